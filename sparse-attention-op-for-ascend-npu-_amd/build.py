@@ -23,6 +23,8 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -52,13 +54,18 @@ HIP_FLAGS = [
     # prologue needs first) into SGPRs at wave launch; 16 dwords is the most
     # the user SGPRs hold, and only scalar arguments qualify.
     "-mllvm", "-amdgpu-kernarg-preload-count=16",
-    # Device code only: no NaN operands, so fmaxf needs no quieting
-    # canonicalisation of its inputs (which doubled the row-max work).  The
-    # kernels never form NaN themselves (masked scores are -inf and an
-    # all-masked row's max is taken as 0).  Host code keeps IEEE NaN
-    # semantics: the C ABI rejects a NaN scale.
-    "-Xarch_device", "-fno-honor-nans",
 ]
+# Device code only: no NaN operands, so fmaxf needs no quieting
+# canonicalisation of its inputs (which doubled the row-max work).  The
+# attention kernels never form NaN themselves (masked scores are -inf and an
+# all-masked row's max is taken as 0).  Host code keeps IEEE NaN
+# semantics: the C ABI rejects a NaN scale.
+NO_NANS_DEFAULT = ["-Xarch_device", "-fno-honor-nans"]
+# The selection ranks scores that are not a number: its file keeps NaN semantics.
+NO_NANS = {"trianglemix_select.hip": []}
+
+HIP_SOURCES = ["trianglemix_kernel.hip", "trianglemix_wide.hip", "trianglemix_cache.hip", "trianglemix_rows.hip",
+               "trianglemix_select.hip", "trianglemix_capi.cpp", "trianglemix_pages_capi.cpp"]
 
 
 def _run(cmd: list[str]) -> None:
@@ -85,10 +92,18 @@ def build_hip_library(phase_clocks: bool = False, plan_override: bool = False) -
     dst = PHASE_CLOCK_LIB if phase_clocks else (PLAN_OVERRIDE_LIB if plan_override else HIP_LIB)
     tmp = dst.with_suffix(".so.tmp")
     defines = (["-DTRIANGLEMIX_PHASE_CLOCKS"] if phase_clocks else []) + (["-DTRIANGLEMIX_PLAN_OVERRIDE"] if plan_override else [])
-    _run([hipcc, *HIP_FLAGS, *defines, "-shared", f"-I{INCLUDE}",
-          str(CSRC / "trianglemix_kernel.hip"), str(CSRC / "trianglemix_wide.hip"), str(CSRC / "trianglemix_cache.hip"),
-          str(CSRC / "trianglemix_capi.cpp"),
-          "-o", str(tmp)])
+    # One object per source, compiled side by side; the names differ per process, so that two builds of one tree
+    # do not meet.
+    with tempfile.TemporaryDirectory() as objects:
+        def compile_one(source: str) -> str:
+            obj = str(Path(objects) / (source + ".o"))
+            _run([hipcc, *HIP_FLAGS, *NO_NANS.get(source, NO_NANS_DEFAULT), *defines, f"-I{INCLUDE}", "-c",
+                  str(CSRC / source), "-o", obj])
+            return obj
+
+        with ThreadPoolExecutor(max_workers=min(len(HIP_SOURCES), os.cpu_count() or 1)) as pool:
+            objs = list(pool.map(compile_one, HIP_SOURCES))
+        _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", str(tmp)])
     _atomic_replace(tmp, dst)
     return dst
 
@@ -105,7 +120,7 @@ def build_torch_adapter() -> Path:
     tmp = TORCH_LIB.with_suffix(".so.tmp")
     _run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-          *incs, str(CSRC / "trianglemix_torch.cpp"),
+          *incs, str(CSRC / "trianglemix_torch.cpp"), str(CSRC / "trianglemix_pages_torch.cpp"),
           f"-L{PKG}", "-ltrianglemix",
           f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python",
           f"-L{ROCM / 'lib'}", "-lamdhip64",

@@ -24,6 +24,7 @@
 #include "../../include/trianglemix.h"
 #include "trianglemix_internal.h"
 #include "trianglemix_kernel.h"
+#include "trianglemix_pages.h"
 
 static_assert(TM_WORKSPACE_COUNTER_BYTES == tmx::kCounterBytes, "the public counter block size is the kernel's");
 static_assert(TM_MAX_WORKSPACE_BYTES == tmx::kMaxWorkspaceBytes, "the public workspace bound is the planner's");
@@ -691,6 +692,20 @@ int check_chunk_table(int64_t table_cols, int64_t first_token, int64_t num_token
 }
 
 }  // namespace
+
+namespace tmx {
+
+int report(int status, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  std::vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
+  va_end(ap);
+  return status;
+}
+
+unsigned long long workspace_tag(const void* workspace) { return workspace_epoch(workspace); }
+
+}  // namespace tmx
 
 extern "C" {
 

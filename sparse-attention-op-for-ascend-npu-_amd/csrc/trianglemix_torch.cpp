@@ -27,6 +27,8 @@
 //   trianglemix::write_chunk_kv(key, value, key_cache!, value_cache!, block_table, query_start) -> ()
 //   trianglemix::chunk_slots(block_table, query_start, num_tokens) -> Tensor
 //
+// The paged serving operators are registered in trianglemix_pages_torch.cpp.
+//
 // Input and output checks restate check_inputs / check_output (:29-97) with
 // the same predicates and messages ("GPU" for "NPU").  Launches go on the
 // current HIP stream of the query's device under a device guard, with no
@@ -58,8 +60,32 @@
 
 #include "../../include/trianglemix.h"
 #include "trianglemix_internal.h"
+#include "trianglemix_torch.h"
 
 namespace trianglemix_rocm {
+
+// Split-KV workspace for a launch on `stream` (see the file comment).
+at::Tensor workspace_for(const at::Tensor& like, int64_t bytes, void* stream) {
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  TORCH_CHECK(hipStreamIsCapturing(static_cast<hipStream_t>(stream), &capture) == hipSuccess,
+              "hipStreamIsCapturing failed");
+  const auto options = like.options().dtype(at::kByte);
+  if (capture != hipStreamCaptureStatusNone) return at::empty({bytes}, options);
+  static std::mutex mutex;
+  static std::map<std::pair<int, void*>, at::Tensor> cache;  // the buffer of each (device, stream)
+  std::lock_guard<std::mutex> lock(mutex);
+  at::Tensor& held = cache[{like.device().index(), stream}];
+  if (!held.defined() || held.numel() < bytes) {
+    held = at::Tensor();  // released first, so that its memory may serve the larger buffer
+    held = at::empty({bytes}, options);
+  }
+  return held;
+}
+
+void check_status(int status, const char* what) {
+  TORCH_CHECK(status == TM_OK, what, " failed (", tm_status_string(status), "): ", tm_last_error());
+}
+
 namespace {
 
 void check_inputs(const at::Tensor& query, const at::Tensor& key_cache, const at::Tensor& value_cache,
@@ -98,28 +124,6 @@ void check_output(const at::Tensor& query, const at::Tensor& key_cache, const at
   at::assert_no_overlap(output, key_cache);
   at::assert_no_overlap(output, value_cache);
   at::assert_no_overlap(output, block_table);
-}
-
-// Split-KV workspace for a launch on `stream` (see the file comment).
-at::Tensor workspace_for(const at::Tensor& like, int64_t bytes, void* stream) {
-  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-  TORCH_CHECK(hipStreamIsCapturing(static_cast<hipStream_t>(stream), &capture) == hipSuccess,
-              "hipStreamIsCapturing failed");
-  const auto options = like.options().dtype(at::kByte);
-  if (capture != hipStreamCaptureStatusNone) return at::empty({bytes}, options);
-  static std::mutex mutex;
-  static std::map<std::pair<int, void*>, at::Tensor> cache;  // the buffer of each (device, stream)
-  std::lock_guard<std::mutex> lock(mutex);
-  at::Tensor& held = cache[{like.device().index(), stream}];
-  if (!held.defined() || held.numel() < bytes) {
-    held = at::Tensor();  // released first, so that its memory may serve the larger buffer
-    held = at::empty({bytes}, options);
-  }
-  return held;
-}
-
-void check_status(int status, const char* what) {
-  TORCH_CHECK(status == TM_OK, what, " failed (", tm_status_string(status), "): ", tm_last_error());
 }
 
 // Launch one chunk; `prompt_len < 0` selects the dense causal companion.
