@@ -65,7 +65,7 @@ NO_NANS_DEFAULT = ["-Xarch_device", "-fno-honor-nans"]
 NO_NANS = {"trianglemix_select.hip": []}
 
 HIP_SOURCES = ["trianglemix_kernel.hip", "trianglemix_wide.hip", "trianglemix_cache.hip", "trianglemix_rows.hip",
-               "trianglemix_select.hip", "trianglemix_capi.cpp", "trianglemix_pages_capi.cpp"]
+               "trianglemix_blocks.hip", "trianglemix_select.hip", "trianglemix_capi.cpp", "trianglemix_pages_capi.cpp"]
 
 
 def _run(cmd: list[str]) -> None:

@@ -1,0 +1,554 @@
+// Attention of large groups of query rows over lists of KV pages, for MI355X
+// (gfx950): selection blocks of a prefill chunk, and large draft trees.  Work,
+// lists and merge as in trianglemix_lists.h; groups of few rows run in
+// trianglemix_rows.hip.
+//
+// A workgroup is four waves of 32 rows each over the same K/V; two workgroups
+// share a CU, so that one's softmax, start-up and end run beside the other's
+// MFMAs.  Tiles are 32 keys (8 KB of K, 8 KB of V), DMA'd into three K and
+// three V slots (distinct objects: the compiler sees that the prefetch does
+// not alias the reads): K three tiles, V two tiles ahead of the tile in hand,
+// 64 KB in flight per CU.  Waves 0 and 1 load K, 2 and 3 load V.
+//
+// Software pipeline: iteration i issues the QK^T MFMAs of tile i + 1 between
+// the exponentials of tile i, then the PV MFMAs of tile i between the row max of
+// tile i + 1.  Only tiles that every row attends whole run there: lists are
+// ascending, so the tiles that need a mask (the keys at and after the block's
+// first row, the end of a tree's context, the tree itself) are the last ones,
+// and run one after the other in a plain loop behind it, with what the pipeline leaves
+// over.  There V entries that are not finite are kept out of the product and
+// added only to rows that attend them, so that what a row does not attend
+// cannot reach it.
+//
+// Contractions (per wave, v_mfma_f32_32x32x16):
+//   S^T (32 keys x 32 rows) = K Q^T, O^T (128 x 32 rows) += V^T P^T,
+// lane l holding row l % 32, accumulator element v key 8 (v / 4) + 4 (l / 32) + v % 4;
+// the scores of a lane are the k-slots of its PV operand.  Numerics as in
+// trianglemix_rows.hip.
+
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include "trianglemix_lists.h"
+
+namespace tmx {
+namespace {
+
+constexpr int kBlockWaves = kBlockRows / 32;
+constexpr int kBlockThreads = kBlockWaves * 64;
+constexpr int kDmaShare = kDmaPerTile / 2;  // two waves share a tile's DMA
+constexpr int kAhead = 3;                   // MFMA steps between an LDS operand read and its use
+static_assert(kBlockWaves == 4 && kPartialBytes == kBlockRows * (kHeadDim + 4) * 4, "the record of four waves");
+
+__device__ __forceinline__ i16x8_t k_operand_of(const char* kt, const int* k_off, int c) {
+  return __builtin_bit_cast(i16x8_t, k_operand(kt, k_off, c));
+}
+__device__ __forceinline__ i16x8_t v_operand_of(const char* vt, const int* v_off, int k) {
+  return __builtin_bit_cast(i16x8_t, v_operand(vt, v_off, k));
+}
+
+template <class Type, bool kTree>
+__global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(const RowsParams p) {
+  typedef typename Type::elem elem;
+  __shared__ __attribute__((aligned(1024))) char k_lds0[kTileBytes];
+  __shared__ __attribute__((aligned(1024))) char k_lds1[kTileBytes];
+  __shared__ __attribute__((aligned(1024))) char k_lds2[kTileBytes];
+  __shared__ __attribute__((aligned(1024))) char v_lds0[kTileBytes];
+  __shared__ __attribute__((aligned(1024))) char v_lds1[kTileBytes];
+  __shared__ __attribute__((aligned(1024))) char v_lds2[kTileBytes];
+  __shared__ ListLds<kTree> lists;
+  __shared__ int s_last;
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool loads_k = wave < 2;
+  const GroupDivider by_group(p.group);
+  const int page_row_bytes = p.kv_heads * kRowBytes;
+  const float c2 = p.scale_log2;
+
+  const int64_t total = plan_units<kTree, kBlockRows, kBlockThreads>(p, lists);
+  const int64_t per_run = max((int64_t)p.min_units, (int64_t)((uint64_t)(total + p.workgroups - 1) / (unsigned)p.workgroups));
+  const int run = run_of_workgroup();
+  int64_t unit = run * per_run;
+  const int64_t unit_end = min(total, unit + per_run);
+
+  while (unit < unit_end) {
+    const Segment g = find_segment<kTree, kBlockRows>(p, lists, unit, unit_end);
+    // Lane values are derived anew in every segment: kept over the loop they
+    // would take registers that the tile loop needs.
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int n = lane & 31, half = lane >> 5;
+
+    // ---- the tiles of the segment ----
+    // Tile t < list_tiles is keys 32 (t % 4) .. of page t / 4 of the list; a
+    // tree's own tiles follow.  All have 32 valid keys but the list's last,
+    // which has `cut`, and the tree's last.
+    int entry = 0, list_pages;
+    bool in_lds = false;
+    int list_tiles, cut, tiles_end;
+    if constexpr (kTree) {
+      list_pages = g.units - 1;
+      list_tiles = (g.context + kKvTile - 1) / kKvTile;
+      cut = g.context - (list_tiles - 1) * kKvTile;
+      tiles_end = g.hi == g.units ? list_tiles + (g.tokens + kKvTile - 1) / kKvTile : 4 * g.hi;
+    } else {
+      list_pages = selected_list<kBlockThreads>(p, lists, g, entry, in_lds);
+    }
+    auto logical_of = [&](int i) {  // page i of the list, i uniform
+      if constexpr (kTree) return i;
+      else return in_lds ? __builtin_amdgcn_readfirstlane(lists.list[i]) : __builtin_amdgcn_readlane(entry, i & 63);
+    };
+    if constexpr (!kTree) {
+      const int end = g.pos0 + g.tokens;  // behind the block's last row
+      const int held = list_pages > 0 ? min(kPageSize, end - logical_of(list_pages - 1) * kPageSize) : 0;
+      list_tiles = list_pages > 0 ? 4 * (list_pages - 1) + (held + kKvTile - 1) / kKvTile : 0;
+      cut = held - (held - 1) / kKvTile * kKvTile;
+      tiles_end = min(4 * g.hi, list_tiles);
+    }
+    const int t0 = 4 * g.lo;
+    const int tiles = max(0, tiles_end - t0);
+    // The leading tiles that every row attends whole.
+    int plain;
+    if constexpr (kTree) {
+      plain = min(g.context / kKvTile, tiles_end) - t0;
+    } else {
+      const int first = max(g.pos0, 0);  // the first row's position
+      int pages = min(g.hi, list_pages);
+      while (pages > g.lo && logical_of(pages - 1) * kPageSize + kPageSize - 1 > first) --pages;
+      plain = 4 * (pages - g.lo);
+      if (pages < min(g.hi, list_pages) && pages >= g.lo) {
+        plain += max(0, (first + 1 - logical_of(pages) * kPageSize) / kKvTile);
+      }
+      plain = min(plain, tiles);
+    }
+
+    // ---- page numbers: 64 pages a register, block b in the one of its parity ----
+    auto load_pages = [&](int block) {
+      const int i = 64 * block + lane;
+      int phys = -1;
+      if (i < list_pages) {
+        int logical = i;
+        if constexpr (!kTree) logical = in_lds ? lists.list[i] : entry;
+        phys = p.block_table[g.request * p.table_stride + logical];
+        if (phys >= p.num_pages) phys = -1;
+      }
+      return phys;
+    };
+    const int block0 = g.lo >> 6;
+    int phys_even = load_pages(block0 + (block0 & 1));
+    int phys_odd = load_pages(block0 + 1 - (block0 & 1));
+    auto phys_of = [&](int page) {
+      return __builtin_amdgcn_readlane((page >> 6) & 1 ? phys_odd : phys_even, page & 63);
+    };
+    int refill_tile = 4 * (64 * (block0 + 1) + 32);  // K of this tile on its way: the block after next is due
+    auto refill = [&](int t) {
+      if (__builtin_expect(t >= refill_tile, 0)) {
+        const int block = (t >> 8) + 1;
+        int phys = load_pages(block);
+        asm volatile("" : "+v"(phys));  // landed before the paths join
+        if (block & 1) phys_odd = phys; else phys_even = phys;
+        refill_tile += 256;
+      }
+    };
+
+    // ---- rows ----
+    const int rows = min(kBlockRows, g.tokens * p.group - g.row_base);
+    const bool active = 32 * wave < rows;
+    const int my_row = 32 * wave + n;
+    const int my_token = by_group.token(g.row_base + my_row);
+    const int my_head = g.row_base + my_row - my_token * p.group;
+    const bool my_ok = my_row < rows;
+    uint64_t my_mask = 0;
+    if constexpr (kTree) {
+      if (my_ok) my_mask = (uint64_t)p.tree_mask[g.row0 + my_token];
+    }
+    i16x8_t q[8];
+    {
+      const uint16_t* const src = p.query + (int64_t)(g.row0 + (my_ok ? my_token : 0)) * p.query_stride +
+                                  (int64_t)(g.kv_head * p.group + (my_ok ? my_head : 0)) * kHeadDim + 8 * half;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) q[c] = *reinterpret_cast<const i16x8_t*>(src + 16 * c);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // Q ahead of the tiles' DMA
+
+    // ---- DMA: this wave's half of a tile of K (waves 0, 1) or V (2, 3) ----
+    const int dma_row = 16 * (wave & 1) + (lane >> 4);
+    int dma_chunk[kDmaShare];
+#pragma unroll
+    for (int j = 0; j < kDmaShare; ++j) {
+      const int row = dma_row + 4 * j;
+      dma_chunk[j] = 16 * (loads_k ? k_slot(row, lane & 15) : v_slot(row, lane & 15));
+    }
+    const char* const cache = loads_k ? p.key_cache : p.value_cache;
+    const int64_t page_stride = loads_k ? p.key_page_stride : p.value_page_stride;
+    // Tile t of the list or tree; past the segment's end an empty range.
+    auto source = [&](int t, int& rb) {
+      const char* base;
+      rb = page_row_bytes;
+      int valid = t == list_tiles - 1 ? cut : kKvTile;
+      if (kTree && t >= list_tiles) {
+        const int at = (t - list_tiles) * kKvTile;
+        rb = (int)(loads_k ? p.draft_key_stride : p.draft_value_stride);
+        base = (loads_k ? p.draft_key : p.draft_value) + (int64_t)(g.row0 + at) * rb;
+        valid = g.tokens - at;
+        valid = min(valid, kKvTile);
+      } else {
+        const int phys = phys_of(t >> 2);
+        base = cache + max(phys, 0) * page_stride + (t & 3) * (kKvTile * page_row_bytes);
+        if (phys < 0) valid = 0;
+      }
+      if (t >= tiles_end) valid = 0;
+      return __builtin_amdgcn_make_buffer_rsrc((void*)(base + g.kv_head * kRowBytes), (short)0,
+                                               valid > 0 ? (valid - 1) * rb + kRowBytes : 0, kBufferFlags);
+    };
+    auto dma = [&](__amdgpu_buffer_rsrc_t rsrc, int rb, char* slot, int j) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, TM_LDS(slot + ((wave & 1) * kDmaShare + j) * 1024), 16,
+                                               (unsigned)((dma_row + 4 * j) * rb + dma_chunk[j]), 0, 0, 0);
+    };
+    auto load_tile = [&](int t, char* slot) {
+      int rb;
+      const __amdgpu_buffer_rsrc_t rsrc = source(t, rb);
+#pragma unroll
+      for (int j = 0; j < kDmaShare; ++j) dma(rsrc, rb, slot, j);
+    };
+    if (loads_k) {
+      load_tile(t0, k_lds0);
+      load_tile(t0 + 1, k_lds1);
+      load_tile(t0 + 2, k_lds2);
+    } else {
+      load_tile(t0, v_lds0);
+      load_tile(t0 + 1, v_lds1);
+    }
+
+    // ---- operand addresses in a slot ----
+    int k_off[8], v_off[4];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) k_off[c] = n * kRowBytes + 16 * k_slot(n, 2 * c + half);
+    const int v_key = 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int d = 32 * m + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      v_off[m] = v_key * kRowBytes + 16 * v_slot(v_key, d >> 3) + 2 * (d & 7);
+    }
+
+    float m_run = -INFINITY, l_run = 0.0f;  // of the row; the sum over this lane's keys
+    f32x16_t o[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) o[m] = f32x16_t{};
+    // The row's running max takes in a tile's; returns the exponentials' shift.
+    auto raise = [&](float top) {
+      if (__any(top > m_run + kLazyRescale)) {
+        const float m_new = fmaxf(m_run, top);
+        const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+        l_run *= alpha;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) o[m] *= alpha;
+        m_run = m_new;
+      }
+      return m_run == -INFINITY ? 0.0f : m_run;
+    };
+    auto row_top = [&](const f32x16_t& s) {
+      float top = s[0];
+#pragma unroll
+      for (int v = 1; v < 16; ++v) top = fmaxf(top, s[v]);
+      return half_max(top) * c2;
+    };
+    auto scores = [&](const char* ks) {
+      f32x16_t s = f32x16_t{};
+      i16x8_t kf[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) kf[c] = k_operand_of(ks, k_off, c);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) s = Type::mfma32(kf[c], q[c], s);
+      return s;
+    };
+
+    // ---- the pipeline ----
+    const int fast = plain > 3 ? (plain - 1) / 3 * 3 : 0;
+    if (fast > 0) {
+      if (loads_k) wait_dma_but<2 * kDmaShare>();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      f32x16_t s_a = f32x16_t{}, s_b = f32x16_t{};
+      float top = -INFINITY;
+      if (active) {
+        s_a = scores(k_lds0);
+        if (phys_of(t0 >> 2) < 0) s_a = f32x16_t{} - INFINITY;
+        top = row_top(s_a);
+      }
+      // Iteration it: scores of tile it in s_cur, their row max in `top`.  K of
+      // it + 1 in kr, V of it in vr; K of it + 3 goes into kw, V of it + 2 into vw.
+      auto iteration = [&](int it, f32x16_t& s_cur, f32x16_t& s_nxt, const char* kr, const char* vr, char* kw,
+                           char* vw) {
+        wait_dma_but<kDmaShare>();  // K of it + 1, V of it have landed
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();  // for every wave, and the slots kw, vw are read
+        asm volatile("" ::: "memory");
+        const int t_load = t0 + it + (loads_k ? 3 : 2);
+        refill(t_load);
+        int rb;
+        const __amdgpu_buffer_rsrc_t src = source(t_load, rb);
+        char* const slot = loads_k ? kw : vw;
+        if (!active) {
+#pragma unroll
+          for (int j = 0; j < kDmaShare; ++j) dma(src, rb, slot, j);
+          return;
+        }
+        const float shift = raise(top);
+        i16x8_t kf[8], va[8];
+        float px[16], sum = 0.0f;
+        auto expo = [&](int e) {
+          px[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s_cur[e], c2, -shift));
+          sum += px[e];
+        };
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) kf[k] = k_operand_of(kr, k_off, k);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if ((k & 1) == 0) dma(src, rb, slot, k >> 1);
+          if (k + kAhead < 8) kf[k + kAhead] = k_operand_of(kr, k_off, k + kAhead);
+          else va[k + kAhead - 8] = v_operand_of(vr, v_off, k + kAhead - 8);
+          s_nxt = Type::mfma32(kf[k], q[k], k == 0 ? f32x16_t{} : s_nxt);
+          expo(k);
+          if ((k & 1) == 0) expo(8 + (k >> 1));
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        typename Type::vec pb[2];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pb[0][e] = (elem)px[e];
+        asm volatile("" ::"v"(pb[0]), "v"(px[8]), "v"(px[9]), "v"(px[10]), "v"(px[11]), "v"(sum));
+        if (phys_of((t0 + it + 1) >> 2) < 0) s_nxt = f32x16_t{} - INFINITY;  // a page without keys
+        float next = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (k + kAhead < 8) va[k + kAhead] = v_operand_of(vr, v_off, k + kAhead);
+          if (k < 4) {
+            expo(12 + k);
+            if (k == 3) {
+#pragma unroll
+              for (int e = 8; e < 16; ++e) pb[1][e - 8] = (elem)px[e];
+            }
+          }
+          o[k & 3] = Type::mfma32(va[k], __builtin_bit_cast(i16x8_t, pb[k >> 2]), o[k & 3]);
+          next = fmaxf(fmaxf(next, s_nxt[2 * k]), s_nxt[2 * k + 1]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        l_run += sum;
+        top = half_max(next) * c2;
+      };
+      // Scores swap buffers every tile and slots turn every three: six tiles a
+      // round, or three and a copy.
+      int it = 0;
+      for (; it + 3 < fast; it += 6) {
+        iteration(it, s_a, s_b, k_lds1, v_lds0, k_lds0, v_lds2);
+        iteration(it + 1, s_b, s_a, k_lds2, v_lds1, k_lds1, v_lds0);
+        iteration(it + 2, s_a, s_b, k_lds0, v_lds2, k_lds2, v_lds1);
+        iteration(it + 3, s_b, s_a, k_lds1, v_lds0, k_lds0, v_lds2);
+        iteration(it + 4, s_a, s_b, k_lds2, v_lds1, k_lds1, v_lds0);
+        iteration(it + 5, s_b, s_a, k_lds0, v_lds2, k_lds2, v_lds1);
+      }
+      if (it < fast) {
+        iteration(it, s_a, s_b, k_lds1, v_lds0, k_lds0, v_lds2);
+        iteration(it + 1, s_b, s_a, k_lds2, v_lds1, k_lds1, v_lds0);
+        iteration(it + 2, s_a, s_b, k_lds0, v_lds2, k_lds2, v_lds1);
+      }
+    }
+
+    // ---- the rest, with masks: K on its way up to tile it + 2, V up to it + 1 ----
+    for (int it = fast; it < tiles; ++it) {
+      wait_dma();
+      __syncthreads();
+      const int t = t0 + it;
+      const int turn = it % 3;
+      if (loads_k) {
+        if (it > fast) load_tile(t + 2, turn == 0 ? k_lds2 : turn == 1 ? k_lds0 : k_lds1);
+      } else {
+        load_tile(t + 2, turn == 0 ? v_lds2 : turn == 1 ? v_lds0 : v_lds1);
+      }
+      if (!active) continue;
+      const char* const ks = turn == 0 ? k_lds0 : turn == 1 ? k_lds1 : k_lds2;
+      const char* const vs = turn == 0 ? v_lds0 : turn == 1 ? v_lds1 : v_lds2;
+      f32x16_t s = scores(ks);
+      if (it >= plain || phys_of(t >> 2) < 0) {
+        int thr = -1;  // the last key offset in the tile that the row attends
+        uint32_t bits = ~0u;
+        if (kTree && t >= list_tiles) {
+          thr = g.tokens - 1 - (t - list_tiles) * kKvTile;
+          bits = (uint32_t)(my_mask >> ((t - list_tiles) * kKvTile));
+        } else if (phys_of(t >> 2) >= 0) {
+          if constexpr (kTree) {
+            thr = g.context - 1 - t * kKvTile;
+          } else {
+            thr = (my_ok ? g.pos0 + my_token : -1) - logical_of(t >> 2) * kPageSize - (t & 3) * kKvTile;
+          }
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int key = elem_key(v) + 4 * half;
+          const bool seen = key <= thr && ((bits >> key) & 1) != 0;
+          s[v] = seen ? s[v] : -INFINITY;
+        }
+      }
+      const float shift = raise(row_top(s));
+      typename Type::vec pb[2];
+      float sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c2, -shift));
+        sum += x;
+        pb[e >> 3][e & 7] = (elem)x;
+      }
+      l_run += sum;
+      i16x8_t va[8];
+      bool bad = false;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        va[k] = v_operand_of(vs, v_off, k);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) bad |= ((unsigned)va[k][e] & Type::kExp) == Type::kExp;
+      }
+      if (__builtin_expect(!__any(bad), 1)) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k & 3] = Type::mfma32(va[k], __builtin_bit_cast(i16x8_t, pb[k >> 2]), o[k & 3]);
+      } else {
+        // The finite entries, then for each other kind an indicator's product: it
+        // is positive in the rows that attend such an entry.
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+#pragma unroll
+          for (int kind = 0; kind < 4; ++kind) {  // finite, +inf, -inf, NaN
+            f32x16_t has = f32x16_t{};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              // read anew and opaque: kept over the kinds they would spill
+              asm volatile("" ::: "memory");
+              u32x4_t a = __builtin_bit_cast(u32x4_t, v_operand_of(vs, v_off, m + 4 * j));
+              asm volatile("" : "+v"(a));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) a[e] = only_kind<Type>(a[e], kind) | only_kind<Type>(a[e] >> 16, kind) << 16;
+              if (kind == 0) o[m] = Type::mfma32(__builtin_bit_cast(i16x8_t, a), __builtin_bit_cast(i16x8_t, pb[j]), o[m]);
+              else has = Type::mfma32(__builtin_bit_cast(i16x8_t, a), __builtin_bit_cast(i16x8_t, pb[j]), has);
+            }
+            if (kind > 0) {
+              // opaque: the compiler takes no operand for a NaN; +inf and -inf give one by themselves
+              float odd = __uint_as_float(kind == 1 ? 0x7f800000u : kind == 2 ? 0xff800000u : 0x7fc00000u);
+              asm volatile("" : "+v"(odd));
+#pragma unroll
+              for (int v = 0; v < 16; ++v) o[m][v] += has[v] > 0.0f ? odd : 0.0f;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+    }
+    wait_dma();
+    __syncthreads();  // no slot is read or written any more
+
+    // Rows out: normalised and rounded, gathered in the wave's slot as whole
+    // rows (8-byte pieces in, 16-byte chunks out, chunk c of row r at c ^ (r %
+    // 16)), stored through L2 in whole cache lines.
+    char* const stage = wave == 0 ? k_lds0 : wave == 1 ? k_lds1 : wave == 2 ? k_lds2 : v_lds0;
+    auto store_rows = [&](float l) {
+      const float l_row = half_sum(l);
+      const float inv = l_row > 0.0f ? 1.0f / l_row : 0.0f;
+      typedef elem elem4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          elem4 y;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = (elem)(o[m][4 * c + e] * inv);
+          *reinterpret_cast<elem4*>(stage + n * kRowBytes + 16 * ((4 * m + c) ^ (n & 15)) + 8 * half) = y;
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = 4 * j + (lane >> 4), c = lane & 15;
+        const u32x4_t y = *reinterpret_cast<const u32x4_t*>(stage + r * kRowBytes + 16 * (c ^ (r & 15)));
+        const int row = 32 * wave + r;
+        const int t = by_group.token(g.row_base + row);
+        const int h = g.row_base + row - t * p.group;
+        if (row < rows && t >= g.held) {
+          *reinterpret_cast<u32x4_t*>(p.out + ((int64_t)(g.row0 + t) * p.heads + g.kv_head * p.group + h) * kHeadDim +
+                                      8 * c) = y;
+        }
+      }
+    };
+    if (g.lo == 0 && g.hi == g.units) {
+      if (active) store_rows(l_run);
+    } else {
+      // ---- a group of several runs ----
+      const Shared shared(g, per_run);
+      const __amdgpu_buffer_rsrc_t rec = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)p.partials, (short)0, (int)((unsigned)p.workgroups * 2u * (unsigned)kPartialBytes), kBufferFlags);
+      // record: O [wave][d-block, quarter][lane][4], then row maxima and lane sums [wave][lane]
+      auto piece = [&](int i) { return (unsigned)(((wave * 16 + i) * 64 + lane) * 16); };
+      const unsigned at_max = (unsigned)(kBlockRows * kHeadDim * 4 + (wave * 64 + lane) * 4);
+      const unsigned at_sum = at_max + kBlockThreads * 4;
+      if (active) {
+        const unsigned own = shared.record(run, (unsigned)kPartialBytes);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const f32x4_t x = {o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2],
+                             o[i >> 2][4 * (i & 3) + 3]};
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, x), rec, own + piece(i), 0, kCpolAgent);
+        }
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(m_run), rec, own + at_max, 0, kCpolAgent);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l_run), rec, own + at_sum, 0, kCpolAgent);
+      }
+      if (last_to_arrive(p, shared, &s_last) && active) {
+        float top = -INFINITY;
+#pragma unroll 4
+        for (int r = shared.first_run; r <= shared.last_run; ++r) {
+          top = fmaxf(top, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                               rec, shared.record(r, (unsigned)kPartialBytes) + at_max, 0, kCpolAgent)));
+        }
+        const float shift = top == -INFINITY ? 0.0f : top;
+        float l = 0.0f;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) o[m] = f32x16_t{};
+        for (int r = shared.first_run; r <= shared.last_run; ++r) {
+          const unsigned from = shared.record(r, (unsigned)kPartialBytes);
+          const float mr = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rec, from + at_max, 0, kCpolAgent));
+          const float lr = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rec, from + at_sum, 0, kCpolAgent));
+          f32x4_t x[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            x[i] = __builtin_bit_cast(f32x4_t,
+                                      __builtin_amdgcn_raw_buffer_load_b128(rec, from + piece(i), 0, kCpolAgent));
+          }
+          const float w = __builtin_amdgcn_exp2f(mr - shift);
+          l += lr * w;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i >> 2][4 * (i & 3) + e] += x[i][e] * w;
+          }
+        }
+        store_rows(l);
+      }
+    }
+    unit = g.first + g.hi;
+    __syncthreads();
+  }
+}
+
+template <class Type, bool kTree>
+hipError_t launch_type(const RowsParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL((blocks_attention_kernel<Type, kTree>), dim3((unsigned)p.workgroups), dim3(kBlockThreads), 0,
+                     stream, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_blocks_attention(const RowsParams& p, bool fp16, hipStream_t stream) {
+  if (p.selected == nullptr) return fp16 ? launch_type<Fp16, true>(p, stream) : launch_type<Bf16, true>(p, stream);
+  return fp16 ? launch_type<Fp16, false>(p, stream) : launch_type<Bf16, false>(p, stream);
+}
+
+}  // namespace tmx

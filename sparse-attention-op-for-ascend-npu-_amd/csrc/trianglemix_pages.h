@@ -78,12 +78,17 @@ struct RowsParams {
   int min_units;            // fewest pages a workgroup takes
   float scale_log2;
 };
-// Rows of one workgroup in the shapes of the kernel.
-constexpr int kRowShapes[] = {16, 32, 64, 128, 256};
-// Bytes of one workgroup's two partial records (O, row maxima, row sums) with
-// this many rows.
-constexpr int64_t rows_partial_bytes(int shape_rows) { return int64_t(2) * shape_rows * (kHeadDim + 2) * 4; }
+// Groups of up to kRowShapes rows run in trianglemix_rows.hip, in the smallest
+// shape that holds them; larger ones in trianglemix_blocks.hip, kBlockRows rows
+// a workgroup.
+constexpr int kRowShapes[] = {16, 32, 64};
+constexpr int kBlockRows = 128;
+// A run of units leaves at most two partial records of this many bytes.
+constexpr int64_t rows_partial_bytes(int rows) {
+  return rows == kBlockRows ? kPartialBytes : int64_t(rows) * (kHeadDim + 2) * 4;
+}
 hipError_t launch_rows_attention(const RowsParams& p, int shape_rows, bool fp16, hipStream_t stream);
+hipError_t launch_blocks_attention(const RowsParams& p, bool fp16, hipStream_t stream);
 
 // From trianglemix_capi.cpp: the calling thread's last error text (returns
 // status), and the arrival tag of a launch on this workspace.

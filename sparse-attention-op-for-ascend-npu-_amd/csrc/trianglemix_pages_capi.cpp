@@ -179,12 +179,12 @@ int check_select(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, i
   return st;
 }
 
-// The smallest shape that holds `rows` rows, else the largest.
+// Rows of the workgroup shape for groups of `rows` rows.
 int shape_for(int64_t rows) {
   for (int s : tmx::kRowShapes) {
     if (rows <= s) return s;
   }
-  return tmx::kRowShapes[4];
+  return tmx::kBlockRows;
 }
 
 struct RowsPlan {
@@ -192,16 +192,24 @@ struct RowsPlan {
   int64_t workspace_bytes;
 };
 
-// Workgroups of the attention kernels: one per CU (its LDS holds one), fewer
-// when the units would not give each min_units; a multiple of the 8 XCDs.
-RowsPlan rows_plan(int64_t rows, int64_t most_units) {
+// As many workgroups as the GPU holds at once, fewer when the units would not
+// give each min_units; a multiple of the 8 XCDs.
+RowsPlan rows_plan(int shape, int64_t most_units) {
   RowsPlan r;
-  r.shape = shape_for(rows);
+  r.shape = shape;
   r.min_units = 1;
-  const int64_t wanted = std::min<int64_t>(kComputeUnits, (most_units + r.min_units - 1) / r.min_units);
+  const int64_t slots = kComputeUnits * (shape == tmx::kBlockRows ? 2 : 1);  // of its LDS a CU holds two, or one
+  const int64_t wanted = std::min<int64_t>(slots, (most_units + r.min_units - 1) / r.min_units);
   r.workgroups = (int)((wanted + 7) / 8 * 8);
-  r.workspace_bytes = tmx::kCounterBytes + r.workgroups * tmx::rows_partial_bytes(r.shape);
+  r.workspace_bytes = tmx::kCounterBytes + 2 * r.workgroups * tmx::rows_partial_bytes(r.shape);
   return r;
+}
+
+int launch_attention(const tmx::RowsParams& p, const RowsPlan& plan, int dtype, void* stream) {
+  const bool fp16 = dtype == TM_FP16;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  return launched(plan.shape == tmx::kBlockRows ? tmx::launch_blocks_attention(p, fp16, s)
+                                                : tmx::launch_rows_attention(p, plan.shape, fp16, s));
 }
 
 int check_selected(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t count) {
@@ -219,7 +227,7 @@ RowsPlan selected_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_he
   const int64_t group_rows = std::min<int64_t>(rows, tmx::kSelectRows) * (heads / kv_heads);
   const int shape = shape_for(group_rows);
   const int64_t blocks = (rows + tmx::kSelectRows - 1) / tmx::kSelectRows;
-  return rows_plan(group_rows, batch * blocks * kv_heads * ((group_rows + shape - 1) / shape) * count);
+  return rows_plan(shape, batch * blocks * kv_heads * ((group_rows + shape - 1) / shape) * count);
 }
 
 int check_tree(int64_t total_rows, int64_t batch, int64_t heads, int64_t kv_heads, int64_t table_cols) {
@@ -236,7 +244,7 @@ RowsPlan tree_plan(int64_t total_rows, int64_t batch, int64_t heads, int64_t kv_
   const int64_t nodes = std::min<int64_t>((total_rows + batch - 1) / batch, tmx::kMaxTreeNodes);
   const int shape = shape_for(nodes * group);
   const int64_t groups = kv_heads * (batch + total_rows * group / shape);
-  return rows_plan(nodes * group, groups * (table_cols + 1));
+  return rows_plan(shape, groups * (table_cols + 1));
 }
 
 }  // namespace
@@ -425,7 +433,7 @@ int tm_selected_page_attention(const void* query, int64_t query_stride, const vo
   p.workgroups = plan.workgroups;
   p.min_units = plan.min_units;
   p.scale_log2 = scale * 1.4426950408889634f;
-  return launched(tmx::launch_rows_attention(p, plan.shape, dtype == TM_FP16, static_cast<hipStream_t>(stream)));
+  return launch_attention(p, plan, dtype, stream);
 }
 
 int64_t tm_tree_attention_workspace_size(int64_t total_rows, int64_t batch, int64_t heads, int64_t kv_heads,
@@ -505,7 +513,7 @@ int tm_tree_attention(const void* query, int64_t query_stride, const void* key, 
   p.workgroups = plan.workgroups;
   p.min_units = plan.min_units;
   p.scale_log2 = scale * 1.4426950408889634f;
-  return launched(tmx::launch_rows_attention(p, plan.shape, dtype == TM_FP16, static_cast<hipStream_t>(stream)));
+  return launch_attention(p, plan, dtype, stream);
 }
 
 }  // extern "C"

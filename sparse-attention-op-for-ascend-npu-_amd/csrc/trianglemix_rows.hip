@@ -1,21 +1,8 @@
-// Attention of groups of query rows over lists of KV pages, for MI355X
-// (gfx950): attention over selected pages, and over draft trees.
+// Attention of small groups of query rows over lists of KV pages, for MI355X
+// (gfx950): a decoding step over selected pages, and draft trees.
 //
-// Work
-// ----
-// A group is the query rows that read the same K/V: (request, KV head) with
-// all heads of the GQA group, and the rows of one selection block (32 tokens)
-// or of one draft tree; rows are numbered token * G + head of the group, and a
-// group of more rows than a workgroup's shape holds is cut into several.  A
-// unit is one page (128 keys) of one group; a tree's own nodes are its group's
-// last unit.  The units of all groups, in a row, are dealt to the workgroups
-// in equal contiguous runs, so every workgroup streams the same number of pages
-// whatever the lengths in the batch are, and the grid does not depend on them:
-// lengths are read on the device, a captured call can be replayed with others.
-// A group whose units lie in one workgroup is written by it.  Otherwise each
-// of its workgroups leaves an fp32 partial (O, row max, row sum) in the
-// workspace and counts its arrival, and the one that arrives last merges them
-// in order (the same sums whichever is last) and writes the rows.
+// Work, lists and merge as in trianglemix_lists.h; groups of more rows run in
+// trianglemix_blocks.hip.
 //
 // A workgroup is four waves = RW row parts x KW = 4 / RW key parts; a wave owns
 // 16 NT rows.  Each page goes HBM -> LDS by DMA, 32 KB of K and 32 KB of V, one
@@ -44,39 +31,12 @@
 
 #include <stdint.h>
 
-#include "trianglemix_device.h"
-#include "trianglemix_pages.h"
+#include "trianglemix_lists.h"
 
 namespace tmx {
 namespace {
 
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef short i16x8_t __attribute__((ext_vector_type(8)));
-
-struct Bf16 {
-  typedef __bf16 elem;
-  typedef bf16x8_t vec;
-  static constexpr unsigned kExp = 0x7f80;  // exponent bits: all set in infinities and NaNs
-  static constexpr short kOne = 0x3f80;
-  static __device__ __forceinline__ f32x4_t mfma(i16x8_t a, i16x8_t b, f32x4_t c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
-  }
-};
-struct Fp16 {
-  typedef _Float16 elem;
-  typedef f16x8_t vec;
-  static constexpr unsigned kExp = 0x7c00;
-  static constexpr short kOne = 0x3c00;
-  static __device__ __forceinline__ f32x4_t mfma(i16x8_t a, i16x8_t b, f32x4_t c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
-  }
-};
-
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * 64;
 constexpr int kSlotBytes = kPageSize * kRowBytes;  // 32 KB: K or V of one page
-constexpr int kDmaPerWave = 2 * 8;                 // 1 KB instructions of a wave per page: its 32 keys of K and V
-constexpr int kCpolAgent = 16;                     // sc1: seen by every XCD
 
 // Max / sum over the four lanes that hold one row (l, l ^ 16, l ^ 32, l ^ 48).
 __device__ __forceinline__ float row_max(float x) {
@@ -102,29 +62,16 @@ __device__ __forceinline__ i16x8_t v_operand16(const char* vt, int off) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// A value that every lane holds alike, in scalar registers.
-__device__ __forceinline__ int64_t uniform64(int64_t x) {
-  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) |
-                   (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
-}
-
-// A run of consecutive units of one group.
-struct Segment {
-  int request, kv_head;
-  int row0;        // first query row (token) of the group in query / out
-  int tokens;      // its tokens
-  int row_base;    // first of its rows (token * group + head) this workgroup holds
-  int pos0;        // position of token row0 (selected pages)
-  int held;        // first tokens without a row (negative positions)
-  int lo, hi;      // pages
-  int units;       // pages of the whole group
-  int64_t first;   // the group's first unit
-};
-
-template <class Type, int NT, int RW, bool kTree>
-__global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsParams p) {
-  constexpr int KW = kWaves / RW;
+// RW row parts x KW key parts, one wave each, of 16 NT rows.
+template <class Type, int NT, int RW, int KW, bool kTree>
+__global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel(const RowsParams p) {
+  constexpr int kWaves = RW * KW;
+  constexpr int kThreads = kWaves * 64;
+  constexpr int kWaveKeys = kPageSize / kWaves;  // keys of a page that a wave loads
+  constexpr int kDma = kWaveKeys / 4;            // by this many 1 KB instructions each for K and V
   constexpr int kWaveRows = 16 * NT;
+  static_assert(kWaves % 4 == 0 && kWaves * kWaveRows * kHeadDim * 4 <= 4 * kSlotBytes, "the waves' O fit the slots");
+  static_assert(RW > 1 || KW == 4, "without row parts a wave loads the 32 keys that it reads");
   constexpr int kRows = kWaveRows * RW;
   typedef typename Type::elem elem;
 
@@ -133,12 +80,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
   __shared__ __attribute__((aligned(1024))) char k_lds1[kSlotBytes];
   __shared__ __attribute__((aligned(1024))) char v_lds1[kSlotBytes];
   __shared__ float s_max[kWaves][kWaveRows], s_sum[kWaves][kWaveRows];
-  // trees: running unit counts of the requests; selected pages: the list of one
-  // selection, and the set it is made from
-  __shared__ int64_t s_units[kTree ? kMaxBatch : 1];
-  __shared__ unsigned s_set[kTree ? 1 : kMaxTableCols / 32];
-  __shared__ int s_list[kTree ? 1 : kMaxSelected];
-  __shared__ int s_count[kWaves];
+  __shared__ ListLds<kTree> lists;
   __shared__ int s_last;
 
   const int tid = threadIdx.x;
@@ -149,165 +91,27 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
   const int rw = wave % RW, kw = wave / RW;
   const int G = p.group;
 
-  // Workgroups are dispatched round-robin over the 8 XCDs: neighbouring runs of
-  // units, which share K/V pages where selections overlap, go to one XCD.
-  const int run = (int)((blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8);
+  const GroupDivider by_group(p.group);
+  const int page_row_bytes = p.kv_heads * kRowBytes;
 
-  // ---- the plan: units, and this workgroup's run of them ----
-  auto tree_of = [&](int b, int& row0, int& tokens, int& pages) {
-    const int at = p.tree_offsets[b], end = p.tree_offsets[b + 1];
-    row0 = min(max(at, 0), p.total_rows);
-    tokens = min(min(max(end, row0), p.total_rows) - row0, kMaxTreeNodes);
-    const int context = min(max(p.lens[b], 0), p.table_cols * kPageSize);
-    pages = (context + kPageSize - 1) / kPageSize;
-  };
-  int64_t total;
-  if constexpr (kTree) {
-    // four consecutive requests a thread, prefix sums over the workgroup
-    int64_t mine[4], sum = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int b = 4 * tid + i;
-      mine[i] = 0;
-      if (b < p.batch) {
-        int row0, tokens, pages;
-        tree_of(b, row0, tokens, pages);
-        mine[i] = (int64_t)p.kv_heads * ((tokens * G + kRows - 1) / kRows) * (pages + 1);
-      }
-      sum += mine[i];
-    }
-    int64_t* scan = reinterpret_cast<int64_t*>(k_lds0);
-    scan[tid] = sum;
-    __syncthreads();
-    for (int d = 1; d < kThreads; d <<= 1) {
-      const int64_t add = tid >= d ? scan[tid - d] : 0;
-      __syncthreads();
-      scan[tid] += add;
-      __syncthreads();
-    }
-    int64_t upto = scan[tid] - sum;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      upto += mine[i];
-      s_units[4 * tid + i] = upto;
-    }
-    __syncthreads();
-    total = uniform64(s_units[p.batch - 1]);
-    __syncthreads();
-  } else {
-    const int row_parts = (min(p.rows, kSelectRows) * G + kRows - 1) / kRows;
-    total = (int64_t)p.batch * p.blocks * p.kv_heads * row_parts * p.count;
-  }
-  const int64_t per_run = max((int64_t)p.min_units, (total + p.workgroups - 1) / p.workgroups);
+  const int64_t total = plan_units<kTree, kRows, kThreads>(p, lists);
+  const int64_t per_run = max((int64_t)p.min_units, (int64_t)((uint64_t)(total + p.workgroups - 1) / (unsigned)p.workgroups));
+  const int run = run_of_workgroup();
   int64_t unit = run * per_run;
   const int64_t unit_end = min(total, unit + per_run);
 
-  const int page_row_bytes = p.kv_heads * kRowBytes;
-
   while (unit < unit_end) {
-    Segment g;
-    bool draft_last = false;
-    int context = 0;  // trees: keys of the cache; selected pages: unused
-    int row_parts;
-    if constexpr (kTree) {
-      int lo = 0, hi = p.batch - 1;  // the request whose running count first passes `unit`
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (s_units[mid] > unit) hi = mid; else lo = mid + 1;
-      }
-      g.request = __builtin_amdgcn_readfirstlane(lo);
-      int pages;
-      tree_of(g.request, g.row0, g.tokens, pages);
-      g.units = pages + 1;
-      row_parts = (g.tokens * G + kRows - 1) / kRows;
-      const int64_t before = g.request > 0 ? uniform64(s_units[g.request - 1]) : 0;
-      const int local = (int)((unit - before) / g.units);
-      g.kv_head = local / row_parts;
-      g.row_base = (local % row_parts) * kRows;
-      g.first = before + (int64_t)local * g.units;
-      context = min(max(p.lens[g.request], 0), p.table_cols * kPageSize);
-      g.pos0 = 0;
-      g.held = 0;
-    } else {
-      row_parts = (min(p.rows, kSelectRows) * G + kRows - 1) / kRows;
-      g.units = p.count;
-      int64_t id = unit / p.count;
-      g.first = id * p.count;
-      // KV head outermost: the blocks of one head share its pages
-      g.row_base = (int)(id % row_parts) * kRows;
-      id /= row_parts;
-      const int blk = (int)(id % p.blocks);
-      id /= p.blocks;
-      g.request = (int)(id % p.batch);
-      g.kv_head = (int)(id / p.batch);
-      g.row0 = g.request * p.rows + blk * kSelectRows;
-      g.tokens = min(kSelectRows, p.rows - blk * kSelectRows);
-      g.pos0 = max(p.lens[g.request], 0) - p.rows + blk * kSelectRows;
-      g.held = max(0, -g.pos0);
-    }
-    g.lo = (int)(unit - g.first);
-    g.hi = (int)(min(unit_end, g.first + g.units) - g.first);
+    const Segment g = find_segment<kTree, kRows>(p, lists, unit, unit_end);
     const bool whole = g.lo == 0 && g.hi == g.units;
     const int valid_rows = min(kRows, g.tokens * G - g.row_base);  // may be <= 0 for a block's last row part
 
     // ---- the pages: list index i -> logical page; physical page or -1 ----
     const int32_t* const table = p.block_table + g.request * p.table_stride;
-    int list_len;        // pages of the list
-    bool in_lds = false;  // the list is in s_list, else (selected) in entry / (tree) the index itself
+    int list_len;  // pages of the list
+    bool in_lds = false;
     int entry = 0;
-    if constexpr (kTree) {
-      list_len = g.units - 1;
-    } else {
-      const int last = g.pos0 + g.tokens - 1;
-      const int possible = last < 0 ? 0 : min(p.table_cols, last / kPageSize + 1);
-      const int32_t* const chosen =
-          p.selected + ((int64_t)(g.row0 - g.request * p.rows) / kSelectRows + (int64_t)g.request * p.blocks) *
-                           p.kv_heads * p.count + (int64_t)g.kv_head * p.count;
-      bool sorted = false;
-      if (p.count <= 64) {
-        // As select_pages leaves it: ascending, what is no page of the block behind.
-        entry = lane < p.count ? chosen[lane] : -1;
-        const bool ok = entry >= 0 && entry < possible;
-        const int before = __shfl_up(ok ? entry : 0x7fffffff, 1);
-        sorted = !__any(ok && lane > 0 && before >= entry);
-        list_len = __popcll(__ballot(ok));
-      }
-      if (!sorted) {
-        // Any order, entries repeated or out of range: through the set of pages.
-        const int words = (possible + 31) / 32;
-        __syncthreads();
-        for (int i = tid; i < words; i += kThreads) s_set[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < p.count; i += kThreads) {
-          const int e = chosen[i];
-          if (e >= 0 && e < possible) atomicOr(&s_set[e >> 5], 1u << (e & 31));
-        }
-        __syncthreads();
-        int base = 0;
-        for (int w0 = 0; w0 < words; w0 += kThreads) {
-          unsigned bits = w0 + tid < words ? s_set[w0 + tid] : 0;
-          const int n = __popc(bits);
-          int upto = n;
-          for (int d = 1; d < 64; d <<= 1) {
-            const int add = __shfl_up(upto, d);
-            if (lane >= d) upto += add;
-          }
-          if (lane == 63) s_count[wave] = upto;
-          __syncthreads();
-          int at = base + upto - n;
-          for (int w = 0; w < wave; ++w) at += s_count[w];
-          base += s_count[0] + s_count[1] + s_count[2] + s_count[3];
-          while (bits) {  // at most count entries in all
-            s_list[at++] = 32 * (w0 + tid) + __ffs(bits) - 1;
-            bits &= bits - 1;
-          }
-          __syncthreads();
-        }
-        list_len = base;
-        in_lds = true;
-      }
-    }
-    list_len = __builtin_amdgcn_readfirstlane(list_len);
+    if constexpr (kTree) list_len = g.units - 1;
+    else list_len = selected_list<kThreads>(p, lists, g, entry, in_lds);
     // Pages 64 t .. 64 t + 63 of the list, one a lane.
     int logical64 = 0, phys64 = 0;
     auto load_pages = [&](int t) {
@@ -315,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
       if constexpr (kTree) {
         logical64 = i;
       } else {
-        logical64 = !in_lds ? entry : i < list_len ? s_list[i] : 0;
+        logical64 = !in_lds ? entry : i < list_len ? lists.list[i] : 0;
       }
       phys64 = i < list_len ? table[logical64] : -1;
       if (phys64 >= p.num_pages) phys64 = -1;
@@ -329,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int r = rw * kWaveRows + 16 * n + col;
-      const int t = (g.row_base + r) / G;
+      const int t = by_group.token(g.row_base + r);
       const int h = g.row_base + r - t * G;
       const bool ok = r < valid_rows;
       row_pos[n] = ok ? g.pos0 + t : -1;
@@ -358,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
       for (int m = 0; m < 8; ++m) o[m][n] = f32x4_t{};
     }
 
-    // ---- DMA of page i into a slot pair: this wave's 32 keys ----
+    // ---- DMA of page i into a slot pair: this wave's share of the keys ----
     auto issue = [&](int i, char* k_slot_base, char* v_slot_base) {
       const char *kb, *vb;
       int k_rb = page_row_bytes, v_rb = page_row_bytes, valid;
@@ -374,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
         kb = p.key_cache + at * p.key_page_stride;
         vb = p.value_cache + at * p.value_page_stride;
         if constexpr (kTree) {
-          valid = min(kPageSize, context - i * kPageSize);
+          valid = min(kPageSize, g.context - i * kPageSize);
         } else {
           const int logical = __builtin_amdgcn_readlane(logical64, i & 63);
           valid = min(kPageSize, g.pos0 + g.tokens - logical * kPageSize);
@@ -388,15 +192,15 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
       const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
           (void*)vb, (short)0, valid > 0 ? (valid - 1) * v_rb + kRowBytes : 0, kBufferFlags);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int row = 32 * wave + 4 * j + quad;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, TM_LDS(k_slot_base + wave * kTileBytes + j * 1024), 16,
+      for (int j = 0; j < kDma; ++j) {
+        const int row = kWaveKeys * wave + 4 * j + quad;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, TM_LDS(k_slot_base + (wave * kDma + j) * 1024), 16,
                                                  (unsigned)(row * k_rb + 16 * k_slot(row, col)), 0, 0, 0);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int row = 32 * wave + 4 * j + quad;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, TM_LDS(v_slot_base + wave * kTileBytes + j * 1024), 16,
+      for (int j = 0; j < kDma; ++j) {
+        const int row = kWaveKeys * wave + 4 * j + quad;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, TM_LDS(v_slot_base + (wave * kDma + j) * 1024), 16,
                                                  (unsigned)(row * v_rb + 16 * v_slot(row, col)), 0, 0, 0);
       }
     };
@@ -417,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
           const int row = 16 * u + col;
           const i16x8_t a = *reinterpret_cast<const i16x8_t*>(kt + row * kRowBytes + 16 * k_slot(row, 4 * c + quad));
 #pragma unroll
-          for (int n = 0; n < NT; ++n) s[u][n] = Type::mfma(a, q[n][c], s[u][n]);
+          for (int n = 0; n < NT; ++n) s[u][n] = Type::mfma16(a, q[n][c], s[u][n]);
         }
       }
       if (masked) {
@@ -479,32 +283,28 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
           for (int e = 0; e < 8; ++e) bad |= ((unsigned)a[e] & Type::kExp) == Type::kExp;
         }
         if (__any(bad)) {
+          // The finite entries, then for each other kind an indicator's product:
+          // it is positive in the rows that attend such an entry.
 #pragma unroll
           for (int m = 0; m < 8; ++m) {
-            const i16x8_t a = v_at(m);
-            i16x8_t finite, plus, minus, nan;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const unsigned bits = (unsigned)a[e] & 0x7fffu;
-              finite[e] = bits < Type::kExp ? a[e] : (short)0;
-              plus[e] = bits == Type::kExp && a[e] >= 0 ? Type::kOne : (short)0;
-              minus[e] = bits == Type::kExp && a[e] < 0 ? Type::kOne : (short)0;
-              nan[e] = bits > Type::kExp ? Type::kOne : (short)0;
-            }
+            for (int kind = 0; kind < 4; ++kind) {  // finite, +inf, -inf, NaN
+              asm volatile("" ::: "memory");
+              u32x4_t a = __builtin_bit_cast(u32x4_t, v_at(m));
+              asm volatile("" : "+v"(a));
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              o[m][n] = Type::mfma(finite, pb[n], o[m][n]);
-              const f32x4_t has_plus = Type::mfma(plus, pb[n], f32x4_t{});
-              const f32x4_t has_minus = Type::mfma(minus, pb[n], f32x4_t{});
-              const f32x4_t has_nan = Type::mfma(nan, pb[n], f32x4_t{});
+              for (int e = 0; e < 4; ++e) a[e] = only_kind<Type>(a[e], kind) | only_kind<Type>(a[e] >> 16, kind) << 16;
+              // opaque: the compiler takes no operand for a NaN; +inf and -inf give one by themselves
+              float odd = __uint_as_float(kind == 1 ? 0x7f800000u : kind == 2 ? 0xff800000u : 0x7fc00000u);
+              asm volatile("" : "+v"(odd));
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                if (has_nan[i] > 0.0f || (has_plus[i] > 0.0f && has_minus[i] > 0.0f)) {
-                  o[m][n][i] = __uint_as_float(0x7fc00000u);
-                } else if (has_plus[i] > 0.0f) {
-                  o[m][n][i] += __uint_as_float(0x7f800000u);
-                } else if (has_minus[i] > 0.0f) {
-                  o[m][n][i] += __uint_as_float(0xff800000u);
+              for (int n = 0; n < NT; ++n) {
+                if (kind == 0) {
+                  o[m][n] = Type::mfma16(__builtin_bit_cast(i16x8_t, a), pb[n], o[m][n]);
+                } else {
+                  const f32x4_t has = Type::mfma16(__builtin_bit_cast(i16x8_t, a), pb[n], f32x4_t{});
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) o[m][n][i] += has[i] > 0.0f ? odd : 0.0f;
                 }
               }
             }
@@ -516,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
       for (int m = 0; m < 8; ++m) {
         const i16x8_t a = v_at(m);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) o[m][n] = Type::mfma(a, pb[n], o[m][n]);
+        for (int n = 0; n < NT; ++n) o[m][n] = Type::mfma16(a, pb[n], o[m][n]);
       }
     };
 
@@ -534,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
       } else {
         const bool bad = __builtin_amdgcn_readlane(phys64, i & 63) < 0;
         if constexpr (kTree) {
-          last_seen = bad ? -1 : min(kPageSize, context - i * kPageSize) - 1;
+          last_seen = bad ? -1 : min(kPageSize, g.context - i * kPageSize) - 1;
           first_hidden = last_seen + 1;
 #pragma unroll
           for (int n = 0; n < NT; ++n) thr[n] = last_seen;
@@ -573,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
           if ((i & 63) == 0 && i > g.lo) load_pages(i >> 6);
           issue(i + 1, kb, vb);
         }
-        wait_dma_but<kDmaPerWave>();
+        wait_dma_but<2 * kDma>();
       } else {
         wait_dma();
       }
@@ -595,9 +395,15 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
       if (i < last_page) step(i, k_lds0, v_lds0, k_lds1, v_lds1);
     }
 
-    // ---- the key parts' sums through LDS; wave w's O in slot w ----
+    // ---- the key parts' sums through LDS; each wave's O in its part of a slot ----
     __syncthreads();
-    char* const own = wave == 0 ? k_lds0 : wave == 1 ? v_lds0 : wave == 2 ? k_lds1 : v_lds1;
+    auto o_slot = [&](int w) {
+      constexpr int kPerSlot = kWaves / 4;
+      const int at = w / kPerSlot;
+      char* const slot = at == 0 ? k_lds0 : at == 1 ? v_lds0 : at == 2 ? k_lds1 : v_lds1;
+      return slot + (w % kPerSlot) * (kWaveRows * kHeadDim * 4);
+    };
+    char* const own = o_slot(wave);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const float l = row_sum(l_run[n]);
@@ -626,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
     // 16 threads a row, 8 dims each.
     const int r0 = tid >> 4, c8 = tid & 15;
     auto store_row = [&](int r, const float* acc, float l) {
-      const int t = (g.row_base + r) / G;
+      const int t = by_group.token(g.row_base + r);
       const int h = g.row_base + r - t * G;
       if (t < g.held) return;  // before the request's first token: no row
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
@@ -637,10 +443,9 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
                                              8 * c8) = y;
     };
     // the workgroups that share the group, and where their partials lie
-    const int first_run = (int)(g.first / per_run);
-    const int last_run = (int)((g.first + g.units - 1) / per_run);
+    const Shared shared(g, per_run);
     constexpr int kRecord = kRows * (kHeadDim + 2);
-    auto record = [&](int r) { return (unsigned)((2 * r + (r == first_run ? 1 : 0)) * (kRecord * 4)); };
+    auto record = [&](int r) { return shared.record(r, kRecord * 4); };
     const __amdgpu_buffer_rsrc_t rec = __builtin_amdgcn_make_buffer_rsrc(
         (void*)p.partials, (short)0, whole ? 0 : (int)((unsigned)p.workgroups * 2u * (kRecord * 4u)), kBufferFlags);
     for (int r = r0; r < valid_rows; r += kThreads / 16) {
@@ -653,8 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
       for (int k = 0; k < KW; ++k) {
         const float mk = s_max[rp + RW * k][row];
         l += mk == -INFINITY ? 0.0f : s_sum[rp + RW * k][row] * __builtin_amdgcn_exp2f(mk - top);
-        const int w = rp + RW * k;
-        const char* src = w == 0 ? k_lds0 : w == 1 ? v_lds0 : w == 2 ? k_lds1 : v_lds1;
+        const char* src = o_slot(rp + RW * k);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const f32x4_t x = *reinterpret_cast<const f32x4_t*>(src + row * (kHeadDim * 4) +
@@ -682,25 +486,17 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
     }
     if (!whole) {
       // ---- the workgroup that arrives last merges ----
-      // Partials are written through to the level that every XCD sees (sc1) and
-      // each wave waits for its own before the arrival is counted.
-      wait_dma();
-      __syncthreads();
-      unsigned long long* const word = p.counters + first_run;
-      if (tid == 0) s_last = (int)(count_arrival(word, p.epoch) == (unsigned long long)(last_run - first_run + 1));
-      __syncthreads();
-      if (s_last) {
-        if (tid == 0) __hip_atomic_store(word, p.epoch << kEpochShift, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (last_to_arrive(p, shared, &s_last)) {
         for (int r = r0; r < valid_rows; r += kThreads / 16) {
           float top = -INFINITY;
-          for (int s = first_run; s <= last_run; ++s) {
+          for (int s = shared.first_run; s <= shared.last_run; ++s) {
             top = fmaxf(top, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
                                  rec, record(s) + (kRows * kHeadDim + r) * 4, 0, kCpolAgent)));
           }
           const float shift = top == -INFINITY ? 0.0f : top;
           float l = 0.0f, acc[8] = {};
 #pragma unroll 4
-          for (int s = first_run; s <= last_run; ++s) {
+          for (int s = shared.first_run; s <= shared.last_run; ++s) {
             const unsigned at = record(s);
             const float ms = __uint_as_float(
                 __builtin_amdgcn_raw_buffer_load_b32(rec, at + (kRows * kHeadDim + r) * 4, 0, kCpolAgent));
@@ -728,13 +524,11 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
 
 template <class Type, bool kTree>
 hipError_t launch_shape(const RowsParams& p, int shape_rows, hipStream_t stream) {
-  const dim3 grid((unsigned)p.workgroups), block(kThreads);
+  const dim3 grid((unsigned)p.workgroups);
   switch (shape_rows) {
-    case 16: hipLaunchKernelGGL((rows_attention_kernel<Type, 1, 1, kTree>), grid, block, 0, stream, p); break;
-    case 32: hipLaunchKernelGGL((rows_attention_kernel<Type, 2, 1, kTree>), grid, block, 0, stream, p); break;
-    case 64: hipLaunchKernelGGL((rows_attention_kernel<Type, 4, 1, kTree>), grid, block, 0, stream, p); break;
-    case 128: hipLaunchKernelGGL((rows_attention_kernel<Type, 4, 2, kTree>), grid, block, 0, stream, p); break;
-    case 256: hipLaunchKernelGGL((rows_attention_kernel<Type, 4, 4, kTree>), grid, block, 0, stream, p); break;
+    case 16: hipLaunchKernelGGL((rows_attention_kernel<Type, 1, 1, 4, kTree>), grid, dim3(256), 0, stream, p); break;
+    case 32: hipLaunchKernelGGL((rows_attention_kernel<Type, 2, 1, 4, kTree>), grid, dim3(256), 0, stream, p); break;
+    case 64: hipLaunchKernelGGL((rows_attention_kernel<Type, 2, 2, 4, kTree>), grid, dim3(512), 0, stream, p); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
