@@ -66,11 +66,10 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
   const int page_row_bytes = p.kv_heads * kRowBytes;
   const float c2 = p.scale_log2;
 
-  const int64_t total = plan_units<kTree, kBlockRows, kBlockThreads>(p, lists);
-  const int64_t per_run = max((int64_t)p.min_units, (int64_t)((uint64_t)(total + p.workgroups - 1) / (unsigned)p.workgroups));
+  const Plan plan = plan_units<kTree, kBlockRows, kBlockThreads>(p, lists);
   const int run = run_of_workgroup();
-  int64_t unit = run * per_run;
-  const int64_t unit_end = min(total, unit + per_run);
+  int unit = min(run, plan.total / plan.per_run + 1) * plan.per_run;
+  const int unit_end = min(plan.total, unit + plan.per_run);
 
   while (unit < unit_end) {
     const Segment g = find_segment<kTree, kBlockRows>(p, lists, unit, unit_end);
@@ -482,7 +481,7 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
       if (active) store_rows(l_run);
     } else {
       // ---- a group of several runs ----
-      const Shared shared(g, per_run);
+      const Shared shared(g, plan.per_run);
       const __amdgpu_buffer_rsrc_t rec = __builtin_amdgcn_make_buffer_rsrc(
           (void*)p.partials, (short)0, (int)((unsigned)p.workgroups * 2u * (unsigned)kPartialBytes), kBufferFlags);
       // record: O [wave][d-block, quarter][lane][4], then row maxima and lane sums [wave][lane]
@@ -501,33 +500,40 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l_run), rec, own + at_sum, 0, kCpolAgent);
       }
       if (last_to_arrive(p, shared, &s_last) && active) {
-        float top = -INFINITY;
-#pragma unroll 4
-        for (int r = shared.first_run; r <= shared.last_run; ++r) {
-          top = fmaxf(top, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                               rec, shared.record(r, (unsigned)kPartialBytes) + at_max, 0, kCpolAgent)));
-        }
-        const float shift = top == -INFINITY ? 0.0f : top;
-        float l = 0.0f;
+        float top = -INFINITY, l = 0.0f;
 #pragma unroll
         for (int m = 0; m < 4; ++m) o[m] = f32x16_t{};
-        for (int r = shared.first_run; r <= shared.last_run; ++r) {
-          const unsigned from = shared.record(r, (unsigned)kPartialBytes);
-          const float mr = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rec, from + at_max, 0, kCpolAgent));
-          const float lr = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rec, from + at_sum, 0, kCpolAgent));
-          f32x4_t x[16];
+        // two partials' loads in flight at a time
+        for (int r = shared.first_run; r <= shared.last_run; r += 2) {
+          float mr[2], lr[2];
+          f32x4_t x[2][16];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            // past the last one its loads fall outside the buffer's range
+            const unsigned from =
+                r + j <= shared.last_run ? shared.record(r + j, (unsigned)kPartialBytes) : kOutOfRange;
+            mr[j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rec, from + at_max, 0, kCpolAgent));
+            lr[j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rec, from + at_sum, 0, kCpolAgent));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              x[j][i] = __builtin_bit_cast(f32x4_t,
+                                           __builtin_amdgcn_raw_buffer_load_b128(rec, from + piece(i), 0, kCpolAgent));
+            }
+          }
+          if (r + 1 > shared.last_run) mr[1] = -INFINITY;
+          const float next = fmaxf(top, fmaxf(mr[0], mr[1]));
+          const float shift = next == -INFINITY ? 0.0f : next;
+          const float keep = __builtin_amdgcn_exp2f(top - shift);
+          const float w0 = __builtin_amdgcn_exp2f(mr[0] - shift), w1 = __builtin_amdgcn_exp2f(mr[1] - shift);
+          l = l * keep + lr[0] * w0 + lr[1] * w1;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            x[i] = __builtin_bit_cast(f32x4_t,
-                                      __builtin_amdgcn_raw_buffer_load_b128(rec, from + piece(i), 0, kCpolAgent));
-          }
-          const float w = __builtin_amdgcn_exp2f(mr - shift);
-          l += lr * w;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[i >> 2][4 * (i & 3) + e] += x[i][e] * w;
+            for (int e = 0; e < 4; ++e) {
+              o[i >> 2][4 * (i & 3) + e] = o[i >> 2][4 * (i & 3) + e] * keep + x[0][i][e] * w0 + x[1][i][e] * w1;
+            }
           }
+          top = next;
         }
         store_rows(l);
       }

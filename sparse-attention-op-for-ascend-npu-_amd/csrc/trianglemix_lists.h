@@ -68,12 +68,6 @@ __device__ __forceinline__ unsigned only_kind(unsigned bits, int kind) {
 
 constexpr int kCpolAgent = 16;  // sc1: written to, read from, the level that every XCD sees
 
-// A value that every lane holds alike, in scalar registers.
-__device__ __forceinline__ int64_t uniform64(int64_t x) {
-  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) |
-                   (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
-}
-
 // Workgroups are dispatched round-robin over the 8 XCDs: neighbouring runs of
 // units, which share K/V pages where selections overlap, go to one XCD (the
 // grid is a multiple of 8).
@@ -93,8 +87,8 @@ template <bool kTree>
 struct ListLds;
 template <>
 struct ListLds<true> {
-  int64_t units[kMaxBatch];  // running unit counts of the requests
-  int64_t scan[16];          // wave totals
+  int units[kMaxBatch];  // running unit counts of the requests
+  int64_t scan[16];      // wave totals
 };
 template <>
 struct ListLds<false> {
@@ -114,7 +108,7 @@ struct Segment {
   int context;    // keys of the cache (trees)
   int lo, hi;     // its units
   int units;      // units of the whole group
-  int64_t first;  // the group's first unit
+  int first;      // the group's first unit
 };
 
 // r / group for the rows of a group (below 2048): exact, as r * group < 65536.
@@ -126,9 +120,13 @@ struct GroupDivider {
 static_assert(kMaxTreeNodes * kMaxGroup <= 2048 && kSelectRows * kMaxGroup <= 2048 && 2047 * kMaxGroup < 65536,
               "rows of a group");
 
-// All units; for trees the running counts too.  Every thread of the workgroup calls it.
+// All units (the host keeps them to kMaxUnits), dealt to the runs in equal parts;
+// for trees the running counts too.  Every thread of the workgroup calls it.
+struct Plan {
+  int total, per_run;
+};
 template <bool kTree, int kRows, int kThreads>
-__device__ __forceinline__ int64_t plan_units(const RowsParams& p, ListLds<kTree>& lds) {
+__device__ __forceinline__ Plan plan_units(const RowsParams& p, ListLds<kTree>& lds) {
   if constexpr (kTree) {
     // consecutive requests a thread, prefix sums over the workgroup
     constexpr int kEach = kMaxBatch / kThreads;
@@ -141,12 +139,13 @@ __device__ __forceinline__ int64_t plan_units(const RowsParams& p, ListLds<kTree
       if (b < p.batch) {
         int row0, tokens, context;
         tree_of(p, b, row0, tokens, context);
-        mine[i] = (int64_t)p.kv_heads * ((tokens * p.group + kRows - 1) / kRows) *
+        mine[i] = (int64_t)(p.kv_heads * ((tokens * p.group + kRows - 1) / kRows)) *
                   ((context + kPageSize - 1) / kPageSize + 1);
       }
       sum += mine[i];
     }
     int64_t upto = sum;
+#pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int64_t add = __shfl_up(upto, d);
       if (lane >= d) upto += add;
@@ -158,20 +157,19 @@ __device__ __forceinline__ int64_t plan_units(const RowsParams& p, ListLds<kTree
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       upto += mine[i];
-      lds.units[kEach * tid + i] = upto;
+      lds.units[kEach * tid + i] = (int)min(upto, (int64_t)kMaxUnits);  // more only with offsets that are none
     }
     __syncthreads();
-    return uniform64(lds.units[p.batch - 1]);
+    const int total = __builtin_amdgcn_readfirstlane(lds.units[p.batch - 1]);
+    return Plan{total, max(1, (int)((unsigned)(total + p.workgroups - 1) / (unsigned)p.workgroups))};
   } else {
-    const int row_parts = (min(p.rows, kSelectRows) * p.group + kRows - 1) / kRows;
-    return (int64_t)p.batch * p.blocks * p.kv_heads * row_parts * p.count;
+    return Plan{p.total_units, p.per_run};
   }
 }
 
 // The segment that begins at `unit` and ends with the group or before unit_end.
 template <bool kTree, int kRows>
-__device__ __forceinline__ Segment find_segment(const RowsParams& p, const ListLds<kTree>& lds, int64_t unit,
-                                                int64_t unit_end) {
+__device__ __forceinline__ Segment find_segment(const RowsParams& p, const ListLds<kTree>& lds, int unit, int unit_end) {
   Segment g;
   if constexpr (kTree) {
     // the request whose running count first passes `unit` (entries past the batch hold the total)
@@ -187,18 +185,18 @@ __device__ __forceinline__ Segment find_segment(const RowsParams& p, const ListL
     tree_of(p, lo, g.row0, g.tokens, g.context);
     g.units = (g.context + kPageSize - 1) / kPageSize + 1;
     const int row_parts = (g.tokens * p.group + kRows - 1) / kRows;
-    const int64_t before = lo > 0 ? uniform64(lds.units[lo - 1]) : 0;
-    const int local = (int)((uint64_t)(unit - before) / (unsigned)g.units);
+    const int before = lo > 0 ? __builtin_amdgcn_readfirstlane(lds.units[lo - 1]) : 0;
+    const int local = (int)((unsigned)(unit - before) / (unsigned)g.units);
     g.kv_head = local / row_parts;
     g.row_base = (local % row_parts) * kRows;
-    g.first = before + (int64_t)local * g.units;
+    g.first = before + local * g.units;
     g.pos0 = 0;
     g.held = 0;
   } else {
     const unsigned row_parts = (unsigned)(min(p.rows, kSelectRows) * p.group + kRows - 1) / kRows;
     g.units = p.count;
-    uint64_t id = (uint64_t)unit / (unsigned)p.count;
-    g.first = (int64_t)(id * (unsigned)p.count);
+    unsigned id = (unsigned)unit / (unsigned)p.count;
+    g.first = (int)(id * (unsigned)p.count);
     // KV head outermost: the blocks of one head share its pages
     g.row_base = (int)(id % row_parts) * kRows;
     id /= row_parts;
@@ -212,8 +210,8 @@ __device__ __forceinline__ Segment find_segment(const RowsParams& p, const ListL
     g.held = max(0, -g.pos0);
     g.context = 0;
   }
-  g.lo = (int)(unit - g.first);
-  g.hi = (int)(min(unit_end, g.first + g.units) - g.first);
+  g.lo = unit - g.first;
+  g.hi = min(unit_end - g.first, g.units);
   return g;
 }
 
@@ -280,9 +278,9 @@ __device__ __forceinline__ int selected_list(const RowsParams& p, ListLds<false>
 // and one for a group that begins in it and goes on behind it.
 struct Shared {
   int first_run, last_run;
-  __device__ Shared(const Segment& g, int64_t per_run)
-      : first_run((int)((uint64_t)g.first / (uint64_t)per_run)),
-        last_run((int)((uint64_t)(g.first + g.units - 1) / (uint64_t)per_run)) {}
+  __device__ Shared(const Segment& g, int per_run)
+      : first_run((int)((unsigned)g.first / (unsigned)per_run)),
+        last_run((int)((unsigned)(g.first + g.units - 1) / (unsigned)per_run)) {}
   __device__ unsigned record(int r, unsigned bytes) const { return (unsigned)(2 * r + (r == first_run ? 1 : 0)) * bytes; }
 };
 

@@ -19,6 +19,7 @@ constexpr int kMaxKvHeads = 256;
 constexpr int kMaxBatch = 1024;       // requests of one call
 constexpr int kMaxSelected = 1024;    // pages of one selection
 constexpr int kMaxTableCols = 16384;  // logical pages of a request (2,097,152 tokens)
+constexpr int kMaxUnits = 1 << 30;    // pages of 128 keys that a call may read, per KV head and group of rows
 constexpr int kMaxTreeNodes = 64;     // one 64-bit mask word per node
 
 struct BoundsParams {
@@ -75,7 +76,7 @@ struct RowsParams {
   int table_cols, batch, heads, kv_heads, group, num_pages, total_rows;
   int rows, blocks, count;  // selected pages: rows per request, row blocks per request, pages per selection
   int workgroups;           // of the grid
-  int min_units;            // fewest pages a workgroup takes
+  int total_units, per_run;  // selected pages: all units, and those of a workgroup
   float scale_log2;
 };
 // Groups of up to kRowShapes rows run in trianglemix_rows.hip, in the smallest

@@ -188,21 +188,28 @@ int shape_for(int64_t rows) {
 }
 
 struct RowsPlan {
-  int shape, workgroups, min_units;
-  int64_t workspace_bytes;
+  int shape, workgroups;
+  int64_t units, workspace_bytes;
 };
 
-// As many workgroups as the GPU holds at once, fewer when the units would not
-// give each min_units; a multiple of the 8 XCDs.
-RowsPlan rows_plan(int shape, int64_t most_units) {
+// As many workgroups as the GPU holds at once, fewer when there are not as
+// many units (pages of groups of rows); a multiple of the 8 XCDs.
+RowsPlan rows_plan(int shape, int64_t units) {
   RowsPlan r;
   r.shape = shape;
-  r.min_units = 1;
+  r.units = units;
   const int64_t slots = kComputeUnits * (shape == tmx::kBlockRows ? 2 : 1);  // of its LDS a CU holds two, or one
-  const int64_t wanted = std::min<int64_t>(slots, (most_units + r.min_units - 1) / r.min_units);
-  r.workgroups = (int)((wanted + 7) / 8 * 8);
+  r.workgroups = (int)((std::min<int64_t>(slots, units) + 7) / 8 * 8);
   r.workspace_bytes = tmx::kCounterBytes + 2 * r.workgroups * tmx::rows_partial_bytes(r.shape);
   return r;
+}
+
+int check_units(int64_t units) {
+  if (units > tmx::kMaxUnits) {
+    return report(TM_ERR_UNSUPPORTED, "the call may read %lld pages of 128 keys; the limit is %d", (long long)units,
+                  tmx::kMaxUnits);
+  }
+  return TM_OK;
 }
 
 int launch_attention(const tmx::RowsParams& p, const RowsPlan& plan, int dtype, void* stream) {
@@ -369,7 +376,9 @@ int64_t tm_selected_page_attention_workspace_size(int64_t batch, int64_t rows, i
                                                   int64_t count) {
   report(TM_OK, "%s", "");
   if (check_selected(batch, rows, heads, kv_heads, count) != TM_OK) return -1;
-  return batch == 0 || rows == 0 ? 0 : selected_plan(batch, rows, heads, kv_heads, count).workspace_bytes;
+  if (batch == 0 || rows == 0) return 0;
+  const RowsPlan plan = selected_plan(batch, rows, heads, kv_heads, count);
+  return check_units(plan.units) == TM_OK ? plan.workspace_bytes : -1;
 }
 
 int tm_selected_page_attention(const void* query, int64_t query_stride, const void* key_cache,
@@ -392,7 +401,8 @@ int tm_selected_page_attention(const void* query, int64_t query_stride, const vo
   if (st == TM_OK) st = check_element(pages, 4);
   if (st != TM_OK) return st;
   const RowsPlan plan = selected_plan(batch, rows, heads, kv_heads, count);
-  st = check_workspace(workspace, workspace_bytes, plan.workspace_bytes);
+  st = check_units(plan.units);
+  if (st == TM_OK) st = check_workspace(workspace, workspace_bytes, plan.workspace_bytes);
   if (st != TM_OK) return st;
   const int64_t blocks = (rows + tmx::kSelectRows - 1) / tmx::kSelectRows;
   const Range written[] = {{out, batch * rows * heads * kHeadBytes, "out"},
@@ -431,7 +441,8 @@ int tm_selected_page_attention(const void* query, int64_t query_stride, const vo
   p.blocks = (int)blocks;
   p.count = (int)count;
   p.workgroups = plan.workgroups;
-  p.min_units = plan.min_units;
+  p.total_units = (int)plan.units;
+  p.per_run = (int)((plan.units + plan.workgroups - 1) / plan.workgroups);
   p.scale_log2 = scale * 1.4426950408889634f;
   return launch_attention(p, plan, dtype, stream);
 }
@@ -440,8 +451,9 @@ int64_t tm_tree_attention_workspace_size(int64_t total_rows, int64_t batch, int6
                                          int64_t table_cols) {
   report(TM_OK, "%s", "");
   if (check_tree(total_rows, batch, heads, kv_heads, table_cols) != TM_OK) return -1;
-  return batch == 0 || total_rows == 0 ? 0
-                                       : tree_plan(total_rows, batch, heads, kv_heads, table_cols).workspace_bytes;
+  if (batch == 0 || total_rows == 0) return 0;
+  const RowsPlan plan = tree_plan(total_rows, batch, heads, kv_heads, table_cols);
+  return check_units(plan.units) == TM_OK ? plan.workspace_bytes : -1;
 }
 
 int tm_tree_attention(const void* query, int64_t query_stride, const void* key, int64_t key_stride,
@@ -468,7 +480,8 @@ int tm_tree_attention(const void* query, int64_t query_stride, const void* key, 
   if (st == TM_OK) st = check_element(tree_mask, 8);
   if (st != TM_OK) return st;
   const RowsPlan plan = tree_plan(total_rows, batch, heads, kv_heads, table_cols);
-  st = check_workspace(workspace, workspace_bytes, plan.workspace_bytes);
+  st = check_units(plan.units);
+  if (st == TM_OK) st = check_workspace(workspace, workspace_bytes, plan.workspace_bytes);
   if (st != TM_OK) return st;
   const Range written[] = {{out, total_rows * heads * kHeadBytes, "out"},
                            {workspace, plan.workspace_bytes, "workspace"}};
@@ -511,7 +524,6 @@ int tm_tree_attention(const void* query, int64_t query_stride, const void* key, 
   p.num_pages = (int)num_pages;
   p.total_rows = (int)total_rows;
   p.workgroups = plan.workgroups;
-  p.min_units = plan.min_units;
   p.scale_log2 = scale * 1.4426950408889634f;
   return launch_attention(p, plan, dtype, stream);
 }

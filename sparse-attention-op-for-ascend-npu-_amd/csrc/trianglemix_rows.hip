@@ -94,11 +94,10 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
   const GroupDivider by_group(p.group);
   const int page_row_bytes = p.kv_heads * kRowBytes;
 
-  const int64_t total = plan_units<kTree, kRows, kThreads>(p, lists);
-  const int64_t per_run = max((int64_t)p.min_units, (int64_t)((uint64_t)(total + p.workgroups - 1) / (unsigned)p.workgroups));
+  const Plan plan = plan_units<kTree, kRows, kThreads>(p, lists);
   const int run = run_of_workgroup();
-  int64_t unit = run * per_run;
-  const int64_t unit_end = min(total, unit + per_run);
+  int unit = min(run, plan.total / plan.per_run + 1) * plan.per_run;
+  const int unit_end = min(plan.total, unit + plan.per_run);
 
   while (unit < unit_end) {
     const Segment g = find_segment<kTree, kRows>(p, lists, unit, unit_end);
@@ -443,7 +442,7 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
                                              8 * c8) = y;
     };
     // the workgroups that share the group, and where their partials lie
-    const Shared shared(g, per_run);
+    const Shared shared(g, plan.per_run);
     constexpr int kRecord = kRows * (kHeadDim + 2);
     auto record = [&](int r) { return shared.record(r, kRecord * 4); };
     const __amdgpu_buffer_rsrc_t rec = __builtin_amdgcn_make_buffer_rsrc(
@@ -487,33 +486,84 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
     if (!whole) {
       // ---- the workgroup that arrives last merges ----
       if (last_to_arrive(p, shared, &s_last)) {
-        for (int r = r0; r < valid_rows; r += kThreads / 16) {
-          float top = -INFINITY;
-          for (int s = shared.first_run; s <= shared.last_run; ++s) {
-            top = fmaxf(top, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                                 rec, record(s) + (kRows * kHeadDim + r) * 4, 0, kCpolAgent)));
-          }
-          const float shift = top == -INFINITY ? 0.0f : top;
-          float l = 0.0f, acc[8] = {};
-#pragma unroll 4
-          for (int s = shared.first_run; s <= shared.last_run; ++s) {
-            const unsigned at = record(s);
-            const float ms = __uint_as_float(
-                __builtin_amdgcn_raw_buffer_load_b32(rec, at + (kRows * kHeadDim + r) * 4, 0, kCpolAgent));
-            const float ls = __uint_as_float(
-                __builtin_amdgcn_raw_buffer_load_b32(rec, at + (kRows * (kHeadDim + 1) + r) * 4, 0, kCpolAgent));
-            const float w = __builtin_amdgcn_exp2f(ms - shift);
-            l += ls * w;
+        // 16 threads a row again; where the rows leave threads over, they share
+        // a row's partials (part pg of `parts` takes every parts-th) and join
+        // through LDS.  Four partials' loads are in flight at a time.
+        int row_slots = 1;
+        while (row_slots < valid_rows && row_slots < kThreads / 16) row_slots *= 2;
+        const int parts = kThreads / 16 / row_slots;
+        const int pg = r0 / row_slots;
+        float* const join = reinterpret_cast<float*>(k_lds0);  // [thread][10]: acc, row max, row sum
+        static_assert(kThreads * 10 * 4 <= kSlotBytes, "the joined values fit a slot");
+        for (int rb = 0; rb < valid_rows; rb += row_slots) {
+          const int r = rb + r0 % row_slots;
+          float top = -INFINITY, l = 0.0f, acc[8] = {};
+          if (r < valid_rows) {
+            for (int s0 = shared.first_run + pg; s0 <= shared.last_run; s0 += 4 * parts) {
+              float ms[4], ls[4];
+              f32x4_t x[4][2];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const f32x4_t x = __builtin_bit_cast(
-                  f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                               rec, at + (r * kHeadDim + 8 * c8 + 4 * half) * 4, 0, kCpolAgent));
+              for (int j = 0; j < 4; ++j) {
+                // past the last one its loads fall outside the buffer's range
+                const int s = s0 + j * parts;
+                const unsigned at = s <= shared.last_run ? record(s) : kOutOfRange;
+                ms[j] = __uint_as_float(
+                    __builtin_amdgcn_raw_buffer_load_b32(rec, at + (kRows * kHeadDim + r) * 4, 0, kCpolAgent));
+                ls[j] = __uint_as_float(
+                    __builtin_amdgcn_raw_buffer_load_b32(rec, at + (kRows * (kHeadDim + 1) + r) * 4, 0, kCpolAgent));
 #pragma unroll
-              for (int e = 0; e < 4; ++e) acc[4 * half + e] += ms == -INFINITY ? 0.0f : x[e] * w;
+                for (int half = 0; half < 2; ++half) {
+                  x[j][half] = __builtin_bit_cast(
+                      f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                   rec, at + (r * kHeadDim + 8 * c8 + 4 * half) * 4, 0, kCpolAgent));
+                }
+              }
+              float next = top;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if (s0 + j * parts > shared.last_run) ms[j] = -INFINITY;
+                next = fmaxf(next, ms[j]);
+              }
+              const float shift = next == -INFINITY ? 0.0f : next;
+              const float keep = __builtin_amdgcn_exp2f(top - shift);
+              l *= keep;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) acc[e] *= keep;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float w = __builtin_amdgcn_exp2f(ms[j] - shift);
+                l += ls[j] * w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[e] += x[j][e >> 2][e & 3] * w;
+              }
+              top = next;
             }
           }
-          store_row(r, acc, l);
+          if (parts > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) join[tid * 10 + e] = acc[e];
+            join[tid * 10 + 8] = top;
+            join[tid * 10 + 9] = l;
+            __syncthreads();
+            if (pg == 0) {
+              float all = top;
+              for (int k = 1; k < parts; ++k) all = fmaxf(all, join[(tid + k * 16 * row_slots) * 10 + 8]);
+              const float shift = all == -INFINITY ? 0.0f : all;
+              const float keep = __builtin_amdgcn_exp2f(top - shift);
+              l *= keep;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) acc[e] *= keep;
+              for (int k = 1; k < parts; ++k) {
+                const float* const from = join + (tid + k * 16 * row_slots) * 10;
+                const float w = __builtin_amdgcn_exp2f(from[8] - shift);
+                l += from[9] * w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[e] += from[e] * w;
+              }
+            }
+          }
+          if (pg == 0 && r < valid_rows) store_row(r, acc, l);
         }
       }
     }
