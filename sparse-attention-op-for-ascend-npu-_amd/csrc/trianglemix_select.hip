@@ -91,38 +91,35 @@ __device__ __forceinline__ float to_float(short x) {
   return kFp16 ? (float)__builtin_bit_cast(_Float16, x) : __uint_as_float((unsigned)(uint16_t)x << 16);
 }
 
-// The sums of each block's rows, one thread per (block, head, dim).
-constexpr int kPoolThreads = 256;
+// The sums of each block's rows, one thread per (block, head, 8 dims), eight
+// rows' loads in flight.
+constexpr int kPoolThreads = 64;
 template <bool kFp16>
 __global__ void __launch_bounds__(kPoolThreads) pool_rows_kernel(const SelectParams p) {
   const int64_t i = (int64_t)blockIdx.x * kPoolThreads + threadIdx.x;
-  const int width = p.heads * kHeadDim;
-  const int64_t block = i / width;
-  if (block >= (int64_t)p.requests * p.slab_blocks) return;
-  const int b = p.request0 + (int)(block / p.slab_blocks);
-  const int t0 = (p.block0 + (int)(block % p.slab_blocks)) * kSelectRows;
+  const int width = p.heads * (kHeadDim / 8);
+  const int block = (int)(i / width);
+  if (block >= p.requests * p.slab_blocks) return;
+  const int b = p.request0 + block / p.slab_blocks;
+  const int t0 = (p.block0 + block % p.slab_blocks) * kSelectRows;
   const int pos0 = max(p.seq_lens[b], 0) - p.rows;
-  const uint16_t* src = p.query + (int64_t)b * p.rows * p.query_stride + i % width;
-  double sum = 0.0;
-  for (int t = max(t0, -pos0); t < min(t0 + kSelectRows, p.rows); ++t) {
-    sum += (double)to_float<kFp16>((short)src[t * p.query_stride]);
+  const int at = (int)(i % width) * 8;
+  const uint16_t* const src = p.query + (int64_t)b * p.rows * p.query_stride + at;
+  const int end = min(t0 + kSelectRows, p.rows);
+  double sum[8] = {};
+  for (int t = max(t0, -pos0); t < end; t += 8) {
+    s16x8_t x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const s16x8_t*>(src + min(t + j, end - 1) * p.query_stride);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += t + j < end ? (double)to_float<kFp16>(x[j][e]) : 0.0;
+    }
   }
-  p.pooled[i] = sum;
-}
-
-// Adds the 16 lanes of a row, the result in all of them.
-template <int kCtrl>
-__device__ __forceinline__ double dpp_add(double x) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, x);
-  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, kCtrl, 0xf, 0xf, true);
-  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), kCtrl, 0xf, 0xf, true);
-  return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-__device__ __forceinline__ double sum16(double x) {
-  x = dpp_add<0xb1>(x);   // quad_perm 1 0 3 2
-  x = dpp_add<0x4e>(x);   // quad_perm 2 3 0 1
-  x = dpp_add<0x141>(x);  // row_half_mirror
-  return dpp_add<0x140>(x);  // row_mirror
+  double* const dst = p.pooled + (int64_t)block * p.heads * kHeadDim + at;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) dst[e] = sum[e];
 }
 
 __device__ __forceinline__ uint64_t score_key(double x) {
@@ -131,81 +128,266 @@ __device__ __forceinline__ uint64_t score_key(double x) {
   return (int64_t)u < 0 ? ~u : u | 0x8000000000000000ull;
 }
 
-// 16 lanes hold one page's bounds (8 dims each), PP pages in turn, and run
-// over the blocks and heads.
-constexpr int kScoreThreads = 256;
-template <bool kFp16, int PP>
-__global__ void __launch_bounds__(kScoreThreads) score_kernel(const SelectParams p) {
-  const int sub = threadIdx.x & 15, slot = threadIdx.x >> 4;
+// max(x, 0) and min(x, 0) of finite numbers by the sign bit.
+__device__ __forceinline__ double positive(double x) { return __builtin_signbit(x) ? 0.0 : x; }
+__device__ __forceinline__ double negative(double x) { return __builtin_signbit(x) ? x : 0.0; }
+
+// The scores as 64-bit matrix products, q+ max + q- min with q+ = max(q, 0), q-
+// = min(q, 0): a wave holds the bounds of 16 pages (lane l: page l % 16, of
+// every 32 dims the eight from 8 (l / 16) on) and runs over tiles of query sums.  A tile is 16 rows
+// (v_mfma_f64_16x16x4) or, for a single block of up to four heads, four
+// (v_mfma_f64_4x4x4, its four blocks taking four pages each): either reached
+// 70-73 TFLOP/s of 78.6, alone, in a probe.  Rows are block * padded + head, the
+// group padded to a power of two.  Infinities and NaNs, which a product with
+// zero would turn into NaN, take a plain loop.
+constexpr int kScoreWaves = 4;
+constexpr int kScoreThreads = kScoreWaves * 64;
+typedef double f64x4_t __attribute__((ext_vector_type(4)));
+
+template <bool kFp16, bool kSmall>
+__global__ void __launch_bounds__(kScoreThreads, kSmall ? 4 : 2) score_kernel(const SelectParams p, int padded) {
+  constexpr int kTileRows = kSmall ? 4 : 16;
+  // The query sums of two row tiles, shared by the waves: rows of 128 and two
+  // doubles, so that 16 rows' reads meet different banks.
+  __shared__ __attribute__((aligned(16))) double s_q[2][kTileRows][kHeadDim + 2];
+  __shared__ int s_odd[2];  // some value of the tile is no finite number
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = lane & 15, quad = lane >> 4;
   const int kv_head = blockIdx.y % p.kv_heads, slab_b = blockIdx.y / p.kv_heads;
   const int b = p.request0 + slab_b;
-  const int page0 = ((int)blockIdx.x * (kScoreThreads / 16) + slot) * PP;
   const int group = p.heads / p.kv_heads;
   const int seq = max(p.seq_lens[b], 0);
   const int pages = min(p.table_cols, (seq + kPageSize - 1) / kPageSize);
-  if ((int)blockIdx.x * (kScoreThreads / 16) * PP >= pages) return;
-  float lo[PP][8], hi[PP][8];
-  bool there[PP];
+  if ((int)blockIdx.x * kScoreWaves * 16 >= pages) return;
+  const int page = ((int)blockIdx.x * kScoreWaves + wave) * 16 + col;
+  const int phys = page < pages ? p.block_table[b * p.table_stride + page] : -1;
+  const bool there = phys >= 0 && phys < p.num_pages;
+  const int64_t at = ((int64_t)(there ? phys : 0) * p.kv_heads + kv_head) * kHeadDim + 8 * quad;
+  s16x8_t raw_lo[4], raw_hi[4];
 #pragma unroll
-  for (int i = 0; i < PP; ++i) {
-    const int phys = page0 + i < pages ? p.block_table[b * p.table_stride + page0 + i] : -1;
-    there[i] = phys >= 0 && phys < p.num_pages;
-    const int64_t at = ((int64_t)(there[i] ? phys : 0) * p.kv_heads + kv_head) * kHeadDim + 8 * sub;
-    const s16x8_t l = *reinterpret_cast<const s16x8_t*>(p.page_min + at);
-    const s16x8_t h = *reinterpret_cast<const s16x8_t*>(p.page_max + at);
+  for (int i = 0; i < 4; ++i) {
+    raw_lo[i] = *reinterpret_cast<const s16x8_t*>(p.page_min + at + 32 * i);
+    raw_hi[i] = *reinterpret_cast<const s16x8_t*>(p.page_max + at + 32 * i);
+  }
+
+  const int rows = p.slab_blocks * padded;
+  const int tiles_per_block = max(1, padded / kTileRows);
+  const int row_tiles = (rows + kTileRows - 1) / kTileRows;
+  // Two dims a thread of each of its rows of the tile; zeros for rows of the padding.
+  constexpr int kShare = kTileRows * (kHeadDim / 2) / kScoreThreads;
+  typedef double f64x2_t __attribute__((ext_vector_type(2)));
+  auto fetch = [&](int row0, f64x2_t* x) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      lo[i][e] = to_float<kFp16>(l[e]);
-      hi[i][e] = to_float<kFp16>(h[e]);
+    for (int j = 0; j < kShare; ++j) {
+      const int row = row0 + (int)threadIdx.x / 64 + j * (kScoreThreads / 64);
+      const int blk = row / padded, g = row & (padded - 1);
+      x[j] = f64x2_t{0.0, 0.0};
+      if (row < rows && g < group) {
+        const int head = kv_head * group + g;
+        if (p.pooled) {
+          x[j] = *reinterpret_cast<const f64x2_t*>(
+              p.pooled + ((int64_t)(slab_b * p.slab_blocks + blk) * p.heads + head) * kHeadDim + 2 * lane);
+        } else {
+          const unsigned two =
+              *reinterpret_cast<const unsigned*>(p.query + b * p.query_stride + (int64_t)head * kHeadDim + 2 * lane);
+          x[j] = f64x2_t{(double)to_float<kFp16>((short)two), (double)to_float<kFp16>((short)(two >> 16))};
+        }
+      }
+    }
+  };
+  auto put = [&](int buffer, const f64x2_t* x) {
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < kShare; ++j) {
+      constexpr uint64_t kExp = 0x7ff0000000000000ull;
+      odd |= (__builtin_bit_cast(uint64_t, x[j][0]) & kExp) == kExp || (__builtin_bit_cast(uint64_t, x[j][1]) & kExp) == kExp;
+      *reinterpret_cast<f64x2_t*>(&s_q[buffer][threadIdx.x / 64 + j * (kScoreThreads / 64)][2 * lane]) = x[j];
+    }
+    if (odd) s_odd[buffer] = 1;
+  };
+  // A workgroup's row tiles: whole blocks, dealt over blockIdx.z.
+  const int stride = (int)gridDim.z * tiles_per_block;
+  auto next_tile = [&](int t) { return (t + 1) % tiles_per_block == 0 ? t + 1 - tiles_per_block + stride : t + 1; };
+  int t = (int)blockIdx.z * tiles_per_block;
+  f64x2_t x[kShare];
+  fetch(t * kTileRows, x);
+  if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
+  __syncthreads();
+  put(0, x);
+
+  bool odd = false;  // some bound is no finite number
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    constexpr short kExp = kFp16 ? 0x7c00 : 0x7f80;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) odd |= (raw_lo[i][e] & kExp) == kExp || (raw_hi[i][e] & kExp) == kExp;
+  }
+  const bool odd_bounds = __any(odd);
+  // Converted once where many row tiles use them, else at each use.
+  double wide_lo[kSmall ? 1 : 32], wide_hi[kSmall ? 1 : 32];
+  if constexpr (!kSmall) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      wide_lo[i] = (double)to_float<kFp16>(raw_lo[i >> 3][i & 7]);
+      wide_hi[i] = (double)to_float<kFp16>(raw_hi[i >> 3][i & 7]);
     }
   }
-  for (int blk = blockIdx.z; blk < p.slab_blocks; blk += gridDim.z) {
-    uint64_t best[PP];
+  auto lo = [&](int i) {
+    if constexpr (kSmall) return (double)to_float<kFp16>(raw_lo[i >> 3][i & 7]);
+    else return wide_lo[i];
+  };
+  auto hi = [&](int i) {
+    if constexpr (kSmall) return (double)to_float<kFp16>(raw_hi[i >> 3][i & 7]);
+    else return wide_hi[i];
+  };
+
+  uint64_t best[4] = {0, 0, 0, 0};
+  int buffer = 0;
+  for (; t < row_tiles; buffer ^= 1) {
+    __syncthreads();  // the tile is in its buffer, the other buffer is read
+    const int next = next_tile(t);
+    const bool more = next < row_tiles;
+    if (more) fetch(next * kTileRows, x);
+    const bool odd_row = s_odd[buffer] != 0;
+    if constexpr (kSmall) {
+      // converted in the loop, not ahead of it in registers that are not there
 #pragma unroll
-    for (int i = 0; i < PP; ++i) best[i] = 0;
-    for (int g = 0; g < group; ++g) {
-      const int head = kv_head * group + g;
-      double q[8];
-      if (p.pooled) {
-        const double* src = p.pooled + (((int64_t)slab_b * p.slab_blocks + blk) * p.heads + head) * kHeadDim + 8 * sub;
+      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(raw_lo[i]), "+v"(raw_hi[i]));
+    }
+    const int row0 = t * kTileRows;
+    {
+      double sum[4] = {};
+      if (__builtin_expect(!odd_bounds && !odd_row, 1)) {
+        // Physical row r of the operand is row 4 (r % 4) + r / 4 of the tile, so
+        // that a lane's four results are rows 4 quad .. 4 quad + 3.
+        const double* const q = &s_q[buffer][kSmall ? (lane & 3) : 4 * (col & 3) + (col >> 2)][8 * quad];
+        if constexpr (kSmall) {
+          double c[4] = {};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q[e] = src[e];
+          for (int i = 0; i < 32; i += 2) {
+            const f64x2_t y = *reinterpret_cast<const f64x2_t*>(q + 32 * (i >> 3) + (i & 7));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              c[2 * j] = __builtin_amdgcn_mfma_f64_4x4x4f64(positive(y[j]), hi(i + j), c[2 * j], 0, 0, 0);
+              c[2 * j + 1] = __builtin_amdgcn_mfma_f64_4x4x4f64(negative(y[j]), lo(i + j), c[2 * j + 1], 0, 0, 0);
+            }
+          }
+          sum[0] = (c[0] + c[1]) + (c[2] + c[3]);
+        } else {
+          f64x4_t c0 = {0.0, 0.0, 0.0, 0.0}, c1 = c0;
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const f64x2_t y = *reinterpret_cast<const f64x2_t*>(q + 32 * (i >> 3) + (i & 7));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              c0 = __builtin_amdgcn_mfma_f64_16x16x4f64(positive(y[j]), hi(i + j), c0, 0, 0, 0);
+              c1 = __builtin_amdgcn_mfma_f64_16x16x4f64(negative(y[j]), lo(i + j), c1, 0, 0, 0);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[i] = c0[i] + c1[i];
+        }
       } else {
-        const s16x8_t x =
-            *reinterpret_cast<const s16x8_t*>(p.query + b * p.query_stride + (int64_t)head * kHeadDim + 8 * sub);
+#pragma unroll 1
+        for (int r = 0; r < kTileRows; ++r) {
+          const double* const q = &s_q[buffer][r][8 * quad];
+          double y = 0.0;
+#pragma unroll 1
+          for (int i = 0; i < 32; ++i) {  // the bounds anew from memory: nothing is kept in registers for this path
+            const int d = 32 * (i >> 3) + (i & 7);
+            const uint16_t bound = q[d] >= 0.0 ? p.page_max[at + d] : p.page_min[at + d];
+            y = __builtin_fma(q[d], (double)to_float<kFp16>((short)bound), y);
+          }
+          y += __shfl_xor(y, 16);
+          y += __shfl_xor(y, 32);
+          if constexpr (kSmall) {
+            sum[0] = r == quad ? y : sum[0];
+          } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q[e] = (double)to_float<kFp16>(x[e]);
+            for (int i = 0; i < 4; ++i) sum[i] = r == 4 * quad + i ? y : sum[i];
+          }
+        }
       }
+      // max over the heads of a block: rows of a lane, then of lanes, then of tiles
 #pragma unroll
-      for (int i = 0; i < PP; ++i) {
-        double sum = 0.0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = __builtin_fma(q[e], (double)(q[e] >= 0.0 ? hi[i][e] : lo[i][e]), sum);
-        const uint64_t key = score_key(sum16(sum));
+      for (int i = 0; i < (kSmall ? 1 : 4); ++i) {
+        const int row = row0 + (kSmall ? quad : 4 * quad + i);
+        const uint64_t key = (row & (padded - 1)) < group ? score_key(sum[i]) : 0;
         best[i] = key > best[i] ? key : best[i];
       }
     }
-    if (sub == 0) {
-      uint64_t* const dst =
-          p.scores + (((int64_t)slab_b * p.slab_blocks + blk) * p.kv_heads + kv_head) * p.table_cols;
+    if ((t + 1) % tiles_per_block == 0 || tiles_per_block == 1) {
+      auto merge = [](uint64_t& y, uint64_t z) { y = z > y ? z : y; };
+      int step = 1;  // rows that one key of a lane stands for
+      if constexpr (!kSmall) {
+        if (padded >= 2) {
+          merge(best[0], best[1]);
+          merge(best[2], best[3]);
+          step = 2;
+        }
+        if (padded >= 4) {
+          merge(best[0], best[2]);
+          step = 4;
+        }
+        if (padded >= 8) merge(best[0], __shfl_xor(best[0], 16));
+        if (padded >= 16) merge(best[0], __shfl_xor(best[0], 32));
+      } else {
+        if (padded >= 2) merge(best[0], __shfl_xor(best[0], 16));
+        if (padded >= 4) merge(best[0], __shfl_xor(best[0], 32));
+      }
+      const int block_row0 = (t / tiles_per_block) * tiles_per_block * kTileRows;
 #pragma unroll
-      for (int i = 0; i < PP; ++i) {
-        if (page0 + i < pages) dst[page0 + i] = there[i] ? best[i] : 0;
+      for (int i = 0; i < (kSmall ? 1 : 4); ++i) {
+        const int row = block_row0 + (kSmall ? quad : 4 * quad + i);
+        if (i % step == 0 && (row & (padded - 1)) == 0 && row < rows && page < pages) {
+          p.scores[((int64_t)(slab_b * p.slab_blocks + row / padded) * p.kv_heads + kv_head) * p.table_cols + page] =
+              there ? best[i] : 0;
+        }
+        best[i] = 0;
       }
     }
+    if (more) {
+      if (threadIdx.x == 0) s_odd[buffer ^ 1] = 0;
+      __syncthreads();
+      put(buffer ^ 1, x);
+    }
+    t = next;
   }
 }
 
 // The `count` largest keys of one (block, KV head), the lowest page first among
 // equal ones, written in the order of the pages.  A key's threshold is found by
-// halving: as soon as exactly `count` keys lie at or above the middle it is
-// done (about 14 steps for 1024 pages); only equal keys take it down to one
-// value.
+// halving between the smallest and the largest key: as soon as exactly `count`
+// keys lie at or above the middle it is done (about 12 steps for 1024 pages);
+// only equal keys take it down to one value.  A row is one wave's (its keys in
+// registers, counts by ballots, no barrier) up to 1024 pages, else a
+// workgroup's of four waves.
 constexpr int kTopThreads = 256;
-template <int KPT>
+// Largest value of the wave's lanes, in all of them.
+template <int kCtrl>
+__device__ __forceinline__ unsigned dpp_max(unsigned x) {
+  const unsigned y = (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, kCtrl, 0xf, 0xf, true);
+  return y > x ? y : x;
+}
+__device__ __forceinline__ unsigned wave_max(unsigned x) {
+  x = dpp_max<0xb1>(x);   // quad_perm 1 0 3 2
+  x = dpp_max<0x4e>(x);   // quad_perm 2 3 0 1
+  x = dpp_max<0x141>(x);  // row_half_mirror
+  x = dpp_max<0x140>(x);  // row_mirror
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = a[0] > a[1] ? a[0] : a[1];
+  const auto c = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return c[0] > c[1] ? c[0] : c[1];
+}
+
+template <int KPT, int W>
 __global__ void __launch_bounds__(kTopThreads) top_pages_kernel(const SelectParams p) {
+  constexpr int kLanes = 64 * W;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row = blockIdx.x;  // of the slab: (request * blocks + block) * kv_heads + head
+  const int within = threadIdx.x % kLanes;
+  // of the slab: (request * blocks + block) * kv_heads + head
+  const int row = (int)blockIdx.x * (kTopThreads / kLanes) + (int)threadIdx.x / kLanes;
+  if (row >= p.requests * p.slab_blocks * p.kv_heads) return;  // W = 1 alone: no barrier follows
   const int kv_head = row % p.kv_heads;
   const int blk = p.block0 + row / p.kv_heads % p.slab_blocks;
   const int b = p.request0 + row / p.kv_heads / p.slab_blocks;
@@ -216,38 +398,101 @@ __global__ void __launch_bounds__(kTopThreads) top_pages_kernel(const SelectPara
   const int recent = first / kPageSize - p.recent_pages + 1;
   const uint64_t* const src = p.scores + (int64_t)row * p.table_cols;
   int32_t* const out = p.out + (((int64_t)b * p.blocks + blk) * p.kv_heads + kv_head) * p.count;
-  __shared__ int s_sum[2][kTopThreads / 64];
+  __shared__ int s_sum[2][W];
+  __shared__ unsigned s_key[2][W];
   int turn = 0;
-  auto total = [&](int mine) {  // of one count per wave, the same in every lane
-    if (lane == 0) s_sum[turn][wave] = mine;
-    __syncthreads();
-    int sum = 0;
+  // One count per wave to their sum, and the sum of the waves before.
+  auto total = [&](int mine, int* before) {
+    if constexpr (W == 1) {
+      if (before) *before = 0;
+      return mine;
+    } else {
+      if (lane == 0) s_sum[turn][wave] = mine;
+      __syncthreads();
+      int sum = 0, ahead = 0;
 #pragma unroll
-    for (int w = 0; w < kTopThreads / 64; ++w) sum += s_sum[turn][w];
-    turn ^= 1;
-    return sum;
+      for (int w = 0; w < W; ++w) {
+        ahead += w < wave ? s_sum[turn][w] : 0;
+        sum += s_sum[turn][w];
+      }
+      turn ^= 1;
+      if (before) *before = ahead;
+      return sum;
+    }
   };
-  // key i of a thread is page i * 256 + threadIdx.x
+  // key i of a thread is page i * kLanes + within
   uint64_t key[KPT];
+  unsigned most = 0, most_neg = 0;  // largest high word, and complement, of the keys that are not always taken
 #pragma unroll
   for (int i = 0; i < KPT; ++i) {
-    const int page = i * kTopThreads + threadIdx.x;
+    const int page = i * kLanes + within;
     key[i] = page < pages ? src[page] : 0;
-    if (key[i] != 0 && p.recent_pages > 0 && page >= recent) key[i] = ~0ull;
-    if (key[i] != 0 && page < p.sink_pages) key[i] = ~0ull;
   }
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {
+    const int page = i * kLanes + within;
+    if (key[i] != 0) {
+      if ((p.recent_pages > 0 && page >= recent) || page < p.sink_pages) {
+        key[i] = ~0ull;
+      } else {
+        const unsigned word = (unsigned)(key[i] >> 32);
+        most = word > most ? word : most;
+        most_neg = ~word > most_neg ? ~word : most_neg;
+      }
+    }
+  }
+  most = wave_max(most);
+  most_neg = wave_max(most_neg);
+  if constexpr (W > 1) {
+    if (lane == 0) {
+      s_key[0][wave] = most;
+      s_key[1][wave] = most_neg;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      most = s_key[0][w] > most ? s_key[0][w] : most;
+      most_neg = s_key[1][w] > most_neg ? s_key[1][w] : most_neg;
+    }
+  }
+  // Sum over the wave of a small count per lane: bit by bit, by ballots.
+  auto wave_total = [&](int n) {
+    int sum = 0;
+#pragma unroll
+    for (int bit = 0; (1 << bit) <= KPT; ++bit) sum += __popcll(__ballot((n >> bit) & 1)) << bit;
+    return total(sum, nullptr);
+  };
   auto at_least = [&](uint64_t bound) {
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < KPT; ++i) n += __popcll(__ballot(key[i] >= bound));
-    return total(n);
+    for (int i = 0; i < KPT; ++i) n += key[i] >= bound ? 1 : 0;
+    return wave_total(n);
+  };
+  auto words_at_least = [&](unsigned bound) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) n += (unsigned)(key[i] >> 32) >= bound ? 1 : 0;
+    return wave_total(n);
   };
   uint64_t bound = 1;  // keys at or above it are taken
   uint64_t equal = 0;  // and of the keys equal to this, the first `rest`
   int rest = 0;
   if (at_least(1) > p.count) {
-    uint64_t low = 1, high = ~0ull;  // more than count keys >= low, at most count >= high
-    int above = at_least(high);
+    // More than count keys >= low, at most count >= high: first by the keys'
+    // high words (most keys differ there), then by the whole keys.
+    unsigned low_word = ~most_neg, high_word = most + 1;
+    int above = words_at_least(high_word);  // those always taken
+    while (above < p.count && high_word - low_word > 1) {
+      const unsigned mid = low_word + (high_word - low_word) / 2;
+      const int n = words_at_least(mid);
+      if (n > p.count) {
+        low_word = mid;
+      } else {
+        high_word = mid;
+        above = n;
+      }
+    }
+    uint64_t low = (uint64_t)low_word << 32, high = (uint64_t)high_word << 32;
     while (above < p.count && high - low > 1) {
       const uint64_t mid = low + (high - low) / 2;
       const int n = at_least(mid);
@@ -264,64 +509,63 @@ __global__ void __launch_bounds__(kTopThreads) top_pages_kernel(const SelectPara
       rest = p.count - above;
     }
   }
+  auto below = [](uint64_t mask) {  // set bits under this lane
+    return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0u));
+  };
   int written = 0, ties = 0;
 #pragma unroll
   for (int i = 0; i < KPT; ++i) {
-    if (i * kTopThreads >= pages) break;
+    if (i * kLanes >= pages) break;
     bool take = key[i] >= bound;
+    int before;
     if (rest > 0) {
       const bool tie = key[i] == equal;
       const uint64_t mask = __ballot(tie);
-      __syncthreads();
-      if (lane == 0) s_sum[0][wave] = __popcll(mask);
-      __syncthreads();
-      int before = ties + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0u));
-      for (int w = 0; w < kTopThreads / 64; ++w) {
-        before += w < wave ? s_sum[0][w] : 0;
-        ties += s_sum[0][w];
-      }
-      take |= tie && before < rest;
+      const int all = total(__popcll(mask), &before);
+      take |= tie && ties + before + below(mask) < rest;
+      ties += all;
     }
     const uint64_t mask = __ballot(take);
-    __syncthreads();
-    if (lane == 0) s_sum[0][wave] = __popcll(mask);
-    __syncthreads();
-    int at = written + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0u));
-    for (int w = 0; w < kTopThreads / 64; ++w) {
-      at += w < wave ? s_sum[0][w] : 0;
-      written += s_sum[0][w];
-    }
-    if (take) out[at] = i * kTopThreads + threadIdx.x;
+    const int all = total(__popcll(mask), &before);
+    if (take) out[written + before + below(mask)] = i * kLanes + within;
+    written += all;
   }
-  for (int i = written + threadIdx.x; i < p.count; i += kTopThreads) out[i] = -1;
+  for (int i = written + within; i < p.count; i += kLanes) out[i] = -1;
 }
 
 template <bool kFp16>
 hipError_t launch_select(const SelectParams& p, hipStream_t stream) {
   const int64_t row_blocks = (int64_t)p.requests * p.slab_blocks;
   if (p.pooled) {
-    const int64_t n = row_blocks * p.heads * kHeadDim;
+    const int64_t n = row_blocks * p.heads * (kHeadDim / 8);
     hipLaunchKernelGGL(pool_rows_kernel<kFp16>, dim3((unsigned)((n + kPoolThreads - 1) / kPoolThreads)),
                        dim3(kPoolThreads), 0, stream, p);
   }
-  constexpr int kSlots = kScoreThreads / 16;
-  if (p.slab_blocks > 1) {
-    const unsigned chunks = (unsigned)((p.table_cols + 4 * kSlots - 1) / (4 * kSlots));
-    const unsigned split = (unsigned)min(p.slab_blocks, 8);
-    hipLaunchKernelGGL((score_kernel<kFp16, 4>), dim3(chunks, (unsigned)(p.requests * p.kv_heads), split),
-                       dim3(kScoreThreads), 0, stream, p);
+  int padded = 1;
+  while (padded < p.heads / p.kv_heads) padded *= 2;
+  const int rows = p.slab_blocks * padded;
+  const unsigned chunks = (unsigned)((p.table_cols + 16 * kScoreWaves - 1) / (16 * kScoreWaves));
+  const unsigned heads = (unsigned)(p.requests * p.kv_heads);
+  if (rows <= 8 && padded <= 4) {
+    hipLaunchKernelGGL((score_kernel<kFp16, true>), dim3(chunks, heads, 1), dim3(kScoreThreads), 0, stream, p, padded);
   } else {
-    const unsigned chunks = (unsigned)((p.table_cols + kSlots - 1) / kSlots);
-    hipLaunchKernelGGL((score_kernel<kFp16, 1>), dim3(chunks, (unsigned)(p.requests * p.kv_heads), 1),
-                       dim3(kScoreThreads), 0, stream, p);
+    // Row tiles are dealt over enough workgroups for two waves per SIMD: the
+    // bounds of a wave's pages are converted once per wave.
+    const int units = (rows + (padded > 16 ? padded : 16) - 1) / (padded > 16 ? padded : 16);
+    const unsigned wanted = (512 + chunks * heads - 1) / (chunks * heads);
+    const unsigned split = wanted < (unsigned)units ? wanted : (unsigned)units;
+    hipLaunchKernelGGL((score_kernel<kFp16, false>), dim3(chunks, heads, split), dim3(kScoreThreads), 0, stream, p,
+                       padded);
   }
-  const dim3 grid((unsigned)(row_blocks * p.kv_heads));
-  if (p.table_cols <= 4 * kTopThreads) {
-    hipLaunchKernelGGL(top_pages_kernel<4>, grid, dim3(kTopThreads), 0, stream, p);
-  } else if (p.table_cols <= 16 * kTopThreads) {
-    hipLaunchKernelGGL(top_pages_kernel<16>, grid, dim3(kTopThreads), 0, stream, p);
+  const unsigned n = (unsigned)(row_blocks * p.kv_heads);
+  if (p.table_cols <= 256) {
+    hipLaunchKernelGGL((top_pages_kernel<4, 1>), dim3((n + 3) / 4), dim3(kTopThreads), 0, stream, p);
+  } else if (p.table_cols <= 1024) {
+    hipLaunchKernelGGL((top_pages_kernel<16, 1>), dim3((n + 3) / 4), dim3(kTopThreads), 0, stream, p);
+  } else if (p.table_cols <= 4096) {
+    hipLaunchKernelGGL((top_pages_kernel<16, 4>), dim3(n), dim3(kTopThreads), 0, stream, p);
   } else {
-    hipLaunchKernelGGL(top_pages_kernel<64>, grid, dim3(kTopThreads), 0, stream, p);
+    hipLaunchKernelGGL((top_pages_kernel<64, 4>), dim3(n), dim3(kTopThreads), 0, stream, p);
   }
   return hipGetLastError();
 }
