@@ -91,35 +91,45 @@ __device__ __forceinline__ float to_float(short x) {
   return kFp16 ? (float)__builtin_bit_cast(_Float16, x) : __uint_as_float((unsigned)(uint16_t)x << 16);
 }
 
-// The sums of each block's rows, one thread per (block, head, 8 dims), eight
-// rows' loads in flight.
-constexpr int kPoolThreads = 64;
+// The sums of each block's rows: four threads per (block, head, 8 dims), each
+// with eight rows' loads in flight, joined through LDS.
+constexpr int kPoolThreads = 256;
+constexpr int kPoolColumns = 64;
 template <bool kFp16>
 __global__ void __launch_bounds__(kPoolThreads) pool_rows_kernel(const SelectParams p) {
-  const int64_t i = (int64_t)blockIdx.x * kPoolThreads + threadIdx.x;
+  __shared__ double s_sum[3][8][kPoolColumns];
+  const int quarter = threadIdx.x / kPoolColumns, column = threadIdx.x % kPoolColumns;
+  const int64_t i = (int64_t)blockIdx.x * kPoolColumns + column;
   const int width = p.heads * (kHeadDim / 8);
   const int block = (int)(i / width);
-  if (block >= p.requests * p.slab_blocks) return;
-  const int b = p.request0 + block / p.slab_blocks;
-  const int t0 = (p.block0 + block % p.slab_blocks) * kSelectRows;
-  const int pos0 = max(p.seq_lens[b], 0) - p.rows;
+  const bool real = block < p.requests * p.slab_blocks;
   const int at = (int)(i % width) * 8;
-  const uint16_t* const src = p.query + (int64_t)b * p.rows * p.query_stride + at;
-  const int end = min(t0 + kSelectRows, p.rows);
   double sum[8] = {};
-  for (int t = max(t0, -pos0); t < end; t += 8) {
+  if (real) {
+    const int b = p.request0 + block / p.slab_blocks;
+    const int t0 = (p.block0 + block % p.slab_blocks) * kSelectRows + 8 * quarter;
+    const uint16_t* const src = p.query + (int64_t)b * p.rows * p.query_stride + at;
+    const int seq = p.seq_lens[b];
     s16x8_t x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const s16x8_t*>(src + min(t + j, end - 1) * p.query_stride);
+    for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const s16x8_t*>(src + min(t0 + j, p.rows - 1) * p.query_stride);
+    const int begin = p.rows - max(seq, 0);  // the first row of the request
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
+      const bool row = t0 + j >= begin && t0 + j < p.rows;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += t + j < end ? (double)to_float<kFp16>(x[j][e]) : 0.0;
+      for (int e = 0; e < 8; ++e) sum[e] += row ? (double)to_float<kFp16>(x[j][e]) : 0.0;
     }
   }
+  if (quarter > 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s_sum[quarter - 1][e][column] = sum[e];
+  }
+  __syncthreads();
+  if (quarter > 0 || !real) return;
   double* const dst = p.pooled + (int64_t)block * p.heads * kHeadDim + at;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) dst[e] = sum[e];
+  for (int e = 0; e < 8; ++e) dst[e] = (sum[e] + s_sum[0][e][column]) + (s_sum[1][e][column] + s_sum[2][e][column]);
 }
 
 __device__ __forceinline__ uint64_t score_key(double x) {
@@ -145,7 +155,7 @@ constexpr int kScoreThreads = kScoreWaves * 64;
 typedef double f64x4_t __attribute__((ext_vector_type(4)));
 
 template <bool kFp16, bool kSmall>
-__global__ void __launch_bounds__(kScoreThreads, kSmall ? 4 : 2) score_kernel(const SelectParams p, int padded) {
+__global__ void __launch_bounds__(kScoreThreads, kSmall ? 4 : 3) score_kernel(const SelectParams p, int padded) {
   constexpr int kTileRows = kSmall ? 4 : 16;
   // The query sums of two row tiles, shared by the waves: rows of 128 and two
   // doubles, so that 16 rows' reads meet different banks.
@@ -223,22 +233,22 @@ __global__ void __launch_bounds__(kScoreThreads, kSmall ? 4 : 2) score_kernel(co
     for (int e = 0; e < 8; ++e) odd |= (raw_lo[i][e] & kExp) == kExp || (raw_hi[i][e] & kExp) == kExp;
   }
   const bool odd_bounds = __any(odd);
-  // Converted once where many row tiles use them, else at each use.
-  double wide_lo[kSmall ? 1 : 32], wide_hi[kSmall ? 1 : 32];
+  // To 32 bits once where many row tiles use them, to 64 bits at each use.
+  float wide_lo[kSmall ? 1 : 32], wide_hi[kSmall ? 1 : 32];
   if constexpr (!kSmall) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      wide_lo[i] = (double)to_float<kFp16>(raw_lo[i >> 3][i & 7]);
-      wide_hi[i] = (double)to_float<kFp16>(raw_hi[i >> 3][i & 7]);
+      wide_lo[i] = to_float<kFp16>(raw_lo[i >> 3][i & 7]);
+      wide_hi[i] = to_float<kFp16>(raw_hi[i >> 3][i & 7]);
     }
   }
   auto lo = [&](int i) {
     if constexpr (kSmall) return (double)to_float<kFp16>(raw_lo[i >> 3][i & 7]);
-    else return wide_lo[i];
+    else return (double)wide_lo[i];
   };
   auto hi = [&](int i) {
     if constexpr (kSmall) return (double)to_float<kFp16>(raw_hi[i >> 3][i & 7]);
-    else return wide_hi[i];
+    else return (double)wide_hi[i];
   };
 
   uint64_t best[4] = {0, 0, 0, 0};
@@ -253,6 +263,9 @@ __global__ void __launch_bounds__(kScoreThreads, kSmall ? 4 : 2) score_kernel(co
       // converted in the loop, not ahead of it in registers that are not there
 #pragma unroll
       for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(raw_lo[i]), "+v"(raw_hi[i]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) asm volatile("" : "+v"(wide_lo[i]), "+v"(wide_hi[i]));
     }
     const int row0 = t * kTileRows;
     {
@@ -356,13 +369,11 @@ __global__ void __launch_bounds__(kScoreThreads, kSmall ? 4 : 2) score_kernel(co
 }
 
 // The `count` largest keys of one (block, KV head), the lowest page first among
-// equal ones, written in the order of the pages.  A key's threshold is found by
-// halving between the smallest and the largest key: as soon as exactly `count`
-// keys lie at or above the middle it is done (about 12 steps for 1024 pages);
-// only equal keys take it down to one value.  A row is one wave's (its keys in
-// registers, counts by ballots, no barrier) up to 1024 pages, else a
-// workgroup's of four waves.
+// equal ones, written in the order of the pages.  The threshold is found by
+// counting keys in 256 bins between the smallest and the largest key, then in
+// the bin that holds it: two levels or three for 1024 pages, eight at most.
 constexpr int kTopThreads = 256;
+static_assert(64 * kTopThreads >= kMaxTableCols, "a workgroup holds a row's keys");
 // Largest value of the wave's lanes, in all of them.
 template <int kCtrl>
 __device__ __forceinline__ unsigned dpp_max(unsigned x) {
@@ -380,14 +391,11 @@ __device__ __forceinline__ unsigned wave_max(unsigned x) {
   return c[0] > c[1] ? c[0] : c[1];
 }
 
-template <int KPT, int W>
+template <int KPT>
 __global__ void __launch_bounds__(kTopThreads) top_pages_kernel(const SelectParams p) {
-  constexpr int kLanes = 64 * W;
+  constexpr int W = kTopThreads / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int within = threadIdx.x % kLanes;
-  // of the slab: (request * blocks + block) * kv_heads + head
-  const int row = (int)blockIdx.x * (kTopThreads / kLanes) + (int)threadIdx.x / kLanes;
-  if (row >= p.requests * p.slab_blocks * p.kv_heads) return;  // W = 1 alone: no barrier follows
+  const int row = blockIdx.x;  // of the slab: (request * blocks + block) * kv_heads + head
   const int kv_head = row % p.kv_heads;
   const int blk = p.block0 + row / p.kv_heads % p.slab_blocks;
   const int b = p.request0 + row / p.kv_heads / p.slab_blocks;
@@ -400,37 +408,33 @@ __global__ void __launch_bounds__(kTopThreads) top_pages_kernel(const SelectPara
   int32_t* const out = p.out + (((int64_t)b * p.blocks + blk) * p.kv_heads + kv_head) * p.count;
   __shared__ int s_sum[2][W];
   __shared__ unsigned s_key[2][W];
+  __shared__ unsigned s_bins[2][256];
   int turn = 0;
   // One count per wave to their sum, and the sum of the waves before.
   auto total = [&](int mine, int* before) {
-    if constexpr (W == 1) {
-      if (before) *before = 0;
-      return mine;
-    } else {
-      if (lane == 0) s_sum[turn][wave] = mine;
-      __syncthreads();
-      int sum = 0, ahead = 0;
+    if (lane == 0) s_sum[turn][wave] = mine;
+    __syncthreads();
+    int sum = 0, ahead = 0;
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        ahead += w < wave ? s_sum[turn][w] : 0;
-        sum += s_sum[turn][w];
-      }
-      turn ^= 1;
-      if (before) *before = ahead;
-      return sum;
+    for (int w = 0; w < W; ++w) {
+      ahead += w < wave ? s_sum[turn][w] : 0;
+      sum += s_sum[turn][w];
     }
+    turn ^= 1;
+    if (before) *before = ahead;
+    return sum;
   };
-  // key i of a thread is page i * kLanes + within
+  // key i of a thread is page 256 i + threadIdx.x
   uint64_t key[KPT];
   unsigned most = 0, most_neg = 0;  // largest high word, and complement, of the keys that are not always taken
 #pragma unroll
   for (int i = 0; i < KPT; ++i) {
-    const int page = i * kLanes + within;
+    const int page = i * kTopThreads + (int)threadIdx.x;
     key[i] = page < pages ? src[page] : 0;
   }
 #pragma unroll
   for (int i = 0; i < KPT; ++i) {
-    const int page = i * kLanes + within;
+    const int page = i * kTopThreads + (int)threadIdx.x;
     if (key[i] != 0) {
       if ((p.recent_pages > 0 && page >= recent) || page < p.sink_pages) {
         key[i] = ~0ull;
@@ -443,71 +447,82 @@ __global__ void __launch_bounds__(kTopThreads) top_pages_kernel(const SelectPara
   }
   most = wave_max(most);
   most_neg = wave_max(most_neg);
-  if constexpr (W > 1) {
-    if (lane == 0) {
-      s_key[0][wave] = most;
-      s_key[1][wave] = most_neg;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      most = s_key[0][w] > most ? s_key[0][w] : most;
-      most_neg = s_key[1][w] > most_neg ? s_key[1][w] : most_neg;
-    }
+  if (lane == 0) {
+    s_key[0][wave] = most;
+    s_key[1][wave] = most_neg;
   }
-  // Sum over the wave of a small count per lane: bit by bit, by ballots.
-  auto wave_total = [&](int n) {
-    int sum = 0;
+  __syncthreads();
 #pragma unroll
-    for (int bit = 0; (1 << bit) <= KPT; ++bit) sum += __popcll(__ballot((n >> bit) & 1)) << bit;
-    return total(sum, nullptr);
-  };
-  auto at_least = [&](uint64_t bound) {
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < KPT; ++i) n += key[i] >= bound ? 1 : 0;
-    return wave_total(n);
-  };
-  auto words_at_least = [&](unsigned bound) {
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < KPT; ++i) n += (unsigned)(key[i] >> 32) >= bound ? 1 : 0;
-    return wave_total(n);
-  };
+  for (int w = 0; w < W; ++w) {
+    most = s_key[0][w] > most ? s_key[0][w] : most;
+    most_neg = s_key[1][w] > most_neg ? s_key[1][w] : most_neg;
+  }
   uint64_t bound = 1;  // keys at or above it are taken
   uint64_t equal = 0;  // and of the keys equal to this, the first `rest`
   int rest = 0;
-  if (at_least(1) > p.count) {
-    // More than count keys >= low, at most count >= high: first by the keys'
-    // high words (most keys differ there), then by the whole keys.
-    unsigned low_word = ~most_neg, high_word = most + 1;
-    int above = words_at_least(high_word);  // those always taken
-    while (above < p.count && high_word - low_word > 1) {
-      const unsigned mid = low_word + (high_word - low_word) / 2;
-      const int n = words_at_least(mid);
-      if (n > p.count) {
-        low_word = mid;
+  int candidates = 0, above = 0;  // keys, and those always taken
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {
+    candidates += __popcll(__ballot(key[i] != 0));
+    above += __popcll(__ballot(key[i] == ~0ull));
+  }
+  candidates = total(candidates, nullptr);
+  above = total(above, nullptr);
+  if (candidates > p.count) {
+    // The keys in [low, high) hold the last one taken.  A level counts them in
+    // 256 bins and goes on in the bin in which the count is reached.
+    uint64_t low = (uint64_t)~most_neg << 32 | (most_neg == ~0u ? 1 : 0), high = ((uint64_t)most + 1) << 32;
+    for (int level = 0; above < p.count; level ^= 1) {
+      const int shift = max(0, 56 - __clzll((long long)(high - low - 1)));
+      s_bins[level][threadIdx.x] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < KPT; ++i) {
+        if (key[i] >= low && key[i] < high) atomicAdd(&s_bins[level][(key[i] - low) >> shift], 1);
+      }
+      __syncthreads();
+      // bins 4 lane .. 4 lane + 3, and how many keys lie in them and the bins above
+      int bin[4], upto = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        bin[j] = s_bins[level][4 * lane + j];
+        upto += bin[j];
+      }
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int add = __shfl_down(upto, d);
+        if (lane + d < 64) upto += add;
+      }
+      // the last lane whose bins and those above reach the count, and in it the bin
+      const int at_lane = 63 - __clzll((long long)__ballot(above + upto >= p.count));
+      int j_at = 0, reached = above + upto, over = reached;
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        over -= bin[j];  // keys above bin j
+        if (over >= p.count) {
+          j_at = j + 1;
+          reached = over;
+        }
+      }
+      const int j = __builtin_amdgcn_readlane(j_at, at_lane);
+      const int with = __builtin_amdgcn_readlane(reached, at_lane);
+      const int in_bin = __builtin_amdgcn_readlane(j_at == 0 ? bin[0] : j_at == 1 ? bin[1] : j_at == 2 ? bin[2] : bin[3], at_lane);
+      low += (uint64_t)(4 * at_lane + j) << shift;
+      if (with == p.count) {
+        bound = low;
+        above = with;
       } else {
-        high_word = mid;
-        above = n;
+        above = with - in_bin;
+        if (shift == 0) {
+          bound = low + 1;
+          equal = low;
+          rest = p.count - above;
+          break;
+        }
+        high = low + (1ull << shift);
       }
     }
-    uint64_t low = (uint64_t)low_word << 32, high = (uint64_t)high_word << 32;
-    while (above < p.count && high - low > 1) {
-      const uint64_t mid = low + (high - low) / 2;
-      const int n = at_least(mid);
-      if (n > p.count) {
-        low = mid;
-      } else {
-        high = mid;
-        above = n;
-      }
-    }
-    bound = high;
-    if (above < p.count) {
-      equal = low;
-      rest = p.count - above;
-    }
+    if (bound == 1) bound = high;  // all that are taken always are
   }
   auto below = [](uint64_t mask) {  // set bits under this lane
     return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0u));
@@ -515,7 +530,7 @@ __global__ void __launch_bounds__(kTopThreads) top_pages_kernel(const SelectPara
   int written = 0, ties = 0;
 #pragma unroll
   for (int i = 0; i < KPT; ++i) {
-    if (i * kLanes >= pages) break;
+    if (i * kTopThreads >= pages) break;
     bool take = key[i] >= bound;
     int before;
     if (rest > 0) {
@@ -527,10 +542,10 @@ __global__ void __launch_bounds__(kTopThreads) top_pages_kernel(const SelectPara
     }
     const uint64_t mask = __ballot(take);
     const int all = total(__popcll(mask), &before);
-    if (take) out[written + before + below(mask)] = i * kLanes + within;
+    if (take) out[written + before + below(mask)] = i * kTopThreads + (int)threadIdx.x;
     written += all;
   }
-  for (int i = written + within; i < p.count; i += kLanes) out[i] = -1;
+  for (int i = written + threadIdx.x; i < p.count; i += kTopThreads) out[i] = -1;
 }
 
 template <bool kFp16>
@@ -538,7 +553,7 @@ hipError_t launch_select(const SelectParams& p, hipStream_t stream) {
   const int64_t row_blocks = (int64_t)p.requests * p.slab_blocks;
   if (p.pooled) {
     const int64_t n = row_blocks * p.heads * (kHeadDim / 8);
-    hipLaunchKernelGGL(pool_rows_kernel<kFp16>, dim3((unsigned)((n + kPoolThreads - 1) / kPoolThreads)),
+    hipLaunchKernelGGL(pool_rows_kernel<kFp16>, dim3((unsigned)((n + kPoolColumns - 1) / kPoolColumns)),
                        dim3(kPoolThreads), 0, stream, p);
   }
   int padded = 1;
@@ -549,23 +564,23 @@ hipError_t launch_select(const SelectParams& p, hipStream_t stream) {
   if (rows <= 8 && padded <= 4) {
     hipLaunchKernelGGL((score_kernel<kFp16, true>), dim3(chunks, heads, 1), dim3(kScoreThreads), 0, stream, p, padded);
   } else {
-    // Row tiles are dealt over enough workgroups for two waves per SIMD: the
+    // Row tiles are dealt over enough workgroups for three waves per SIMD: the
     // bounds of a wave's pages are converted once per wave.
     const int units = (rows + (padded > 16 ? padded : 16) - 1) / (padded > 16 ? padded : 16);
-    const unsigned wanted = (512 + chunks * heads - 1) / (chunks * heads);
+    const unsigned wanted = (768 + chunks * heads - 1) / (chunks * heads);
     const unsigned split = wanted < (unsigned)units ? wanted : (unsigned)units;
     hipLaunchKernelGGL((score_kernel<kFp16, false>), dim3(chunks, heads, split), dim3(kScoreThreads), 0, stream, p,
                        padded);
   }
   const unsigned n = (unsigned)(row_blocks * p.kv_heads);
-  if (p.table_cols <= 256) {
-    hipLaunchKernelGGL((top_pages_kernel<4, 1>), dim3((n + 3) / 4), dim3(kTopThreads), 0, stream, p);
-  } else if (p.table_cols <= 1024) {
-    hipLaunchKernelGGL((top_pages_kernel<16, 1>), dim3((n + 3) / 4), dim3(kTopThreads), 0, stream, p);
-  } else if (p.table_cols <= 4096) {
-    hipLaunchKernelGGL((top_pages_kernel<16, 4>), dim3(n), dim3(kTopThreads), 0, stream, p);
+  if (p.table_cols <= kTopThreads) {
+    hipLaunchKernelGGL(top_pages_kernel<1>, dim3(n), dim3(kTopThreads), 0, stream, p);
+  } else if (p.table_cols <= 4 * kTopThreads) {
+    hipLaunchKernelGGL(top_pages_kernel<4>, dim3(n), dim3(kTopThreads), 0, stream, p);
+  } else if (p.table_cols <= 16 * kTopThreads) {
+    hipLaunchKernelGGL(top_pages_kernel<16>, dim3(n), dim3(kTopThreads), 0, stream, p);
   } else {
-    hipLaunchKernelGGL((top_pages_kernel<64, 4>), dim3(n), dim3(kTopThreads), 0, stream, p);
+    hipLaunchKernelGGL(top_pages_kernel<64>, dim3(n), dim3(kTopThreads), 0, stream, p);
   }
   return hipGetLastError();
 }
