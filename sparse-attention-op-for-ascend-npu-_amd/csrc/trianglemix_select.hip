@@ -141,55 +141,175 @@ __device__ __forceinline__ uint64_t score_key(double x) {
 // max(x, 0) and min(x, 0) of finite numbers by the sign bit.
 __device__ __forceinline__ double positive(double x) { return __builtin_signbit(x) ? 0.0 : x; }
 __device__ __forceinline__ double negative(double x) { return __builtin_signbit(x) ? x : 0.0; }
+__device__ __forceinline__ bool odd_number(double x) {
+  return (__builtin_bit_cast(uint64_t, x) & 0x7ff0000000000000ull) == 0x7ff0000000000000ull;
+}
+__device__ __forceinline__ void keep_larger(uint64_t& x, uint64_t y) { x = y > x ? y : x; }
 
 // The scores as 64-bit matrix products, q+ max + q- min with q+ = max(q, 0), q-
-// = min(q, 0): a wave holds the bounds of 16 pages (lane l: page l % 16, of
-// every 32 dims the eight from 8 (l / 16) on) and runs over tiles of query sums.  A tile is 16 rows
-// (v_mfma_f64_16x16x4) or, for a single block of up to four heads, four
-// (v_mfma_f64_4x4x4, its four blocks taking four pages each): either reached
-// 70-73 TFLOP/s of 78.6, alone, in a probe.  Rows are block * padded + head, the
-// group padded to a power of two.  Infinities and NaNs, which a product with
-// zero would turn into NaN, take a plain loop.
+// = min(q, 0): lane l of a wave holds the bounds of page l % 16 of 16, of every
+// 32 dims the eight from 8 (l / 16) on, and the products run over tiles of
+// rows, block * padded + head with the group padded to a power of two.
+// Infinities and NaNs, which a product with zero would turn into NaN, take a
+// plain loop.
+typedef double f64x4_t __attribute__((ext_vector_type(4)));
+typedef double f64x2_t __attribute__((ext_vector_type(2)));
 constexpr int kScoreWaves = 4;
 constexpr int kScoreThreads = kScoreWaves * 64;
-typedef double f64x4_t __attribute__((ext_vector_type(4)));
 
-template <bool kFp16, bool kSmall>
-__global__ void __launch_bounds__(kScoreThreads, kSmall ? 4 : 3) score_kernel(const SelectParams p, int padded) {
-  constexpr int kTileRows = kSmall ? 4 : 16;
-  // The query sums of two row tiles, shared by the waves: rows of 128 and two
-  // doubles, so that 16 rows' reads meet different banks.
-  __shared__ __attribute__((aligned(16))) double s_q[2][kTileRows][kHeadDim + 2];
+struct Bounds16 {  // a lane's 32 dims of its page
+  s16x8_t lo[4], hi[4];
+};
+__device__ __forceinline__ Bounds16 load_bounds(const SelectParams& p, int64_t at) {
+  Bounds16 x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x.lo[i] = *reinterpret_cast<const s16x8_t*>(p.page_min + at + 32 * i);
+    x.hi[i] = *reinterpret_cast<const s16x8_t*>(p.page_max + at + 32 * i);
+  }
+  return x;
+}
+template <bool kFp16>
+__device__ __forceinline__ bool odd_bounds(const Bounds16& x) {  // some bound of the wave's is no finite number
+  typedef unsigned short u16x8_t __attribute__((ext_vector_type(8)));
+  u16x8_t most = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x8_t, x.lo[i] & (short)0x7fff));
+    most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x8_t, x.hi[i] & (short)0x7fff));
+  }
+  bool odd = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) odd |= most[e] >= (kFp16 ? 0x7c00 : 0x7f80);
+  return __any(odd);
+}
+// The plain sum over a row of 128 (q: its dims from 8 quad on), in all four
+// lanes of a page.  The bounds come anew from memory: nothing is kept in
+// registers for this path.
+template <bool kFp16>
+__device__ double plain_score(const SelectParams& p, int64_t at, const double* q) {
+  double y = 0.0;
+#pragma unroll 1
+  for (int i = 0; i < 32; ++i) {
+    const int d = 32 * (i >> 3) + (i & 7);
+    const uint16_t bound = q[d] >= 0.0 ? p.page_max[at + d] : p.page_min[at + d];
+    y = __builtin_fma(q[d], (double)to_float<kFp16>((short)bound), y);
+  }
+  y += __shfl_xor(y, 16);
+  y += __shfl_xor(y, 32);
+  return y;
+}
+
+// Up to four rows (a decoding step: one block, up to four heads a group):
+// v_mfma_f64_4x4x4, its four blocks taking four pages each.  A wave runs over
+// `tiles` tiles of 16 pages, one tile's bounds ahead; what bounds it is reading
+// them and their conversion to 64 bits.
+template <bool kFp16>
+__global__ void __launch_bounds__(kScoreThreads, 4) score_few_kernel(const SelectParams p, int padded, int tiles) {
+  __shared__ __attribute__((aligned(16))) double s_q[4][kHeadDim + 2];
+  __shared__ __attribute__((aligned(16))) double s_plus[4][kHeadDim + 2], s_minus[4][kHeadDim + 2];
+  __shared__ int s_odd[kScoreWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = lane & 15, quad = lane >> 4;
+  const int kv_head = blockIdx.y, slab_b = blockIdx.z;
+  const int b = p.request0 + slab_b;
+  const int group = p.heads / p.kv_heads;
+  const int page0 = ((int)blockIdx.x * kScoreWaves + wave) * 16 * tiles;
+  // the wave's pages, one a lane; the length is not waited for
+  int phys = page0 + lane < p.table_cols && lane < 16 * tiles ? p.block_table[b * p.table_stride + page0 + lane] : -1;
+  if (phys >= p.num_pages) phys = -1;
+  const int seq = max(p.seq_lens[b], 0);
+  {
+    // one row a wave, two dims a lane
+    const int blk = wave / padded, g = wave & (padded - 1), head = kv_head * group + g;
+    f64x2_t x = {0.0, 0.0};
+    if (blk < p.slab_blocks && g < group) {
+      if (p.pooled) {
+        x = *reinterpret_cast<const f64x2_t*>(
+            p.pooled + ((int64_t)(slab_b * p.slab_blocks + blk) * p.heads + head) * kHeadDim + 2 * lane);
+      } else {
+        const unsigned two =
+            *reinterpret_cast<const unsigned*>(p.query + b * p.query_stride + (int64_t)head * kHeadDim + 2 * lane);
+        x = f64x2_t{(double)to_float<kFp16>((short)two), (double)to_float<kFp16>((short)(two >> 16))};
+      }
+    }
+    *reinterpret_cast<f64x2_t*>(&s_q[wave][2 * lane]) = x;
+    *reinterpret_cast<f64x2_t*>(&s_plus[wave][2 * lane]) = f64x2_t{positive(x[0]), positive(x[1])};
+    *reinterpret_cast<f64x2_t*>(&s_minus[wave][2 * lane]) = f64x2_t{negative(x[0]), negative(x[1])};
+    const bool odd = __any(odd_number(x[0]) || odd_number(x[1]));
+    if (lane == 0) s_odd[wave] = odd ? 1 : 0;
+  }
+  auto place = [&](int t) {  // of the lane's page in tile t; an unused page's bounds are those of page 0
+    return ((int64_t)max(__shfl(phys, 16 * t + col), 0) * p.kv_heads + kv_head) * kHeadDim + 8 * quad;
+  };
+  Bounds16 next = load_bounds(p, place(0));
+  __syncthreads();
+  const bool odd_rows = (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3]) != 0;
+  const int pages = min(p.table_cols, (seq + kPageSize - 1) / kPageSize);
+  for (int t = 0; t < tiles; ++t) {
+    if (page0 + 16 * t >= pages) return;
+    Bounds16 x = next;
+    const int64_t at = place(t);
+    if (t + 1 < tiles) next = load_bounds(p, place(t + 1));
+    double sum = 0.0;
+    if (__builtin_expect(!odd_rows && !odd_bounds<kFp16>(x), 1)) {
+      double c[4] = {};
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        const int d = 8 * quad + 32 * (i >> 3) + (i & 7);
+        const f64x2_t plus = *reinterpret_cast<const f64x2_t*>(&s_plus[lane & 3][d]);
+        const f64x2_t minus = *reinterpret_cast<const f64x2_t*>(&s_minus[lane & 3][d]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const double hi = (double)to_float<kFp16>(x.hi[i >> 3][(i & 7) + j]);
+          const double lo = (double)to_float<kFp16>(x.lo[i >> 3][(i & 7) + j]);
+          c[2 * j] = __builtin_amdgcn_mfma_f64_4x4x4f64(plus[j], hi, c[2 * j], 0, 0, 0);
+          c[2 * j + 1] = __builtin_amdgcn_mfma_f64_4x4x4f64(minus[j], lo, c[2 * j + 1], 0, 0, 0);
+        }
+      }
+      sum = (c[0] + c[1]) + (c[2] + c[3]);
+    } else {
+      for (int r = 0; r < 4; ++r) {
+        const double y = plain_score<kFp16>(p, at, &s_q[r][8 * quad]);
+        sum = r == quad ? y : sum;
+      }
+    }
+    // row `quad` of page `col`: max over the heads of a block
+    uint64_t best = (quad & (padded - 1)) < group ? score_key(sum) : 0;
+    if (padded >= 2) keep_larger(best, __shfl_xor(best, 16));
+    if (padded >= 4) keep_larger(best, __shfl_xor(best, 32));
+    const int page = page0 + 16 * t + col;
+    if ((quad & (padded - 1)) == 0 && quad < p.slab_blocks * padded && page < pages) {
+      p.scores[((int64_t)(slab_b * p.slab_blocks + quad / padded) * p.kv_heads + kv_head) * p.table_cols + page] =
+          __shfl(phys, 16 * t + col) >= 0 ? best : 0;
+    }
+  }
+}
+
+// Many rows: tiles of 16 rows, v_mfma_f64_16x16x4, two tiles' query sums in LDS.
+// A wave keeps the bounds of its 16 pages, converted, over all its row tiles.
+template <bool kFp16>
+__global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectParams p, int padded, int split_bits) {
+  // rows of 128 and two doubles, so that 16 rows' reads meet different banks
+  __shared__ __attribute__((aligned(16))) double s_q[2][16][kHeadDim + 2];
   __shared__ int s_odd[2];  // some value of the tile is no finite number
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, quad = lane >> 4;
-  const int kv_head = blockIdx.y % p.kv_heads, slab_b = blockIdx.y / p.kv_heads;
+  const int kv_head = (int)blockIdx.y >> split_bits, slab_b = blockIdx.z;
   const int b = p.request0 + slab_b;
   const int group = p.heads / p.kv_heads;
-  const int seq = max(p.seq_lens[b], 0);
-  const int pages = min(p.table_cols, (seq + kPageSize - 1) / kPageSize);
-  if ((int)blockIdx.x * kScoreWaves * 16 >= pages) return;
   const int page = ((int)blockIdx.x * kScoreWaves + wave) * 16 + col;
-  const int phys = page < pages ? p.block_table[b * p.table_stride + page] : -1;
-  const bool there = phys >= 0 && phys < p.num_pages;
-  const int64_t at = ((int64_t)(there ? phys : 0) * p.kv_heads + kv_head) * kHeadDim + 8 * quad;
-  s16x8_t raw_lo[4], raw_hi[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    raw_lo[i] = *reinterpret_cast<const s16x8_t*>(p.page_min + at + 32 * i);
-    raw_hi[i] = *reinterpret_cast<const s16x8_t*>(p.page_max + at + 32 * i);
-  }
+  const int phys = page < p.table_cols ? p.block_table[b * p.table_stride + page] : -1;
+  const int seq = max(p.seq_lens[b], 0);
 
   const int rows = p.slab_blocks * padded;
-  const int tiles_per_block = max(1, padded / kTileRows);
-  const int row_tiles = (rows + kTileRows - 1) / kTileRows;
-  // Two dims a thread of each of its rows of the tile; zeros for rows of the padding.
-  constexpr int kShare = kTileRows * (kHeadDim / 2) / kScoreThreads;
-  typedef double f64x2_t __attribute__((ext_vector_type(2)));
+  const int tiles_per_block = max(1, padded / 16);
+  const int row_tiles = (rows + 15) / 16;
+  // Two dims a thread of four of the tile's rows; zeros for rows of the padding.
   auto fetch = [&](int row0, f64x2_t* x) {
 #pragma unroll
-    for (int j = 0; j < kShare; ++j) {
-      const int row = row0 + (int)threadIdx.x / 64 + j * (kScoreThreads / 64);
+    for (int j = 0; j < 4; ++j) {
+      const int row = row0 + wave + 4 * j;
       const int blk = row / padded, g = row & (padded - 1);
       x[j] = f64x2_t{0.0, 0.0};
       if (row < rows && g < group) {
@@ -208,150 +328,85 @@ __global__ void __launch_bounds__(kScoreThreads, kSmall ? 4 : 3) score_kernel(co
   auto put = [&](int buffer, const f64x2_t* x) {
     bool odd = false;
 #pragma unroll
-    for (int j = 0; j < kShare; ++j) {
-      constexpr uint64_t kExp = 0x7ff0000000000000ull;
-      odd |= (__builtin_bit_cast(uint64_t, x[j][0]) & kExp) == kExp || (__builtin_bit_cast(uint64_t, x[j][1]) & kExp) == kExp;
-      *reinterpret_cast<f64x2_t*>(&s_q[buffer][threadIdx.x / 64 + j * (kScoreThreads / 64)][2 * lane]) = x[j];
+    for (int j = 0; j < 4; ++j) {
+      odd |= odd_number(x[j][0]) || odd_number(x[j][1]);
+      *reinterpret_cast<f64x2_t*>(&s_q[buffer][wave + 4 * j][2 * lane]) = x[j];
     }
     if (odd) s_odd[buffer] = 1;
   };
-  // A workgroup's row tiles: whole blocks, dealt over blockIdx.z.
-  const int stride = (int)gridDim.z * tiles_per_block;
-  auto next_tile = [&](int t) { return (t + 1) % tiles_per_block == 0 ? t + 1 - tiles_per_block + stride : t + 1; };
-  int t = (int)blockIdx.z * tiles_per_block;
-  f64x2_t x[kShare];
-  fetch(t * kTileRows, x);
+  // A workgroup's row tiles: whole blocks, dealt over the splits.
+  const int stride = tiles_per_block << split_bits;
+  int t = ((int)blockIdx.y & ((1 << split_bits) - 1)) * tiles_per_block;
+  f64x2_t x[4];
+  fetch(t * 16, x);
+  const bool there = phys >= 0 && phys < p.num_pages;
+  const int64_t at = ((int64_t)(there ? phys : 0) * p.kv_heads + kv_head) * kHeadDim + 8 * quad;
+  const Bounds16 raw = load_bounds(p, at);
   if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
   __syncthreads();
   put(0, x);
-
-  bool odd = false;  // some bound is no finite number
+  const int pages = min(p.table_cols, (seq + kPageSize - 1) / kPageSize);
+  if ((int)blockIdx.x * kScoreWaves * 16 >= pages) return;
+  const bool odd_page = odd_bounds<kFp16>(raw);
+  double lo[32], hi[32];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    constexpr short kExp = kFp16 ? 0x7c00 : 0x7f80;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) odd |= (raw_lo[i][e] & kExp) == kExp || (raw_hi[i][e] & kExp) == kExp;
+  for (int i = 0; i < 32; ++i) {
+    lo[i] = (double)to_float<kFp16>(raw.lo[i >> 3][i & 7]);
+    hi[i] = (double)to_float<kFp16>(raw.hi[i >> 3][i & 7]);
   }
-  const bool odd_bounds = __any(odd);
-  // To 32 bits once where many row tiles use them, to 64 bits at each use.
-  float wide_lo[kSmall ? 1 : 32], wide_hi[kSmall ? 1 : 32];
-  if constexpr (!kSmall) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      wide_lo[i] = to_float<kFp16>(raw_lo[i >> 3][i & 7]);
-      wide_hi[i] = to_float<kFp16>(raw_hi[i >> 3][i & 7]);
-    }
-  }
-  auto lo = [&](int i) {
-    if constexpr (kSmall) return (double)to_float<kFp16>(raw_lo[i >> 3][i & 7]);
-    else return (double)wide_lo[i];
-  };
-  auto hi = [&](int i) {
-    if constexpr (kSmall) return (double)to_float<kFp16>(raw_hi[i >> 3][i & 7]);
-    else return (double)wide_hi[i];
-  };
 
   uint64_t best[4] = {0, 0, 0, 0};
-  int buffer = 0;
-  for (; t < row_tiles; buffer ^= 1) {
+  for (int buffer = 0; t < row_tiles; buffer ^= 1) {
     __syncthreads();  // the tile is in its buffer, the other buffer is read
-    const int next = next_tile(t);
+    const int next = (t + 1) % tiles_per_block == 0 ? t + 1 - tiles_per_block + stride : t + 1;
     const bool more = next < row_tiles;
-    if (more) fetch(next * kTileRows, x);
-    const bool odd_row = s_odd[buffer] != 0;
-    if constexpr (kSmall) {
-      // converted in the loop, not ahead of it in registers that are not there
+    if (more) fetch(next * 16, x);
+    const int row0 = t * 16;
+    f64x4_t sum = {0.0, 0.0, 0.0, 0.0};
+    if (__builtin_expect(!odd_page && s_odd[buffer] == 0, 1)) {
+      // Physical row r of the operand is row 4 (r % 4) + r / 4 of the tile, so
+      // that a lane's four results are rows 4 quad .. 4 quad + 3.
+      const double* const q = &s_q[buffer][4 * (col & 3) + (col >> 2)][8 * quad];
+      f64x4_t c0 = sum, c1 = sum;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(raw_lo[i]), "+v"(raw_hi[i]));
+      for (int i = 0; i < 32; i += 2) {
+        const f64x2_t y = *reinterpret_cast<const f64x2_t*>(q + 32 * (i >> 3) + (i & 7));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          c0 = __builtin_amdgcn_mfma_f64_16x16x4f64(positive(y[j]), hi[i + j], c0, 0, 0, 0);
+          c1 = __builtin_amdgcn_mfma_f64_16x16x4f64(negative(y[j]), lo[i + j], c1, 0, 0, 0);
+        }
+      }
+      sum = c0 + c1;
     } else {
+      for (int r = 0; r < 16; ++r) {
+        const double y = plain_score<kFp16>(p, at, &s_q[buffer][r][8 * quad]);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) asm volatile("" : "+v"(wide_lo[i]), "+v"(wide_hi[i]));
-    }
-    const int row0 = t * kTileRows;
-    {
-      double sum[4] = {};
-      if (__builtin_expect(!odd_bounds && !odd_row, 1)) {
-        // Physical row r of the operand is row 4 (r % 4) + r / 4 of the tile, so
-        // that a lane's four results are rows 4 quad .. 4 quad + 3.
-        const double* const q = &s_q[buffer][kSmall ? (lane & 3) : 4 * (col & 3) + (col >> 2)][8 * quad];
-        if constexpr (kSmall) {
-          double c[4] = {};
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const f64x2_t y = *reinterpret_cast<const f64x2_t*>(q + 32 * (i >> 3) + (i & 7));
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              c[2 * j] = __builtin_amdgcn_mfma_f64_4x4x4f64(positive(y[j]), hi(i + j), c[2 * j], 0, 0, 0);
-              c[2 * j + 1] = __builtin_amdgcn_mfma_f64_4x4x4f64(negative(y[j]), lo(i + j), c[2 * j + 1], 0, 0, 0);
-            }
-          }
-          sum[0] = (c[0] + c[1]) + (c[2] + c[3]);
-        } else {
-          f64x4_t c0 = {0.0, 0.0, 0.0, 0.0}, c1 = c0;
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const f64x2_t y = *reinterpret_cast<const f64x2_t*>(q + 32 * (i >> 3) + (i & 7));
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              c0 = __builtin_amdgcn_mfma_f64_16x16x4f64(positive(y[j]), hi(i + j), c0, 0, 0, 0);
-              c1 = __builtin_amdgcn_mfma_f64_16x16x4f64(negative(y[j]), lo(i + j), c1, 0, 0, 0);
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum[i] = c0[i] + c1[i];
-        }
-      } else {
-#pragma unroll 1
-        for (int r = 0; r < kTileRows; ++r) {
-          const double* const q = &s_q[buffer][r][8 * quad];
-          double y = 0.0;
-#pragma unroll 1
-          for (int i = 0; i < 32; ++i) {  // the bounds anew from memory: nothing is kept in registers for this path
-            const int d = 32 * (i >> 3) + (i & 7);
-            const uint16_t bound = q[d] >= 0.0 ? p.page_max[at + d] : p.page_min[at + d];
-            y = __builtin_fma(q[d], (double)to_float<kFp16>((short)bound), y);
-          }
-          y += __shfl_xor(y, 16);
-          y += __shfl_xor(y, 32);
-          if constexpr (kSmall) {
-            sum[0] = r == quad ? y : sum[0];
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] = r == 4 * quad + i ? y : sum[i];
-          }
-        }
-      }
-      // max over the heads of a block: rows of a lane, then of lanes, then of tiles
-#pragma unroll
-      for (int i = 0; i < (kSmall ? 1 : 4); ++i) {
-        const int row = row0 + (kSmall ? quad : 4 * quad + i);
-        const uint64_t key = (row & (padded - 1)) < group ? score_key(sum[i]) : 0;
-        best[i] = key > best[i] ? key : best[i];
+        for (int i = 0; i < 4; ++i) sum[i] = r == 4 * quad + i ? y : sum[i];
       }
     }
-    if ((t + 1) % tiles_per_block == 0 || tiles_per_block == 1) {
-      auto merge = [](uint64_t& y, uint64_t z) { y = z > y ? z : y; };
+    // max over the heads of a block: rows of a lane, then of lanes, then of tiles
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (((row0 + 4 * quad + i) & (padded - 1)) < group) keep_larger(best[i], score_key(sum[i]));
+    }
+    if ((t + 1) % tiles_per_block == 0) {
       int step = 1;  // rows that one key of a lane stands for
-      if constexpr (!kSmall) {
-        if (padded >= 2) {
-          merge(best[0], best[1]);
-          merge(best[2], best[3]);
-          step = 2;
-        }
-        if (padded >= 4) {
-          merge(best[0], best[2]);
-          step = 4;
-        }
-        if (padded >= 8) merge(best[0], __shfl_xor(best[0], 16));
-        if (padded >= 16) merge(best[0], __shfl_xor(best[0], 32));
-      } else {
-        if (padded >= 2) merge(best[0], __shfl_xor(best[0], 16));
-        if (padded >= 4) merge(best[0], __shfl_xor(best[0], 32));
+      if (padded >= 2) {
+        keep_larger(best[0], best[1]);
+        keep_larger(best[2], best[3]);
+        step = 2;
       }
-      const int block_row0 = (t / tiles_per_block) * tiles_per_block * kTileRows;
+      if (padded >= 4) {
+        keep_larger(best[0], best[2]);
+        step = 4;
+      }
+      if (padded >= 8) keep_larger(best[0], __shfl_xor(best[0], 16));
+      if (padded >= 16) keep_larger(best[0], __shfl_xor(best[0], 32));
+      const int block_row0 = (t / tiles_per_block) * tiles_per_block * 16;
 #pragma unroll
-      for (int i = 0; i < (kSmall ? 1 : 4); ++i) {
-        const int row = block_row0 + (kSmall ? quad : 4 * quad + i);
+      for (int i = 0; i < 4; ++i) {
+        const int row = block_row0 + 4 * quad + i;
         if (i % step == 0 && (row & (padded - 1)) == 0 && row < rows && page < pages) {
           p.scores[((int64_t)(slab_b * p.slab_blocks + row / padded) * p.kv_heads + kv_head) * p.table_cols + page] =
               there ? best[i] : 0;
@@ -559,18 +614,23 @@ hipError_t launch_select(const SelectParams& p, hipStream_t stream) {
   int padded = 1;
   while (padded < p.heads / p.kv_heads) padded *= 2;
   const int rows = p.slab_blocks * padded;
-  const unsigned chunks = (unsigned)((p.table_cols + 16 * kScoreWaves - 1) / (16 * kScoreWaves));
-  const unsigned heads = (unsigned)(p.requests * p.kv_heads);
-  if (rows <= 8 && padded <= 4) {
-    hipLaunchKernelGGL((score_kernel<kFp16, true>), dim3(chunks, heads, 1), dim3(kScoreThreads), 0, stream, p, padded);
+  const unsigned requests = (unsigned)p.requests, kv_heads = (unsigned)p.kv_heads;
+  if (rows <= 4) {
+    // Four tiles of pages a wave once that still gives every SIMD two waves.
+    const unsigned wide = (unsigned)((p.table_cols + 64 * kScoreWaves - 1) / (64 * kScoreWaves));
+    const int tiles = wide * kv_heads * requests >= 512 ? 4 : 1;
+    const unsigned chunks = (unsigned)((p.table_cols + 16 * tiles * kScoreWaves - 1) / (16 * tiles * kScoreWaves));
+    hipLaunchKernelGGL(score_few_kernel<kFp16>, dim3(chunks, kv_heads, requests), dim3(kScoreThreads), 0, stream, p,
+                       padded, tiles);
   } else {
-    // Row tiles are dealt over enough workgroups for three waves per SIMD: the
+    // Row tiles are dealt over enough workgroups for two waves per SIMD: the
     // bounds of a wave's pages are converted once per wave.
+    const unsigned chunks = (unsigned)((p.table_cols + 16 * kScoreWaves - 1) / (16 * kScoreWaves));
     const int units = (rows + (padded > 16 ? padded : 16) - 1) / (padded > 16 ? padded : 16);
-    const unsigned wanted = (768 + chunks * heads - 1) / (chunks * heads);
-    const unsigned split = wanted < (unsigned)units ? wanted : (unsigned)units;
-    hipLaunchKernelGGL((score_kernel<kFp16, false>), dim3(chunks, heads, split), dim3(kScoreThreads), 0, stream, p,
-                       padded);
+    int split_bits = 0;
+    while ((2 << split_bits) <= units && (chunks * kv_heads * requests << split_bits) < 512) ++split_bits;
+    hipLaunchKernelGGL(score_kernel<kFp16>, dim3(chunks, kv_heads << split_bits, requests), dim3(kScoreThreads), 0,
+                       stream, p, padded, split_bits);
   }
   const unsigned n = (unsigned)(row_blocks * p.kv_heads);
   if (p.table_cols <= kTopThreads) {
