@@ -3,12 +3,12 @@
 // lists and merge as in trianglemix_lists.h; groups of few rows run in
 // trianglemix_rows.hip.
 //
-// A workgroup is four waves of 32 rows each over the same K/V; two workgroups
-// share a CU, so that one's softmax, start-up and end run beside the other's
-// MFMAs.  Tiles are 32 keys (8 KB of K, 8 KB of V), DMA'd into three K and
-// three V slots (distinct objects: the compiler sees that the prefetch does
-// not alias the reads): K three tiles, V two tiles ahead of the tile in hand,
-// 64 KB in flight per CU.  Waves 0 and 1 load K, 2 and 3 load V.
+// A workgroup is four or eight waves of 32 rows each over the same K/V; two of
+// four waves or one of eight share a CU, so two waves of a SIMD run one's
+// softmax beside the other's MFMAs.  Tiles are 32 keys (8 KB of K, 8 KB of V),
+// DMA'd into NS K and NS V slots (distinct objects: the compiler sees that the
+// prefetch does not alias the reads): K NS tiles, V NS - 1 tiles ahead of the
+// tile in hand.  One half of the waves loads K, the other V.
 //
 // Software pipeline: iteration i issues the QK^T MFMAs of tile i + 1 between
 // the exponentials of tile i, then the PV MFMAs of tile i between the row max of
@@ -35,11 +35,10 @@
 namespace tmx {
 namespace {
 
-constexpr int kBlockWaves = kBlockRows / 32;
-constexpr int kBlockThreads = kBlockWaves * 64;
-constexpr int kDmaShare = kDmaPerTile / 2;  // two waves share a tile's DMA
-constexpr int kAhead = 3;                   // MFMA steps between an LDS operand read and its use
-static_assert(kBlockWaves == 4 && kPartialBytes == kBlockRows * (kHeadDim + 4) * 4, "the record of four waves");
+constexpr int kAhead = 3;  // MFMA steps between an LDS operand read and its use
+static_assert(kPartialBytes == 128 * (kHeadDim + 4) * 4, "the record of four waves");
+template <int J>
+struct Index { static constexpr int value = J; };
 
 __device__ __forceinline__ i16x8_t k_operand_of(const char* kt, const int* k_off, int c) {
   return __builtin_bit_cast(i16x8_t, k_operand(kt, k_off, c));
@@ -48,20 +47,51 @@ __device__ __forceinline__ i16x8_t v_operand_of(const char* vt, const int* v_off
   return __builtin_bit_cast(i16x8_t, v_operand(vt, v_off, k));
 }
 
-template <class Type, bool kTree>
-__global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(const RowsParams p) {
+template <class Type, int W, bool kTree>
+__global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsParams p) {
   typedef typename Type::elem elem;
+  constexpr int NS = W == 4 ? 3 : 6;  // slots; 64 KB (of two workgroups) or 80 KB in flight per CU
+  constexpr int kUnroll = 6;          // scores swap buffers every tile, slots turn every NS
+  constexpr int kBlockRows = 32 * W;
+  constexpr int kBlockThreads = 64 * W;
+  constexpr int kLoaders = W / 2;                   // waves that share the DMA of K, and of V
+  constexpr int kDmaShare = kDmaPerTile / kLoaders;
+  constexpr unsigned kRecordBytes = (unsigned)kPartialBytes * (W / 4);
+  static_assert((W == 4 || W == 8) && kUnroll % NS == 0 && kUnroll % 2 == 0, "supported shapes");
   __shared__ __attribute__((aligned(1024))) char k_lds0[kTileBytes];
   __shared__ __attribute__((aligned(1024))) char k_lds1[kTileBytes];
   __shared__ __attribute__((aligned(1024))) char k_lds2[kTileBytes];
+  __shared__ __attribute__((aligned(1024))) char k_lds3[NS > 3 ? kTileBytes : 16];
+  __shared__ __attribute__((aligned(1024))) char k_lds4[NS > 4 ? kTileBytes : 16];
+  __shared__ __attribute__((aligned(1024))) char k_lds5[NS > 5 ? kTileBytes : 16];
   __shared__ __attribute__((aligned(1024))) char v_lds0[kTileBytes];
   __shared__ __attribute__((aligned(1024))) char v_lds1[kTileBytes];
   __shared__ __attribute__((aligned(1024))) char v_lds2[kTileBytes];
+  __shared__ __attribute__((aligned(1024))) char v_lds3[NS > 3 ? kTileBytes : 16];
+  __shared__ __attribute__((aligned(1024))) char v_lds4[NS > 4 ? kTileBytes : 16];
+  __shared__ __attribute__((aligned(1024))) char v_lds5[NS > 5 ? kTileBytes : 16];
   __shared__ ListLds<kTree> lists;
   __shared__ int s_last;
+  // Slot j, named statically or picked (where nothing is prefetched beside the reads).
+  auto k_at = [&](auto j) -> char* {
+    constexpr int i = decltype(j)::value % NS;
+    return i == 0 ? k_lds0 : i == 1 ? k_lds1 : i == 2 ? k_lds2 : i == 3 ? k_lds3 : i == 4 ? k_lds4 : k_lds5;
+  };
+  auto v_at = [&](auto j) -> char* {
+    constexpr int i = decltype(j)::value % NS;
+    return i == 0 ? v_lds0 : i == 1 ? v_lds1 : i == 2 ? v_lds2 : i == 3 ? v_lds3 : i == 4 ? v_lds4 : v_lds5;
+  };
+  auto k_pick = [&](int i) -> char* {
+    if (NS > 3 && i >= 3) return i == 3 ? k_lds3 : i == 4 ? k_lds4 : k_lds5;
+    return i == 0 ? k_lds0 : i == 1 ? k_lds1 : k_lds2;
+  };
+  auto v_pick = [&](int i) -> char* {
+    if (NS > 3 && i >= 3) return i == 3 ? v_lds3 : i == 4 ? v_lds4 : v_lds5;
+    return i == 0 ? v_lds0 : i == 1 ? v_lds1 : v_lds2;
+  };
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const bool loads_k = wave < 2;
+  const bool loads_k = wave < kLoaders;
   const GroupDivider by_group(p.group);
   const int page_row_bytes = p.kv_heads * kRowBytes;
   const float c2 = p.scale_log2;
@@ -123,15 +153,19 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
     }
 
     // ---- page numbers: 64 pages a register, block b in the one of its parity ----
+    bool bad_pages = false;  // some page of those loaded is none of the cache
     auto load_pages = [&](int block) {
       const int i = 64 * block + lane;
       int phys = -1;
+      bool bad = false;
       if (i < list_pages) {
         int logical = i;
         if constexpr (!kTree) logical = in_lds ? lists.list[i] : entry;
         phys = p.block_table[g.request * p.table_stride + logical];
         if (phys >= p.num_pages) phys = -1;
+        if (phys < 0) bad = true;
       }
+      bad_pages |= __any(bad) != 0;
       return phys;
     };
     const int block0 = g.lo >> 6;
@@ -154,33 +188,32 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
     // ---- rows ----
     const int rows = min(kBlockRows, g.tokens * p.group - g.row_base);
     const bool active = 32 * wave < rows;
-    const int my_row = 32 * wave + n;
-    const int my_token = by_group.token(g.row_base + my_row);
-    const int my_head = g.row_base + my_row - my_token * p.group;
-    const bool my_ok = my_row < rows;
-    uint64_t my_mask = 0;
-    if constexpr (kTree) {
-      if (my_ok) my_mask = (uint64_t)p.tree_mask[g.row0 + my_token];
-    }
     i16x8_t q[8];
     {
-      const uint16_t* const src = p.query + (int64_t)(g.row0 + (my_ok ? my_token : 0)) * p.query_stride +
-                                  (int64_t)(g.kv_head * p.group + (my_ok ? my_head : 0)) * kHeadDim + 8 * half;
+      const int row = 32 * wave + n;
+      const int token = by_group.token(g.row_base + row);
+      const int head = g.row_base + row - token * p.group;
+      const bool ok = row < rows;
+      const uint16_t* const src = p.query + (int64_t)(g.row0 + (ok ? token : 0)) * p.query_stride +
+                                  (int64_t)(g.kv_head * p.group + (ok ? head : 0)) * kHeadDim + 8 * half;
 #pragma unroll
       for (int c = 0; c < 8; ++c) q[c] = *reinterpret_cast<const i16x8_t*>(src + 16 * c);
     }
     __builtin_amdgcn_sched_barrier(0);  // Q ahead of the tiles' DMA
 
-    // ---- DMA: this wave's half of a tile of K (waves 0, 1) or V (2, 3) ----
-    const int dma_row = 16 * (wave & 1) + (lane >> 4);
+    // ---- DMA: this wave's share of a tile of K or V ----
+    const int dma_row = 4 * kDmaShare * (wave % kLoaders) + (lane >> 4);
     int dma_chunk[kDmaShare];
 #pragma unroll
     for (int j = 0; j < kDmaShare; ++j) {
       const int row = dma_row + 4 * j;
       dma_chunk[j] = 16 * (loads_k ? k_slot(row, lane & 15) : v_slot(row, lane & 15));
     }
-    const char* const cache = loads_k ? p.key_cache : p.value_cache;
+    const char* const cache = (loads_k ? p.key_cache : p.value_cache) + g.kv_head * kRowBytes;
     const int64_t page_stride = loads_k ? p.key_page_stride : p.value_page_stride;
+    const int draft_rb = kTree ? (int)(loads_k ? p.draft_key_stride : p.draft_value_stride) : 0;
+    const char* const draft =
+        kTree ? (loads_k ? p.draft_key : p.draft_value) + (int64_t)g.row0 * draft_rb + g.kv_head * kRowBytes : nullptr;
     // Tile t of the list or tree; past the segment's end an empty range.
     auto source = [&](int t, int& rb) {
       const char* base;
@@ -188,21 +221,20 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
       int valid = t == list_tiles - 1 ? cut : kKvTile;
       if (kTree && t >= list_tiles) {
         const int at = (t - list_tiles) * kKvTile;
-        rb = (int)(loads_k ? p.draft_key_stride : p.draft_value_stride);
-        base = (loads_k ? p.draft_key : p.draft_value) + (int64_t)(g.row0 + at) * rb;
-        valid = g.tokens - at;
-        valid = min(valid, kKvTile);
+        rb = draft_rb;
+        base = draft + (int64_t)at * draft_rb;
+        valid = min(g.tokens - at, kKvTile);
       } else {
         const int phys = phys_of(t >> 2);
         base = cache + max(phys, 0) * page_stride + (t & 3) * (kKvTile * page_row_bytes);
         if (phys < 0) valid = 0;
       }
       if (t >= tiles_end) valid = 0;
-      return __builtin_amdgcn_make_buffer_rsrc((void*)(base + g.kv_head * kRowBytes), (short)0,
-                                               valid > 0 ? (valid - 1) * rb + kRowBytes : 0, kBufferFlags);
+      return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, valid > 0 ? (valid - 1) * rb + kRowBytes : 0,
+                                               kBufferFlags);
     };
     auto dma = [&](__amdgpu_buffer_rsrc_t rsrc, int rb, char* slot, int j) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, TM_LDS(slot + ((wave & 1) * kDmaShare + j) * 1024), 16,
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, TM_LDS(slot + ((wave % kLoaders) * kDmaShare + j) * 1024), 16,
                                                (unsigned)((dma_row + 4 * j) * rb + dma_chunk[j]), 0, 0, 0);
     };
     auto load_tile = [&](int t, char* slot) {
@@ -215,9 +247,19 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
       load_tile(t0, k_lds0);
       load_tile(t0 + 1, k_lds1);
       load_tile(t0 + 2, k_lds2);
+      if (NS > 3) {
+        load_tile(t0 + 3, k_lds3);
+        load_tile(t0 + 4, k_lds4);
+        load_tile(t0 + 5, k_lds5);
+      }
     } else {
       load_tile(t0, v_lds0);
       load_tile(t0 + 1, v_lds1);
+      if (NS > 3) {
+        load_tile(t0 + 2, v_lds2);
+        load_tile(t0 + 3, v_lds3);
+        load_tile(t0 + 4, v_lds4);
+      }
     }
 
     // ---- operand addresses in a slot ----
@@ -264,9 +306,9 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
     };
 
     // ---- the pipeline ----
-    const int fast = plain > 3 ? (plain - 1) / 3 * 3 : 0;
+    const int fast = max(plain - 1, 0);
     if (fast > 0) {
-      if (loads_k) wait_dma_but<2 * kDmaShare>();
+      if (loads_k) wait_dma_but<(NS - 1) * kDmaShare>();
       asm volatile("" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
@@ -274,22 +316,24 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
       float top = -INFINITY;
       if (active) {
         s_a = scores(k_lds0);
-        if (phys_of(t0 >> 2) < 0) s_a = f32x16_t{} - INFINITY;
+        if (bad_pages && phys_of(t0 >> 2) < 0) s_a = f32x16_t{} - INFINITY;
         top = row_top(s_a);
       }
-      // Iteration it: scores of tile it in s_cur, their row max in `top`.  K of
-      // it + 1 in kr, V of it in vr; K of it + 3 goes into kw, V of it + 2 into vw.
-      auto iteration = [&](int it, f32x16_t& s_cur, f32x16_t& s_nxt, const char* kr, const char* vr, char* kw,
-                           char* vw) {
-        wait_dma_but<kDmaShare>();  // K of it + 1, V of it have landed
+      // Iteration it, it % NS = j: scores of tile it in s_cur, their row max in
+      // `top`; K of it + NS and V of it + NS - 1 go into the slots just read.
+      auto iteration = [&](auto j, int it, f32x16_t& s_cur, f32x16_t& s_nxt) {
+        constexpr int J = decltype(j)::value;
+        const char* const kr = k_at(Index<J + 1>{});
+        const char* const vr = v_at(Index<J>{});
+        wait_dma_but<(NS - 2) * kDmaShare>();  // K of it + 1, V of it have landed
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();  // for every wave, and the slots kw, vw are read
+        __builtin_amdgcn_s_barrier();  // for every wave, and the slots that are filled next are read
         asm volatile("" ::: "memory");
-        const int t_load = t0 + it + (loads_k ? 3 : 2);
+        const int t_load = t0 + it + (loads_k ? NS : NS - 1);
         refill(t_load);
         int rb;
         const __amdgpu_buffer_rsrc_t src = source(t_load, rb);
-        char* const slot = loads_k ? kw : vw;
+        char* const slot = loads_k ? k_at(Index<J>{}) : v_at(Index<J + NS - 1>{});
         if (!active) {
 #pragma unroll
           for (int j = 0; j < kDmaShare; ++j) dma(src, rb, slot, j);
@@ -306,7 +350,7 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
         for (int k = 0; k < kAhead; ++k) kf[k] = k_operand_of(kr, k_off, k);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          if ((k & 1) == 0) dma(src, rb, slot, k >> 1);
+          if (k % (8 / kDmaShare) == 0) dma(src, rb, slot, k / (8 / kDmaShare));
           if (k + kAhead < 8) kf[k + kAhead] = k_operand_of(kr, k_off, k + kAhead);
           else va[k + kAhead - 8] = v_operand_of(vr, v_off, k + kAhead - 8);
           s_nxt = Type::mfma32(kf[k], q[k], k == 0 ? f32x16_t{} : s_nxt);
@@ -318,7 +362,9 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
 #pragma unroll
         for (int e = 0; e < 8; ++e) pb[0][e] = (elem)px[e];
         asm volatile("" ::"v"(pb[0]), "v"(px[8]), "v"(px[9]), "v"(px[10]), "v"(px[11]), "v"(sum));
-        if (phys_of((t0 + it + 1) >> 2) < 0) s_nxt = f32x16_t{} - INFINITY;  // a page without keys
+        if (__builtin_expect(bad_pages, 0)) {
+          if (phys_of((t0 + it + 1) >> 2) < 0) s_nxt = f32x16_t{} - INFINITY;  // a page without keys
+        }
         float next = -INFINITY;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -337,38 +383,46 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
         l_run += sum;
         top = half_max(next) * c2;
       };
-      // Scores swap buffers every tile and slots turn every three: six tiles a
-      // round, or three and a copy.
-      int it = 0;
-      for (; it + 3 < fast; it += 6) {
-        iteration(it, s_a, s_b, k_lds1, v_lds0, k_lds0, v_lds2);
-        iteration(it + 1, s_b, s_a, k_lds2, v_lds1, k_lds1, v_lds0);
-        iteration(it + 2, s_a, s_b, k_lds0, v_lds2, k_lds2, v_lds1);
-        iteration(it + 3, s_b, s_a, k_lds1, v_lds0, k_lds0, v_lds2);
-        iteration(it + 4, s_a, s_b, k_lds2, v_lds1, k_lds1, v_lds0);
-        iteration(it + 5, s_b, s_a, k_lds0, v_lds2, k_lds2, v_lds1);
-      }
-      if (it < fast) {
-        iteration(it, s_a, s_b, k_lds1, v_lds0, k_lds0, v_lds2);
-        iteration(it + 1, s_b, s_a, k_lds2, v_lds1, k_lds1, v_lds0);
-        iteration(it + 2, s_a, s_b, k_lds0, v_lds2, k_lds2, v_lds1);
+      for (int it = 0;;) {
+        iteration(Index<0>{}, it, s_a, s_b);
+        if (++it == fast) break;
+        iteration(Index<1>{}, it, s_b, s_a);
+        if (++it == fast) break;
+        iteration(Index<2>{}, it, s_a, s_b);
+        if (++it == fast) break;
+        iteration(Index<3>{}, it, s_b, s_a);
+        if (++it == fast) break;
+        iteration(Index<4>{}, it, s_a, s_b);
+        if (++it == fast) break;
+        iteration(Index<5>{}, it, s_b, s_a);
+        if (++it == fast) break;
       }
     }
 
-    // ---- the rest, with masks: K on its way up to tile it + 2, V up to it + 1 ----
+    // ---- the rest, with masks: K on its way up to tile it + NS - 1, V up to it + NS - 2 ----
+    int tail_lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(tail_lane));
+    const int my_row = 32 * wave + (tail_lane & 31);
+    const int my_token = by_group.token(g.row_base + my_row);
+    const bool my_ok = my_row < rows;
+    uint64_t my_mask = 0;
+    if constexpr (kTree) {
+      if (my_ok) my_mask = (uint64_t)p.tree_mask[g.row0 + my_token];
+    }
     for (int it = fast; it < tiles; ++it) {
       wait_dma();
       __syncthreads();
       const int t = t0 + it;
-      const int turn = it % 3;
+      const int turn = it % NS;
+      const int fill = turn == 0 ? NS - 1 : turn - 1;
       if (loads_k) {
-        if (it > fast) load_tile(t + 2, turn == 0 ? k_lds2 : turn == 1 ? k_lds0 : k_lds1);
+        if (it > fast) load_tile(t + NS - 1, k_pick(fill));
       } else {
-        load_tile(t + 2, turn == 0 ? v_lds2 : turn == 1 ? v_lds0 : v_lds1);
+        load_tile(t + NS - 1, v_pick(fill));
       }
       if (!active) continue;
-      const char* const ks = turn == 0 ? k_lds0 : turn == 1 ? k_lds1 : k_lds2;
-      const char* const vs = turn == 0 ? v_lds0 : turn == 1 ? v_lds1 : v_lds2;
+      const char* const ks = k_pick(turn);
+      const char* const vs = v_pick(turn);
       f32x16_t s = scores(ks);
       if (it >= plain || phys_of(t >> 2) < 0) {
         int thr = -1;  // the last key offset in the tile that the row attends
@@ -448,7 +502,7 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
     // Rows out: normalised and rounded, gathered in the wave's slot as whole
     // rows (8-byte pieces in, 16-byte chunks out, chunk c of row r at c ^ (r %
     // 16)), stored through L2 in whole cache lines.
-    char* const stage = wave == 0 ? k_lds0 : wave == 1 ? k_lds1 : wave == 2 ? k_lds2 : v_lds0;
+    char* const stage = wave < NS ? k_pick(wave) : v_pick(wave - NS);
     auto store_rows = [&](float l) {
       const float l_row = half_sum(l);
       const float inv = l_row > 0.0f ? 1.0f / l_row : 0.0f;
@@ -483,13 +537,13 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
       // ---- a group of several runs ----
       const Shared shared(g, plan.per_run);
       const __amdgpu_buffer_rsrc_t rec = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)p.partials, (short)0, (int)((unsigned)p.workgroups * 2u * (unsigned)kPartialBytes), kBufferFlags);
+          (void*)p.partials, (short)0, (int)((unsigned)p.workgroups * 2u * kRecordBytes), kBufferFlags);
       // record: O [wave][d-block, quarter][lane][4], then row maxima and lane sums [wave][lane]
       auto piece = [&](int i) { return (unsigned)(((wave * 16 + i) * 64 + lane) * 16); };
       const unsigned at_max = (unsigned)(kBlockRows * kHeadDim * 4 + (wave * 64 + lane) * 4);
       const unsigned at_sum = at_max + kBlockThreads * 4;
       if (active) {
-        const unsigned own = shared.record(run, (unsigned)kPartialBytes);
+        const unsigned own = shared.record(run, kRecordBytes);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const f32x4_t x = {o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2],
@@ -511,7 +565,7 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
           for (int j = 0; j < 2; ++j) {
             // past the last one its loads fall outside the buffer's range
             const unsigned from =
-                r + j <= shared.last_run ? shared.record(r + j, (unsigned)kPartialBytes) : kOutOfRange;
+                r + j <= shared.last_run ? shared.record(r + j, kRecordBytes) : kOutOfRange;
             mr[j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rec, from + at_max, 0, kCpolAgent));
             lr[j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rec, from + at_sum, 0, kCpolAgent));
 #pragma unroll
@@ -544,17 +598,23 @@ __global__ void __launch_bounds__(kBlockThreads, 2) blocks_attention_kernel(cons
 }
 
 template <class Type, bool kTree>
-hipError_t launch_type(const RowsParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL((blocks_attention_kernel<Type, kTree>), dim3((unsigned)p.workgroups), dim3(kBlockThreads), 0,
-                     stream, p);
+hipError_t launch_type(const RowsParams& p, int shape_rows, hipStream_t stream) {
+  const dim3 grid((unsigned)p.workgroups);
+  if (shape_rows == 128) {
+    hipLaunchKernelGGL((blocks_attention_kernel<Type, 4, kTree>), grid, dim3(256), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL((blocks_attention_kernel<Type, 8, kTree>), grid, dim3(512), 0, stream, p);
+  }
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_blocks_attention(const RowsParams& p, bool fp16, hipStream_t stream) {
-  if (p.selected == nullptr) return fp16 ? launch_type<Fp16, true>(p, stream) : launch_type<Bf16, true>(p, stream);
-  return fp16 ? launch_type<Fp16, false>(p, stream) : launch_type<Bf16, false>(p, stream);
+hipError_t launch_blocks_attention(const RowsParams& p, int shape_rows, bool fp16, hipStream_t stream) {
+  if (p.selected == nullptr) {
+    return fp16 ? launch_type<Fp16, true>(p, shape_rows, stream) : launch_type<Bf16, true>(p, shape_rows, stream);
+  }
+  return fp16 ? launch_type<Fp16, false>(p, shape_rows, stream) : launch_type<Bf16, false>(p, shape_rows, stream);
 }
 
 }  // namespace tmx

@@ -79,17 +79,17 @@ struct RowsParams {
   int total_units, per_run;  // selected pages: all units, and those of a workgroup
   float scale_log2;
 };
-// Groups of up to kRowShapes rows run in trianglemix_rows.hip, in the smallest
-// shape that holds them; larger ones in trianglemix_blocks.hip, kBlockRows rows
-// a workgroup.
-constexpr int kRowShapes[] = {16, 32, 64};
-constexpr int kBlockRows = 128;
+// Rows of one workgroup: groups of rows run in the smallest shape that holds
+// them, up to 64 rows in trianglemix_rows.hip, else in trianglemix_blocks.hip;
+// more rows than the largest in several workgroups.
+constexpr int kRowShapes[] = {16, 32, 64, 128, 256};
+constexpr int kMostStreamRows = 64;
 // A run of units leaves at most two partial records of this many bytes.
 constexpr int64_t rows_partial_bytes(int rows) {
-  return rows == kBlockRows ? kPartialBytes : int64_t(rows) * (kHeadDim + 2) * 4;
+  return rows > kMostStreamRows ? kPartialBytes * (rows / 128) : int64_t(rows) * (kHeadDim + 2) * 4;
 }
 hipError_t launch_rows_attention(const RowsParams& p, int shape_rows, bool fp16, hipStream_t stream);
-hipError_t launch_blocks_attention(const RowsParams& p, bool fp16, hipStream_t stream);
+hipError_t launch_blocks_attention(const RowsParams& p, int shape_rows, bool fp16, hipStream_t stream);
 
 // From trianglemix_capi.cpp: the calling thread's last error text (returns
 // status), and the arrival tag of a launch on this workspace.

@@ -184,7 +184,7 @@ int shape_for(int64_t rows) {
   for (int s : tmx::kRowShapes) {
     if (rows <= s) return s;
   }
-  return tmx::kBlockRows;
+  return tmx::kRowShapes[4];
 }
 
 struct RowsPlan {
@@ -198,7 +198,7 @@ RowsPlan rows_plan(int shape, int64_t units) {
   RowsPlan r;
   r.shape = shape;
   r.units = units;
-  const int64_t slots = kComputeUnits * (shape == tmx::kBlockRows ? 2 : 1);  // of its LDS a CU holds two, or one
+  const int64_t slots = kComputeUnits * (shape == 128 ? 2 : 1);  // that shape's LDS and registers let a CU hold two
   r.workgroups = (int)((std::min<int64_t>(slots, units) + 7) / 8 * 8);
   r.workspace_bytes = tmx::kCounterBytes + 2 * r.workgroups * tmx::rows_partial_bytes(r.shape);
   return r;
@@ -215,8 +215,8 @@ int check_units(int64_t units) {
 int launch_attention(const tmx::RowsParams& p, const RowsPlan& plan, int dtype, void* stream) {
   const bool fp16 = dtype == TM_FP16;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  return launched(plan.shape == tmx::kBlockRows ? tmx::launch_blocks_attention(p, fp16, s)
-                                                : tmx::launch_rows_attention(p, plan.shape, fp16, s));
+  return launched(plan.shape > tmx::kMostStreamRows ? tmx::launch_blocks_attention(p, plan.shape, fp16, s)
+                                                     : tmx::launch_rows_attention(p, plan.shape, fp16, s));
 }
 
 int check_selected(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t count) {

@@ -616,12 +616,11 @@ hipError_t launch_select(const SelectParams& p, hipStream_t stream) {
   const int rows = p.slab_blocks * padded;
   const unsigned requests = (unsigned)p.requests, kv_heads = (unsigned)p.kv_heads;
   if (rows <= 4) {
-    // Four tiles of pages a wave once that still gives every SIMD two waves.
+    // Two tiles of pages a wave once that still gives every SIMD four waves.
     // Chunks of pages last: workgroups go round the 8 XCDs, and the chunks past
-    // a request's length have no work (chunk first: 28 us instead of FEWUS for
-    // 32 requests of 16k to 131k tokens).
-    const unsigned wide = (unsigned)((p.table_cols + 64 * kScoreWaves - 1) / (64 * kScoreWaves));
-    const int tiles = wide * kv_heads * requests >= 512 ? 4 : 1;
+    // a request's length have no work.
+    const unsigned wide = (unsigned)((p.table_cols + 32 * kScoreWaves - 1) / (32 * kScoreWaves));
+    const int tiles = wide * kv_heads * requests >= 1024 ? 2 : 1;
     const unsigned chunks = (unsigned)((p.table_cols + 16 * tiles * kScoreWaves - 1) / (16 * tiles * kScoreWaves));
     hipLaunchKernelGGL(score_few_kernel<kFp16>, dim3(kv_heads, requests, chunks), dim3(kScoreThreads), 0, stream, p,
                        padded, tiles);
