@@ -40,11 +40,17 @@ static_assert(kPartialBytes == 128 * (kHeadDim + 4) * 4, "the record of four wav
 template <int J>
 struct Index { static constexpr int value = J; };
 
-__device__ __forceinline__ i16x8_t k_operand_of(const char* kt, const int* k_off, int c) {
-  return __builtin_bit_cast(i16x8_t, k_operand(kt, k_off, c));
+// Operand reads of a tile.  Swizzled addresses differ by an exclusive or alone:
+// one register holds them all.
+__device__ __forceinline__ i16x8_t k_operand_of(const char* kt, int k0, int c) {  // dims 16 c .. 16 c + 15
+  return *reinterpret_cast<const i16x8_t*>(kt + (k0 ^ (32 * c)));
 }
-__device__ __forceinline__ i16x8_t v_operand_of(const char* vt, const int* v_off, int k) {
-  return __builtin_bit_cast(i16x8_t, v_operand(vt, v_off, k));
+__device__ __forceinline__ i16x8_t v_operand_of(const char* vt, int v0, int k) {  // d-block k % 4, keys 16 (k / 4) ..
+  const char* const a = vt + 16 * (k >> 2) * kRowBytes + (v0 ^ (64 * (k & 3)));
+  const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)a);
+  const i16x4_t hi =
+      __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)(a + 8 * kRowBytes));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 template <class Type, int W, bool kTree>
@@ -109,11 +115,34 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     asm volatile("" : "+v"(lane));
     const int n = lane & 31, half = lane >> 5;
 
+    // What needs no page number is loaded first: the selection, then Q.
+    const int32_t* chosen = nullptr;
+    int entry = 0;
+    if constexpr (!kTree) {
+      chosen = selection_of(p, g);
+      entry = selection_entry(p, chosen);
+    }
+    // ---- rows ----
+    const int rows = min(kBlockRows, g.tokens * p.group - g.row_base);
+    const bool active = 32 * wave < rows;
+    i16x8_t q[8];
+    {
+      const int row = 32 * wave + n;
+      const int token = by_group.token(g.row_base + row);
+      const int head = g.row_base + row - token * p.group;
+      const bool ok = row < rows;
+      const uint16_t* const src = p.query + (int64_t)(g.row0 + (ok ? token : 0)) * p.query_stride +
+                                  (int64_t)(g.kv_head * p.group + (ok ? head : 0)) * kHeadDim + 8 * half;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) q[c] = *reinterpret_cast<const i16x8_t*>(src + 16 * c);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
     // ---- the tiles of the segment ----
     // Tile t < list_tiles is keys 32 (t % 4) .. of page t / 4 of the list; a
     // tree's own tiles follow.  All have 32 valid keys but the list's last,
     // which has `cut`, and the tree's last.
-    int entry = 0, list_pages;
+    int list_pages;
     bool in_lds = false;
     int list_tiles, cut, tiles_end;
     if constexpr (kTree) {
@@ -122,7 +151,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
       cut = g.context - (list_tiles - 1) * kKvTile;
       tiles_end = g.hi == g.units ? list_tiles + (g.tokens + kKvTile - 1) / kKvTile : 4 * g.hi;
     } else {
-      list_pages = selected_list<kBlockThreads>(p, lists, g, entry, in_lds);
+      list_pages = selected_list<kBlockThreads>(p, lists, g, chosen, entry, in_lds);
     }
     auto logical_of = [&](int i) {  // page i of the list, i uniform
       if constexpr (kTree) return i;
@@ -185,30 +214,13 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
       }
     };
 
-    // ---- rows ----
-    const int rows = min(kBlockRows, g.tokens * p.group - g.row_base);
-    const bool active = 32 * wave < rows;
-    i16x8_t q[8];
-    {
-      const int row = 32 * wave + n;
-      const int token = by_group.token(g.row_base + row);
-      const int head = g.row_base + row - token * p.group;
-      const bool ok = row < rows;
-      const uint16_t* const src = p.query + (int64_t)(g.row0 + (ok ? token : 0)) * p.query_stride +
-                                  (int64_t)(g.kv_head * p.group + (ok ? head : 0)) * kHeadDim + 8 * half;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) q[c] = *reinterpret_cast<const i16x8_t*>(src + 16 * c);
-    }
-    __builtin_amdgcn_sched_barrier(0);  // Q ahead of the tiles' DMA
-
     // ---- DMA: this wave's share of a tile of K or V ----
     const int dma_row = 4 * kDmaShare * (wave % kLoaders) + (lane >> 4);
-    int dma_chunk[kDmaShare];
-#pragma unroll
-    for (int j = 0; j < kDmaShare; ++j) {
-      const int row = dma_row + 4 * j;
-      dma_chunk[j] = 16 * (loads_k ? k_slot(row, lane & 15) : v_slot(row, lane & 15));
-    }
+    // Lane i of instruction j fills slot i % 16 of key row dma_row + 4 j, which
+    // holds chunk k_slot or v_slot of the row.
+    const int dma_chunk = 16 * (loads_k ? k_slot(dma_row, lane & 15) : v_slot(dma_row, lane & 15));
+    const int dma_turn = loads_k ? 64 : 0;
+    static_assert(kDmaShare <= 4, "the rows of a wave's instructions differ in bits 2 and 3");
     const char* const cache = (loads_k ? p.key_cache : p.value_cache) + g.kv_head * kRowBytes;
     const int64_t page_stride = loads_k ? p.key_page_stride : p.value_page_stride;
     const int draft_rb = kTree ? (int)(loads_k ? p.draft_key_stride : p.draft_value_stride) : 0;
@@ -235,7 +247,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     };
     auto dma = [&](__amdgpu_buffer_rsrc_t rsrc, int rb, char* slot, int j) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, TM_LDS(slot + ((wave % kLoaders) * kDmaShare + j) * 1024), 16,
-                                               (unsigned)((dma_row + 4 * j) * rb + dma_chunk[j]), 0, 0, 0);
+                                               (unsigned)((dma_row + 4 * j) * rb + (dma_chunk ^ (dma_turn * j))), 0, 0, 0);
     };
     auto load_tile = [&](int t, char* slot) {
       int rb;
@@ -263,15 +275,10 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     }
 
     // ---- operand addresses in a slot ----
-    int k_off[8], v_off[4];
-#pragma unroll
-    for (int c = 0; c < 8; ++c) k_off[c] = n * kRowBytes + 16 * k_slot(n, 2 * c + half);
+    int k_off = n * kRowBytes + 16 * k_slot(n, half);
     const int v_key = 4 * half + ((lane & 15) >> 2);
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      const int d = 32 * m + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-      v_off[m] = v_key * kRowBytes + 16 * v_slot(v_key, d >> 3) + 2 * (d & 7);
-    }
+    const int v_dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    int v_off = v_key * kRowBytes + 16 * v_slot(v_key, v_dim >> 3) + 2 * (v_dim & 7);
 
     float m_run = -INFINITY, l_run = 0.0f;  // of the row; the sum over this lane's keys
     f32x16_t o[4];
@@ -306,8 +313,9 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     };
 
     // ---- the pipeline ----
-    const int fast = max(plain - 1, 0);
-    if (fast > 0) {
+    // The first `plain` tiles; `next`: this wave's next tile to load.
+    int next = loads_k ? NS : NS - 1;
+    if (plain > 0) {
       if (loads_k) wait_dma_but<(NS - 1) * kDmaShare>();
       asm volatile("" ::: "memory");
       __builtin_amdgcn_s_barrier();
@@ -334,6 +342,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
         int rb;
         const __amdgpu_buffer_rsrc_t src = source(t_load, rb);
         char* const slot = loads_k ? k_at(Index<J>{}) : v_at(Index<J + NS - 1>{});
+        asm volatile("" : "+v"(k_off), "+v"(v_off));  // addresses are formed here, not held over the loop
         if (!active) {
 #pragma unroll
           for (int j = 0; j < kDmaShare; ++j) dma(src, rb, slot, j);
@@ -383,7 +392,8 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
         l_run += sum;
         top = half_max(next) * c2;
       };
-      for (int it = 0;;) {
+      const int fast = plain - 1;
+      for (int it = 0; it < fast;) {
         iteration(Index<0>{}, it, s_a, s_b);
         if (++it == fast) break;
         iteration(Index<1>{}, it, s_b, s_a);
@@ -395,11 +405,33 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
         iteration(Index<4>{}, it, s_a, s_b);
         if (++it == fast) break;
         iteration(Index<5>{}, it, s_b, s_a);
-        if (++it == fast) break;
+        ++it;
+      }
+      next += fast;
+      // The last of them: its scores are there, no tile of the pipeline follows.
+      wait_dma();
+      __syncthreads();
+      if (active) {
+        if (fast & 1) s_a = s_b;
+        const char* const vr = v_pick(fast % NS);
+        const float shift = raise(top);
+        typename Type::vec pb[2];
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s_a[e], c2, -shift));
+          sum += x;
+          pb[e >> 3][e & 7] = (elem)x;
+        }
+        l_run += sum;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          o[k & 3] = Type::mfma32(v_operand_of(vr, v_off, k), __builtin_bit_cast(i16x8_t, pb[k >> 2]), o[k & 3]);
+        }
       }
     }
 
-    // ---- the rest, with masks: K on its way up to tile it + NS - 1, V up to it + NS - 2 ----
+    // ---- the rest, with masks, one tile after the other ----
     int tail_lane = threadIdx.x & 63;
     asm volatile("" : "+v"(tail_lane));
     const int my_row = 32 * wave + (tail_lane & 31);
@@ -409,17 +441,13 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     if constexpr (kTree) {
       if (my_ok) my_mask = (uint64_t)p.tree_mask[g.row0 + my_token];
     }
-    for (int it = fast; it < tiles; ++it) {
+    for (int it = max(plain, 0); it < tiles; ++it) {
       wait_dma();
       __syncthreads();
       const int t = t0 + it;
       const int turn = it % NS;
-      const int fill = turn == 0 ? NS - 1 : turn - 1;
-      if (loads_k) {
-        if (it > fast) load_tile(t + NS - 1, k_pick(fill));
-      } else {
-        load_tile(t + NS - 1, v_pick(fill));
-      }
+      // the slots of the tiles before this one are free
+      for (; next < min(it + NS, tiles); ++next) load_tile(t0 + next, loads_k ? k_pick(next % NS) : v_pick(next % NS));
       if (!active) continue;
       const char* const ks = k_pick(turn);
       const char* const vs = v_pick(turn);

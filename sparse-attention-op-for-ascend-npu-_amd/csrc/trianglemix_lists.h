@@ -88,6 +88,7 @@ struct ListLds;
 template <>
 struct ListLds<true> {
   int units[kMaxBatch];  // running unit counts of the requests
+  int row0[kMaxBatch], tokens[kMaxBatch], context[kMaxBatch];  // their trees (tree_of)
   int64_t scan[16];      // wave totals
 };
 template <>
@@ -139,6 +140,9 @@ __device__ __forceinline__ Plan plan_units(const RowsParams& p, ListLds<kTree>& 
       if (b < p.batch) {
         int row0, tokens, context;
         tree_of(p, b, row0, tokens, context);
+        lds.row0[b] = row0;
+        lds.tokens[b] = tokens;
+        lds.context[b] = context;
         mine[i] = (int64_t)(p.kv_heads * ((tokens * p.group + kRows - 1) / kRows)) *
                   ((context + kPageSize - 1) / kPageSize + 1);
       }
@@ -182,7 +186,9 @@ __device__ __forceinline__ Segment find_segment(const RowsParams& p, const ListL
       }
     }
     g.request = lo;
-    tree_of(p, lo, g.row0, g.tokens, g.context);
+    g.row0 = __builtin_amdgcn_readfirstlane(lds.row0[lo]);
+    g.tokens = __builtin_amdgcn_readfirstlane(lds.tokens[lo]);
+    g.context = __builtin_amdgcn_readfirstlane(lds.context[lo]);
     g.units = (g.context + kPageSize - 1) / kPageSize + 1;
     const int row_parts = (g.tokens * p.group + kRows - 1) / kRows;
     const int before = lo > 0 ? __builtin_amdgcn_readfirstlane(lds.units[lo - 1]) : 0;
@@ -215,23 +221,29 @@ __device__ __forceinline__ Segment find_segment(const RowsParams& p, const ListL
   return g;
 }
 
+// A selection's list in memory, and its first 64 entries, one a lane: loaded
+// apart from their use, so that other loads can go along.
+__device__ __forceinline__ const int32_t* selection_of(const RowsParams& p, const Segment& g) {
+  const int blk = (g.row0 - g.request * p.rows) / kSelectRows;
+  return p.selected + (((int64_t)g.request * p.blocks + blk) * p.kv_heads + g.kv_head) * p.count;
+}
+__device__ __forceinline__ int selection_entry(const RowsParams& p, const int32_t* chosen) {
+  const int lane = threadIdx.x & 63;
+  return lane < p.count ? chosen[lane] : -1;
+}
+
 // The pages of a selection, ascending, each once: in `entry` (page i in lane i;
 // in_lds false) or in lds.list.  Returns how many.  Every thread of the
-// workgroup calls it.
+// workgroup calls it, with selection_entry in `entry`.
 template <int kThreads>
-__device__ __forceinline__ int selected_list(const RowsParams& p, ListLds<false>& lds, const Segment& g, int& entry,
-                                             bool& in_lds) {
+__device__ __forceinline__ int selected_list(const RowsParams& p, ListLds<false>& lds, const Segment& g,
+                                             const int32_t* chosen, int& entry, bool& in_lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int last = g.pos0 + g.tokens - 1;
   const int possible = last < 0 ? 0 : min(p.table_cols, last / kPageSize + 1);
-  const int blk = (g.row0 - g.request * p.rows) / kSelectRows;
-  const int32_t* const chosen =
-      p.selected + (((int64_t)g.request * p.blocks + blk) * p.kv_heads + g.kv_head) * p.count;
   in_lds = false;
-  entry = 0;
   if (p.count <= 64) {
     // As select_pages leaves it: ascending, what is no page of the block behind.
-    entry = lane < p.count ? chosen[lane] : -1;
     const bool ok = entry >= 0 && entry < possible;
     const int before = __shfl_up(ok ? entry : 0x7fffffff, 1);
     if (!__any(ok && lane > 0 && before >= entry)) {

@@ -104,27 +104,13 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
     const bool whole = g.lo == 0 && g.hi == g.units;
     const int valid_rows = min(kRows, g.tokens * G - g.row_base);  // may be <= 0 for a block's last row part
 
-    // ---- the pages: list index i -> logical page; physical page or -1 ----
-    const int32_t* const table = p.block_table + g.request * p.table_stride;
-    int list_len;  // pages of the list
-    bool in_lds = false;
+    // What needs no page number is loaded first: the selection, then Q.
+    const int32_t* chosen = nullptr;
     int entry = 0;
-    if constexpr (kTree) list_len = g.units - 1;
-    else list_len = selected_list<kThreads>(p, lists, g, entry, in_lds);
-    // Pages 64 t .. 64 t + 63 of the list, one a lane.
-    int logical64 = 0, phys64 = 0;
-    auto load_pages = [&](int t) {
-      const int i = 64 * t + lane;
-      if constexpr (kTree) {
-        logical64 = i;
-      } else {
-        logical64 = !in_lds ? entry : i < list_len ? lists.list[i] : 0;
-      }
-      phys64 = i < list_len ? table[logical64] : -1;
-      if (phys64 >= p.num_pages) phys64 = -1;
-    };
-    const int last_page = kTree ? g.hi : min(g.hi, list_len);  // pages g.lo .. last_page - 1 are read
-
+    if constexpr (!kTree) {
+      chosen = selection_of(p, g);
+      entry = selection_entry(p, chosen);
+    }
     // ---- Q ----
     i16x8_t q[NT][4];
     int row_pos[NT];  // selected pages: the row's position; trees: unused
@@ -150,6 +136,26 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
         q[n][c] = x;
       }
     }
+
+    // ---- the pages: list index i -> logical page; physical page or -1 ----
+    const int32_t* const table = p.block_table + g.request * p.table_stride;
+    int list_len;  // pages of the list
+    bool in_lds = false;
+    if constexpr (kTree) list_len = g.units - 1;
+    else list_len = selected_list<kThreads>(p, lists, g, chosen, entry, in_lds);
+    // Pages 64 t .. 64 t + 63 of the list, one a lane.
+    int logical64 = 0, phys64 = 0;
+    auto load_pages = [&](int t) {
+      const int i = 64 * t + lane;
+      if constexpr (kTree) {
+        logical64 = i;
+      } else {
+        logical64 = !in_lds ? entry : i < list_len ? lists.list[i] : 0;
+      }
+      phys64 = i < list_len ? table[logical64] : -1;
+      if (phys64 >= p.num_pages) phys64 = -1;
+    };
+    const int last_page = kTree ? g.hi : min(g.hi, list_len);  // pages g.lo .. last_page - 1 are read
 
     float m_run[NT], l_run[NT];
     f32x4_t o[8][NT];
