@@ -96,6 +96,15 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     return i == 0 ? v_lds0 : i == 1 ? v_lds1 : v_lds2;
   };
 
+  // Parameters that only a segment's ends need are read again there: held over
+  // the tile loop they would push its scalars into vector registers.
+  auto late = []() -> const RowsParams& {
+    typedef const __attribute__((address_space(4))) RowsParams* Kernarg;
+    Kernarg at = (Kernarg)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const RowsParams*)at;
+  };
+
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool loads_k = wave < kLoaders;
   const GroupDivider by_group(p.group);
@@ -190,8 +199,9 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
       if (i < list_pages) {
         int logical = i;
         if constexpr (!kTree) logical = in_lds ? lists.list[i] : entry;
-        phys = p.block_table[g.request * p.table_stride + logical];
-        if (phys >= p.num_pages) phys = -1;
+        const RowsParams& l = late();
+        phys = l.block_table[g.request * l.table_stride + logical];
+        if (phys >= l.num_pages) phys = -1;
         if (phys < 0) bad = true;
       }
       bad_pages |= __any(bad) != 0;
@@ -439,7 +449,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     const bool my_ok = my_row < rows;
     uint64_t my_mask = 0;
     if constexpr (kTree) {
-      if (my_ok) my_mask = (uint64_t)p.tree_mask[g.row0 + my_token];
+      if (my_ok) my_mask = (uint64_t)late().tree_mask[g.row0 + my_token];
     }
     for (int it = max(plain, 0); it < tiles; ++it) {
       wait_dma();
@@ -532,6 +542,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     // 16)), stored through L2 in whole cache lines.
     char* const stage = wave < NS ? k_pick(wave) : v_pick(wave - NS);
     auto store_rows = [&](float l) {
+      const RowsParams& q = late();
       const float l_row = half_sum(l);
       const float inv = l_row > 0.0f ? 1.0f / l_row : 0.0f;
       typedef elem elem4 __attribute__((ext_vector_type(4)));
@@ -552,9 +563,9 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
         const u32x4_t y = *reinterpret_cast<const u32x4_t*>(stage + r * kRowBytes + 16 * (c ^ (r & 15)));
         const int row = 32 * wave + r;
         const int t = by_group.token(g.row_base + row);
-        const int h = g.row_base + row - t * p.group;
+        const int h = g.row_base + row - t * q.group;
         if (row < rows && t >= g.held) {
-          *reinterpret_cast<u32x4_t*>(p.out + ((int64_t)(g.row0 + t) * p.heads + g.kv_head * p.group + h) * kHeadDim +
+          *reinterpret_cast<u32x4_t*>(q.out + ((int64_t)(g.row0 + t) * q.heads + g.kv_head * q.group + h) * kHeadDim +
                                       8 * c) = y;
         }
       }
@@ -565,7 +576,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
       // ---- a group of several runs ----
       const Shared shared(g, plan.per_run);
       const __amdgpu_buffer_rsrc_t rec = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)p.partials, (short)0, (int)((unsigned)p.workgroups * 2u * kRecordBytes), kBufferFlags);
+          (void*)late().partials, (short)0, (int)((unsigned)late().workgroups * 2u * kRecordBytes), kBufferFlags);
       // record: O [wave][d-block, quarter][lane][4], then row maxima and lane sums [wave][lane]
       auto piece = [&](int i) { return (unsigned)(((wave * 16 + i) * 64 + lane) * 16); };
       const unsigned at_max = (unsigned)(kBlockRows * kHeadDim * 4 + (wave * 64 + lane) * 4);
@@ -581,7 +592,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(m_run), rec, own + at_max, 0, kCpolAgent);
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l_run), rec, own + at_sum, 0, kCpolAgent);
       }
-      if (last_to_arrive(p, shared, &s_last) && active) {
+      if (last_to_arrive(late(), shared, &s_last) && active) {
         float top = -INFINITY, l = 0.0f;
 #pragma unroll
         for (int m = 0; m < 4; ++m) o[m] = f32x16_t{};
