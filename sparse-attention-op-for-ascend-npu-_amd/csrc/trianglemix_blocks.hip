@@ -56,8 +56,8 @@ __device__ __forceinline__ i16x8_t v_operand_of(const char* vt, int v0, int k) {
 template <class Type, int W, bool kTree>
 __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsParams p) {
   typedef typename Type::elem elem;
-  constexpr int NS = W == 4 ? 3 : 6;  // slots; 64 KB (of two workgroups) or 80 KB in flight per CU
-  constexpr int kUnroll = 6;          // scores swap buffers every tile, slots turn every NS
+  constexpr int NS = W == 4 ? 4 : 6;  // slots; 64 KB (of two workgroups) or 80 KB in flight per CU
+  constexpr int kUnroll = W == 4 ? 4 : 6;          // scores swap buffers every tile, slots turn every NS
   constexpr int kBlockRows = 32 * W;
   constexpr int kBlockThreads = 64 * W;
   constexpr int kLoaders = W / 2;                   // waves that share the DMA of K, and of V
@@ -269,16 +269,16 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
       load_tile(t0, k_lds0);
       load_tile(t0 + 1, k_lds1);
       load_tile(t0 + 2, k_lds2);
-      if (NS > 3) {
-        load_tile(t0 + 3, k_lds3);
+      if (NS > 3) load_tile(t0 + 3, k_lds3);
+      if (NS > 4) {
         load_tile(t0 + 4, k_lds4);
         load_tile(t0 + 5, k_lds5);
       }
     } else {
       load_tile(t0, v_lds0);
       load_tile(t0 + 1, v_lds1);
-      if (NS > 3) {
-        load_tile(t0 + 2, v_lds2);
+      if (NS > 3) load_tile(t0 + 2, v_lds2);
+      if (NS > 4) {
         load_tile(t0 + 3, v_lds3);
         load_tile(t0 + 4, v_lds4);
       }
@@ -412,10 +412,12 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
         if (++it == fast) break;
         iteration(Index<3>{}, it, s_b, s_a);
         if (++it == fast) break;
-        iteration(Index<4>{}, it, s_a, s_b);
-        if (++it == fast) break;
-        iteration(Index<5>{}, it, s_b, s_a);
-        ++it;
+        if constexpr (kUnroll == 6) {
+          iteration(Index<4>{}, it, s_a, s_b);
+          if (++it == fast) break;
+          iteration(Index<5>{}, it, s_b, s_a);
+          ++it;
+        }
       }
       next += fast;
       // The last of them: its scores are there, no tile of the pipeline follows.
@@ -493,13 +495,16 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
       }
       l_run += sum;
       i16x8_t va[8];
-      bool bad = false;
+      typedef unsigned short u16x8_t __attribute__((ext_vector_type(8)));
+      u16x8_t size = {};
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         va[k] = v_operand_of(vs, v_off, k);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) bad |= ((unsigned)va[k][e] & Type::kExp) == Type::kExp;
+        size = __builtin_elementwise_max(size, __builtin_bit_cast(u16x8_t, va[k] & (short)0x7fff));
       }
+      bool bad = false;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bad |= size[e] >= Type::kExp;
       if (__builtin_expect(!__any(bad), 1)) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) o[k & 3] = Type::mfma32(va[k], __builtin_bit_cast(i16x8_t, pb[k >> 2]), o[k & 3]);

@@ -88,7 +88,7 @@ struct ListLds;
 template <>
 struct ListLds<true> {
   int units[kMaxBatch];  // running unit counts of the requests
-  int row0[kMaxBatch], tokens[kMaxBatch], context[kMaxBatch];  // their trees (tree_of)
+  int row0[kMaxBatch], size[kMaxBatch];  // their trees (tree_of): first row, context * 128 + tokens
   int64_t scan[16];      // wave totals
 };
 template <>
@@ -99,6 +99,7 @@ struct ListLds<false> {
 };
 
 // A run of consecutive units of one group.
+static_assert(kMaxTreeNodes < 128 && (int64_t)kMaxTableCols * kPageSize * 128 < (int64_t(1) << 31), "a tree's size in 32 bits");
 struct Segment {
   int request, kv_head;
   int row0;       // first query row (token) of the group in query / out
@@ -141,8 +142,7 @@ __device__ __forceinline__ Plan plan_units(const RowsParams& p, ListLds<kTree>& 
         int row0, tokens, context;
         tree_of(p, b, row0, tokens, context);
         lds.row0[b] = row0;
-        lds.tokens[b] = tokens;
-        lds.context[b] = context;
+        lds.size[b] = context * 128 + tokens;
         mine[i] = (int64_t)(p.kv_heads * ((tokens * p.group + kRows - 1) / kRows)) *
                   ((context + kPageSize - 1) / kPageSize + 1);
       }
@@ -165,7 +165,9 @@ __device__ __forceinline__ Plan plan_units(const RowsParams& p, ListLds<kTree>& 
     }
     __syncthreads();
     const int total = __builtin_amdgcn_readfirstlane(lds.units[p.batch - 1]);
-    return Plan{total, max(1, (int)((unsigned)(total + p.workgroups - 1) / (unsigned)p.workgroups))};
+    const int usual = (int)((unsigned)total / (unsigned)(p.kv_heads * p.batch));  // units of a group of one row part
+    return Plan{total, max(min_run_units(usual, kRows),
+                           (int)((unsigned)(total + p.workgroups - 1) / (unsigned)p.workgroups))};
   } else {
     return Plan{p.total_units, p.per_run};
   }
@@ -187,8 +189,9 @@ __device__ __forceinline__ Segment find_segment(const RowsParams& p, const ListL
     }
     g.request = lo;
     g.row0 = __builtin_amdgcn_readfirstlane(lds.row0[lo]);
-    g.tokens = __builtin_amdgcn_readfirstlane(lds.tokens[lo]);
-    g.context = __builtin_amdgcn_readfirstlane(lds.context[lo]);
+    const int size = __builtin_amdgcn_readfirstlane(lds.size[lo]);
+    g.tokens = size & 127;
+    g.context = size >> 7;
     g.units = (g.context + kPageSize - 1) / kPageSize + 1;
     const int row_parts = (g.tokens * p.group + kRows - 1) / kRows;
     const int before = lo > 0 ? __builtin_amdgcn_readfirstlane(lds.units[lo - 1]) : 0;

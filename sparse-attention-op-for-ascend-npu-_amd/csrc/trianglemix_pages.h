@@ -80,13 +80,19 @@ struct RowsParams {
   float scale_log2;
 };
 // Rows of one workgroup: groups of rows run in the smallest shape that holds
-// them, up to 64 rows in trianglemix_rows.hip, else in trianglemix_blocks.hip;
+// them, up to 32 rows in trianglemix_rows.hip, else in trianglemix_blocks.hip;
 // more rows than the largest in several workgroups.
-constexpr int kRowShapes[] = {16, 32, 64, 128, 256};
-constexpr int kMostStreamRows = 64;
+constexpr int kRowShapes[] = {16, 32, 128, 256};
+constexpr int kMostStreamRows = 32;
 // A run of units leaves at most two partial records of this many bytes.
 constexpr int64_t rows_partial_bytes(int rows) {
   return rows > kMostStreamRows ? kPartialBytes * (rows / 128) : int64_t(rows) * (kHeadDim + 2) * 4;
+}
+// Fewest units of a run where a group has `units`: a small group is not split
+// (its partials and their merge cost more than reading three pages one after the
+// other), a run of the large shapes takes two.
+__host__ __device__ constexpr int min_run_units(int units, int rows) {
+  return units <= 3 ? (units < 1 ? 1 : units) : rows > kMostStreamRows ? 2 : 1;
 }
 hipError_t launch_rows_attention(const RowsParams& p, int shape_rows, bool fp16, hipStream_t stream);
 hipError_t launch_blocks_attention(const RowsParams& p, int shape_rows, bool fp16, hipStream_t stream);

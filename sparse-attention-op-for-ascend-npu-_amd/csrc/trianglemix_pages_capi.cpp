@@ -184,22 +184,23 @@ int shape_for(int64_t rows) {
   for (int s : tmx::kRowShapes) {
     if (rows <= s) return s;
   }
-  return tmx::kRowShapes[4];
+  return tmx::kRowShapes[3];
 }
 
 struct RowsPlan {
   int shape, workgroups;
-  int64_t units, workspace_bytes;
+  int64_t units, per_run, workspace_bytes;
 };
 
 // As many workgroups as the GPU holds at once, fewer when there are not as
 // many units (pages of groups of rows); a multiple of the 8 XCDs.
-RowsPlan rows_plan(int shape, int64_t units) {
+RowsPlan rows_plan(int shape, int64_t units, int64_t min_units) {
   RowsPlan r;
   r.shape = shape;
   r.units = units;
   const int64_t slots = kComputeUnits * (shape == 128 ? 2 : 1);  // that shape's LDS and registers let a CU hold two
-  r.workgroups = (int)((std::min<int64_t>(slots, units) + 7) / 8 * 8);
+  r.workgroups = (int)((std::min<int64_t>(slots, (units + min_units - 1) / min_units) + 7) / 8 * 8);
+  r.per_run = std::max(min_units, (units + r.workgroups - 1) / r.workgroups);
   r.workspace_bytes = tmx::kCounterBytes + 2 * r.workgroups * tmx::rows_partial_bytes(r.shape);
   return r;
 }
@@ -234,7 +235,8 @@ RowsPlan selected_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_he
   const int64_t group_rows = std::min<int64_t>(rows, tmx::kSelectRows) * (heads / kv_heads);
   const int shape = shape_for(group_rows);
   const int64_t blocks = (rows + tmx::kSelectRows - 1) / tmx::kSelectRows;
-  return rows_plan(shape, batch * blocks * kv_heads * ((group_rows + shape - 1) / shape) * count);
+  return rows_plan(shape, batch * blocks * kv_heads * ((group_rows + shape - 1) / shape) * count,
+                   tmx::min_run_units((int)count, shape));
 }
 
 int check_tree(int64_t total_rows, int64_t batch, int64_t heads, int64_t kv_heads, int64_t table_cols) {
@@ -244,14 +246,15 @@ int check_tree(int64_t total_rows, int64_t batch, int64_t heads, int64_t kv_head
   return st;
 }
 
-// The shape fits the average tree: larger trees of the batch take several
-// workgroups' rows.
+// The shape holds the trees that the batch's average lets expect: equal ones
+// where the rows divide evenly, else up to a third more than it.  A larger tree
+// takes several row parts, each reading the request's K/V again.
 RowsPlan tree_plan(int64_t total_rows, int64_t batch, int64_t heads, int64_t kv_heads, int64_t table_cols) {
   const int64_t group = heads / kv_heads;
-  const int64_t nodes = std::min<int64_t>((total_rows + batch - 1) / batch, tmx::kMaxTreeNodes);
-  const int shape = shape_for(nodes * group);
+  const int64_t expected = total_rows % batch == 0 ? total_rows / batch : (4 * total_rows + 3 * batch - 1) / (3 * batch);
+  const int shape = shape_for(std::min<int64_t>(expected, tmx::kMaxTreeNodes) * group);
   const int64_t groups = kv_heads * (batch + total_rows * group / shape);
-  return rows_plan(shape, groups * (table_cols + 1));
+  return rows_plan(shape, groups * (table_cols + 1), 1);  // the device deals the units that there are
 }
 
 }  // namespace
@@ -442,7 +445,7 @@ int tm_selected_page_attention(const void* query, int64_t query_stride, const vo
   p.count = (int)count;
   p.workgroups = plan.workgroups;
   p.total_units = (int)plan.units;
-  p.per_run = (int)((plan.units + plan.workgroups - 1) / plan.workgroups);
+  p.per_run = (int)plan.per_run;
   p.scale_log2 = scale * 1.4426950408889634f;
   return launch_attention(p, plan, dtype, stream);
 }

@@ -210,11 +210,15 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
       }
     };
 
-    const int v_key = 4 * quad + (col >> 2);
+    // Swizzled operand addresses differ by an exclusive or alone: K of dims 32 c ..
+    // at k_off ^ 64 c, V of dims 16 m .. at v_off ^ 32 m.
+    const int k_off = col * kRowBytes + 16 * k_slot(col, quad);
+    const int v_key = 4 * quad + (col >> 2), v_dim = 4 * (col & 3);
+    const int v_off = v_key * kRowBytes + 16 * v_slot(v_key, v_dim >> 3) + 2 * (v_dim & 7);
     const float c2 = p.scale_log2;
 
-    // One tile of 32 keys, the first at offset t32 of its page.  thr(n): the
-    // last key offset in the page that row n attends; draft: by mask bits.
+    // One tile of 32 keys, the first at offset t32 of its page.  thr[n]: the last
+    // key offset in the page that row n attends; draft: by mask bits too.
     auto tile = [&](const char* kt, const char* vt, int t32, bool draft, bool masked, const int* thr) {
       f32x4_t s[2][NT];
 #pragma unroll
@@ -223,8 +227,7 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
         for (int n = 0; n < NT; ++n) s[u][n] = f32x4_t{};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const int row = 16 * u + col;
-          const i16x8_t a = *reinterpret_cast<const i16x8_t*>(kt + row * kRowBytes + 16 * k_slot(row, 4 * c + quad));
+          const i16x8_t a = *reinterpret_cast<const i16x8_t*>(kt + 16 * u * kRowBytes + (k_off ^ (64 * c)));
 #pragma unroll
           for (int n = 0; n < NT; ++n) s[u][n] = Type::mfma16(a, q[n][c], s[u][n]);
         }
@@ -232,13 +235,15 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
       if (masked) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+          const int limit = thr[n] - t32 - 4 * quad;  // of 16 u + i
+          uint32_t bits = ~0u;
+          if (kTree && draft) bits = (uint32_t)(row_mask[n] >> (t32 & 63)) >> (4 * quad);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int key = t32 + 16 * u + 4 * quad + i;
-              bool seen = key <= thr[n];
-              if (kTree && draft) seen = seen && ((row_mask[n] >> (key & 63)) & 1) != 0;
+              bool seen = 16 * u + i <= limit;
+              if (kTree) seen = seen && (bits & (1u << (16 * u + i))) != 0;
               s[u][n][i] = seen ? s[u][n][i] : -INFINITY;
             }
           }
@@ -274,20 +279,18 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
         l_run[n] += add;
         pb[n] = __builtin_bit_cast(i16x8_t, pv);
       }
-      // V^T of dims 16 m .. 16 m + 15
-      auto v_at = [&](int m) {
-        const int d = 16 * m + 4 * (col & 3);
-        return v_operand16(vt, v_key * kRowBytes + 16 * v_slot(v_key, d >> 3) + 2 * (d & 7));
-      };
+      auto v_at = [&](int m) { return v_operand16(vt, v_off ^ (32 * m)); };  // V^T of dims 16 m .. 16 m + 15
       if (masked) {
-        bool bad = false;
+        typedef unsigned short u16x8_t __attribute__((ext_vector_type(8)));
+        u16x8_t size = {};
 #pragma unroll
         for (int m = 0; m < 8; ++m) {
-          const i16x8_t a = v_at(m);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) bad |= ((unsigned)a[e] & Type::kExp) == Type::kExp;
+          size = __builtin_elementwise_max(size, __builtin_bit_cast(u16x8_t, v_at(m) & (short)0x7fff));
         }
-        if (__any(bad)) {
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) bad |= size[e] >= Type::kExp;
+        if (__builtin_expect(__any(bad) != 0, 0)) {
           // The finite entries, then for each other kind an indicator's product:
           // it is positive in the rows that attend such an entry.
 #pragma unroll
@@ -584,7 +587,6 @@ hipError_t launch_shape(const RowsParams& p, int shape_rows, hipStream_t stream)
   switch (shape_rows) {
     case 16: hipLaunchKernelGGL((rows_attention_kernel<Type, 1, 1, 4, kTree>), grid, dim3(256), 0, stream, p); break;
     case 32: hipLaunchKernelGGL((rows_attention_kernel<Type, 2, 1, 4, kTree>), grid, dim3(256), 0, stream, p); break;
-    case 64: hipLaunchKernelGGL((rows_attention_kernel<Type, 2, 2, 4, kTree>), grid, dim3(512), 0, stream, p); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
