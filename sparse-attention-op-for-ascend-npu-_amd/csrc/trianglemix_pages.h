@@ -79,18 +79,19 @@ struct RowsParams {
   int total_units, per_run;  // selected pages: all units, and those of a workgroup
   float scale_log2;
 };
-// Rows of one workgroup: groups of rows run in the smallest shape that holds
-// them, up to 32 rows in trianglemix_rows.hip, else in trianglemix_blocks.hip;
-// more rows than the largest in several workgroups.
-constexpr int kRowShapes[] = {16, 32, 128, 256};
-constexpr int kMostStreamRows = 32;
+// Rows of one workgroup: groups of up to 32 rows run in trianglemix_rows.hip,
+// larger ones in trianglemix_blocks.hip, of more than 256 rows in several
+// workgroups.  Measured: 24 pages for each of 64 requests' 4 rows a KV head
+// 137 us with 16 rows, 152 with 256; a 28-row tree 9.4 with 32, 11.1 with 256.
+constexpr int kFewRows = 16, kMostStreamRows = 32, kHalfBlockRows = 128, kBlockRows = 256;
 // A run of units leaves at most two partial records of this many bytes.
 constexpr int64_t rows_partial_bytes(int rows) {
   return rows > kMostStreamRows ? kPartialBytes * (rows / 128) : int64_t(rows) * (kHeadDim + 2) * 4;
 }
-// Fewest units of a run where a group has `units`: a small group is not split
-// (its partials and their merge cost more than reading three pages one after the
-// other), a run of the large shapes takes two.
+// Fewest units of a run where a group has `units`: a small group is not split,
+// as its partials and their merge cost more than reading three pages one after the
+// other (a 7-node tree behind 77 tokens: 9.5 us in one run, 11.0 in two; 64
+// blocks of three pages each: 26.2 and 26.9); a run of the large shapes takes two.
 __host__ __device__ constexpr int min_run_units(int units, int rows) {
   return units <= 3 ? (units < 1 ? 1 : units) : rows > kMostStreamRows ? 2 : 1;
 }

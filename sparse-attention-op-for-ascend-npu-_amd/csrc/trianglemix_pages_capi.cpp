@@ -181,10 +181,7 @@ int check_select(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, i
 
 // Rows of the workgroup shape for groups of `rows` rows.
 int shape_for(int64_t rows) {
-  for (int s : tmx::kRowShapes) {
-    if (rows <= s) return s;
-  }
-  return tmx::kRowShapes[3];
+  return rows <= tmx::kFewRows ? tmx::kFewRows : rows <= tmx::kMostStreamRows ? tmx::kMostStreamRows : tmx::kBlockRows;
 }
 
 struct RowsPlan {
@@ -198,7 +195,7 @@ RowsPlan rows_plan(int shape, int64_t units, int64_t min_units) {
   RowsPlan r;
   r.shape = shape;
   r.units = units;
-  const int64_t slots = kComputeUnits * (shape == 128 ? 2 : 1);  // that shape's LDS and registers let a CU hold two
+  const int64_t slots = kComputeUnits * (shape == tmx::kHalfBlockRows ? 2 : 1);  // a CU holds two of that shape
   r.workgroups = (int)((std::min<int64_t>(slots, (units + min_units - 1) / min_units) + 7) / 8 * 8);
   r.per_run = std::max(min_units, (units + r.workgroups - 1) / r.workgroups);
   r.workspace_bytes = tmx::kCounterBytes + 2 * r.workgroups * tmx::rows_partial_bytes(r.shape);
@@ -233,8 +230,19 @@ int check_selected(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads,
 
 RowsPlan selected_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t count) {
   const int64_t group_rows = std::min<int64_t>(rows, tmx::kSelectRows) * (heads / kv_heads);
-  const int shape = shape_for(group_rows);
+  int shape = shape_for(group_rows);
   const int64_t blocks = (rows + tmx::kSelectRows - 1) / tmx::kSelectRows;
+  // Blocks of one request find each other's pages in the L2: with work enough
+  // they are bound by the MFMAs, and two workgroups of four waves a CU keep those
+  // busier than one of eight whose other waves have no rows.  Else memory
+  // bounds the call, and the eight waves' 80 KB in flight and half as many partials
+  // serve it better.  128 rows a group, 4 | 8 waves: 64 blocks x 32 pages of
+  // 131072 tokens 170 | 197 us, 64 x 8 of 8192 45 | 56, 32 x 16 of 8192 52 | 52,
+  // 16 x 16 of 8192 38 | 36, one block x 64 pages of each of 32 requests 224 | 216.
+  if (shape == tmx::kBlockRows && group_rows <= tmx::kHalfBlockRows && blocks > 1 &&
+      batch * blocks * kv_heads * count >= 4096) {
+    shape = tmx::kHalfBlockRows;
+  }
   return rows_plan(shape, batch * blocks * kv_heads * ((group_rows + shape - 1) / shape) * count,
                    tmx::min_run_units((int)count, shape));
 }
@@ -247,11 +255,13 @@ int check_tree(int64_t total_rows, int64_t batch, int64_t heads, int64_t kv_head
 }
 
 // The shape holds the trees that the batch's average lets expect: equal ones
-// where the rows divide evenly, else up to a third more than it.  A larger tree
-// takes several row parts, each reading the request's K/V again.
+// where the rows divide evenly, else up to a quarter more than it.  A larger tree
+// takes several row parts, each reading the request's K/V again: 32 trees of 5 to
+// 10 nodes (up to 40 rows a KV head) take 146 us in the shape for 256 rows, 151 in
+// parts of 32; of 4 to 8 nodes 207 and, in one part each, 194.
 RowsPlan tree_plan(int64_t total_rows, int64_t batch, int64_t heads, int64_t kv_heads, int64_t table_cols) {
   const int64_t group = heads / kv_heads;
-  const int64_t expected = total_rows % batch == 0 ? total_rows / batch : (4 * total_rows + 3 * batch - 1) / (3 * batch);
+  const int64_t expected = total_rows % batch == 0 ? total_rows / batch : (5 * total_rows + 4 * batch - 1) / (4 * batch);
   const int shape = shape_for(std::min<int64_t>(expected, tmx::kMaxTreeNodes) * group);
   const int64_t groups = kv_heads * (batch + total_rows * group / shape);
   return rows_plan(shape, groups * (table_cols + 1), 1);  // the device deals the units that there are

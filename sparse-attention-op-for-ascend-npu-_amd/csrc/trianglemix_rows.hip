@@ -4,12 +4,19 @@
 // Work, lists and merge as in trianglemix_lists.h; groups of more rows run in
 // trianglemix_blocks.hip.
 //
-// A workgroup is four waves = RW row parts x KW = 4 / RW key parts; a wave owns
-// 16 NT rows.  Each page goes HBM -> LDS by DMA, 32 KB of K and 32 KB of V, one
-// page ahead of the one being read (two K and two V slots, distinct objects,
-// so that the compiler sees that the prefetch does not alias the reads): 64 KB
-// in flight per CU.  With one row part each wave loads and reads its own 32
-// keys of every page and no barrier is needed; with more the page is shared.
+// A workgroup is four waves over the same 16 NT rows; wave w has keys 32 w ..
+// 32 w + 31 of every page.  Each page goes HBM -> LDS by DMA, 32 KB of K and
+// 32 KB of V, one page ahead of the one being read (two K and two V slots,
+// distinct objects, so that the compiler sees that the prefetch does not alias
+// the reads): 64 KB in flight per CU.  A wave loads what it reads itself, so
+// the page loop has no barrier; the waves' sums meet in LDS behind it.
+//
+// What bounds it: memory.  24 pages of each KV head for 64 requests of 2000 to
+// 16384 tokens (798 MB of K and V) take 137 us, 5.8 TB/s, where a library copy
+// of 2 GiB moves 4.9 (read and written).  One
+// request's few pages are bound by latency instead (8 us for 64 pages x 8 KV
+// heads: launch, lengths, selection, table, page, merge, each waiting for the
+// one before).
 //
 // Contractions (per wave, 32 keys x 16 rows, v_mfma_f32_16x16x32)
 //   S^T (keys x rows) = K Q^T     A = K rows from LDS, B = Q in registers
@@ -62,24 +69,22 @@ __device__ __forceinline__ i16x8_t v_operand16(const char* vt, int off) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// RW row parts x KW key parts, one wave each, of 16 NT rows.
-template <class Type, int NT, int RW, int KW, bool kTree>
-__global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel(const RowsParams p) {
-  constexpr int kWaves = RW * KW;
-  constexpr int kThreads = kWaves * 64;
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * 64;
+
+template <class Type, int NT, bool kTree>
+__global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsParams p) {
   constexpr int kWaveKeys = kPageSize / kWaves;  // keys of a page that a wave loads
   constexpr int kDma = kWaveKeys / 4;            // by this many 1 KB instructions each for K and V
-  constexpr int kWaveRows = 16 * NT;
-  static_assert(kWaves % 4 == 0 && kWaves * kWaveRows * kHeadDim * 4 <= 4 * kSlotBytes, "the waves' O fit the slots");
-  static_assert(RW > 1 || KW == 4, "without row parts a wave loads the 32 keys that it reads");
-  constexpr int kRows = kWaveRows * RW;
+  constexpr int kRows = 16 * NT;
+  static_assert(kWaves == 4 && kRows * kHeadDim * 4 <= kSlotBytes, "each wave's O fits a slot");
   typedef typename Type::elem elem;
 
   __shared__ __attribute__((aligned(1024))) char k_lds0[kSlotBytes];
   __shared__ __attribute__((aligned(1024))) char v_lds0[kSlotBytes];
   __shared__ __attribute__((aligned(1024))) char k_lds1[kSlotBytes];
   __shared__ __attribute__((aligned(1024))) char v_lds1[kSlotBytes];
-  __shared__ float s_max[kWaves][kWaveRows], s_sum[kWaves][kWaveRows];
+  __shared__ float s_max[kWaves][kRows], s_sum[kWaves][kRows];
   __shared__ ListLds<kTree> lists;
   __shared__ int s_last;
 
@@ -88,7 +93,6 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
   const int lane = tid & 63;
   const int col = lane & 15;   // row of the wave's 16-row tile
   const int quad = lane >> 4;
-  const int rw = wave % RW, kw = wave / RW;
   const int G = p.group;
 
   const GroupDivider by_group(p.group);
@@ -102,7 +106,7 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
   while (unit < unit_end) {
     const Segment g = find_segment<kTree, kRows>(p, lists, unit, unit_end);
     const bool whole = g.lo == 0 && g.hi == g.units;
-    const int valid_rows = min(kRows, g.tokens * G - g.row_base);  // may be <= 0 for a block's last row part
+    const int valid_rows = min(kRows, g.tokens * G - g.row_base);
 
     // What needs no page number is loaded first: the selection, then Q.
     const int32_t* chosen = nullptr;
@@ -117,7 +121,7 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
     uint64_t row_mask[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = rw * kWaveRows + 16 * n + col;
+      const int r = 16 * n + col;
       const int t = by_group.token(g.row_base + r);
       const int h = g.row_base + r - t * G;
       const bool ok = r < valid_rows;
@@ -355,16 +359,14 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
         }
       }
       const int tiles = min(4, (last_seen + 32) >> 5);  // tiles with an attended key
-      for (int t = kw; t < tiles; t += KW) {
-        tile(ks + t * kTileBytes, vs + t * kTileBytes, 32 * t, draft, 32 * t + 31 >= first_hidden, thr);
-      }
+      const int t = wave;
+      if (t < tiles) tile(ks + t * kTileBytes, vs + t * kTileBytes, 32 * t, draft, 32 * t + 31 >= first_hidden, thr);
     };
 
     // Page i in the slots (ka, va), page i + 1 on its way into (kb, vb).
     int table_block = g.lo >> 6;
     load_pages(table_block);
     auto step = [&](int i, char* ka, char* va, char* kb, char* vb) {
-      if constexpr (RW > 1) __syncthreads();  // every wave has read (kb, vb)
       if (i + 1 < last_page) {
         // the page numbers of page i + 1; page i's are needed below
         const int keep_phys = __builtin_amdgcn_readlane(phys64, i & 63);
@@ -385,15 +387,10 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
       } else {
         wait_dma();
       }
-      if constexpr (RW > 1) {
-        __syncthreads();
-      } else {
-        asm volatile("" ::: "memory");
-      }
+      asm volatile("" ::: "memory");
       page(i, ka, va);
     };
     if (g.lo < last_page) {
-      if constexpr (RW > 1) __syncthreads();
       issue(g.lo, k_lds0, v_lds0);
       int i = g.lo;
       for (; i + 1 < last_page; i += 2) {
@@ -403,14 +400,9 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
       if (i < last_page) step(i, k_lds0, v_lds0, k_lds1, v_lds1);
     }
 
-    // ---- the key parts' sums through LDS; each wave's O in its part of a slot ----
+    // ---- the waves' sums through LDS; each wave's O in a slot ----
     __syncthreads();
-    auto o_slot = [&](int w) {
-      constexpr int kPerSlot = kWaves / 4;
-      const int at = w / kPerSlot;
-      char* const slot = at == 0 ? k_lds0 : at == 1 ? v_lds0 : at == 2 ? k_lds1 : v_lds1;
-      return slot + (w % kPerSlot) * (kWaveRows * kHeadDim * 4);
-    };
+    auto o_slot = [&](int w) { return w == 0 ? k_lds0 : w == 1 ? v_lds0 : w == 2 ? k_lds1 : v_lds1; };
     char* const own = o_slot(wave);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -425,7 +417,7 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
     for (int n = 0; n < NT; ++n) {
       float top = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < KW; ++k) top = fmaxf(top, s_max[rw + RW * k][16 * n + col]);
+      for (int k = 0; k < kWaves; ++k) top = fmaxf(top, s_max[k][16 * n + col]);
       const float w = m_run[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - top);
       const int row = 16 * n + col;
 #pragma unroll
@@ -457,20 +449,19 @@ __global__ void __launch_bounds__(RW* KW * 64, RW* KW / 4) rows_attention_kernel
     const __amdgpu_buffer_rsrc_t rec = __builtin_amdgcn_make_buffer_rsrc(
         (void*)p.partials, (short)0, whole ? 0 : (int)((unsigned)p.workgroups * 2u * (kRecord * 4u)), kBufferFlags);
     for (int r = r0; r < valid_rows; r += kThreads / 16) {
-      const int rp = r / kWaveRows, row = r % kWaveRows;
       float top = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < KW; ++k) top = fmaxf(top, s_max[rp + RW * k][row]);
+      for (int k = 0; k < kWaves; ++k) top = fmaxf(top, s_max[k][r]);
       float l = 0.0f, acc[8] = {};
 #pragma unroll
-      for (int k = 0; k < KW; ++k) {
-        const float mk = s_max[rp + RW * k][row];
-        l += mk == -INFINITY ? 0.0f : s_sum[rp + RW * k][row] * __builtin_amdgcn_exp2f(mk - top);
-        const char* src = o_slot(rp + RW * k);
+      for (int k = 0; k < kWaves; ++k) {
+        const float mk = s_max[k][r];
+        l += mk == -INFINITY ? 0.0f : s_sum[k][r] * __builtin_amdgcn_exp2f(mk - top);
+        const char* src = o_slot(k);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const f32x4_t x = *reinterpret_cast<const f32x4_t*>(src + row * (kHeadDim * 4) +
-                                                              16 * ((2 * c8 + half) ^ (row & 15)));
+          const f32x4_t x = *reinterpret_cast<const f32x4_t*>(src + r * (kHeadDim * 4) +
+                                                              16 * ((2 * c8 + half) ^ (r & 15)));
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[4 * half + e] += x[e];
         }
@@ -585,8 +576,8 @@ template <class Type, bool kTree>
 hipError_t launch_shape(const RowsParams& p, int shape_rows, hipStream_t stream) {
   const dim3 grid((unsigned)p.workgroups);
   switch (shape_rows) {
-    case 16: hipLaunchKernelGGL((rows_attention_kernel<Type, 1, 1, 4, kTree>), grid, dim3(256), 0, stream, p); break;
-    case 32: hipLaunchKernelGGL((rows_attention_kernel<Type, 2, 1, 4, kTree>), grid, dim3(256), 0, stream, p); break;
+    case 16: hipLaunchKernelGGL((rows_attention_kernel<Type, 1, kTree>), grid, dim3(256), 0, stream, p); break;
+    case 32: hipLaunchKernelGGL((rows_attention_kernel<Type, 2, kTree>), grid, dim3(256), 0, stream, p); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();

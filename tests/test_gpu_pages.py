@@ -197,6 +197,9 @@ def check_attention(gpu, query, keys, values, table, lens, pages, query_d=None):
     ([1111], 70, 4, 2, 6),
     ([300], 300, 4, 1, 3),             # a whole prompt
     ([50, 10, 0], 64, 4, 1, 2),        # more rows than tokens
+    ([900], 260, 32, 8, 64),           # work enough for two workgroups a CU: 128 rows
+    ([700, 3, 1025, 40], 64, 24, 8, 64),  # 96 rows of 128
+    ([8300], 40, 8, 4, 1024),          # 64 rows, lists of 65 pages
 ])
 def test_attention(gpu, dtype, lens, rows, heads, kv_heads, count):
     print(f"attend {lens} {rows} {heads}/{kv_heads} {count} {dtype}", flush=True)
@@ -235,15 +238,18 @@ def test_long_lists(gpu, count, rows):
     check_attention(gpu, query, keys, values, table, lens, shuffled)
 
 
+@pytest.mark.parametrize("rows,count", [(20, 4), (64, 1024)])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
-def test_bad_pages_and_values_nobody_attends(gpu, dtype):
+def test_bad_pages_and_values_nobody_attends(gpu, dtype, rows, count):
     """Pages that are none, pages not chosen full of NaN, NaN and infinities at positions a row does not attend."""
-    lens, rows = [700, 450], 20
+    print(f"attend bad pages {rows} {count} {dtype}", flush=True)
+    lens = [700, 450]
     keys, values, table = make_cache(lens, 1, dtype, seed=21)
     pages = random_lists(lens, rows, 1, 4, seed=22)
+    pages = torch.cat([pages, torch.full((*pages.shape[:-1], count - 4), -1, dtype=torch.int32)], dim=-1)
     for b in range(2):
         for j in range(table.shape[1]):
-            if j not in pages[b, 0, 0].tolist() and table[b, j] >= 0:
+            if j not in pages[b].flatten().tolist() and table[b, j] >= 0:
                 keys[table[b, j].item()] = values[table[b, j].item()] = float("nan")
     # position 695: attended by the rows from 695 on alone
     page, slot = table[0, 695 // 128].item(), 695 % 128
@@ -261,7 +267,7 @@ def test_bad_pages_and_values_nobody_attends(gpu, dtype):
     finite = want.isfinite()
     assert torch.equal(got.isfinite(), finite)
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
-    assert (~finite).any() and finite[:15].all()
+    assert (~finite).any() and finite[:rows - 5].all()
     tol = tolerance(want, size, values[values.isfinite()], 512, dtype)
     assert bool(((got - want).abs() <= tol)[finite].all())
 
