@@ -23,7 +23,8 @@
  * Query head h reads KV head h / (heads / kv_heads), any group of 1 to 32.
  * Tokens past table_cols * 128 have no page and no keys.
  * Limits: 1024 requests, 16384 table columns, 256 heads, 2^21 query rows,
- * 1024 pages per selection, 64 nodes per tree, 2^22 cache pages.
+ * 1024 pages per selection, 64 nodes per tree, 2^22 cache pages, and 2^30 pages
+ * of attention work (pages per group, KV heads and groups of rows together).
  */
 #ifndef TRIANGLEMIX_PAGES_H
 #define TRIANGLEMIX_PAGES_H

@@ -16,6 +16,8 @@ Modules:
 * ``attention`` -- floating-point restatement of the reference's masked paged
   GQA attention: a float64 numpy version for small cases and a float32
   PyTorch CPU version (the reference's own oracle method) for larger ones.
+* ``pages``     -- key bounds of pages, page selection, attention over selected
+  pages and over draft trees, in 64 bits (no counterpart in the reference).
 
 Each function cites the reference file:line it restates.  How every function
 is pinned (reference known-answer tests, closed forms, brute force, library

@@ -9,9 +9,10 @@ Modules mirror the reference's plugin package ``vllm_ascend_trianglemix``:
 reasons), ``config``, ``stats`` (counters), ``native`` (library bootstrap),
 plus ``router`` (per-layer routing), ``vllm_rocm`` (the vLLM-ROCm seam:
 ``register`` patches vLLM v1's Triton attention backend), ``counters``
-(structured counter log and its run aggregator), ``cache`` (paged KV write), ``calibrate``
-(crossover gates), ``cabi`` (C ABI binding) and ``workload`` (seeded
-synthetic chunks, work accounting).
+(structured counter log and its run aggregator), ``cache`` (paged KV write),
+``pages`` (attention over selected pages), ``tree`` (attention of draft
+trees), ``calibrate`` (crossover gates), ``cabi`` (C ABI binding) and
+``workload`` (seeded synthetic chunks, work accounting).
 """
 
 from .kernel import (  # noqa: F401

@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in ``include/trianglemix.h``.
+"""ctypes binding of the C ABI in ``include/trianglemix.h`` and ``include/trianglemix_pages.h``.
 
 For callers that do not go through ``torch.ops`` (and for the parity tests,
 which exercise the C boundary directly).  Tensors are only used for their
@@ -74,7 +74,10 @@ _WORKSPACES: dict = {}
 
 
 def _workspace(query, query_start, seq_len, prompt_len, workspace, stream):
-    need = workspace_size(query.shape[0], query_start, seq_len, prompt_len)
+    return _workspace_of(query, workspace_size(query.shape[0], query_start, seq_len, prompt_len), workspace, stream)
+
+
+def _workspace_of(query, need, workspace, stream):
     if need == 0:
         return None, 0
     if workspace is None:
@@ -135,3 +138,72 @@ def reshape_and_cache(key, value, key_cache, value_cache, slot_mapping, *, strea
     _check(lib.tm_reshape_and_cache(
         key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), slot_mapping.data_ptr(),
         key.shape[0], key.stride(0), value.stride(0), key_cache.shape[0], st))
+
+
+def _dtype(tensor) -> int:
+    import torch
+
+    return {torch.bfloat16: 0, torch.float16: 1}.get(tensor.dtype, -1)  # TM_BF16, TM_FP16
+
+
+def _need(size, *geometry) -> int:
+    n = size(*geometry)
+    if n < 0:
+        raise TriangleMixError(TM_ERR_INVALID_ARGUMENT, load_hip_library().tm_last_error().decode())
+    return int(n)
+
+
+def update_page_bounds(key_cache, block_table, seq_lens, num_tokens: int, page_min, page_max, *, stream=None) -> None:
+    """``pages.update_page_bounds`` through the C ABI."""
+    lib = load_hip_library()
+    _check(lib.tm_update_page_bounds(
+        key_cache.data_ptr(), key_cache.stride(0), block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(),
+        num_tokens, page_min.data_ptr(), page_max.data_ptr(), block_table.shape[0], block_table.shape[1],
+        key_cache.shape[0], key_cache.shape[2], _dtype(key_cache), _stream(key_cache, stream)))
+
+
+def select_pages(query, page_min, page_max, block_table, seq_lens, out, *, sink_pages: int = 1, recent_pages: int = 1,
+                 stream=None, workspace=None) -> None:
+    """``pages.select_pages`` through the C ABI; ``out`` holds the count."""
+    lib = load_hip_library()
+    st = _stream(query, stream)
+    (batch, cols), heads, kv = block_table.shape, query.shape[1], page_min.shape[1]
+    rows = query.shape[0] // max(batch, 1)
+    need = _need(lib.tm_select_pages_workspace_size, batch, rows, heads, kv, cols)
+    ws_ptr, ws_bytes = _workspace_of(query, need, workspace, st)
+    _check(lib.tm_select_pages(
+        query.data_ptr(), query.stride(0), page_min.data_ptr(), page_max.data_ptr(), block_table.data_ptr(),
+        block_table.stride(0), seq_lens.data_ptr(), out.data_ptr(), batch, rows, heads, kv, cols, page_min.shape[0],
+        out.shape[-1], sink_pages, recent_pages, _dtype(query), ws_ptr, ws_bytes, st))
+
+
+def selected_page_attention(query, key_cache, value_cache, block_table, seq_lens, pages, out, *, scale: float,
+                            stream=None, workspace=None) -> None:
+    """``pages.selected_page_attention`` through the C ABI."""
+    lib = load_hip_library()
+    st = _stream(query, stream)
+    (batch, cols), heads, kv, count = block_table.shape, query.shape[1], key_cache.shape[2], pages.shape[-1]
+    rows = query.shape[0] // max(batch, 1)
+    need = _need(lib.tm_selected_page_attention_workspace_size, batch, rows, heads, kv, count)
+    ws_ptr, ws_bytes = _workspace_of(query, need, workspace, st)
+    _check(lib.tm_selected_page_attention(
+        query.data_ptr(), query.stride(0), key_cache.data_ptr(), key_cache.stride(0), value_cache.data_ptr(),
+        value_cache.stride(0), block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(), pages.data_ptr(),
+        out.data_ptr(), batch, rows, heads, kv, cols, key_cache.shape[0], count, float(scale), _dtype(query), ws_ptr,
+        ws_bytes, st))
+
+
+def tree_attention(query, key, value, key_cache, value_cache, block_table, context_lens, tree_offsets, tree_mask, out, *,
+                   scale: float, stream=None, workspace=None) -> None:
+    """``tree.tree_attention`` through the C ABI."""
+    lib = load_hip_library()
+    st = _stream(query, stream)
+    (batch, cols), (total, heads), kv = block_table.shape, query.shape[:2], key_cache.shape[2]
+    need = _need(lib.tm_tree_attention_workspace_size, total, batch, heads, kv, cols)
+    ws_ptr, ws_bytes = _workspace_of(query, need, workspace, st)
+    _check(lib.tm_tree_attention(
+        query.data_ptr(), query.stride(0), key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0),
+        key_cache.data_ptr(), key_cache.stride(0), value_cache.data_ptr(), value_cache.stride(0),
+        block_table.data_ptr(), block_table.stride(0), context_lens.data_ptr(), tree_offsets.data_ptr(),
+        tree_mask.data_ptr(), out.data_ptr(), total, batch, heads, kv, cols, key_cache.shape[0], float(scale),
+        _dtype(query), ws_ptr, ws_bytes, st))

@@ -84,6 +84,19 @@ def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
                                   ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int64)]
     lib.tm_reshape_and_cache.restype = ctypes.c_int
     lib.tm_reshape_and_cache.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, i64, vp]
+    i32, f32 = ctypes.c_int, ctypes.c_float
+    for name, args in {
+        "tm_update_page_bounds": [vp, i64, vp, i64, vp, i64, vp, vp, i64, i64, i64, i64, i32, vp],
+        "tm_select_pages": [vp, i64, vp, vp, vp, i64, vp, vp, *[i64] * 9, i32, vp, i64, vp],
+        "tm_selected_page_attention": [vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, *[i64] * 7, f32, i32, vp, i64, vp],
+        "tm_tree_attention": [vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, *[i64] * 6, f32, i32,
+                              vp, i64, vp],
+    }.items():
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name).argtypes = args
+    for name in ("tm_select_pages", "tm_selected_page_attention", "tm_tree_attention"):
+        size = getattr(lib, f"{name}_workspace_size")
+        size.restype, size.argtypes = i64, [i64] * 5
     del i32p
     return lib
 
