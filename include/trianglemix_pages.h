@@ -48,8 +48,9 @@ extern "C" {
  * last num_tokens tokens of a request's first seq_lens[b], over the page's
  * tokens below seq_lens[b], into page_min / page_max [num_pages, kv_heads, 128]
  * (contiguous, the keys' type, exact).  A NaN among the keys makes both bounds
- * of its dim NaN.  Other pages' bounds are left as they were.  Call it after
- * the tokens' K rows are in the cache.
+ * of its dim NaN.  Other pages' bounds are left as they were.  A length past
+ * the table counts as the table's.  Call it after the tokens' K rows are in the
+ * cache.
  */
 int tm_update_page_bounds(const void* key_cache, int64_t key_page_stride, const int32_t* block_table,
                           int64_t table_stride, const int32_t* seq_lens, int64_t num_tokens, void* page_min,

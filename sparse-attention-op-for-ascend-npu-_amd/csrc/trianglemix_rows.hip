@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
           for (int n = 0; n < NT; ++n) thr[n] = last_seen;
         } else {
           const int key0 = __builtin_amdgcn_readlane(logical64, i & 63) * kPageSize;
-          last_seen = bad ? -1 : g.pos0 + g.tokens - 1 - key0;
+          last_seen = bad ? -1 : min(g.pos0 + g.tokens - 1 - key0, kPageSize - 1);
           first_hidden = g.pos0 + 1 - key0;
 #pragma unroll
           for (int n = 0; n < NT; ++n) thr[n] = row_pos[n] - key0;

@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) score_few_kernel(const Selec
   // the wave's pages, one a lane; the length is not waited for
   int phys = page0 + lane < p.table_cols && lane < 16 * tiles ? p.block_table[b * p.table_stride + page0 + lane] : -1;
   if (phys >= p.num_pages) phys = -1;
-  const int seq = max(p.seq_lens[b], 0);
+  const int seq = min(max(p.seq_lens[b], 0), p.table_cols * kPageSize);
   {
     // one row a wave, two dims a lane
     const int blk = wave / padded, g = wave & (padded - 1), head = kv_head * group + g;
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) score_few_kernel(const Selec
   Bounds16 next = load_bounds(p, place(0));
   __syncthreads();
   const bool odd_rows = (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3]) != 0;
-  const int pages = min(p.table_cols, (seq + kPageSize - 1) / kPageSize);
+  const int pages = (seq + kPageSize - 1) / kPageSize;
   for (int t = 0; t < tiles; ++t) {
     if (page0 + 16 * t >= pages) return;
     Bounds16 x = next;
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPar
   const int group = p.heads / p.kv_heads;
   const int page = ((int)blockIdx.z * kScoreWaves + wave) * 16 + col;
   const int phys = page < p.table_cols ? p.block_table[b * p.table_stride + page] : -1;
-  const int seq = max(p.seq_lens[b], 0);
+  const int seq = min(max(p.seq_lens[b], 0), p.table_cols * kPageSize);
 
   const int rows = p.slab_blocks * padded;
   const int tiles_per_block = max(1, padded / 16);
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPar
   if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
   __syncthreads();
   put(0, x);
-  const int pages = min(p.table_cols, (seq + kPageSize - 1) / kPageSize);
+  const int pages = (seq + kPageSize - 1) / kPageSize;
   if ((int)blockIdx.z * kScoreWaves * 16 >= pages) return;
   const bool odd_page = odd_bounds<kFp16>(raw);
   double lo[32], hi[32];

@@ -340,6 +340,21 @@ def test_captured_and_replayed_with_other_lengths(gpu):
         assert (out[[i for i, n in enumerate(one) if n == 0]] == 3.0).all()
 
 
+@pytest.mark.parametrize("length", [10000, 2 ** 31 - 100, 2 ** 31 - 1])
+@pytest.mark.parametrize("rows,heads", [(1, 8), (1, 32), (3, 2), (33, 32)])
+def test_lengths_past_the_table(gpu, length, rows, heads):
+    """Positions behind every page: the table's pages whole, whatever the distance."""
+    print(f"pages past the table {length} {rows} {heads}", flush=True)
+    keys, values, table = make_cache([500, 128], 1, BF16, seed=61)
+    lens = ints([length, length - 7])
+    low, high = bounds_of(keys, table, [500, 128])
+    query = make_rows(2 * rows, heads, BF16, 62)
+    want = OP.select_pages(query, low, high, table, lens, 3, 1, 1)
+    got = TP.select_pages(query.to(gpu), low.to(gpu), high.to(gpu), table.to(gpu), lens.to(gpu), 3).cpu()
+    assert torch.equal(got, want) and (want[0] >= 0).all()
+    check_attention(gpu, query, keys, values, table, lens.tolist(), want)
+
+
 def test_calls_on_two_streams_at_once(gpu):
     print("pages two streams", flush=True)
     lens = [128 * 60]
