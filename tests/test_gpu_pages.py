@@ -373,3 +373,39 @@ def test_calls_on_two_streams_at_once(gpu):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, alone[i]) for o in outs[i])
+
+
+def test_two_graphs_replayed_at_once(gpu):
+    """Two captured calls, each with its own workspace, replayed side by side with eager calls on the capture stream."""
+    print("pages two graphs", flush=True)
+    lens = [128 * 60]
+    keys, values, table = make_cache(lens, 2, BF16, seed=71)
+    keys, values, table, lens = keys.to(gpu), values.to(gpu), table.to(gpu), ints(lens, gpu)
+    low, high = TP.page_bounds_like(keys)
+    TP.update_page_bounds(keys, table, lens, 128 * 60, low, high)
+    queries = [make_rows(rows, 8, BF16, 72 + rows).to(gpu) for rows in (1, 70)]
+
+    def step(query, out):
+        pages = TP.select_pages(query, low, high, table, lens, 40)
+        return TP.selected_page_attention(query, keys, values, table, lens, pages, SCALE, out=out)
+
+    want = [step(q, torch.zeros_like(q)) for q in queries]
+    outs = [torch.zeros_like(q) for q in queries]
+    graphs = []
+    for q, out in zip(queries, outs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            step(q, out)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for out in outs:
+            out.fill_(9.0)
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    graph.replay()
+        eager = step(queries[1], torch.zeros_like(queries[1]))
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[1])
+        assert all(torch.equal(out, w) for out, w in zip(outs, want))
