@@ -62,7 +62,8 @@ def chunk_plan(query_tokens: int, query_start: int, seq_len: int, prompt_len: in
     return parts.value, tiles.value, items.value
 
 
-# Split-KV workspace per (device, stream), at most MAX_WORKSPACE_BYTES.  Its
+# Split-KV workspace per (device, stream), at most MAX_WORKSPACE_BYTES (the
+# paged serving operators' may be 2.1 MiB larger).  Its
 # contents before a call do not matter (the library tags every arrival word
 # for its workspace), so a buffer is never cleared.  One buffer is kept per
 # (device, stream), allocated on that stream; a call that needs more replaces
