@@ -183,17 +183,18 @@ __device__ __forceinline__ bool odd_bounds(const Bounds16& x) {  // some bound o
   for (int e = 0; e < 8; ++e) odd |= most[e] >= (kFp16 ? 0x7c00 : 0x7f80);
   return __any(odd);
 }
-// The plain sum over a row of 128 (q: its dims from 8 quad on), in all four
-// lanes of a page.  The bounds come anew from memory: nothing is kept in
+// The plain sum over a row of 128 (plus and minus its parts, from 8 quad on), in
+// all four lanes of a page.  The bounds come anew from memory: nothing is kept in
 // registers for this path.
 template <bool kFp16>
-__device__ double plain_score(const SelectParams& p, int64_t at, const double* q) {
+__device__ double plain_score(const SelectParams& p, int64_t at, const double* plus, const double* minus) {
   double y = 0.0;
 #pragma unroll 1
   for (int i = 0; i < 32; ++i) {
     const int d = 32 * (i >> 3) + (i & 7);
-    const uint16_t bound = q[d] >= 0.0 ? p.page_max[at + d] : p.page_min[at + d];
-    y = __builtin_fma(q[d], (double)to_float<kFp16>((short)bound), y);
+    const double q = plus[d] + minus[d];
+    const uint16_t bound = q >= 0.0 ? p.page_max[at + d] : p.page_min[at + d];
+    y = __builtin_fma(q, (double)to_float<kFp16>((short)bound), y);
   }
   y += __shfl_xor(y, 16);
   y += __shfl_xor(y, 32);
@@ -205,11 +206,11 @@ __device__ double plain_score(const SelectParams& p, int64_t at, const double* q
 // `tiles` tiles of 16 pages, one tile's bounds ahead; what bounds it is reading
 // them and their conversion to 64 bits.
 template <bool kFp16>
-__global__ void __launch_bounds__(kScoreThreads, 4) score_few_kernel(const SelectParams p, int padded, int tiles) {
-  __shared__ __attribute__((aligned(16))) double s_q[4][kHeadDim + 2];
+__global__ void __launch_bounds__(kScoreThreads, 4) score_few_kernel(const SelectParams p, int padded_bits, int tiles) {
   __shared__ __attribute__((aligned(16))) double s_plus[4][kHeadDim + 2], s_minus[4][kHeadDim + 2];
   __shared__ int s_odd[kScoreWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int padded = 1 << padded_bits;
   const int col = lane & 15, quad = lane >> 4;
   const int kv_head = blockIdx.x, slab_b = blockIdx.y;
   const int b = p.request0 + slab_b;
@@ -221,7 +222,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) score_few_kernel(const Selec
   const int seq = min(max(p.seq_lens[b], 0), p.table_cols * kPageSize);
   {
     // one row a wave, two dims a lane
-    const int blk = wave / padded, g = wave & (padded - 1), head = kv_head * group + g;
+    const int blk = wave >> padded_bits, g = wave & (padded - 1), head = kv_head * group + g;
     f64x2_t x = {0.0, 0.0};
     if (blk < p.slab_blocks && g < group) {
       if (p.pooled) {
@@ -233,7 +234,6 @@ __global__ void __launch_bounds__(kScoreThreads, 4) score_few_kernel(const Selec
         x = f64x2_t{(double)to_float<kFp16>((short)two), (double)to_float<kFp16>((short)(two >> 16))};
       }
     }
-    *reinterpret_cast<f64x2_t*>(&s_q[wave][2 * lane]) = x;
     *reinterpret_cast<f64x2_t*>(&s_plus[wave][2 * lane]) = f64x2_t{positive(x[0]), positive(x[1])};
     *reinterpret_cast<f64x2_t*>(&s_minus[wave][2 * lane]) = f64x2_t{negative(x[0]), negative(x[1])};
     const bool odd = __any(odd_number(x[0]) || odd_number(x[1]));
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) score_few_kernel(const Selec
       sum = (c[0] + c[1]) + (c[2] + c[3]);
     } else {
       for (int r = 0; r < 4; ++r) {
-        const double y = plain_score<kFp16>(p, at, &s_q[r][8 * quad]);
+        const double y = plain_score<kFp16>(p, at, &s_plus[r][8 * quad], &s_minus[r][8 * quad]);
         sum = r == quad ? y : sum;
       }
     }
@@ -280,20 +280,23 @@ __global__ void __launch_bounds__(kScoreThreads, 4) score_few_kernel(const Selec
     if (padded >= 4) keep_larger(best, __shfl_xor(best, 32));
     const int page = page0 + 16 * t + col;
     if ((quad & (padded - 1)) == 0 && quad < p.slab_blocks * padded && page < pages) {
-      p.scores[((int64_t)(slab_b * p.slab_blocks + quad / padded) * p.kv_heads + kv_head) * p.table_cols + page] =
+      p.scores[((int64_t)(slab_b * p.slab_blocks + (quad >> padded_bits)) * p.kv_heads + kv_head) * p.table_cols + page] =
           __shfl(phys, 16 * t + col) >= 0 ? best : 0;
     }
   }
 }
 
-// Many rows: tiles of 16 rows, v_mfma_f64_16x16x4, two tiles' query sums in LDS.
-// A wave keeps the bounds of its 16 pages, converted, over all its row tiles.
+// Many rows: tiles of 16 rows, v_mfma_f64_16x16x4, two tiles' query sums in LDS,
+// q+ and q- apart: the loop over the products has no other instructions, which
+// would not run beside 64-bit MFMAs.  A wave keeps the bounds of its 16 pages,
+// converted, over all its row tiles.
 template <bool kFp16>
-__global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectParams p, int padded, int split_bits) {
+__global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectParams p, int padded_bits, int split_bits) {
   // rows of 128 and two doubles, so that 16 rows' reads meet different banks
-  __shared__ __attribute__((aligned(16))) double s_q[2][16][kHeadDim + 2];
+  __shared__ __attribute__((aligned(16))) double s_plus[2][16][kHeadDim + 2], s_minus[2][16][kHeadDim + 2];
   __shared__ int s_odd[2];  // some value of the tile is no finite number
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int padded = 1 << padded_bits;
   const int col = lane & 15, quad = lane >> 4;
   const int kv_head = (int)blockIdx.x >> split_bits, slab_b = blockIdx.y;
   const int b = p.request0 + slab_b;
@@ -303,14 +306,14 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPar
   const int seq = min(max(p.seq_lens[b], 0), p.table_cols * kPageSize);
 
   const int rows = p.slab_blocks * padded;
-  const int tiles_per_block = max(1, padded / 16);
+  const int tile_bits = max(0, padded_bits - 4), tiles_per_block = 1 << tile_bits;
   const int row_tiles = (rows + 15) / 16;
   // Two dims a thread of four of the tile's rows; zeros for rows of the padding.
   auto fetch = [&](int row0, f64x2_t* x) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int row = row0 + wave + 4 * j;
-      const int blk = row / padded, g = row & (padded - 1);
+      const int blk = row >> padded_bits, g = row & (padded - 1);
       x[j] = f64x2_t{0.0, 0.0};
       if (row < rows && g < group) {
         const int head = kv_head * group + g;
@@ -330,7 +333,8 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPar
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       odd |= odd_number(x[j][0]) || odd_number(x[j][1]);
-      *reinterpret_cast<f64x2_t*>(&s_q[buffer][wave + 4 * j][2 * lane]) = x[j];
+      *reinterpret_cast<f64x2_t*>(&s_plus[buffer][wave + 4 * j][2 * lane]) = f64x2_t{positive(x[j][0]), positive(x[j][1])};
+      *reinterpret_cast<f64x2_t*>(&s_minus[buffer][wave + 4 * j][2 * lane]) = f64x2_t{negative(x[j][0]), negative(x[j][1])};
     }
     if (odd) s_odd[buffer] = 1;
   };
@@ -358,7 +362,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPar
   uint64_t best[4] = {0, 0, 0, 0};
   for (int buffer = 0; t < row_tiles; buffer ^= 1) {
     __syncthreads();  // the tile is in its buffer, the other buffer is read
-    const int next = (t + 1) % tiles_per_block == 0 ? t + 1 - tiles_per_block + stride : t + 1;
+    const int next = ((t + 1) & (tiles_per_block - 1)) == 0 ? t + 1 - tiles_per_block + stride : t + 1;
     const bool more = next < row_tiles;
     if (more) fetch(next * 16, x);
     const int row0 = t * 16;
@@ -366,21 +370,23 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPar
     if (__builtin_expect(!odd_page && s_odd[buffer] == 0, 1)) {
       // Physical row r of the operand is row 4 (r % 4) + r / 4 of the tile, so
       // that a lane's four results are rows 4 quad .. 4 quad + 3.
-      const double* const q = &s_q[buffer][4 * (col & 3) + (col >> 2)][8 * quad];
+      const double* const plus = &s_plus[buffer][4 * (col & 3) + (col >> 2)][8 * quad];
+      const double* const minus = &s_minus[buffer][4 * (col & 3) + (col >> 2)][8 * quad];
       f64x4_t c0 = sum, c1 = sum;
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
-        const f64x2_t y = *reinterpret_cast<const f64x2_t*>(q + 32 * (i >> 3) + (i & 7));
+        const f64x2_t x = *reinterpret_cast<const f64x2_t*>(plus + 32 * (i >> 3) + (i & 7));
+        const f64x2_t y = *reinterpret_cast<const f64x2_t*>(minus + 32 * (i >> 3) + (i & 7));
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          c0 = __builtin_amdgcn_mfma_f64_16x16x4f64(positive(y[j]), hi[i + j], c0, 0, 0, 0);
-          c1 = __builtin_amdgcn_mfma_f64_16x16x4f64(negative(y[j]), lo[i + j], c1, 0, 0, 0);
+          c0 = __builtin_amdgcn_mfma_f64_16x16x4f64(x[j], hi[i + j], c0, 0, 0, 0);
+          c1 = __builtin_amdgcn_mfma_f64_16x16x4f64(y[j], lo[i + j], c1, 0, 0, 0);
         }
       }
       sum = c0 + c1;
     } else {
       for (int r = 0; r < 16; ++r) {
-        const double y = plain_score<kFp16>(p, at, &s_q[buffer][r][8 * quad]);
+        const double y = plain_score<kFp16>(p, at, &s_plus[buffer][r][8 * quad], &s_minus[buffer][r][8 * quad]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] = r == 4 * quad + i ? y : sum[i];
       }
@@ -390,7 +396,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPar
     for (int i = 0; i < 4; ++i) {
       if (((row0 + 4 * quad + i) & (padded - 1)) < group) keep_larger(best[i], score_key(sum[i]));
     }
-    if ((t + 1) % tiles_per_block == 0) {
+    if (((t + 1) & (tiles_per_block - 1)) == 0) {
       int step = 1;  // rows that one key of a lane stands for
       if (padded >= 2) {
         keep_larger(best[0], best[1]);
@@ -403,12 +409,12 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPar
       }
       if (padded >= 8) keep_larger(best[0], __shfl_xor(best[0], 16));
       if (padded >= 16) keep_larger(best[0], __shfl_xor(best[0], 32));
-      const int block_row0 = (t / tiles_per_block) * tiles_per_block * 16;
+      const int block_row0 = ((t >> tile_bits) << tile_bits) * 16;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = block_row0 + 4 * quad + i;
         if (i % step == 0 && (row & (padded - 1)) == 0 && row < rows && page < pages) {
-          p.scores[((int64_t)(slab_b * p.slab_blocks + row / padded) * p.kv_heads + kv_head) * p.table_cols + page] =
+          p.scores[((int64_t)(slab_b * p.slab_blocks + (row >> padded_bits)) * p.kv_heads + kv_head) * p.table_cols + page] =
               there ? best[i] : 0;
         }
         best[i] = 0;
@@ -611,8 +617,9 @@ hipError_t launch_select(const SelectParams& p, hipStream_t stream) {
     hipLaunchKernelGGL(pool_rows_kernel<kFp16>, dim3((unsigned)((n + kPoolColumns - 1) / kPoolColumns)),
                        dim3(kPoolThreads), 0, stream, p);
   }
-  int padded = 1;
-  while (padded < p.heads / p.kv_heads) padded *= 2;
+  int padded_bits = 0;
+  while ((1 << padded_bits) < p.heads / p.kv_heads) ++padded_bits;
+  const int padded = 1 << padded_bits;
   const int rows = p.slab_blocks * padded;
   const unsigned requests = (unsigned)p.requests, kv_heads = (unsigned)p.kv_heads;
   if (rows <= 4) {
@@ -623,7 +630,7 @@ hipError_t launch_select(const SelectParams& p, hipStream_t stream) {
     const int tiles = wide * kv_heads * requests >= 1024 ? 2 : 1;
     const unsigned chunks = (unsigned)((p.table_cols + 16 * tiles * kScoreWaves - 1) / (16 * tiles * kScoreWaves));
     hipLaunchKernelGGL(score_few_kernel<kFp16>, dim3(kv_heads, requests, chunks), dim3(kScoreThreads), 0, stream, p,
-                       padded, tiles);
+                       padded_bits, tiles);
   } else {
     // Row tiles are dealt over enough workgroups for two waves per SIMD: the
     // bounds of a wave's pages are converted once per wave.
@@ -632,7 +639,7 @@ hipError_t launch_select(const SelectParams& p, hipStream_t stream) {
     int split_bits = 0;
     while ((2 << split_bits) <= units && (chunks * kv_heads * requests << split_bits) < 512) ++split_bits;
     hipLaunchKernelGGL(score_kernel<kFp16>, dim3(kv_heads << split_bits, requests, chunks), dim3(kScoreThreads), 0,
-                       stream, p, padded, split_bits);
+                       stream, p, padded_bits, split_bits);
   }
   const unsigned n = (unsigned)(row_blocks * p.kv_heads);
   if (p.table_cols <= kTopThreads) {
