@@ -3,20 +3,23 @@
 // lists and merge as in trianglemix_lists.h; groups of few rows run in
 // trianglemix_rows.hip.
 //
-// A workgroup is four or eight waves of 32 rows each over the same K/V; two of
-// four waves or one of eight share a CU, so two waves of a SIMD run one's
-// softmax beside the other's MFMAs.  Tiles are 32 keys (8 KB of K, 8 KB of V),
-// DMA'd into NS K and NS V slots (distinct objects: the compiler sees that the
-// prefetch does not alias the reads): K NS tiles, V NS - 1 tiles ahead of the
-// tile in hand.  One half of the waves loads K, the other V.
+// A workgroup is W waves = W / KP row parts of 32 rows x KP key parts: eight row
+// parts for groups of more than 128 rows, four row parts x two key parts for
+// smaller ones, or two workgroups of four row parts a CU (when which: the plans
+// in trianglemix_pages_capi.cpp).  So a SIMD has two waves, and runs one's softmax
+// beside the other's MFMAs.  The loop goes in steps of 32 KP keys, a wave taking
+// the 32 of its key part (8 KB of K, 8 KB of V), DMA'd into NS K and NS V slots
+// (distinct objects: the compiler sees that the prefetch does not alias the
+// reads): K NS steps, V NS - 1 steps ahead of the one in hand.  One half of the
+// waves loads K, the other V.  Key parts join through LDS behind the loop.
 //
-// Software pipeline: iteration i issues the QK^T MFMAs of tile i + 1 between
-// the exponentials of tile i, then the PV MFMAs of tile i between the row max of
-// tile i + 1.  Only tiles that every row attends whole run there: lists are
-// ascending, so the tiles that need a mask (the keys at and after the block's
+// Software pipeline: iteration i issues the QK^T MFMAs of step i + 1 between
+// the exponentials of step i, then the PV MFMAs of step i between the row max of
+// step i + 1.  Only steps that every row attends whole run there: lists are
+// ascending, so the steps that need a mask (the keys at and after the block's
 // first row, the end of a tree's context, the tree itself) are the last ones,
-// and run one after the other in a plain loop behind it, with what the pipeline leaves
-// over.  There V entries that are not finite are kept out of the product and
+// and run one after the other in a plain loop behind it, with what the pipeline
+// leaves over.  There V entries that are not finite are kept out of the product and
 // added only to rows that attend them, so that what a row does not attend
 // cannot reach it.
 //
@@ -29,9 +32,9 @@
 // What bounds it: with pages that the L2 holds the MFMAs and the exponentials
 // beside them, 975 to 1000 TFLOP/s over 2048 rows x 128 pages, where a bf16
 // library product of 8192^3 reaches 1377; with pages read once, memory: 32 trees
-// of up to 32 nodes over 8000 tokens each take 200 us, 5.3 TB/s.  Short lists
-// pay for the start (lengths, selection, Q and table before the first tile, 7
-// us) and the partials of split groups: 512 rows x 16 pages take 36 us.
+// of up to 32 nodes over 8000 tokens each take 192 us, 5.5 TB/s.  Short lists
+// pay for the start (lengths, selection, Q and table before the first step, 7
+// us) and the partials of split groups: 512 rows x 16 pages take 34 us.
 
 #include <hip/hip_runtime.h>
 
@@ -60,29 +63,34 @@ __device__ __forceinline__ i16x8_t v_operand_of(const char* vt, int v0, int k) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-template <class Type, int W, bool kTree>
+// W waves: W / KP row parts of 32 rows x KP key parts.
+template <class Type, int W, int KP, bool kTree>
 __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsParams p) {
   typedef typename Type::elem elem;
-  constexpr int NS = W == 4 ? 4 : 6;  // slots; 64 KB (of two workgroups) or 80 KB in flight per CU
-  constexpr int kUnroll = W == 4 ? 4 : 6;          // scores swap buffers every tile, slots turn every NS
-  constexpr int kGroupRows = 32 * W;
+  constexpr int kRowParts = W / KP;
+  constexpr int NS = W == 4 ? 4 : 6 / KP;  // slots of a step; 64 KB (of two workgroups) or 80 KB in flight per CU
+  constexpr int kUnroll = W == 4 ? 4 : 6;  // scores swap buffers every step, slots turn every NS
+  constexpr int kStep = KP * kKvTile;  // keys of a step
+  constexpr int kSteps = kPageSize / kStep;  // steps of a page
+  constexpr int kStepBytes = KP * kTileBytes;
+  constexpr int kGroupRows = 32 * kRowParts;
   constexpr int kBlockThreads = 64 * W;
   constexpr int kLoaders = W / 2;                   // waves that share the DMA of K, and of V
-  constexpr int kDmaShare = kDmaPerTile / kLoaders;
-  constexpr unsigned kRecordBytes = (unsigned)kPartialBytes * (W / 4);
-  static_assert((W == 4 || W == 8) && kUnroll % NS == 0 && kUnroll % 2 == 0, "supported shapes");
-  __shared__ __attribute__((aligned(1024))) char k_lds0[kTileBytes];
-  __shared__ __attribute__((aligned(1024))) char k_lds1[kTileBytes];
-  __shared__ __attribute__((aligned(1024))) char k_lds2[kTileBytes];
-  __shared__ __attribute__((aligned(1024))) char k_lds3[NS > 3 ? kTileBytes : 16];
-  __shared__ __attribute__((aligned(1024))) char k_lds4[NS > 4 ? kTileBytes : 16];
-  __shared__ __attribute__((aligned(1024))) char k_lds5[NS > 5 ? kTileBytes : 16];
-  __shared__ __attribute__((aligned(1024))) char v_lds0[kTileBytes];
-  __shared__ __attribute__((aligned(1024))) char v_lds1[kTileBytes];
-  __shared__ __attribute__((aligned(1024))) char v_lds2[kTileBytes];
-  __shared__ __attribute__((aligned(1024))) char v_lds3[NS > 3 ? kTileBytes : 16];
-  __shared__ __attribute__((aligned(1024))) char v_lds4[NS > 4 ? kTileBytes : 16];
-  __shared__ __attribute__((aligned(1024))) char v_lds5[NS > 5 ? kTileBytes : 16];
+  constexpr int kDmaShare = KP * kDmaPerTile / kLoaders;
+  constexpr unsigned kRecordBytes = (unsigned)kPartialBytes * (kRowParts / 4);
+  static_assert((W == 8 || W == 4) && (KP == 1 || (KP == 2 && W == 8)) && kUnroll % NS == 0 && kUnroll % 2 == 0, "supported shapes");
+  __shared__ __attribute__((aligned(1024))) char k_lds0[kStepBytes];
+  __shared__ __attribute__((aligned(1024))) char k_lds1[kStepBytes];
+  __shared__ __attribute__((aligned(1024))) char k_lds2[kStepBytes];
+  __shared__ __attribute__((aligned(1024))) char k_lds3[NS > 3 ? kStepBytes : 16];
+  __shared__ __attribute__((aligned(1024))) char k_lds4[NS > 4 ? kStepBytes : 16];
+  __shared__ __attribute__((aligned(1024))) char k_lds5[NS > 5 ? kStepBytes : 16];
+  __shared__ __attribute__((aligned(1024))) char v_lds0[kStepBytes];
+  __shared__ __attribute__((aligned(1024))) char v_lds1[kStepBytes];
+  __shared__ __attribute__((aligned(1024))) char v_lds2[kStepBytes];
+  __shared__ __attribute__((aligned(1024))) char v_lds3[NS > 3 ? kStepBytes : 16];
+  __shared__ __attribute__((aligned(1024))) char v_lds4[NS > 4 ? kStepBytes : 16];
+  __shared__ __attribute__((aligned(1024))) char v_lds5[NS > 5 ? kStepBytes : 16];
   __shared__ ListLds<kTree> lists;
   __shared__ int s_last;
   // Slot j, named statically or picked (where nothing is prefetched beside the reads).
@@ -113,6 +121,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
   };
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row_part = wave % kRowParts, key_part = wave / kRowParts;
   const bool loads_k = wave < kLoaders;
   const GroupDivider by_group(p.group);
   const int page_row_bytes = p.kv_heads * kRowBytes;
@@ -140,10 +149,10 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     }
     // ---- rows ----
     const int rows = min(kGroupRows, g.tokens * p.group - g.row_base);
-    const bool active = 32 * wave < rows;
+    const bool active = 32 * row_part < rows;
     i16x8_t q[8];
     {
-      const int row = 32 * wave + n;
+      const int row = 32 * row_part + n;
       const int token = by_group.token(g.row_base + row);
       const int head = g.row_base + row - token * p.group;
       const bool ok = row < rows;
@@ -154,18 +163,18 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     }
     __builtin_amdgcn_sched_barrier(0);
 
-    // ---- the tiles of the segment ----
-    // Tile t < list_tiles is keys 32 (t % 4) .. of page t / 4 of the list; a
-    // tree's own tiles follow.  All have 32 valid keys but the list's last,
-    // which has `cut`, and the tree's last.
+    // ---- the steps of the segment ----
+    // Step t < list_tiles is keys kStep (t % kSteps) .. of page t / kSteps of the
+    // list; a tree's own steps follow.  All have kStep valid keys but the list's
+    // last, which has `cut`, and the tree's last.
     int list_pages;
     bool in_lds = false;
     int list_tiles, cut, tiles_end;
     if constexpr (kTree) {
       list_pages = g.units - 1;
-      list_tiles = (g.context + kKvTile - 1) / kKvTile;
-      cut = g.context - (list_tiles - 1) * kKvTile;
-      tiles_end = g.hi == g.units ? list_tiles + (g.tokens + kKvTile - 1) / kKvTile : 4 * g.hi;
+      list_tiles = (g.context + kStep - 1) / kStep;
+      cut = g.context - (list_tiles - 1) * kStep;
+      tiles_end = g.hi == g.units ? list_tiles + (g.tokens + kStep - 1) / kStep : kSteps * g.hi;
     } else {
       list_pages = selected_list<kBlockThreads>(p, lists, g, chosen, entry, in_lds);
     }
@@ -176,23 +185,23 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     if constexpr (!kTree) {
       const int end = g.pos0 + g.tokens;  // behind the block's last row
       const int held = list_pages > 0 ? min(kPageSize, end - logical_of(list_pages - 1) * kPageSize) : 0;
-      list_tiles = list_pages > 0 ? 4 * (list_pages - 1) + (held + kKvTile - 1) / kKvTile : 0;
-      cut = held - (held - 1) / kKvTile * kKvTile;
-      tiles_end = min(4 * g.hi, list_tiles);
+      list_tiles = list_pages > 0 ? kSteps * (list_pages - 1) + (held + kStep - 1) / kStep : 0;
+      cut = held - (held - 1) / kStep * kStep;
+      tiles_end = min(kSteps * g.hi, list_tiles);
     }
-    const int t0 = 4 * g.lo;
+    const int t0 = kSteps * g.lo;
     const int tiles = max(0, tiles_end - t0);
     // The leading tiles that every row attends whole.
     int plain;
     if constexpr (kTree) {
-      plain = min(g.context / kKvTile, tiles_end) - t0;
+      plain = min(g.context / kStep, tiles_end) - t0;
     } else {
       const int first = max(g.pos0, 0);  // the first row's position
       int pages = min(g.hi, list_pages);
       while (pages > g.lo && logical_of(pages - 1) * kPageSize + kPageSize - 1 > first) --pages;
-      plain = 4 * (pages - g.lo);
+      plain = kSteps * (pages - g.lo);
       if (pages < min(g.hi, list_pages) && pages >= g.lo) {
-        plain += max(0, (first + 1 - logical_of(pages) * kPageSize) / kKvTile);
+        plain += max(0, (first + 1 - logical_of(pages) * kPageSize) / kStep);
       }
       plain = min(plain, tiles);
     }
@@ -220,14 +229,14 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     auto phys_of = [&](int page) {
       return __builtin_amdgcn_readlane((page >> 6) & 1 ? phys_odd : phys_even, page & 63);
     };
-    int refill_tile = 4 * (64 * (block0 + 1) + 32);  // K of this tile on its way: the block after next is due
+    int refill_tile = kSteps * (64 * (block0 + 1) + 32);  // K of this tile on its way: the block after next is due
     auto refill = [&](int t) {
       if (__builtin_expect(t >= refill_tile, 0)) {
-        const int block = (t >> 8) + 1;
+        const int block = t / (64 * kSteps) + 1;
         int phys = load_pages(block);
         asm volatile("" : "+v"(phys));  // landed before the paths join
         if (block & 1) phys_odd = phys; else phys_even = phys;
-        refill_tile += 256;
+        refill_tile += 64 * kSteps;
       }
     };
 
@@ -247,15 +256,15 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     auto source = [&](int t, int& rb) {
       const char* base;
       rb = page_row_bytes;
-      int valid = t == list_tiles - 1 ? cut : kKvTile;
+      int valid = t == list_tiles - 1 ? cut : kStep;
       if (kTree && t >= list_tiles) {
-        const int at = (t - list_tiles) * kKvTile;
+        const int at = (t - list_tiles) * kStep;
         rb = draft_rb;
         base = draft + (int64_t)at * draft_rb;
-        valid = min(g.tokens - at, kKvTile);
+        valid = min(g.tokens - at, kStep);
       } else {
-        const int phys = phys_of(t >> 2);
-        base = cache + max(phys, 0) * page_stride + (t & 3) * (kKvTile * page_row_bytes);
+        const int phys = phys_of(t / kSteps);
+        base = cache + max(phys, 0) * page_stride + (t % kSteps) * (kStep * page_row_bytes);
         if (phys < 0) valid = 0;
       }
       if (t >= tiles_end) valid = 0;
@@ -292,10 +301,10 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     }
 
     // ---- operand addresses in a slot ----
-    int k_off = n * kRowBytes + 16 * k_slot(n, half);
+    int k_off = key_part * kTileBytes + n * kRowBytes + 16 * k_slot(n, half);
     const int v_key = 4 * half + ((lane & 15) >> 2);
     const int v_dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    int v_off = v_key * kRowBytes + 16 * v_slot(v_key, v_dim >> 3) + 2 * (v_dim & 7);
+    int v_off = key_part * kTileBytes + v_key * kRowBytes + 16 * v_slot(v_key, v_dim >> 3) + 2 * (v_dim & 7);
 
     float m_run = -INFINITY, l_run = 0.0f;  // of the row; the sum over this lane's keys
     f32x16_t o[4];
@@ -341,7 +350,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
       float top = -INFINITY;
       if (active) {
         s_a = scores(k_lds0);
-        if (bad_pages && phys_of(t0 >> 2) < 0) s_a = f32x16_t{} - INFINITY;
+        if (bad_pages && phys_of(t0 / kSteps) < 0) s_a = f32x16_t{} - INFINITY;
         top = row_top(s_a);
       }
       // Iteration it, it % NS = j: scores of tile it in s_cur, their row max in
@@ -389,7 +398,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
         for (int e = 0; e < 8; ++e) pb[0][e] = (elem)px[e];
         asm volatile("" ::"v"(pb[0]), "v"(px[8]), "v"(px[9]), "v"(px[10]), "v"(px[11]), "v"(sum));
         if (__builtin_expect(bad_pages, 0)) {
-          if (phys_of((t0 + it + 1) >> 2) < 0) s_nxt = f32x16_t{} - INFINITY;  // a page without keys
+          if (phys_of((t0 + it + 1) / kSteps) < 0) s_nxt = f32x16_t{} - INFINITY;  // a page without keys
         }
         float next = -INFINITY;
 #pragma unroll
@@ -453,7 +462,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     // ---- the rest, with masks, one tile after the other ----
     int tail_lane = threadIdx.x & 63;
     asm volatile("" : "+v"(tail_lane));
-    const int my_row = 32 * wave + (tail_lane & 31);
+    const int my_row = 32 * row_part + (tail_lane & 31);
     const int my_token = by_group.token(g.row_base + my_row);
     const bool my_ok = my_row < rows;
     uint64_t my_mask = 0;
@@ -471,17 +480,19 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
       const char* const ks = k_pick(turn);
       const char* const vs = v_pick(turn);
       f32x16_t s = scores(ks);
-      if (it >= plain || phys_of(t >> 2) < 0) {
+      if (it >= plain || phys_of(t / kSteps) < 0) {
         int thr = -1;  // the last key offset in the tile that the row attends
         uint32_t bits = ~0u;
         if (kTree && t >= list_tiles) {
-          thr = g.tokens - 1 - (t - list_tiles) * kKvTile;
-          bits = (uint32_t)(my_mask >> ((t - list_tiles) * kKvTile));
-        } else if (phys_of(t >> 2) >= 0) {
+          const int at = (t - list_tiles) * kStep + key_part * kKvTile;
+          thr = g.tokens - 1 - at;
+          bits = (uint32_t)(my_mask >> (at & 63));
+        } else if (phys_of(t / kSteps) >= 0) {
           if constexpr (kTree) {
-            thr = g.context - 1 - t * kKvTile;
+            thr = g.context - 1 - t * kStep - key_part * kKvTile;
           } else {
-            thr = (my_ok ? g.pos0 + my_token : -1) - logical_of(t >> 2) * kPageSize - (t & 3) * kKvTile;
+            thr = (my_ok ? g.pos0 + my_token : -1) - logical_of(t / kSteps) * kPageSize - (t % kSteps) * kStep -
+                  key_part * kKvTile;
           }
         }
 #pragma unroll
@@ -549,6 +560,39 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
     wait_dma();
     __syncthreads();  // no slot is read or written any more
 
+    // ---- the key parts' sums: the second's through LDS ----
+    if constexpr (KP == 2) {
+      char* const at = row_part < NS ? k_pick(row_part) : v_pick(row_part - NS);
+      float* const sums = reinterpret_cast<float*>(v_pick(NS - 1)) + 2 * (64 * row_part + lane);
+      static_assert(kRowParts - NS < NS - 1 && 64 * 64 * 4 <= kStepBytes, "a wave's O fits a slot");
+      if (active && key_part == 1) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const f32x4_t x = {o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2],
+                             o[i >> 2][4 * (i & 3) + 3]};
+          *reinterpret_cast<f32x4_t*>(at + (64 * i + lane) * 16) = x;
+        }
+        sums[0] = m_run;
+        sums[1] = l_run;
+      }
+      __syncthreads();
+      if (active && key_part == 0) {
+        const float other = sums[0];
+        const float top = fmaxf(m_run, other);
+        const float shift = top == -INFINITY ? 0.0f : top;
+        const float w0 = __builtin_amdgcn_exp2f(m_run - shift), w1 = __builtin_amdgcn_exp2f(other - shift);
+        l_run = l_run * w0 + sums[1] * w1;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const f32x4_t x = *reinterpret_cast<const f32x4_t*>(at + (64 * i + lane) * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i >> 2][4 * (i & 3) + e] = o[i >> 2][4 * (i & 3) + e] * w0 + x[e] * w1;
+        }
+        m_run = top;
+      }
+    }
+    const bool writes = active && key_part == 0;
+
     // Rows out: normalised and rounded, gathered in the wave's slot as whole
     // rows (8-byte pieces in, 16-byte chunks out, chunk c of row r at c ^ (r %
     // 16)), stored through L2 in whole cache lines.
@@ -573,7 +617,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
       for (int j = 0; j < 8; ++j) {
         const int r = 4 * j + (lane >> 4), c = lane & 15;
         const u32x4_t y = *reinterpret_cast<const u32x4_t*>(stage + r * kRowBytes + 16 * (c ^ (r & 15)));
-        const int row = 32 * wave + r;
+        const int row = 32 * row_part + r;
         const int t = by_group.token(g.row_base + row);
         const int h = g.row_base + row - t * q.group;
         if (row < rows && t >= g.held) {
@@ -583,17 +627,17 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
       }
     };
     if (g.lo == 0 && g.hi == g.units) {
-      if (active) store_rows(l_run);
+      if (writes) store_rows(l_run);
     } else {
       // ---- a group of several runs ----
       const Shared shared(g, plan.per_run);
       const __amdgpu_buffer_rsrc_t rec = __builtin_amdgcn_make_buffer_rsrc(
           (void*)late().partials, (short)0, (int)((unsigned)late().workgroups * 2u * kRecordBytes), kBufferFlags);
       // record: O [wave][d-block, quarter][lane][4], then row maxima and lane sums [wave][lane]
-      auto piece = [&](int i) { return (unsigned)(((wave * 16 + i) * 64 + lane) * 16); };
-      const unsigned at_max = (unsigned)(kGroupRows * kHeadDim * 4 + (wave * 64 + lane) * 4);
-      const unsigned at_sum = at_max + kBlockThreads * 4;
-      if (active) {
+      auto piece = [&](int i) { return (unsigned)(((row_part * 16 + i) * 64 + lane) * 16); };
+      const unsigned at_max = (unsigned)(kGroupRows * kHeadDim * 4 + (row_part * 64 + lane) * 4);
+      const unsigned at_sum = at_max + kRowParts * 64 * 4;
+      if (writes) {
         const unsigned own = shared.record(run, kRecordBytes);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -604,7 +648,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(m_run), rec, own + at_max, 0, kCpolAgent);
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l_run), rec, own + at_sum, 0, kCpolAgent);
       }
-      if (last_to_arrive(late(), shared, &s_last) && active) {
+      if (last_to_arrive(late(), shared, &s_last) && writes) {
         float top = -INFINITY, l = 0.0f;
 #pragma unroll
         for (int m = 0; m < 4; ++m) o[m] = f32x16_t{};
@@ -652,11 +696,11 @@ template <class Type, bool kTree>
 hipError_t launch_type(const RowsParams& p, int shape_rows, hipStream_t stream) {
   const dim3 grid((unsigned)p.workgroups);
   if (shape_rows == kBlockRows) {
-    hipLaunchKernelGGL((blocks_attention_kernel<Type, 8, kTree>), grid, dim3(512), 0, stream, p);
+    hipLaunchKernelGGL((blocks_attention_kernel<Type, 8, 1, kTree>), grid, dim3(512), 0, stream, p);
+  } else if (kTree || p.workgroups <= kComputeUnits) {
+    hipLaunchKernelGGL((blocks_attention_kernel<Type, 8, 2, kTree>), grid, dim3(512), 0, stream, p);
   } else if constexpr (!kTree) {
-    hipLaunchKernelGGL((blocks_attention_kernel<Type, 4, kTree>), grid, dim3(256), 0, stream, p);
-  } else {
-    return hipErrorInvalidValue;  // trees are bound by memory: eight waves
+    hipLaunchKernelGGL((blocks_attention_kernel<Type, 4, 1, kTree>), grid, dim3(256), 0, stream, p);
   }
   return hipGetLastError();
 }

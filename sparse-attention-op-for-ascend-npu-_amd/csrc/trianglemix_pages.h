@@ -82,7 +82,9 @@ struct RowsParams {
 // Rows of one workgroup: groups of up to 32 rows run in trianglemix_rows.hip,
 // larger ones in trianglemix_blocks.hip, of more than 256 rows in several
 // workgroups.  Measured: 24 pages for each of 64 requests' 4 rows a KV head
-// 137 us with 16 rows, 152 with 256; a 28-row tree 9.4 with 32, 11.1 with 256.
+// 137 us with 16 rows, 152 with 256; a 28-row tree 9.4 with 32, 11.1 with 256;
+// 32 trees of up to 128 rows over 8000 tokens 192 with 128, 208 with 256.
+constexpr int kComputeUnits = 256;  // of an MI355X, in 8 XCDs
 constexpr int kFewRows = 16, kMostStreamRows = 32, kHalfBlockRows = 128, kBlockRows = 256;
 // A run of units leaves at most two partial records of this many bytes.
 constexpr int64_t rows_partial_bytes(int rows) {

@@ -18,7 +18,6 @@ using tmx::report;
 constexpr int64_t kMaxRows = int64_t(1) << 21;
 constexpr int64_t kMaxHeads = 256;
 constexpr int64_t kHeadBytes = tmx::kHeadDim * 2;
-constexpr int kComputeUnits = 256;  // of an MI355X, in 8 XCDs
 
 struct Range {
   const void* at;
@@ -181,7 +180,10 @@ int check_select(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, i
 
 // Rows of the workgroup shape for groups of `rows` rows.
 int shape_for(int64_t rows) {
-  return rows <= tmx::kFewRows ? tmx::kFewRows : rows <= tmx::kMostStreamRows ? tmx::kMostStreamRows : tmx::kBlockRows;
+  for (int shape : {tmx::kFewRows, tmx::kMostStreamRows, tmx::kHalfBlockRows}) {
+    if (rows <= shape) return shape;
+  }
+  return tmx::kBlockRows;
 }
 
 struct RowsPlan {
@@ -189,13 +191,12 @@ struct RowsPlan {
   int64_t units, per_run, workspace_bytes;
 };
 
-// As many workgroups as the GPU holds at once, fewer when there are not as
+// As many workgroups as `slots`, what the GPU holds at once, fewer when there are not as
 // many units (pages of groups of rows); a multiple of the 8 XCDs.
-RowsPlan rows_plan(int shape, int64_t units, int64_t min_units) {
+RowsPlan rows_plan(int shape, int64_t units, int64_t min_units, int64_t slots = tmx::kComputeUnits) {
   RowsPlan r;
   r.shape = shape;
   r.units = units;
-  const int64_t slots = kComputeUnits * (shape == tmx::kHalfBlockRows ? 2 : 1);  // a CU holds two of that shape
   r.workgroups = (int)((std::min<int64_t>(slots, (units + min_units - 1) / min_units) + 7) / 8 * 8);
   r.per_run = std::max(min_units, (units + r.workgroups - 1) / r.workgroups);
   r.workspace_bytes = tmx::kCounterBytes + 2 * r.workgroups * tmx::rows_partial_bytes(r.shape);
@@ -230,21 +231,18 @@ int check_selected(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads,
 
 RowsPlan selected_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t count) {
   const int64_t group_rows = std::min<int64_t>(rows, tmx::kSelectRows) * (heads / kv_heads);
-  int shape = shape_for(group_rows);
+  const int shape = shape_for(group_rows);
   const int64_t blocks = (rows + tmx::kSelectRows - 1) / tmx::kSelectRows;
-  // Blocks of one request find each other's pages in the L2: with work enough
-  // they are bound by the MFMAs, and two workgroups of four waves a CU keep those
-  // busier than one of eight whose other waves have no rows.  Else memory
-  // bounds the call, and the eight waves' 80 KB in flight and half as many partials
-  // serve it better.  128 rows a group, 4 | 8 waves: 64 blocks x 32 pages of
-  // 131072 tokens 170 | 197 us, 64 x 8 of 8192 45 | 56, 32 x 16 of 8192 52 | 52,
-  // 16 x 16 of 8192 38 | 36, one block x 64 pages of each of 32 requests 224 | 216.
-  if (shape == tmx::kBlockRows && group_rows <= tmx::kHalfBlockRows && blocks > 1 &&
-      batch * blocks * kv_heads * count >= 4096) {
-    shape = tmx::kHalfBlockRows;
-  }
-  return rows_plan(shape, batch * blocks * kv_heads * ((group_rows + shape - 1) / shape) * count,
-                   tmx::min_run_units((int)count, shape));
+  const int64_t groups = batch * blocks * kv_heads * ((group_rows + shape - 1) / shape);
+  // Groups of up to 128 rows run in workgroups of eight waves, one a CU.  With two
+  // groups a CU and more, in workgroups of four, two a CU: one starts its next
+  // group beside the other's tiles.  Eight | four waves: 512 groups of 32 pages
+  // of 131072 tokens 182 | 170 us, of 8 pages of 8192 tokens 52 | 45; 256 groups
+  // of 32 pages 79 | 83, of 64 pages, each read once, 200 | 224; 128 groups of 16
+  // pages 34 | 38.  (Lists of 4 to 8 pages lose 0.5 to 1 us of 20 to 25 by the key
+  // parts' join against eight row parts, four of them empty.)
+  const bool two = shape == tmx::kHalfBlockRows && groups >= 2 * tmx::kComputeUnits;
+  return rows_plan(shape, groups * count, tmx::min_run_units((int)count, shape), (two ? 2 : 1) * tmx::kComputeUnits);
 }
 
 int check_tree(int64_t total_rows, int64_t batch, int64_t heads, int64_t kv_heads, int64_t table_cols) {
@@ -257,7 +255,7 @@ int check_tree(int64_t total_rows, int64_t batch, int64_t heads, int64_t kv_head
 // The shape holds the trees that the batch's average lets expect: equal ones
 // where the rows divide evenly, else up to a quarter more than it.  A larger tree
 // takes several row parts, each reading the request's K/V again: 32 trees of 5 to
-// 10 nodes (up to 40 rows a KV head) take 146 us in the shape for 256 rows, 151 in
+// 10 nodes (up to 40 rows a KV head) take 146 us in the shape for 128 rows, 151 in
 // parts of 32; of 4 to 8 nodes 207 and, in one part each, 194.
 RowsPlan tree_plan(int64_t total_rows, int64_t batch, int64_t heads, int64_t kv_heads, int64_t table_cols) {
   const int64_t group = heads / kv_heads;

@@ -197,9 +197,11 @@ def check_attention(gpu, query, keys, values, table, lens, pages, query_d=None):
     ([1111], 70, 4, 2, 6),
     ([300], 300, 4, 1, 3),             # a whole prompt
     ([50, 10, 0], 64, 4, 1, 2),        # more rows than tokens
-    ([900], 260, 32, 8, 64),           # work enough for two workgroups a CU: 128 rows
+    ([900], 260, 32, 8, 64),           # 128 rows, lists longer than the table
     ([700, 3, 1025, 40], 64, 24, 8, 64),  # 96 rows of 128
     ([8300], 40, 8, 4, 1024),          # 64 rows, lists of 65 pages
+    ([700], 260, 128, 64, 5),          # 576 groups: two workgroups a CU, split groups
+    ([400, 3], 130, 128, 64, 3),       # 640 groups in one piece each, the second request's mostly without rows
 ])
 def test_attention(gpu, dtype, lens, rows, heads, kv_heads, count):
     print(f"attend {lens} {rows} {heads}/{kv_heads} {count} {dtype}", flush=True)
@@ -238,14 +240,14 @@ def test_long_lists(gpu, count, rows):
     check_attention(gpu, query, keys, values, table, lens, shuffled)
 
 
-@pytest.mark.parametrize("rows,count", [(20, 4), (64, 1024)])
+@pytest.mark.parametrize("rows,count,heads,kv", [(20, 4, 4, 1), (64, 1024, 4, 1), (160, 4, 128, 64)])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
-def test_bad_pages_and_values_nobody_attends(gpu, dtype, rows, count):
+def test_bad_pages_and_values_nobody_attends(gpu, dtype, rows, count, heads, kv):
     """Pages that are none, pages not chosen full of NaN, NaN and infinities at positions a row does not attend."""
-    print(f"attend bad pages {rows} {count} {dtype}", flush=True)
+    print(f"attend bad pages {rows} {count} {heads}/{kv} {dtype}", flush=True)
     lens = [700, 450]
-    keys, values, table = make_cache(lens, 1, dtype, seed=21)
-    pages = random_lists(lens, rows, 1, 4, seed=22)
+    keys, values, table = make_cache(lens, kv, dtype, seed=21)
+    pages = random_lists(lens, rows, kv, 4, seed=22)
     pages = torch.cat([pages, torch.full((*pages.shape[:-1], count - 4), -1, dtype=torch.int32)], dim=-1)
     for b in range(2):
         for j in range(table.shape[1]):
@@ -259,7 +261,7 @@ def test_bad_pages_and_values_nobody_attends(gpu, dtype, rows, count):
     keys[page, 700 % 128:] = float("nan")
     table[1, pages[1, 0, 0, 0].item()] = -1
     table[1, pages[1, 0, 0, 1].item()] = keys.shape[0] + 3
-    query = make_rows(2 * rows, 4, dtype, 23)
+    query = make_rows(2 * rows, heads, dtype, 23)
     out = torch.zeros_like(query)
     want, size, _ = OP.selected_attention(query, keys, values, table, ints(lens), pages, SCALE, out)
     got = TP.selected_page_attention(query.to(gpu), keys.to(gpu), values.to(gpu), table.to(gpu), ints(lens, gpu),
