@@ -527,8 +527,11 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
 #pragma unroll
         for (int k = 0; k < 8; ++k) o[k & 3] = Type::mfma32(va[k], __builtin_bit_cast(i16x8_t, pb[k >> 2]), o[k & 3]);
       } else {
-        // The finite entries, then for each other kind an indicator's product: it
-        // is positive in the rows that attend such an entry.
+        // The finite entries, then for each other kind the product of indicators
+        // (such an entry; the key attended, whatever its weight rounded to).
+        i16x8_t attended[2];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) attended[e >> 3][e & 7] = s[e] != -INFINITY ? Type::kOne : 0;
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
 #pragma unroll
@@ -543,7 +546,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
 #pragma unroll
               for (int e = 0; e < 4; ++e) a[e] = only_kind<Type>(a[e], kind) | only_kind<Type>(a[e] >> 16, kind) << 16;
               if (kind == 0) o[m] = Type::mfma32(__builtin_bit_cast(i16x8_t, a), __builtin_bit_cast(i16x8_t, pb[j]), o[m]);
-              else has = Type::mfma32(__builtin_bit_cast(i16x8_t, a), __builtin_bit_cast(i16x8_t, pb[j]), has);
+              else has = Type::mfma32(__builtin_bit_cast(i16x8_t, a), attended[j], has);
             }
             if (kind > 0) {
               // opaque: the compiler takes no operand for a NaN; +inf and -inf give one by themselves

@@ -295,8 +295,14 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
 #pragma unroll
         for (int e = 0; e < 8; ++e) bad |= size[e] >= Type::kExp;
         if (__builtin_expect(__any(bad) != 0, 0)) {
-          // The finite entries, then for each other kind an indicator's product:
-          // it is positive in the rows that attend such an entry.
+          // The finite entries, then for each other kind the product of indicators
+          // (such an entry; the key attended, whatever its weight rounded to).
+          i16x8_t attended[NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) attended[n][e] = s[e >> 2][n][e & 3] != -INFINITY ? Type::kOne : 0;
+          }
 #pragma unroll
           for (int m = 0; m < 8; ++m) {
 #pragma unroll
@@ -314,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
                 if (kind == 0) {
                   o[m][n] = Type::mfma16(__builtin_bit_cast(i16x8_t, a), pb[n], o[m][n]);
                 } else {
-                  const f32x4_t has = Type::mfma16(__builtin_bit_cast(i16x8_t, a), pb[n], f32x4_t{});
+                  const f32x4_t has = Type::mfma16(__builtin_bit_cast(i16x8_t, a), attended[n], f32x4_t{});
 #pragma unroll
                   for (int i = 0; i < 4; ++i) o[m][n][i] += has[i] > 0.0f ? odd : 0.0f;
                 }

@@ -240,7 +240,7 @@ def test_long_lists(gpu, count, rows):
     check_attention(gpu, query, keys, values, table, lens, shuffled)
 
 
-@pytest.mark.parametrize("rows,count,heads,kv", [(20, 4, 4, 1), (64, 1024, 4, 1), (160, 4, 128, 64)])
+@pytest.mark.parametrize("rows,count,heads,kv", [(20, 4, 4, 1), (64, 1024, 4, 1), (160, 4, 128, 64), (32, 4, 8, 1)])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 def test_bad_pages_and_values_nobody_attends(gpu, dtype, rows, count, heads, kv):
     """Pages that are none, pages not chosen full of NaN, NaN and infinities at positions a row does not attend."""
