@@ -29,10 +29,10 @@
 // scores in units of log2(e); P is rounded to the input type for the PV
 // product (the row sum adds the unrounded values), the output once.  A row
 // without keys gives zeros.  K and V rows past a page's valid keys are never
-// read from memory (the DMA's range ends there and gives zeros).  In tiles where some row masks a
-// key, V entries that are not finite are kept out of the product and added
-// only to rows that attend them, so that what a row does not attend cannot
-// reach it.
+// read from memory (the DMA's range ends there and gives zeros).  In tiles where
+// some row masks a key, V entries that are not finite are kept out of the product
+// and added only to rows that attend them, so that what a row does not attend
+// cannot reach it.  (Elsewhere an infinity whose weight rounds to zero gives NaN.)
 
 #include <hip/hip_runtime.h>
 
