@@ -560,6 +560,7 @@ __global__ void __launch_bounds__(W * 64, 2) blocks_attention_kernel(const RowsP
         }
       }
     }
+    m_run = row_shift(m_run, half_sum(l_run));
     wait_dma();
     __syncthreads();  // no slot is read or written any more
 

@@ -66,6 +66,12 @@ __device__ __forceinline__ unsigned only_kind(unsigned bits, int kind) {
   return bits == (kind == 1 ? Type::kExp : Type::kExp | 0x8000u) ? (unsigned)Type::kOne : 0;
 }
 
+// A row max takes no NaN in: where all scores of a row were NaN it is still -inf,
+// but the row sum is NaN, and the row must not pass for one without keys.
+__device__ __forceinline__ float row_shift(float max, float sum) {
+  return max == -INFINITY && (__float_as_uint(sum) & 0x7fffffffu) != 0 ? 0.0f : max;
+}
+
 constexpr int kCpolAgent = 16;  // sc1: written to, read from, the level that every XCD sees
 
 // Workgroups are dispatched round-robin over the 8 XCDs: neighbouring runs of

@@ -413,6 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attention_kernel(const RowsP
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const float l = row_sum(l_run[n]);
+      m_run[n] = row_shift(m_run[n], l);
       if (quad == 0) {
         s_max[wave][16 * n + col] = m_run[n];
         s_sum[wave][16 * n + col] = l;

@@ -274,6 +274,24 @@ def test_bad_pages_and_values_nobody_attends(gpu, dtype, rows, count, heads, kv)
     assert bool(((got - want).abs() <= tol)[finite].all())
 
 
+@pytest.mark.parametrize("length,rows,heads,kv", [(1, 1, 4, 1), (300, 1, 32, 1), (300, 20, 4, 1), (300, 33, 16, 1),
+                                                  (300, 256, 128, 64)])
+def test_queries_and_keys_that_are_no_numbers(gpu, length, rows, heads, kv):
+    """A NaN among a row's queries or attended keys makes the row NaN, not one without keys, and no other row."""
+    print(f"attend NaN {length} {rows} {heads}/{kv}", flush=True)
+    keys, values, table = make_cache([length], kv, BF16, seed=81)
+    query = make_rows(rows, heads, BF16, 82)
+    query[0, 1, 7] = query[-1, -1, 0] = float("nan")
+    keys[table[0, 0].item(), 0, 0, 3] = float("nan")  # the first KV head's first key
+    pages = random_lists([length], rows, kv, 3, seed=83)
+    want, size, _ = OP.selected_attention(query, keys, values, table, ints([length]), pages, SCALE, torch.zeros_like(query))
+    got = TP.selected_page_attention(query.to(gpu), keys.to(gpu), values.to(gpu), table.to(gpu), ints([length], gpu),
+                                     pages.to(gpu), SCALE).cpu().double()
+    assert torch.equal(got.isnan(), want.isnan()) and want[0, 1].isnan().all() and want[-1, -1].isnan().all()
+    real = ~want.isnan()
+    assert bool(((got - want).abs() <= tolerance(want, size, values, 384, BF16))[real].all())
+
+
 def test_attention_equals_the_dense_companion_over_all_pages(gpu):
     """Write a chunk's K/V, bounds, selection of every page, attention: as dense causal attention."""
     from trianglemix import cache, kernel
