@@ -16,7 +16,6 @@
 // rows that the operator leaves as they were.
 
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
