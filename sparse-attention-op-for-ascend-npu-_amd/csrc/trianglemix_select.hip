@@ -239,18 +239,26 @@ __global__ void __launch_bounds__(kScoreThreads, 4) score_few_kernel(const Selec
     const bool odd = __any(odd_number(x[0]) || odd_number(x[1]));
     if (lane == 0) s_odd[wave] = odd ? 1 : 0;
   }
-  auto place = [&](int t) {  // of the lane's page in tile t; an unused page's bounds are those of page 0
-    return ((int64_t)max(__shfl(phys, 16 * t + col), 0) * p.kv_heads + kv_head) * kHeadDim + 8 * quad;
+  // The lane's page in tile t, -1 for none.  Another lane holds it, so every lane
+  // must be active here: one that is masked off gives a zero, page 0.
+  auto page_of = [&](int t) { return __shfl(phys, 16 * t + col); };
+  auto place = [&](int page) {  // an unused page's bounds are those of page 0
+    return ((int64_t)max(page, 0) * p.kv_heads + kv_head) * kHeadDim + 8 * quad;
   };
-  Bounds16 next = load_bounds(p, place(0));
+  int next_page = page_of(0);
+  Bounds16 next = load_bounds(p, place(next_page));
   __syncthreads();
   const bool odd_rows = (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3]) != 0;
   const int pages = (seq + kPageSize - 1) / kPageSize;
   for (int t = 0; t < tiles; ++t) {
     if (page0 + 16 * t >= pages) return;
     Bounds16 x = next;
-    const int64_t at = place(t);
-    if (t + 1 < tiles) next = load_bounds(p, place(t + 1));
+    const int here = next_page;
+    const int64_t at = place(here);
+    if (t + 1 < tiles) {
+      next_page = page_of(t + 1);
+      next = load_bounds(p, place(next_page));
+    }
     double sum = 0.0;
     if (__builtin_expect(!odd_rows && !odd_bounds<kFp16>(x), 1)) {
       double c[4] = {};
@@ -281,7 +289,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) score_few_kernel(const Selec
     const int page = page0 + 16 * t + col;
     if ((quad & (padded - 1)) == 0 && quad < p.slab_blocks * padded && page < pages) {
       p.scores[((int64_t)(slab_b * p.slab_blocks + (quad >> padded_bits)) * p.kv_heads + kv_head) * p.table_cols + page] =
-          __shfl(phys, 16 * t + col) >= 0 ? best : 0;
+          here >= 0 ? best : 0;
     }
   }
 }

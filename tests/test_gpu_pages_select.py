@@ -1,0 +1,87 @@
+"""Page selection of batches that decode over wide tables, against a ranking of all pages in 64 bits.
+
+Scoring takes two tiles of 16 pages a wave once requests x KV heads x chunks of 128 pages reach 1024.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from oracle import pages as OP
+from pages_cases import make_rows
+from trianglemix import pages as TP
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def ranked(query, low, high, table, lens, count, sink, recent):
+    """``oracle.pages.select_pages`` of finite bounds, with the scores of a request as one product."""
+    batch, kv = table.shape[0], low.shape[1]
+    rows, group = query.shape[0] // batch, query.shape[1] // kv
+    blocks = -(-rows // 32)
+    out = torch.full((batch, blocks, kv, count), -1, dtype=torch.int32)
+    low, high = low.double(), high.double()
+    for b, n in enumerate(lens.tolist()):
+        for i in range(blocks):
+            first, last = OP.block_rows(n, rows, i)
+            if last < first:
+                continue
+            at = b * rows + first - (max(n, 0) - rows)
+            total = query[at:at + last - first + 1].double().sum(dim=0).view(kv, group, 128)
+            j = torch.arange(min(table.shape[1], last // 128 + 1))
+            there = (table[b, j] >= 0) & (table[b, j] < low.shape[0])
+            phys = table[b, j].long() * there
+            score = (total.clamp(min=0) @ high[phys].permute(1, 2, 0) + total.clamp(max=0) @ low[phys].permute(1, 2, 0))
+            score = score.amax(dim=1)  # [kv, pages]
+            forced = (j < sink) | ((j >= first // 128 - recent + 1) if recent > 0 else False)
+            score = score.masked_fill(forced, float("inf"))[:, there]
+            best = score.sort(dim=1, descending=True, stable=True).indices[:, :count].sort(dim=1).values
+            out[b, i, :, :best.shape[1]] = j[there][best].to(torch.int32)
+    return out
+
+
+def make_batch(batch, kv_heads, cols, pages, dtype, seed):
+    """(low, high, table, lens): random bounds, a third of the table's entries no page of the cache.
+
+    Physical page 0 has by far the largest bounds and is in no request's table.
+    """
+    g = torch.Generator().manual_seed(seed)
+    low = torch.randn(pages, kv_heads, 128, generator=g) - 1
+    high = low + 2 + torch.rand(pages, kv_heads, 128, generator=g)
+    low[0], high[0] = -60.0, 60.0
+    table = torch.randint(1, pages, (batch, cols), generator=g).to(torch.int32)
+    nothing = torch.tensor([-1, pages, -2 ** 31, 2 ** 31 - 1], dtype=torch.int32)
+    bad = torch.rand(batch, cols, generator=g) < 1 / 3
+    table[bad] = nothing[torch.randint(0, 4, (int(bad.sum()),), generator=g)]
+    lens = torch.randint(1, cols * 128 + 1, (batch,), generator=g).to(torch.int32)
+    lens[0], lens[1], lens[2], lens[3] = cols * 128, 0, 1, 17 * 128 + 5
+    table[0, 0] = table[0, -1] = table[3, 17] = -1  # the first and the most recent page
+    return low.to(dtype), high.to(dtype), table, lens
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows,group,batch,kv_heads,cols", [
+    (1, 1, 32, 8, 512), (1, 2, 64, 4, 500), (1, 4, 32, 8, 512), (1, 3, 64, 8, 300),  # decoding, 1 to 4 heads a group
+    (3, 4, 32, 8, 512), (32, 1, 64, 8, 257),                                        # one block of several rows
+    (40, 2, 32, 8, 512), (128, 1, 64, 4, 512),                                      # two blocks, four
+])
+def test_pages_that_are_none_in_every_tile(gpu, dtype, rows, group, batch, kv_heads, cols):
+    print(f"select two tiles {rows} {group} {batch} {kv_heads} {cols} {dtype}", flush=True)
+    assert -(-cols // 128) * kv_heads * batch >= 1024
+    low, high, table, lens = make_batch(batch, kv_heads, cols, 900, dtype, seed=rows + group + cols)
+    query = make_rows(batch * rows, group * kv_heads, dtype, 3)
+    for count, sink, recent in ((16, 1, 1), (9, 3, 4)):
+        want = ranked(query, low, high, table, lens, count, sink, recent)
+        got = TP.select_pages(query.to(gpu), low.to(gpu), high.to(gpu), table.to(gpu), lens.to(gpu), count,
+                              sink_pages=sink, recent_pages=recent).cpu()
+        assert torch.equal(got, want), f"{int((got != want).any(dim=-1).sum())} of {got[..., 0].numel()} selections differ"
+
+
+def test_ranking_equals_the_oracle():
+    """The ranking above, on a small case, against the oracle's own loop."""
+    low, high, table, lens = make_batch(4, 2, 20, 30, BF16, seed=1)
+    for rows in (1, 5, 40):
+        query = make_rows(4 * rows, 6, BF16, 2)
+        assert torch.equal(ranked(query, low, high, table, lens, 6, 1, 2),
+                           OP.select_pages(query, low, high, table, lens, 6, 1, 2))
