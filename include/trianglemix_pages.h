@@ -76,7 +76,10 @@ int tm_select_pages(const void* query, int64_t query_stride, const void* page_mi
                     int64_t num_pages, int64_t count, int64_t sink_pages, int64_t recent_pages, int dtype,
                     void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Workspace bytes of that call (any contents), or -1 for what it refuses. */
+/* Workspace bytes of that call, or -1 for what it refuses.  Any contents,
+ * 16-byte aligned.  The call enqueues several launches that hand it on, so it
+ * is one call's own until the last of them has run: no other call's launches,
+ * from another thread on the same stream either, may come between them. */
 int64_t tm_select_pages_workspace_size(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads,
                                        int64_t table_cols);
 

@@ -11,9 +11,11 @@
 //
 // Shapes, types, devices and overlaps are checked here or in the library, on
 // the host; launches go on the current HIP stream of the query's device under
-// a device guard, with no synchronisation, with the adapter's workspace
-// (trianglemix_torch.cpp).  The functional attention forms return zeros in the
-// rows that the operator leaves as they were.
+// a device guard, with no synchronisation.  The attention operators, one launch
+// each, take the adapter's workspace (trianglemix_torch.cpp); select_pages, which
+// keeps scores from one launch to the next, a buffer of each call's own.  The
+// functional attention forms return zeros in the rows that the operator leaves
+// as they were.
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -100,14 +102,20 @@ void* stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.de
 void* ptr(const at::Tensor& t) { return t.data_ptr(); }
 const int32_t* ints(const at::Tensor& t) { return t.data_ptr<int32_t>(); }
 
+// Of a call's launches.  The stream's shared buffer serves calls of one launch: the
+// launches of two host threads on a stream come in any order, so what a launch
+// leaves for the next one of its call must be out of the other's reach
+// (kPerCall; the caching allocator hands it out again in stream order).
+enum class Buffer { kShared, kPerCall };
 struct Workspace {
   at::Tensor held;
   void* at = nullptr;
   int64_t bytes = 0;
-  Workspace(const at::Tensor& like, int64_t need, void* stream, const char* what) {
+  Workspace(const at::Tensor& like, int64_t need, void* stream, const char* what, Buffer buffer = Buffer::kShared) {
     TORCH_CHECK(need >= 0, what, " failed (TM_ERR): ", tm_last_error());
     if (need == 0) return;
-    held = workspace_for(like, need, stream);
+    held = buffer == Buffer::kPerCall ? at::empty({need}, like.options().dtype(at::kByte))
+                                      : workspace_for(like, need, stream);
     at = held.data_ptr();
     bytes = need;
   }
@@ -147,7 +155,7 @@ at::Tensor& select_pages_out(const at::Tensor& query, const at::Tensor& page_min
   c10::OptionalDeviceGuard guard(query.device());
   void* stream = stream_of(query);
   const Workspace ws(query, tm_select_pages_workspace_size(batch, rows, heads, kv_heads, block_table.size(1)), stream,
-                     "select_pages");
+                     "select_pages", Buffer::kPerCall);
   check_status(tm_select_pages(ptr(query), row_stride(query), ptr(page_min), ptr(page_max), ints(block_table),
                                table_stride(block_table), ints(seq_lens), out.data_ptr<int32_t>(), batch, rows, heads,
                                kv_heads, block_table.size(1), page_min.size(0), count, sink_pages, recent_pages, dtype,

@@ -611,7 +611,9 @@ __global__ void __launch_bounds__(kTopThreads) top_pages_kernel(const SelectPara
     }
     const uint64_t mask = __ballot(take);
     const int all = total(__popcll(mask), &before);
-    if (take) out[written + before + below(mask)] = i * kTopThreads + (int)threadIdx.x;
+    // a workspace that others write to meanwhile may show more keys always taken than fit
+    const int at = written + before + below(mask);
+    if (take && at < p.count) out[at] = i * kTopThreads + (int)threadIdx.x;
     written += all;
   }
   for (int i = written + threadIdx.x; i < p.count; i += kTopThreads) out[i] = -1;

@@ -38,7 +38,8 @@
 // torch_npu's.  Its contents do not matter (the library tags each arrival
 // word for its workspace), so no buffer is ever cleared.  Outside stream
 // capture one buffer is kept per (device, stream) and shared by the launches
-// on that stream, which run in order; a call that needs more replaces it,
+// on that stream, which run in order (nothing in it outlives a launch; a call
+// of several launches takes a buffer of its own); a call that needs more replaces it,
 // and the old buffer goes back to the caching allocator, which hands its
 // memory out again only in stream order.  Under stream capture every call
 // takes a buffer of its own from the capture's private pool, which the

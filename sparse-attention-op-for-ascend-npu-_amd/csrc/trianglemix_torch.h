@@ -9,7 +9,8 @@
 namespace trianglemix_rocm {
 
 // Workspace of at least `bytes` for a launch on `stream`: the buffer kept for
-// this device and stream, or under stream capture one of the capture's own.
+// this device and stream, or under stream capture one of the capture's own.  Any
+// other launch on the stream may use it too: it holds nothing between launches.
 at::Tensor workspace_for(const at::Tensor& like, int64_t bytes, void* stream);
 
 // Raises the library's last error unless the status is TM_OK.

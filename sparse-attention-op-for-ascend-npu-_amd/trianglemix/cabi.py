@@ -82,16 +82,21 @@ def _workspace_of(query, need, workspace, stream):
     if need == 0:
         return None, 0
     if workspace is None:
-        import torch
-
         key = (query.device.index, int(stream))
         held = _WORKSPACES.get(key)
         if held is None or held.numel() < need:
             _WORKSPACES.pop(key, None)
-            with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=query.device)):
-                held = _WORKSPACES[key] = torch.empty(need, dtype=torch.uint8, device=query.device)
+            held = _WORKSPACES[key] = _buffer(query, need, stream)
         workspace = held
     return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _buffer(query, need, stream):
+    """Memory of the caching allocator that is handed out again in this stream's order."""
+    import torch
+
+    with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=query.device)):
+        return torch.empty(need, dtype=torch.uint8, device=query.device)
 
 
 def triangle_paged_sparse_attention(query, key_cache, value_cache, block_table, out, *, query_start: int,
@@ -171,6 +176,9 @@ def select_pages(query, page_min, page_max, block_table, seq_lens, out, *, sink_
     (batch, cols), heads, kv = block_table.shape, query.shape[1], page_min.shape[1]
     rows = query.shape[0] // max(batch, 1)
     need = _need(lib.tm_select_pages_workspace_size, batch, rows, heads, kv, cols)
+    if workspace is None and need > 0:
+        # scores that one launch of the call leaves for the next: out of reach of other threads' calls on the stream
+        workspace = _buffer(query, need, st)
     ws_ptr, ws_bytes = _workspace_of(query, need, workspace, st)
     _check(lib.tm_select_pages(
         query.data_ptr(), query.stride(0), page_min.data_ptr(), page_max.data_ptr(), block_table.data_ptr(),
