@@ -79,8 +79,10 @@ def _workspace(query, query_start, seq_len, prompt_len, workspace, stream):
 
 
 def _workspace_of(query, need, workspace, stream):
+    """(buffer, pointer, bytes).  The caller keeps the buffer until its launch is enqueued: another thread's call
+    may replace the one that is kept for the stream meanwhile, and its memory would go to whoever asks next."""
     if need == 0:
-        return None, 0
+        return None, None, 0
     if workspace is None:
         key = (query.device.index, int(stream))
         held = _WORKSPACES.get(key)
@@ -88,7 +90,7 @@ def _workspace_of(query, need, workspace, stream):
             _WORKSPACES.pop(key, None)
             held = _WORKSPACES[key] = _buffer(query, need, stream)
         workspace = held
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def _buffer(query, need, stream):
@@ -104,7 +106,7 @@ def triangle_paged_sparse_attention(query, key_cache, value_cache, block_table, 
                                     workspace=None) -> None:
     lib = load_hip_library()
     st = _stream(query, stream)
-    ws_ptr, ws_bytes = _workspace(query, query_start, seq_len, prompt_len, workspace, st)
+    _held, ws_ptr, ws_bytes = _workspace(query, query_start, seq_len, prompt_len, workspace, st)
     _check(lib.tm_triangle_paged_sparse_attention(
         query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(), out.data_ptr(),
         query.shape[0], key_cache.shape[0], block_table.shape[-1], query_start, seq_len, prompt_len,
@@ -126,7 +128,7 @@ def dense_paged_causal_attention(query, key_cache, value_cache, block_table, out
                                  seq_len: int, scale: float, stream=None, workspace=None) -> None:
     lib = load_hip_library()
     st = _stream(query, stream)
-    ws_ptr, ws_bytes = _workspace(query, query_start, seq_len, None, workspace, st)
+    _held, ws_ptr, ws_bytes = _workspace(query, query_start, seq_len, None, workspace, st)
     _check(lib.tm_dense_paged_causal_attention(
         query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(), out.data_ptr(),
         query.shape[0], key_cache.shape[0], block_table.shape[-1], query_start, seq_len,
@@ -179,7 +181,7 @@ def select_pages(query, page_min, page_max, block_table, seq_lens, out, *, sink_
     if workspace is None and need > 0:
         # scores that one launch of the call leaves for the next: out of reach of other threads' calls on the stream
         workspace = _buffer(query, need, st)
-    ws_ptr, ws_bytes = _workspace_of(query, need, workspace, st)
+    _held, ws_ptr, ws_bytes = _workspace_of(query, need, workspace, st)
     _check(lib.tm_select_pages(
         query.data_ptr(), query.stride(0), page_min.data_ptr(), page_max.data_ptr(), block_table.data_ptr(),
         block_table.stride(0), seq_lens.data_ptr(), out.data_ptr(), batch, rows, heads, kv, cols, page_min.shape[0],
@@ -194,7 +196,7 @@ def selected_page_attention(query, key_cache, value_cache, block_table, seq_lens
     (batch, cols), heads, kv, count = block_table.shape, query.shape[1], key_cache.shape[2], pages.shape[-1]
     rows = query.shape[0] // max(batch, 1)
     need = _need(lib.tm_selected_page_attention_workspace_size, batch, rows, heads, kv, count)
-    ws_ptr, ws_bytes = _workspace_of(query, need, workspace, st)
+    _held, ws_ptr, ws_bytes = _workspace_of(query, need, workspace, st)
     _check(lib.tm_selected_page_attention(
         query.data_ptr(), query.stride(0), key_cache.data_ptr(), key_cache.stride(0), value_cache.data_ptr(),
         value_cache.stride(0), block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(), pages.data_ptr(),
@@ -209,7 +211,7 @@ def tree_attention(query, key, value, key_cache, value_cache, block_table, conte
     st = _stream(query, stream)
     (batch, cols), (total, heads), kv = block_table.shape, query.shape[:2], key_cache.shape[2]
     need = _need(lib.tm_tree_attention_workspace_size, total, batch, heads, kv, cols)
-    ws_ptr, ws_bytes = _workspace_of(query, need, workspace, st)
+    _held, ws_ptr, ws_bytes = _workspace_of(query, need, workspace, st)
     _check(lib.tm_tree_attention(
         query.data_ptr(), query.stride(0), key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0),
         key_cache.data_ptr(), key_cache.stride(0), value_cache.data_ptr(), value_cache.stride(0),
