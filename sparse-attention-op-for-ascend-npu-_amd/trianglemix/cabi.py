@@ -68,7 +68,9 @@ def chunk_plan(query_tokens: int, query_start: int, seq_len: int, prompt_len: in
 # for its workspace), so a buffer is never cleared.  One buffer is kept per
 # (device, stream), allocated on that stream; a call that needs more replaces
 # it, and PyTorch's caching allocator hands the old buffer's memory out again
-# only in that stream's order, after the work queued on it.
+# only in that stream's order, after the work queued on it.  Under stream
+# capture every call takes a buffer of its own from the graph's pool, so no
+# graph depends on a buffer that is replaced here or shares it with another.
 WORKSPACE_COUNTER_BYTES = 65536
 MAX_WORKSPACE_BYTES = 64 << 20
 _WORKSPACES: dict = {}
@@ -83,6 +85,8 @@ def _workspace_of(query, need, workspace, stream):
     may replace the one that is kept for the stream meanwhile, and its memory would go to whoever asks next."""
     if need == 0:
         return None, None, 0
+    if workspace is None and _capturing(query, stream):
+        workspace = _buffer(query, need, stream)  # from the graph's own pool, which it keeps for its replays
     if workspace is None:
         key = (query.device.index, int(stream))
         held = _WORKSPACES.get(key)
@@ -91,6 +95,15 @@ def _workspace_of(query, need, workspace, stream):
             held = _WORKSPACES[key] = _buffer(query, need, stream)
         workspace = held
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _capturing(query, stream) -> bool:
+    import torch
+
+    if not torch.cuda.is_available():
+        return False
+    with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=query.device)):
+        return torch.cuda.is_current_stream_capturing()
 
 
 def _buffer(query, need, stream):
