@@ -174,6 +174,12 @@ def _need(size, *geometry) -> int:
     return int(n)
 
 
+def _rows_per_request(query, batch: int) -> int:
+    if query.shape[0] % max(batch, 1) or (batch == 0 and query.shape[0]):
+        raise TriangleMixError(TM_ERR_INVALID_ARGUMENT, "query must hold the same number of rows for each request")
+    return query.shape[0] // max(batch, 1)
+
+
 def update_page_bounds(key_cache, block_table, seq_lens, num_tokens: int, page_min, page_max, *, stream=None) -> None:
     """``pages.update_page_bounds`` through the C ABI."""
     lib = load_hip_library()
@@ -189,7 +195,7 @@ def select_pages(query, page_min, page_max, block_table, seq_lens, out, *, sink_
     lib = load_hip_library()
     st = _stream(query, stream)
     (batch, cols), heads, kv = block_table.shape, query.shape[1], page_min.shape[1]
-    rows = query.shape[0] // max(batch, 1)
+    rows = _rows_per_request(query, batch)
     need = _need(lib.tm_select_pages_workspace_size, batch, rows, heads, kv, cols)
     if workspace is None and need > 0:
         # scores that one launch of the call leaves for the next: out of reach of other threads' calls on the stream
@@ -207,7 +213,7 @@ def selected_page_attention(query, key_cache, value_cache, block_table, seq_lens
     lib = load_hip_library()
     st = _stream(query, stream)
     (batch, cols), heads, kv, count = block_table.shape, query.shape[1], key_cache.shape[2], pages.shape[-1]
-    rows = query.shape[0] // max(batch, 1)
+    rows = _rows_per_request(query, batch)
     need = _need(lib.tm_selected_page_attention_workspace_size, batch, rows, heads, kv, count)
     _held, ws_ptr, ws_bytes = _workspace_of(query, need, workspace, st)
     _check(lib.tm_selected_page_attention(

@@ -1,4 +1,4 @@
-"""Workspaces of the ctypes binding, with a stand-in for the library: what a call holds until its launch is enqueued."""
+"""The ctypes binding with a stand-in for the library: what a call holds until its launch is enqueued, what it refuses."""
 
 from __future__ import annotations
 
@@ -64,3 +64,23 @@ def test_a_buffer_lives_until_its_call_has_launched(monkeypatch, kind):
     monkeypatch.setattr(cabi, "_WORKSPACES", {})
     calls()[kind]()
     assert len(made) == 2 and alive == [True]
+
+
+@pytest.mark.parametrize("kind", ["selected", "select"])
+@pytest.mark.parametrize("requests,rows", [(2, 3), (2, 5), (3, 4), (0, 4)])
+def test_rows_that_do_not_divide_are_refused(monkeypatch, kind, requests, rows):
+    """Not taken as fewer rows a request, the second one's beginning in the first one's."""
+    launched = []
+    monkeypatch.setattr(cabi, "load_hip_library", lambda: Library([1024], lambda: launched.append(kind)))
+    monkeypatch.setattr(cabi, "_buffer", lambda query, need, stream: torch.empty(need, dtype=torch.uint8))
+    monkeypatch.setattr(cabi, "_WORKSPACES", {})
+    q = torch.zeros(rows, 8, 128, dtype=torch.bfloat16)
+    cache = torch.zeros(3, 128, 2, 128, dtype=torch.bfloat16)
+    table, lens = torch.zeros(requests, 3, dtype=torch.int32), torch.zeros(requests, dtype=torch.int32)
+    pages = torch.zeros(requests, 1, 2, 4, dtype=torch.int32)
+    with pytest.raises(cabi.TriangleMixError, match="same number of rows"):
+        if kind == "select":
+            cabi.select_pages(q, cache[:, 0], cache[:, 0], table, lens, pages, stream=0)
+        else:
+            cabi.selected_page_attention(q, cache, cache, table, lens, pages, q, scale=1.0, stream=0)
+    assert not launched
