@@ -54,8 +54,9 @@ def make_batch(batch, kv_heads, cols, pages, dtype, seed):
     bad = torch.rand(batch, cols, generator=g) < 1 / 3
     table[bad] = nothing[torch.randint(0, 4, (int(bad.sum()),), generator=g)]
     lens = torch.randint(1, cols * 128 + 1, (batch,), generator=g).to(torch.int32)
-    lens[0], lens[1], lens[2], lens[3] = cols * 128, 0, 1, 17 * 128 + 5
-    table[0, 0] = table[0, -1] = table[3, 17] = -1  # the first and the most recent page
+    lens[:4] = torch.tensor([cols * 128, 0, 1, 17 * 128 + 5])[:batch]
+    table[0, 0] = table[0, -1] = -1  # the first and the most recent page
+    table[3:4, 17] = -1
     return low.to(dtype), high.to(dtype), table, lens
 
 
@@ -85,3 +86,30 @@ def test_ranking_equals_the_oracle():
         query = make_rows(4 * rows, 6, BF16, 2)
         assert torch.equal(ranked(query, low, high, table, lens, 6, 1, 2),
                            OP.select_pages(query, low, high, table, lens, 6, 1, 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,rows,heads,kv_heads", [
+    (64, 1, 8, 8),     # 40 requests, then 24
+    (24, 40, 16, 8),   # pooled rows: 19 requests of two blocks, then 5
+    (2, 1607, 16, 8),  # one request's 51 blocks: 39, then 12, with seven rows in the last one; then the other request's
+])
+def test_calls_of_several_slabs(gpu, batch, rows, heads, kv_heads):
+    """Scores past the workspace's 40 MiB: several launches over it, each with its part of the requests and blocks."""
+    from trianglemix import cabi
+
+    print(f"select slabs {batch} {rows} {heads} {kv_heads}", flush=True)
+    cols, blocks = 16384, -(-rows // 32)
+    each = kv_heads * cols * 8 + (heads * 128 * 8 if rows > 1 else 0)
+    assert batch * blocks * each > 40 << 20
+    assert cabi.load_hip_library().tm_select_pages_workspace_size(batch, rows, heads, kv_heads, cols) <= 40 << 20
+    low, high, table, _ = make_batch(batch, kv_heads, cols, 900, BF16, seed=rows)
+    g = torch.Generator().manual_seed(rows)
+    lens = torch.randint(1, 60 * 128, (batch,), generator=g).to(torch.int32)
+    lens[-1] = 130 * 128 + 77
+    query = make_rows(batch * rows, heads, BF16, 4)
+    want = ranked(query, low, high, table, lens, 12, 1, 1)
+    out = torch.full_like(want, 7, device=gpu)
+    TP.select_pages(query.to(gpu), low.to(gpu), high.to(gpu), table.to(gpu), lens.to(gpu), 12, out=out)
+    assert torch.equal(out.cpu(), want)
+    assert all(not torch.equal(want[0], want[b]) for b in range(1, batch))
