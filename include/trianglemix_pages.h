@@ -50,7 +50,9 @@ extern "C" {
  * (contiguous, the keys' type, exact).  A NaN among the keys makes both bounds
  * of its dim NaN.  Other pages' bounds are left as they were.  A length past
  * the table counts as the table's.  Call it after the tokens' K rows are in the
- * cache.
+ * cache.  Requests may share pages that hold the same number of tokens for each
+ * of them (a common prefix of full pages); with different lengths in a shared
+ * page its bounds would be either's, in any mixture.
  */
 int tm_update_page_bounds(const void* key_cache, int64_t key_page_stride, const int32_t* block_table,
                           int64_t table_stride, const int32_t* seq_lens, int64_t num_tokens, void* page_min,
@@ -86,9 +88,16 @@ int64_t tm_select_pages_workspace_size(int64_t batch, int64_t rows, int64_t head
 /*
  * Causal attention of each query row over the keys k <= p of the pages that
  * `pages` [batch, ceil(rows / 32), kv_heads, count] int32 lists for its block
- * and KV head: one softmax over them, fp32 accumulation, rounded once.  The
- * list is a set: any order, an entry twice counts once, an entry that is no
- * page up to the block's last row is ignored.  A row without keys gives zeros.
+ * and KV head.  The list is a set: any order, an entry twice counts once, an
+ * entry that is no page up to the block's last row is ignored.
+ *
+ * Numerics, of this operator and of tm_tree_attention: scores, softmax
+ * statistics and sums in fp32; the weights are rounded to the inputs' type for
+ * their product with V (the sum that they are divided by takes them unrounded),
+ * the result once more.  A row without keys gives zeros.  A key whose score is
+ * -infinity counts as one that the row does not attend.  NaN, and infinities in V,
+ * reach the rows that attend their key and no other; an infinity whose weight
+ * rounds to zero may arrive as NaN.
  */
 int tm_selected_page_attention(const void* query, int64_t query_stride, const void* key_cache,
                                int64_t key_page_stride, const void* value_cache, int64_t value_page_stride,
