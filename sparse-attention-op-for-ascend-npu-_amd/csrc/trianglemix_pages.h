@@ -15,7 +15,6 @@ namespace tmx {
 // are those of trianglemix_kernel.h).
 constexpr int kSelectRows = 32;       // query rows that share one selection
 constexpr int kMaxGroup = 32;         // query heads per KV head
-constexpr int kMaxKvHeads = 256;
 constexpr int kMaxBatch = 1024;       // requests of one call
 constexpr int kMaxSelected = 1024;    // pages of one selection
 constexpr int kMaxTableCols = 16384;  // logical pages of a request (2,097,152 tokens)
