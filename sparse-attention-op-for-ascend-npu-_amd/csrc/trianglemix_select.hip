@@ -151,7 +151,9 @@ __device__ __forceinline__ void keep_larger(uint64_t& x, uint64_t y) { x = y > x
 // 32 dims the eight from 8 (l / 16) on, and the products run over tiles of
 // rows, block * padded + head with the group padded to a power of two.
 // Infinities and NaNs, which a product with zero would turn into NaN, take a
-// plain loop.
+// plain loop: the rows that hold one for all pages, the pages that hold one by
+// themselves, so that a page's score does not hang on its neighbours' bounds (the two
+// forms may differ in the last bit).
 typedef double f64x4_t __attribute__((ext_vector_type(4)));
 typedef double f64x2_t __attribute__((ext_vector_type(2)));
 constexpr int kScoreWaves = 4;
@@ -169,8 +171,9 @@ __device__ __forceinline__ Bounds16 load_bounds(const SelectParams& p, int64_t a
   }
   return x;
 }
+// Bit j: some bound of the wave's page j is no finite number.
 template <bool kFp16>
-__device__ __forceinline__ bool odd_bounds(const Bounds16& x) {  // some bound of the wave's is no finite number
+__device__ __forceinline__ unsigned odd_bounds(const Bounds16& x) {
   typedef unsigned short u16x8_t __attribute__((ext_vector_type(8)));
   u16x8_t most = {};
 #pragma unroll
@@ -181,7 +184,10 @@ __device__ __forceinline__ bool odd_bounds(const Bounds16& x) {  // some bound o
   bool odd = false;
 #pragma unroll
   for (int e = 0; e < 8; ++e) odd |= most[e] >= (kFp16 ? 0x7c00 : 0x7f80);
-  return __any(odd);
+  uint64_t lanes = __ballot(odd);
+  lanes |= lanes >> 32;
+  lanes |= lanes >> 16;
+  return (unsigned)lanes & 0xffffu;
 }
 // The plain sum over a row of 128 (plus and minus its parts, from 8 quad on), in
 // all four lanes of a page.  The bounds come anew from memory: nothing is kept in
@@ -260,7 +266,8 @@ __global__ void __launch_bounds__(kScoreThreads, 4) score_few_kernel(const Selec
       next = load_bounds(p, place(next_page));
     }
     double sum = 0.0;
-    if (__builtin_expect(!odd_rows && !odd_bounds<kFp16>(x), 1)) {
+    const unsigned plain = odd_rows ? 0xffffu : odd_bounds<kFp16>(x);  // pages that take the plain loop
+    if (__builtin_expect(!odd_rows, 1)) {
       double c[4] = {};
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
@@ -276,10 +283,11 @@ __global__ void __launch_bounds__(kScoreThreads, 4) score_few_kernel(const Selec
         }
       }
       sum = (c[0] + c[1]) + (c[2] + c[3]);
-    } else {
+    }
+    if (__builtin_expect(plain != 0, 0)) {
       for (int r = 0; r < 4; ++r) {
         const double y = plain_score<kFp16>(p, at, &s_plus[r][8 * quad], &s_minus[r][8 * quad]);
-        sum = r == quad ? y : sum;
+        sum = r == quad && (plain >> col & 1) != 0 ? y : sum;
       }
     }
     // row `quad` of page `col`: max over the heads of a block
@@ -359,7 +367,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPar
   put(0, x);
   const int pages = (seq + kPageSize - 1) / kPageSize;
   if ((int)blockIdx.z * kScoreWaves * 16 >= pages) return;
-  const bool odd_page = odd_bounds<kFp16>(raw);
+  const unsigned odd_pages = odd_bounds<kFp16>(raw);
   double lo[32], hi[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
@@ -375,7 +383,8 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPar
     if (more) fetch(next * 16, x);
     const int row0 = t * 16;
     f64x4_t sum = {0.0, 0.0, 0.0, 0.0};
-    if (__builtin_expect(!odd_page && s_odd[buffer] == 0, 1)) {
+    const unsigned plain = __builtin_amdgcn_readfirstlane(s_odd[buffer]) != 0 ? 0xffffu : odd_pages;
+    if (__builtin_expect(plain != 0xffffu, 1)) {
       // Physical row r of the operand is row 4 (r % 4) + r / 4 of the tile, so
       // that a lane's four results are rows 4 quad .. 4 quad + 3.
       const double* const plus = &s_plus[buffer][4 * (col & 3) + (col >> 2)][8 * quad];
@@ -392,11 +401,12 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const SelectPar
         }
       }
       sum = c0 + c1;
-    } else {
+    }
+    if (__builtin_expect(plain != 0, 0)) {
       for (int r = 0; r < 16; ++r) {
         const double y = plain_score<kFp16>(p, at, &s_plus[buffer][r][8 * quad], &s_minus[buffer][r][8 * quad]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i] = r == 4 * quad + i ? y : sum[i];
+        for (int i = 0; i < 4; ++i) sum[i] = r == 4 * quad + i && (plain >> col & 1) != 0 ? y : sum[i];
       }
     }
     // max over the heads of a block: rows of a lane, then of lanes, then of tiles

@@ -113,3 +113,39 @@ def test_calls_of_several_slabs(gpu, batch, rows, heads, kv_heads):
     TP.select_pages(query.to(gpu), low.to(gpu), high.to(gpu), table.to(gpu), lens.to(gpu), 12, out=out)
     assert torch.equal(out.cpu(), want)
     assert all(not torch.equal(want[0], want[b]) for b in range(1, batch))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows,group", [(1, 1), (1, 3), (33, 2), (70, 8), (1, 32)])
+def test_equal_pages_beside_odd_bounds(gpu, dtype, rows, group):
+    """Two logical pages with the same bounds have the same score, also where sums round and a neighbour is infinite."""
+    print(f"select equal pages {rows} {group} {dtype}", flush=True)
+    batch, kv, cols, pages = 32, 8, 64, 8
+    g = torch.Generator().manual_seed(rows + group)
+
+    def wide(*shape, bits):  # values of many magnitudes: their products' sum takes more than 53 bits
+        return torch.randn(*shape, generator=g) * 2.0 ** torch.randint(-bits, bits + 1, shape, generator=g)
+
+    bits = 7 if dtype == FP16 else 25
+    low, high = wide(pages, kv, 128, bits=bits), wide(pages, kv, 128, bits=bits)
+    low, high = torch.minimum(low, high).to(dtype), torch.maximum(low, high).to(dtype)
+    low[1:], high[1:] = 0, 0
+    low[0] -= 1
+    high[0] += 1
+    high[2, :, 5] = float("inf")
+    query = wide(batch * rows, group * kv, 128, bits=bits).to(dtype)
+    query[..., 5] = -query[..., 5].abs() - 0.25  # takes the lower bound there, which is zero
+    table = torch.ones(batch, cols, dtype=torch.int32)
+    table[:, 3] = table[:, 40] = 0
+    table[:, 41] = 2
+    lens = torch.full((batch,), cols * 128, dtype=torch.int32)
+    got = TP.select_pages(query.to(gpu), low.to(gpu), high.to(gpu), table.to(gpu), lens.to(gpu), 1 if rows == 1 else 3,
+                          sink_pages=0, recent_pages=0).cpu()
+    # where the sum of page 0's terms is negative, the pages without bounds of their own come first: 0, 1, 2
+    first = (got == 3).any(dim=-1)
+    assert first.float().mean() > 0.8
+    assert not ((got == 40).any(dim=-1) & ~first).any()
+    one = TP.select_pages(query.to(gpu), low.to(gpu), high.to(gpu), table.to(gpu), lens.to(gpu), 1, sink_pages=0,
+                          recent_pages=0).cpu()[..., 0]
+    assert not (one == 40).any(), f"page 40 before page 3 in {int((one == 40).sum())} of {one.numel()} selections"
