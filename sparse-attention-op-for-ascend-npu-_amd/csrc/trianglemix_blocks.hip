@@ -30,7 +30,8 @@
 // trianglemix_rows.hip.
 //
 // What bounds it: with pages that the L2 holds the MFMAs and the exponentials
-// beside them, 975 to 1000 TFLOP/s over 2048 rows x 128 pages, where a bf16
+// beside them, 1028 TFLOP/s over 2048 rows x 128 pages (97 % of the reads hit the
+// L2, MFMAs are busy in half the cycles), where a bf16
 // library product of 8192^3 reaches 1377; with pages read once, memory: 32 trees
 // of up to 32 nodes over 8000 tokens each take 192 us, 5.5 TB/s.  Short lists
 // pay for the start (lengths, selection, Q and table before the first step, 7

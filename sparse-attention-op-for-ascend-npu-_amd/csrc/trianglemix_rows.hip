@@ -12,7 +12,7 @@
 // the page loop has no barrier; the waves' sums meet in LDS behind it.
 //
 // What bounds it: memory.  24 pages of each KV head for 64 requests of 2000 to
-// 16384 tokens (798 MB of K and V) take 137 us, 5.8 TB/s, where a library copy
+// 16384 tokens (798 MB of K and V) take 138 us, 5.8 TB/s, where a library copy
 // of 2 GiB moves 4.9 (read and written).  One
 // request's few pages are bound by latency instead (8 us for 64 pages x 8 KV
 // heads: launch, lengths, selection, table, page, merge, each waiting for the
