@@ -9,6 +9,7 @@ current stream of the query's device).
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 
 from .native import load_hip_library
 
@@ -97,20 +98,30 @@ def _workspace_of(query, need, workspace, stream):
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
-def _capturing(query, stream) -> bool:
+def _on(query, stream):
+    """Makes the stream of the query's device torch's current one, if it is not."""
     import torch
 
-    if not torch.cuda.is_available():
+    if query.device.index == torch.cuda.current_device() and int(stream) == torch.cuda.current_stream().cuda_stream:
+        return nullcontext()
+    return torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=query.device))
+
+
+def _capturing(query, stream) -> bool:
+    if not query.is_cuda:
         return False
-    with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=query.device)):
-        return torch.cuda.is_current_stream_capturing()
+    status = ctypes.c_int()
+    # of the HIP runtime that the library is linked to; asking through torch takes several microseconds more
+    if load_hip_library().hipStreamIsCapturing(ctypes.c_void_p(int(stream)), ctypes.byref(status)) != 0:
+        raise TriangleMixError(TM_ERR_LAUNCH, "hipStreamIsCapturing failed")
+    return status.value != 0
 
 
 def _buffer(query, need, stream):
     """Memory of the caching allocator that is handed out again in this stream's order."""
     import torch
 
-    with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=query.device)):
+    with _on(query, stream):
         return torch.empty(need, dtype=torch.uint8, device=query.device)
 
 
@@ -198,8 +209,10 @@ def select_pages(query, page_min, page_max, block_table, seq_lens, out, *, sink_
     rows = _rows_per_request(query, batch)
     need = _need(lib.tm_select_pages_workspace_size, batch, rows, heads, kv, cols)
     if workspace is None and need > 0:
+        import torch
+
         # scores that one launch of the call leaves for the next: out of reach of other threads' calls on the stream
-        workspace = _buffer(query, need, st)
+        workspace = _buffer(query, need, st) if stream is not None else query.new_empty(need, dtype=torch.uint8)
     _held, ws_ptr, ws_bytes = _workspace_of(query, need, workspace, st)
     _check(lib.tm_select_pages(
         query.data_ptr(), query.stride(0), page_min.data_ptr(), page_max.data_ptr(), block_table.data_ptr(),
