@@ -61,11 +61,15 @@ HIP_FLAGS = [
 # all-masked row's max is taken as 0).  Host code keeps IEEE NaN
 # semantics: the C ABI rejects a NaN scale.
 NO_NANS_DEFAULT = ["-Xarch_device", "-fno-honor-nans"]
-# The selection ranks scores that are not a number: its file keeps NaN semantics.
-NO_NANS = {"trianglemix_select.hip": []}
+# The selection ranks scores that are not a number, the rotated write keeps NaN in an 8-bit cache: their files keep
+# NaN semantics.
+NO_NANS = {"trianglemix_select.hip": [], "trianglemix_rotary.hip": []}
 
 HIP_SOURCES = ["trianglemix_kernel.hip", "trianglemix_wide.hip", "trianglemix_cache.hip", "trianglemix_rows.hip",
-               "trianglemix_blocks.hip", "trianglemix_select.hip", "trianglemix_capi.cpp", "trianglemix_pages_capi.cpp"]
+               "trianglemix_blocks.hip", "trianglemix_select.hip", "trianglemix_rotary.hip", "trianglemix_cached.hip",
+               "trianglemix_capi.cpp", "trianglemix_pages_capi.cpp", "trianglemix_cached_capi.cpp"]
+
+TORCH_SOURCES = ["trianglemix_torch.cpp", "trianglemix_pages_torch.cpp", "trianglemix_cached_torch.cpp"]
 
 
 def _run(cmd: list[str]) -> None:
@@ -120,7 +124,7 @@ def build_torch_adapter() -> Path:
     tmp = TORCH_LIB.with_suffix(".so.tmp")
     _run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-          *incs, str(CSRC / "trianglemix_torch.cpp"), str(CSRC / "trianglemix_pages_torch.cpp"),
+          *incs, *(str(CSRC / name) for name in TORCH_SOURCES),
           f"-L{PKG}", "-ltrianglemix",
           f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python",
           f"-L{ROCM / 'lib'}", "-lamdhip64",

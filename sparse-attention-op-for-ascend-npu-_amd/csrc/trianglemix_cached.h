@@ -1,0 +1,64 @@
+// Internal interface of the cached-attention operators (position rotation,
+// rotated cache write, attention over the cache) between their host code and
+// their kernels.
+#ifndef TRIANGLEMIX_CACHED_INTERNAL_H
+#define TRIANGLEMIX_CACHED_INTERNAL_H
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "trianglemix_kernel.h"
+#include "trianglemix_pages.h"
+
+namespace tmx {
+
+enum class CacheType { kSame, kE4m3 };  // of the rows' own type, or 8-bit with a scale for each KV head
+
+struct RotateParams {
+  const uint16_t* query;  // [rows, heads, 128]
+  const uint16_t* key;    // [rows, kv_heads, 128]
+  const uint16_t* value;
+  uint16_t* query_out;
+  int64_t query_stride, key_stride, value_stride, out_stride;  // elements
+  const int64_t* positions;
+  const int64_t* slots;
+  const double* frequencies;
+  char* key_cache;
+  char* value_cache;
+  int64_t key_page_stride, value_page_stride;  // bytes
+  const float* key_scale;
+  const float* value_scale;
+  int64_t num_slots;
+  int rows, heads, kv_heads;  // kv_heads 0: rotation alone
+  int rotary_dim;
+  float magnitude;
+};
+hipError_t launch_rotate(const RotateParams& p, bool interleaved, bool fp16, CacheType cache, hipStream_t stream);
+
+struct CachedParams {
+  const uint16_t* query;  // [batch * rows, heads, 128]
+  int64_t query_stride;   // elements
+  const char* key_cache;
+  const char* value_cache;
+  int64_t key_page_stride, value_page_stride;  // bytes
+  const float* key_scale;                      // [kv_heads], or null
+  const float* value_scale;
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* seq_lens;
+  uint16_t* out;  // [batch * rows, heads, 128]
+  unsigned long long* counters;
+  float* partials;
+  unsigned long long epoch;
+  int table_cols, batch, rows, heads, kv_heads, group, num_pages;
+  int window, sinks;  // window -1: all keys
+  int row_parts;      // workgroups' shares of a (request, KV head)'s rows
+  int workgroups;
+  float scale_log2;
+};
+hipError_t launch_cached_attention(const CachedParams& p, int shape_rows, bool fp16, CacheType cache,
+                                   hipStream_t stream);
+
+}  // namespace tmx
+
+#endif  // TRIANGLEMIX_CACHED_INTERNAL_H

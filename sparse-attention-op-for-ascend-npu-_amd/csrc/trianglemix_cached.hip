@@ -1,0 +1,705 @@
+// Attention of the last tokens of each request over its paged cache, of e4m3
+// numbers or of the queries' own 16-bit type, for MI355X (gfx950).
+//
+// Work.  A group is the query rows of a (request, KV head) that one workgroup
+// holds: all heads of the GQA group times the request's tokens, rows numbered
+// token * G + head, cut into row parts of 16 NT.  A unit is one page (128 keys)
+// of one group: the pages of the first `sinks` keys and those from the window's
+// first key of the request's first row on, or all.  The units of all groups, in a
+// row, are dealt to the workgroups in equal contiguous runs, as in
+// trianglemix_lists.h, with the same partials and merge for groups that a run's
+// end cuts: every workgroup streams the same number of pages whatever the lengths,
+// the grid does not depend on them, and the sums do not depend on which workgroup
+// merges them.
+//
+// A workgroup is four waves over the same rows; wave w has keys 32 w .. 32 w + 31
+// of every page.  K and V go from memory into registers, kDepth - 1 tiles ahead:
+// a wave loads what it multiplies itself, so the page loop has neither LDS nor
+// barriers.  The waves' sums meet in LDS behind it.
+//
+// Contractions (per wave, 32 keys x 16 NT rows, v_mfma_f32_16x16x32)
+//   S^T (keys x rows) = K Q^T     A = K, B = Q
+//   O^T (dims x rows) += V^T P^T  A = V^T, B = P
+// Lane l holds row l % 16.  The keys of S^T's two 16-key halves u are dealt so that
+// accumulator element i of half u in lanes of quad l / 16 is key 8 quad + 4 u + i:
+// the lane's eight scores are its eight k-slots of P.  V^T wants, for one dim, eight
+// keys in a lane: lane l loads dims 8 (l % 16) .. + 7 of keys 8 quad .. + 7, a
+// block of 8 x 8 that it transposes in registers (v_perm); product m has the dims
+// 8 i + m (i the operand's row), so that a lane's results are 32 dims in a row.
+// e4m3 numbers become 16-bit ones on the way (v_cvt_scalef32_pk, exact): K of the
+// queries' type, V fp16 with fp16 weights.
+//
+// Numerics: scores, row max, row sum and O in fp32, exponentials as exp2 of
+// scores in units of log2(e); the weights are rounded for the PV product alone.
+// fp16 weights are 2^7 times themselves (at most 2^15, as the row max may be stale
+// by 2^8): what is 2^-31 of the largest is still a number, so that millions of
+// small ones are not lost.  Keys past a page's valid ones are not read (the
+// buffer's range ends there and gives zeros).  In tiles where some row masks a key,
+// V entries that are not finite are kept out of the product and added only to rows
+// that attend them.
+
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "trianglemix_cached.h"
+#include "trianglemix_lists.h"
+
+namespace tmx {
+namespace {
+
+typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * 64;
+
+// Max / sum over the four lanes that hold one row (l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float row_max(float x) {
+  x = half_max(x);
+  const unsigned u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float row_sum(float x) {
+  x = half_sum(x);
+  const unsigned u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The bits of two 16-bit numbers of type Type from two e4m3 ones.
+template <class Type, bool kHigh>
+__device__ __forceinline__ unsigned from_e4m3(unsigned x) {
+  if constexpr (std::is_same_v<Type, Fp16>) {
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, kHigh));
+  } else {
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, kHigh));
+  }
+}
+
+// A wave's share of a page, 32 keys: what its lanes load, and the operands made of it.
+template <class Type, CacheType kCache>
+struct Tile;
+
+template <class Type>
+struct Tile<Type, CacheType::kSame> {
+  typedef Type Weight;  // of P and V^T
+  static constexpr int kElemBytes = 2;
+  u32x4_t k[2][4], v[8];
+
+  // The first of the eight dims of Q's (and K's) operand c.
+  static __device__ __forceinline__ int q_dim(int c, int quad) { return 32 * c + 8 * quad; }
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t vr, const int* k_off,
+                                       const int* v_off) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) k[u][c] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_off[u] + 64 * c, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, v_off[j], 0, 0);
+  }
+  __device__ __forceinline__ i16x8_t k_operand(int u, int c) const { return __builtin_bit_cast(i16x8_t, k[u][c]); }
+  // Dims 2 w and 2 w + 1 of key j's eight.
+  __device__ __forceinline__ unsigned v_pair(int j, int w) const { return v[j][w]; }
+  // Of number i in memory: 0 finite, 1 +infinity, 2 -infinity, 3 NaN.
+  static __device__ __forceinline__ int odd_kind(const char* at, int i) {
+    const unsigned x = reinterpret_cast<const uint16_t*>(at)[i], size = x & 0x7fffu;
+    return size < Type::kExp ? 0 : size > Type::kExp ? 3 : x == size ? 1 : 2;
+  }
+  // Whether some V entry is no finite number.
+  __device__ __forceinline__ bool odd_value() const {
+    typedef unsigned short u16x8_t __attribute__((ext_vector_type(8)));
+    u16x8_t size = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) size = __builtin_elementwise_max(size, __builtin_bit_cast(u16x8_t, v[j] & 0x7fff7fffu));
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) odd |= size[e] >= Type::kExp;
+    return odd;
+  }
+  // V with zeros in the place of what is no finite number.
+  __device__ __forceinline__ void keep_finite() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const unsigned x = v[j][w];
+        v[j][w] = ((x & 0x7fffu) < Type::kExp ? x & 0xffffu : 0) | ((x & 0x7fff0000u) < (Type::kExp << 16) ? x & 0xffff0000u : 0);
+      }
+    }
+  }
+};
+
+template <class Type>
+struct Tile<Type, CacheType::kE4m3> {
+  typedef Fp16 Weight;
+  static constexpr int kElemBytes = 1;
+  u32x4_t k[2][2];
+  u32x2_t v[8];
+
+  // A 16-byte load holds two operands' dims.
+  static __device__ __forceinline__ int q_dim(int c, int quad) { return 64 * (c >> 1) + 16 * quad + 8 * (c & 1); }
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t kr, __amdgpu_buffer_rsrc_t vr, const int* k_off,
+                                       const int* v_off) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) k[u][c] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_off[u] + 64 * c, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __builtin_amdgcn_raw_buffer_load_b64(vr, v_off[j], 0, 0);
+  }
+  __device__ __forceinline__ i16x8_t k_operand(int u, int c) const {
+    const unsigned lo = k[u][c >> 1][2 * (c & 1)], hi = k[u][c >> 1][2 * (c & 1) + 1];
+    const u32x4_t x = {from_e4m3<Type, false>(lo), from_e4m3<Type, true>(lo), from_e4m3<Type, false>(hi),
+                       from_e4m3<Type, true>(hi)};
+    return __builtin_bit_cast(i16x8_t, x);
+  }
+  __device__ __forceinline__ unsigned v_pair(int j, int w) const {
+    return w & 1 ? from_e4m3<Fp16, true>(v[j][w >> 1]) : from_e4m3<Fp16, false>(v[j][w >> 1]);
+  }
+  static __device__ __forceinline__ int odd_kind(const char* at, int i) {
+    return (reinterpret_cast<const uint8_t*>(at)[i] & 0x7f) == 0x7f ? 3 : 0;
+  }
+  __device__ __forceinline__ bool odd_value() const {
+    unsigned odd = 0;  // NaN is 0x7f or 0xff: the only sizes that a one carries into the sign's place
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) odd |= (v[j][w] & 0x7f7f7f7fu) + 0x01010101u;
+    }
+    return (odd & 0x80808080u) != 0;
+  }
+  __device__ __forceinline__ void keep_finite() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const unsigned odd = ((v[j][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        v[j][w] &= ~((odd >> 7) * 0xffu);
+      }
+    }
+  }
+};
+
+// V^T of dims 8 i + 2 w and 8 i + 2 w + 1: the two operands, eight keys each.
+template <class T>
+__device__ __forceinline__ void v_operands(const T& tile, int w, u32x4_t& even, u32x4_t& odd) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned a = tile.v_pair(2 * j, w), b = tile.v_pair(2 * j + 1, w);
+    even[j] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    odd[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+  }
+}
+
+// A request's pages that some row of it may attend: `sink_pages` from the first
+// on, then first_page .. end_page - 1; at least one unit where it has rows.
+struct Pages {
+  int sink_pages, first_page, end_page;
+  __device__ __forceinline__ Pages(const CachedParams& p, int len) {
+    end_page = (min(len, p.table_cols * kPageSize) + kPageSize - 1) / kPageSize;
+    const int first_key = p.window < 0 ? 0 : max(0, max(0, len - p.rows) - p.window);
+    first_page = min(first_key / kPageSize, end_page);
+    sink_pages = min((int)(((unsigned)p.sinks + kPageSize - 1) / kPageSize), first_page);
+  }
+  __device__ __forceinline__ int units(int len) const {
+    return len > 0 ? max(1, sink_pages + end_page - first_page) : 0;
+  }
+  __device__ __forceinline__ int logical(int i) const { return i < sink_pages ? i : first_page + (i - sink_pages); }
+};
+
+typedef const __attribute__((address_space(4))) int32_t* ConstInts;  // read by scalar loads
+
+template <class Type, CacheType kCache, int NT>
+__global__ void __launch_bounds__(kThreads, kCache == CacheType::kE4m3 ? (NT > 2 ? 1 : 2) : (NT > 1 ? 1 : 2)) cached_attention_kernel(const CachedParams p) {
+  typedef Tile<Type, kCache> Share;
+  typedef typename Share::Weight Weight;
+  typedef typename Type::elem elem;
+  constexpr int kRows = 16 * NT;
+  constexpr int kDepth = kCache == CacheType::kE4m3 && NT == 1 ? 3 : 2;  // tiles in registers, the one in use among them
+  constexpr int kHeadBytes = kHeadDim * Share::kElemBytes;
+  constexpr float kWeightBits = std::is_same_v<Weight, Fp16> ? 7.0f : 0.0f;
+  constexpr int kRecord = kRows * (kHeadDim + 2);  // floats of a partial: O, row max, row sum
+
+  __shared__ __attribute__((aligned(16))) float o_lds[kWaves][16 * kHeadDim];
+  __shared__ float s_max[kWaves][kRows], s_sum[kWaves][kRows];
+  __shared__ float join[kThreads][10];
+  __shared__ unsigned s_odd[kRows][3][4];  // note_odd: a bit a dim, for +infinity, -infinity, NaN
+  __shared__ int s_last;
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  const int col = lane & 15;  // row of the wave's 16-row tile
+  const int quad = lane >> 4;
+  const int G = p.group;
+  const int token_bytes = p.kv_heads * kHeadBytes;
+  const int heads_parts = p.kv_heads * p.row_parts;
+
+  auto clear_odd = [&]() {
+    for (int i = tid; i < kRows * 12; i += kThreads) (&s_odd[0][0][0])[i] = 0;
+  };
+  clear_odd();
+  __syncthreads();
+
+  // ---- the plan: requests base .. base + 63 one a lane, their running unit counts ----
+  auto len_of = [&](int b) { return b < p.batch ? max(p.seq_lens[b], 0) : 0; };
+  int base = 0, len64 = 0, upto64 = 0, before64 = 0;  // before64: units of the requests in front of base
+  auto load_requests = [&]() {
+    len64 = len_of(base + lane);
+    upto64 = Pages(p, len64).units(len64) * heads_parts;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int add = __shfl_up(upto64, d);
+      if (lane >= d) upto64 += add;
+    }
+    upto64 += before64;
+  };
+  load_requests();
+  int total = __builtin_amdgcn_readlane(upto64, 63);
+  for (int b = 64; b < p.batch; b += 64) {
+    const int len = len_of(b + lane);
+    int sum = Pages(p, len).units(len) * heads_parts;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+    total += __builtin_amdgcn_readfirstlane(sum);
+  }
+  const int usual = (int)((unsigned)total / (unsigned)(heads_parts * p.batch));
+  const int per_run = max(min_run_units(usual, kRows > kMostStreamRows ? kMostStreamRows : kRows),
+                          (int)((unsigned)(total + p.workgroups - 1) / (unsigned)p.workgroups));
+  const int run = run_of_workgroup();
+  int unit = min(run, total / per_run + 1) * per_run;
+  const int unit_end = min(total, unit + per_run);
+
+  while (unit < unit_end) {
+    // ---- the group, and its units lo .. hi - 1 of this run ----
+    while (__builtin_amdgcn_readlane(upto64, 63) <= unit) {
+      before64 = __builtin_amdgcn_readlane(upto64, 63);
+      base += 64;
+      load_requests();
+    }
+    const int in_block = __ffsll((unsigned long long)__ballot(upto64 > unit)) - 1;
+    const int request = base + in_block;
+    const int len = __builtin_amdgcn_readlane(len64, in_block);
+    const Pages pages(p, len);
+    const int units = pages.units(len);
+    const int id = (unit - (__builtin_amdgcn_readlane(upto64, in_block) - units * heads_parts)) / units;
+    const int first = __builtin_amdgcn_readlane(upto64, in_block) - (heads_parts - id) * units;  // its first unit
+    const int kv_head = id / p.row_parts;
+    const int row_base = (id % p.row_parts) * kRows;
+    const int lo = unit - first, hi = min(unit_end - first, units);
+    const bool whole = lo == 0 && hi == units;
+    const int valid_rows = min(kRows, p.rows * G - row_base);
+    const int pos0 = len - p.rows;  // position of token 0; a negative one is no row
+    const int first_pos = pos0 + row_base / G, last_pos = pos0 + (row_base + valid_rows - 1) / G;
+    const int tokens = min(len, p.table_cols * kPageSize);  // with a key
+
+    // ---- Q ----
+    i16x8_t q[NT][4];
+    int row_pos[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = row_base + 16 * n + col;
+      const int t = (int)((unsigned)r / (unsigned)G);
+      const bool ok = 16 * n + col < valid_rows;
+      row_pos[n] = ok ? pos0 + t : -1;
+      const uint16_t* const from =
+          p.query + (int64_t)(request * p.rows + t) * p.query_stride + (int64_t)(kv_head * G + (r - t * G)) * kHeadDim;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        q[n][c] = i16x8_t{};
+        if (ok) q[n][c] = *reinterpret_cast<const i16x8_t*>(from + Share::q_dim(c, quad));
+      }
+    }
+
+    float c2 = p.scale_log2, v_scale = 1.0f;
+    if constexpr (kCache == CacheType::kE4m3) {
+      c2 *= p.key_scale[kv_head];
+      v_scale = p.value_scale[kv_head];
+    }
+
+    // ---- pages ----
+    const ConstInts table = (ConstInts)(p.block_table + (int64_t)request * p.table_stride);
+    auto entry = [&](int i) {  // page of the cache, or -1
+      int phys = -1;
+      if (i < hi && pages.logical(i) < pages.end_page) phys = table[pages.logical(i)];
+      return (unsigned)phys < (unsigned)p.num_pages ? phys : -1;
+    };
+    int k_off[2], v_off[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) k_off[u] = (32 * wave + 8 * (col >> 2) + 4 * u + (col & 3)) * token_bytes + 16 * quad;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v_off[j] = (32 * wave + 8 * quad + j) * token_bytes + 8 * Share::kElemBytes * col;
+    auto valid_keys = [&](int i, int phys) {
+      return phys < 0 ? 0 : min(kPageSize, tokens - pages.logical(i) * kPageSize);
+    };
+    auto value_page = [&](int phys) {
+      return p.value_cache + max(phys, 0) * p.value_page_stride + kv_head * kHeadBytes;
+    };
+    auto load = [&](Share& t, int i, int phys) {
+      const int valid = valid_keys(i, phys);
+      const int range = valid > 0 ? (valid - 1) * token_bytes + kHeadBytes : 0;
+      const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(p.key_cache + max(phys, 0) * p.key_page_stride + kv_head * kHeadBytes), (short)0, range, kBufferFlags);
+      const __amdgpu_buffer_rsrc_t vr =
+          __builtin_amdgcn_make_buffer_rsrc((void*)value_page(phys), (short)0, range, kBufferFlags);
+      t.load(kr, vr, k_off, v_off);
+    };
+
+    float m_run[NT], l_run[NT];
+    f32x4_t o[8][NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m_run[n] = -INFINITY;
+      l_run[n] = 0.0f;
+#pragma unroll
+      for (int m = 0; m < 8; ++m) o[m][n] = f32x4_t{};
+    }
+
+    // Notes the V entries of a tile that are no finite numbers for the rows that attend
+    // them, apart from the product: 0 * NaN would reach the others too.
+    auto note_odd = [&](int i, int phys) {
+      const int key0 = pages.logical(i) * kPageSize + 32 * wave;
+      const int keys = min(32, valid_keys(i, phys) - 32 * wave);
+      const int pos = pos0 + (int)((unsigned)(row_base + lane) / (unsigned)G);  // of row `lane`
+      const char* at = value_page(phys) + 32 * wave * token_bytes;
+#pragma unroll 1
+      for (int k = 0; k < keys; ++k, at += token_bytes) {
+        const int lower = Share::odd_kind(at, lane), upper = Share::odd_kind(at, lane + 64);
+        const int key = key0 + k;
+        const bool seen =
+            lane < valid_rows && key <= pos && (p.window < 0 || key >= max(pos, 0) - p.window || key < p.sinks);
+#pragma unroll 1
+        for (int kind = 1; kind < 4; ++kind) {
+          const unsigned long long lo64 = __ballot(lower == kind), hi64 = __ballot(upper == kind);
+          if (seen && (lo64 | hi64) != 0) {
+            unsigned* const to = s_odd[lane][kind - 1];
+            atomicOr(to, (unsigned)lo64);
+            atomicOr(to + 1, (unsigned)(lo64 >> 32));
+            atomicOr(to + 2, (unsigned)hi64);
+            atomicOr(to + 3, (unsigned)(hi64 >> 32));
+          }
+        }
+      }
+    };
+
+    auto compute = [&](Share& t, int i, int phys) {
+      const int key0 = pages.logical(i) * kPageSize + 32 * wave;
+      // the first key that the last row's window holds, and that the first row's does
+      const int last_low = p.window < 0 ? 0 : max(last_pos, 0) - p.window;
+      const int first_low = p.window < 0 ? 0 : max(first_pos, 0) - p.window;
+      if (phys < 0 || key0 > last_pos || (key0 + 31 < first_low && key0 >= p.sinks)) return;
+      const bool masked = key0 + 31 > first_pos || (key0 < last_low && key0 + 31 >= p.sinks);
+      f32x4_t s[2][NT];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[u][n] = f32x4_t{};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const i16x8_t a = t.k_operand(u, c);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) s[u][n] = Type::mfma16(a, q[n][c], s[u][n]);
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int low = p.window < 0 ? 0 : max(row_pos[n], 0) - p.window;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int key = key0 + 8 * quad + e;
+            const bool seen = key <= row_pos[n] && (key >= low || key < p.sinks);
+            s[e >> 2][n][e & 3] = seen ? s[e >> 2][n][e & 3] : -INFINITY;
+          }
+        }
+      }
+      i16x8_t pb[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, s[e >> 2][n][e & 3]);
+        top = row_max(top) * c2;
+        if (__any(top > m_run[n] + kLazyRescale)) {
+          const float m_new = fmaxf(m_run[n], top);
+          const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run[n] - m_new);
+          l_run[n] *= alpha;
+#pragma unroll
+          for (int m = 0; m < 8; ++m) o[m][n] *= alpha;
+          m_run[n] = m_new;
+        }
+        const float shift = kWeightBits - (m_run[n] == -INFINITY ? 0.0f : m_run[n]);
+        typename Weight::vec weight;
+        float add = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][n][e & 3], c2, shift));
+          add += x;
+          weight[e] = (typename Weight::elem)x;
+        }
+        l_run[n] += add;
+        pb[n] = __builtin_bit_cast(i16x8_t, weight);
+      }
+      if (masked && __builtin_expect(__any(t.odd_value()) != 0, 0)) {
+        note_odd(i, phys);
+        t.keep_finite();
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        __builtin_amdgcn_sched_barrier(0);
+        u32x4_t even, odd;
+        v_operands(t, w, even, odd);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          o[2 * w][n] = Weight::mfma16(__builtin_bit_cast(i16x8_t, even), pb[n], o[2 * w][n]);
+          o[2 * w + 1][n] = Weight::mfma16(__builtin_bit_cast(i16x8_t, odd), pb[n], o[2 * w + 1][n]);
+        }
+      }
+    };
+
+    // Tile slot s holds page i + s; the page kDepth - 1 ahead is on its way.
+    Share tile[kDepth];
+    int phys[kDepth];
+#pragma unroll
+    for (int s = 0; s < kDepth; ++s) phys[s] = entry(lo + s);
+#pragma unroll
+    for (int s = 0; s + 1 < kDepth; ++s) load(tile[s], lo + s, phys[s]);
+    for (int i = lo; i < hi; i += kDepth) {
+#pragma unroll
+      for (int s = 0; s < kDepth; ++s) {
+        constexpr int kAhead = kDepth - 1;
+        const int slot = (s + kAhead) % kDepth;
+        load(tile[slot], i + s + kAhead, phys[slot]);
+        const int own = phys[s];
+        phys[s] = entry(i + s + kDepth);
+        if (i + s < hi) compute(tile[s], i + s, own);
+      }
+    }
+
+    // ---- the waves' sums, 16 rows at a time through LDS ----
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float l = row_sum(l_run[n]);
+      m_run[n] = row_shift(m_run[n], l);
+      if (quad == 0) {
+        s_max[wave][16 * n + col] = m_run[n];
+        s_sum[wave][16 * n + col] = l;
+      }
+    }
+    // 16 threads a row, 8 dims each.
+    const int r16 = tid >> 4, c8 = tid & 15;
+    auto store_row = [&](int r, const float* acc, float l) {
+      const int at = row_base + r;
+      const int t = (int)((unsigned)at / (unsigned)G);
+      if (pos0 + t < 0) return;  // before the request's first token: no row
+      const float inv = l > 0.0f ? v_scale / l : 0.0f;
+      // a NaN sum fails the comparison, and must reach the result
+      const float scale = (__float_as_uint(l) & 0x7fffffffu) > 0x7f800000u ? l : inv;
+      typename Type::vec y;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = (elem)(acc[e] * scale);
+      *reinterpret_cast<typename Type::vec*>(
+          p.out + ((int64_t)(request * p.rows + t) * p.heads + kv_head * G + (at - t * G)) * kHeadDim + 8 * c8) = y;
+    };
+    // the workgroups that share the group, and where their partials lie
+    const int first_run = (int)((unsigned)first / (unsigned)per_run);
+    const int last_run = (int)((unsigned)(first + units - 1) / (unsigned)per_run);
+    auto record = [&](int r) { return (unsigned)(2 * r + (r == first_run ? 1 : 0)) * (kRecord * 4u); };
+    const __amdgpu_buffer_rsrc_t rec = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)p.partials, (short)0, whole ? 0 : (int)((unsigned)p.workgroups * 2u * (kRecord * 4u)), kBufferFlags);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      __syncthreads();
+      if (16 * n >= valid_rows) break;
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) top = fmaxf(top, s_max[k][16 * n + col]);
+      const float weight = m_run[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - top);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {  // dims 32 quad + 8 e + 4 half ..
+          f32x4_t x;
+#pragma unroll
+          for (int m = 0; m < 4; ++m) x[m] = m_run[n] == -INFINITY ? 0.0f : o[4 * half + m][n][e] * weight;
+          const int chunk = (8 * quad + 2 * e + half) ^ col;
+          *reinterpret_cast<f32x4_t*>(&o_lds[wave][col * kHeadDim + 4 * chunk]) = x;
+        }
+      }
+      __syncthreads();
+      const int r = 16 * n + r16;
+      if (r < valid_rows) {
+        float all = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) all = fmaxf(all, s_max[k][r]);
+        float l = 0.0f, acc[8] = {};
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+          const float mk = s_max[k][r];
+          l += mk == -INFINITY ? 0.0f : s_sum[k][r] * __builtin_amdgcn_exp2f(mk - all);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const f32x4_t x =
+                *reinterpret_cast<const f32x4_t*>(&o_lds[k][r16 * kHeadDim + 4 * ((2 * c8 + half) ^ r16)]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[4 * half + e] += x[e];
+          }
+        }
+#pragma unroll
+        for (int kind = 0; kind < 3; ++kind) {
+          const unsigned odd = s_odd[r][kind][c8 >> 2] >> (8 * (c8 & 3)) & 0xffu;
+          // bits, and no number that is taken for finite
+          float value = __uint_as_float(kind == 0 ? 0x7f800000u : kind == 1 ? 0xff800000u : 0x7fc00000u);
+          asm volatile("" : "+v"(value));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] += odd >> e & 1 ? value : 0.0f;
+        }
+        if (whole) {
+          store_row(r, acc, l);
+        } else {
+          const unsigned at = record(run);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const f32x4_t x = {acc[4 * half], acc[4 * half + 1], acc[4 * half + 2], acc[4 * half + 3]};
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, x), rec,
+                                                   at + (r * kHeadDim + 8 * c8 + 4 * half) * 4, 0, kCpolAgent);
+          }
+          if (c8 == 0) {
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(all), rec, at + (kRows * kHeadDim + r) * 4, 0,
+                                                  kCpolAgent);
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), rec, at + (kRows * (kHeadDim + 1) + r) * 4, 0,
+                                                  kCpolAgent);
+          }
+        }
+      }
+    }
+
+    if (!whole) {
+      // ---- the workgroup that arrives last merges ----
+      wait_dma();  // this wave's partial stores have completed
+      __syncthreads();
+      unsigned long long* const word = p.counters + first_run;
+      if (tid == 0) {
+        s_last = (int)(count_arrival(word, p.epoch) == (unsigned long long)(last_run - first_run + 1));
+      }
+      __syncthreads();
+      if (s_last) {
+        // The word is left at this launch's tag with a count of zero for the next one.
+        if (tid == 0) __hip_atomic_store(word, p.epoch << kEpochShift, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // 16 threads a row again; where the rows leave threads over, they share a
+        // row's partials (part pg of `parts` takes every parts-th) and join through
+        // LDS.  Four partials' loads are in flight at a time.
+        int row_slots = 1;
+        while (row_slots < valid_rows && row_slots < kThreads / 16) row_slots *= 2;
+        const int parts = kThreads / 16 / row_slots;
+        const int pg = r16 / row_slots;
+        for (int rb = 0; rb < valid_rows; rb += row_slots) {
+          const int r = rb + r16 % row_slots;
+          float top = -INFINITY, l = 0.0f, acc[8] = {};
+          if (r < valid_rows) {
+            for (int s0 = first_run + pg; s0 <= last_run; s0 += 4 * parts) {
+              float ms[4], ls[4];
+              f32x4_t x[4][2];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                // past the last one its loads fall outside the buffer's range
+                const int s = s0 + j * parts;
+                const unsigned at = s <= last_run ? record(s) : kOutOfRange;
+                ms[j] = __uint_as_float(
+                    __builtin_amdgcn_raw_buffer_load_b32(rec, at + (kRows * kHeadDim + r) * 4, 0, kCpolAgent));
+                ls[j] = __uint_as_float(
+                    __builtin_amdgcn_raw_buffer_load_b32(rec, at + (kRows * (kHeadDim + 1) + r) * 4, 0, kCpolAgent));
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  x[j][half] = __builtin_bit_cast(
+                      f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                   rec, at + (r * kHeadDim + 8 * c8 + 4 * half) * 4, 0, kCpolAgent));
+                }
+              }
+              float next = top;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if (s0 + j * parts > last_run) ms[j] = -INFINITY;
+                next = fmaxf(next, ms[j]);
+              }
+              const float shift = next == -INFINITY ? 0.0f : next;
+              const float keep = __builtin_amdgcn_exp2f(top - shift);
+              l *= keep;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) acc[e] *= keep;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float w = __builtin_amdgcn_exp2f(ms[j] - shift);
+                l += ls[j] * w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[e] += x[j][e >> 2][e & 3] * w;
+              }
+              top = next;
+            }
+          }
+          if (parts > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) join[tid][e] = acc[e];
+            join[tid][8] = top;
+            join[tid][9] = l;
+            __syncthreads();
+            if (pg == 0) {
+              float all = top;
+              for (int k = 1; k < parts; ++k) all = fmaxf(all, join[tid + k * 16 * row_slots][8]);
+              const float shift = all == -INFINITY ? 0.0f : all;
+              const float keep = __builtin_amdgcn_exp2f(top - shift);
+              l *= keep;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) acc[e] *= keep;
+              for (int k = 1; k < parts; ++k) {
+                const float* const from = join[tid + k * 16 * row_slots];
+                const float w = __builtin_amdgcn_exp2f(from[8] - shift);
+                l += from[9] * w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[e] += from[e] * w;
+              }
+            }
+          }
+          if (pg == 0 && r < valid_rows) store_row(r, acc, l);
+        }
+      }
+    }
+    unit = first + hi;
+    __syncthreads();
+    clear_odd();
+    __syncthreads();
+  }
+}
+
+template <class Type, CacheType kCache>
+hipError_t launch_shape(const CachedParams& p, int shape_rows, hipStream_t stream) {
+  const dim3 grid((unsigned)p.workgroups), block(kThreads);
+  switch (shape_rows) {
+    case 16: hipLaunchKernelGGL((cached_attention_kernel<Type, kCache, 1>), grid, block, 0, stream, p); break;
+    case 32: hipLaunchKernelGGL((cached_attention_kernel<Type, kCache, 2>), grid, block, 0, stream, p); break;
+    case 64: hipLaunchKernelGGL((cached_attention_kernel<Type, kCache, 4>), grid, block, 0, stream, p); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_cached_attention(const CachedParams& p, int shape_rows, bool fp16, CacheType cache,
+                                   hipStream_t stream) {
+  if (cache == CacheType::kE4m3) {
+    return fp16 ? launch_shape<Fp16, CacheType::kE4m3>(p, shape_rows, stream)
+                : launch_shape<Bf16, CacheType::kE4m3>(p, shape_rows, stream);
+  }
+  return fp16 ? launch_shape<Fp16, CacheType::kSame>(p, shape_rows, stream)
+              : launch_shape<Bf16, CacheType::kSame>(p, shape_rows, stream);
+}
+
+}  // namespace tmx

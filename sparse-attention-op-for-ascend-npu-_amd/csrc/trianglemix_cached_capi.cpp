@@ -1,0 +1,308 @@
+// C ABI of the cached-attention operators (include/trianglemix_cached.h): host
+// checks and launch geometry.  Every check runs before any HIP call.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "../../include/trianglemix_cached.h"
+#include "trianglemix_cached.h"
+#include "trianglemix_checks.h"
+
+namespace {
+
+using namespace tmx;
+
+// Rows of `width` bytes, `stride` bytes apart.
+struct Rows {
+  const void* at;
+  int64_t stride, width, rows;
+  const char* name;
+  Range range() const { return {at, rows > 0 ? (rows - 1) * stride + width : 0, name}; }
+};
+
+// Views of one buffer whose rows lie side by side (a fused projection) do not
+// overlap, though their ranges do.
+bool overlap(const Rows& a, const Rows& b) {
+  if (!tmx::overlap(a.range(), b.range())) return false;
+  if (a.rows == 1 && b.rows == 1) return true;
+  const int64_t stride = a.rows > 1 ? a.stride : b.stride;
+  if (stride <= 0 || (a.rows > 1 && b.rows > 1 && a.stride != b.stride)) return true;
+  const int64_t apart = (int64_t)((uintptr_t)b.at - (uintptr_t)a.at) % stride;
+  const int64_t behind = apart < 0 ? apart + stride : apart;  // b's rows begin so far behind a's
+  return behind < a.width || behind + b.width > stride;
+}
+
+bool same(const Rows& a, const Rows& b) { return a.at == b.at && (a.rows <= 1 || a.stride == b.stride); }
+
+int refuse_overlap(const char* a, const char* b) {
+  return report(TM_ERR_INVALID_ARGUMENT, "%s must not overlap %s", a, b);
+}
+
+int check_rotation(int64_t rows, int64_t rotary_dim, float magnitude) {
+  if (rows < 0) return report(TM_ERR_INVALID_ARGUMENT, "sizes must not be negative");
+  if (rows > kMaxRows) return report(TM_ERR_UNSUPPORTED, "more than %lld rows", (long long)kMaxRows);
+  if (rotary_dim < 16 || rotary_dim > kHeadDim || rotary_dim % 16 != 0) {
+    return report(TM_ERR_UNSUPPORTED, "rotary_dim must be a multiple of 16 from 16 to %d", kHeadDim);
+  }
+  if (!std::isfinite(magnitude)) return report(TM_ERR_INVALID_ARGUMENT, "magnitude must be finite");
+  return TM_OK;
+}
+
+// The cache's type and scales.
+int check_cache_type(int dtype, int cache_dtype, const void* key_scale, const void* value_scale, CacheType* type) {
+  *type = cache_dtype == TM_E4M3 ? CacheType::kE4m3 : CacheType::kSame;
+  if (cache_dtype != TM_E4M3 && cache_dtype != dtype) {
+    return report(TM_ERR_INVALID_ARGUMENT, "the caches must hold numbers of the rows' type or TM_E4M3 ones");
+  }
+  if (cache_dtype == TM_E4M3) {
+    int st = check_element(key_scale, 4);
+    return st == TM_OK ? check_element(value_scale, 4) : st;
+  }
+  if (key_scale || value_scale) return report(TM_ERR_INVALID_ARGUMENT, "caches of the rows' type have no scales");
+  return TM_OK;
+}
+
+int elem_bytes(CacheType type) { return type == CacheType::kE4m3 ? 1 : 2; }
+
+int64_t pages_of(int64_t tokens) { return (tokens + kPageSize - 1) / kPageSize; }
+
+struct CachedPlan {
+  int shape, row_parts, workgroups;
+  int64_t units, workspace_bytes;
+};
+
+int check_cached(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t table_cols, int64_t window,
+                 int64_t sinks) {
+  int st = check_batch(batch, rows, batch * std::max<int64_t>(rows, 0));
+  if (st == TM_OK) st = check_heads(heads, kv_heads);
+  if (st == TM_OK) st = check_table(table_cols, table_cols, batch);
+  if (st != TM_OK) return st;
+  if (window < -1 || sinks < 0 || (window == -1 && sinks != 0)) {
+    return report(TM_ERR_INVALID_ARGUMENT, "window must be -1 (all keys, sinks 0) or more, sinks must not be negative");
+  }
+  return TM_OK;
+}
+
+// The pages that a request's rows can attend at most, its own included.
+int64_t most_units(int64_t rows, int64_t table_cols, int64_t window, int64_t sinks) {
+  if (window < 0 || window >= table_cols * kPageSize) return table_cols;
+  return std::min(table_cols, pages_of(window + rows - 1) + 1 + pages_of(std::min(sinks, table_cols * kPageSize)));
+}
+
+CachedPlan cached_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t table_cols, int64_t window,
+                       int64_t sinks) {
+  CachedPlan r;
+  const int64_t group_rows = rows * (heads / kv_heads);
+  r.shape = group_rows <= 16 ? 16 : group_rows <= 32 ? 32 : 64;
+  r.row_parts = (int)((group_rows + r.shape - 1) / r.shape);
+  r.units = batch * kv_heads * r.row_parts * most_units(rows, table_cols, window, sinks);
+  r.workgroups = (int)((std::min<int64_t>(2 * kComputeUnits, r.units) + 7) / 8 * 8);
+  r.workspace_bytes = kCounterBytes + 2 * int64_t(r.workgroups) * r.shape * (kHeadDim + 2) * 4;
+  return r;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tm_rotate_positions(const void* x, int64_t x_stride, const int64_t* positions, const double* frequencies,
+                        void* out, int64_t out_stride, int64_t rows, int64_t heads, int64_t rotary_dim,
+                        int interleaved, float magnitude, int dtype, void* stream) {
+  int st = check_dtype(dtype);
+  if (st == TM_OK) st = check_rotation(rows, rotary_dim, magnitude);
+  if (st == TM_OK) st = check_heads(heads, heads);
+  if (st == TM_OK) st = check_stride(x_stride, heads * kHeadDim, rows, "x");
+  if (st == TM_OK) st = check_stride(out_stride, heads * kHeadDim, rows, "out");
+  if (st != TM_OK || rows == 0) return st;
+  st = check_aligned({x, out});
+  if (st == TM_OK) st = check_element(positions, 8);
+  if (st == TM_OK) st = check_element(frequencies, 8);
+  if (st != TM_OK) return st;
+  const Rows from{x, x_stride * 2, heads * kHeadBytes, rows, "x"}, to{out, out_stride * 2, heads * kHeadBytes, rows, "out"};
+  if (!same(from, to) && overlap(to, from)) return refuse_overlap("out", "x");
+  const Range written[] = {to.range()};
+  const Range read[] = {{positions, rows * 8, "positions"}, {frequencies, rotary_dim / 2 * 8, "frequencies"}};
+  st = check_overlap(written, read);
+  if (st != TM_OK) return st;
+  RotateParams p{};
+  p.query = static_cast<const uint16_t*>(x);
+  p.query_out = static_cast<uint16_t*>(out);
+  p.query_stride = x_stride;
+  p.out_stride = out_stride;
+  p.positions = positions;
+  p.frequencies = frequencies;
+  p.rows = (int)rows;
+  p.heads = (int)heads;
+  p.rotary_dim = (int)rotary_dim;
+  p.magnitude = magnitude;
+  return launched(launch_rotate(p, interleaved != 0, dtype == TM_FP16, CacheType::kSame, static_cast<hipStream_t>(stream)));
+}
+
+int tm_rotate_and_cache(const void* query, int64_t query_stride, const void* key, int64_t key_stride,
+                        const void* value, int64_t value_stride, const int64_t* positions,
+                        const int64_t* slot_mapping, const double* frequencies, void* query_out,
+                        int64_t query_out_stride, void* key_cache, int64_t key_page_stride, void* value_cache,
+                        int64_t value_page_stride, const float* key_scale, const float* value_scale, int64_t rows,
+                        int64_t heads, int64_t kv_heads, int64_t num_pages, int64_t rotary_dim, int interleaved,
+                        float magnitude, int dtype, int cache_dtype, void* stream) {
+  int st = check_dtype(dtype);
+  if (st == TM_OK) st = check_rotation(rows, rotary_dim, magnitude);
+  if (st == TM_OK) st = check_heads(heads, kv_heads);
+  CacheType type;
+  if (st == TM_OK) st = check_cache_type(dtype, cache_dtype, key_scale, value_scale, &type);
+  if (st == TM_OK) st = check_cache(num_pages, key_page_stride, kv_heads, "key_cache", elem_bytes(type));
+  if (st == TM_OK) st = check_cache(num_pages, value_page_stride, kv_heads, "value_cache", elem_bytes(type));
+  if (st == TM_OK) st = check_stride(query_stride, heads * kHeadDim, rows, "query");
+  if (st == TM_OK) st = check_stride(key_stride, kv_heads * kHeadDim, rows, "key");
+  if (st == TM_OK) st = check_stride(value_stride, kv_heads * kHeadDim, rows, "value");
+  if (st == TM_OK) st = check_stride(query_out_stride, heads * kHeadDim, rows, "query_out");
+  if (st != TM_OK || rows == 0) return st;
+  st = check_aligned({query, key, value, query_out, key_cache, value_cache});
+  if (st == TM_OK) st = check_element(positions, 8);
+  if (st == TM_OK) st = check_element(slot_mapping, 8);
+  if (st == TM_OK) st = check_element(frequencies, 8);
+  if (st != TM_OK) return st;
+  const Rows out{query_out, query_out_stride * 2, heads * kHeadBytes, rows, "query_out"};
+  const Rows q{query, query_stride * 2, heads * kHeadBytes, rows, "query"};
+  const Rows k{key, key_stride * 2, kv_heads * kHeadBytes, rows, "key"};
+  const Rows v{value, value_stride * 2, kv_heads * kHeadBytes, rows, "value"};
+  if (!same(q, out) && overlap(out, q)) return refuse_overlap("query_out", "query");
+  for (const Rows& other : {k, v}) {
+    if (overlap(out, other)) return refuse_overlap("query_out", other.name);
+  }
+  const Range written[] = {
+      out.range(),
+      {key_cache, cache_bytes(num_pages, key_page_stride, kv_heads, elem_bytes(type)), "key_cache"},
+      {value_cache, cache_bytes(num_pages, value_page_stride, kv_heads, elem_bytes(type)), "value_cache"}};
+  const Range small[] = {{positions, rows * 8, "positions"},
+                         {slot_mapping, rows * 8, "slot_mapping"},
+                         {frequencies, rotary_dim / 2 * 8, "frequencies"},
+                         {key_scale, key_scale ? kv_heads * 4 : 0, "key_scale"},
+                         {value_scale, value_scale ? kv_heads * 4 : 0, "value_scale"}};
+  for (const Range& cache : {written[1], written[2]}) {
+    for (const Rows& rows_read : {q, k, v}) {
+      if (tmx::overlap(cache, rows_read.range())) return refuse_overlap(cache.name, rows_read.name);
+    }
+  }
+  const bool interleaved_pages = key_page_stride == value_page_stride && num_pages > 1;
+  const Rows key_pages{key_cache, key_page_stride * elem_bytes(type), kPageSize * kv_heads * kHeadDim * elem_bytes(type),
+                       num_pages, "key_cache"};
+  const Rows value_pages{value_cache, value_page_stride * elem_bytes(type),
+                         kPageSize * kv_heads * kHeadDim * elem_bytes(type), num_pages, "value_cache"};
+  if (interleaved_pages ? overlap(key_pages, value_pages) : tmx::overlap(written[1], written[2])) {
+    return refuse_overlap("key_cache", "value_cache");
+  }
+  for (const Range& w : written) {
+    const Range one[] = {w};
+    st = check_overlap(one, small);
+    if (st != TM_OK) return st;
+  }
+  for (const Range& cache : {written[1], written[2]}) {
+    if (tmx::overlap(written[0], cache)) return refuse_overlap("query_out", cache.name);
+  }
+  RotateParams p{};
+  p.query = static_cast<const uint16_t*>(query);
+  p.key = static_cast<const uint16_t*>(key);
+  p.value = static_cast<const uint16_t*>(value);
+  p.query_out = static_cast<uint16_t*>(query_out);
+  p.query_stride = query_stride;
+  p.key_stride = key_stride;
+  p.value_stride = value_stride;
+  p.out_stride = query_out_stride;
+  p.positions = positions;
+  p.slots = slot_mapping;
+  p.frequencies = frequencies;
+  p.key_cache = static_cast<char*>(key_cache);
+  p.value_cache = static_cast<char*>(value_cache);
+  p.key_page_stride = key_page_stride * elem_bytes(type);
+  p.value_page_stride = value_page_stride * elem_bytes(type);
+  p.key_scale = key_scale;
+  p.value_scale = value_scale;
+  p.num_slots = num_pages * kPageSize;
+  p.rows = (int)rows;
+  p.heads = (int)heads;
+  p.kv_heads = (int)kv_heads;
+  p.rotary_dim = (int)rotary_dim;
+  p.magnitude = magnitude;
+  return launched(launch_rotate(p, interleaved != 0, dtype == TM_FP16, type, static_cast<hipStream_t>(stream)));
+}
+
+int64_t tm_cached_attention_workspace_size(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads,
+                                           int64_t table_cols, int64_t window, int64_t sinks) {
+  report(TM_OK, "%s", "");
+  if (check_cached(batch, rows, heads, kv_heads, table_cols, window, sinks) != TM_OK) return -1;
+  if (batch == 0 || rows == 0) return 0;
+  const CachedPlan plan = cached_plan(batch, rows, heads, kv_heads, table_cols, window, sinks);
+  return check_units(plan.units) == TM_OK ? plan.workspace_bytes : -1;
+}
+
+int tm_cached_attention(const void* query, int64_t query_stride, const void* key_cache, int64_t key_page_stride,
+                        const void* value_cache, int64_t value_page_stride, const float* key_scale,
+                        const float* value_scale, const int32_t* block_table, int64_t table_stride,
+                        const int32_t* seq_lens, void* out, int64_t batch, int64_t rows, int64_t heads,
+                        int64_t kv_heads, int64_t table_cols, int64_t num_pages, int64_t window, int64_t sinks,
+                        float scale, int dtype, int cache_dtype, void* workspace, int64_t workspace_bytes,
+                        void* stream) {
+  int st = check_dtype(dtype);
+  if (st == TM_OK) st = check_cached(batch, rows, heads, kv_heads, table_cols, window, sinks);
+  if (st == TM_OK) st = check_table(table_cols, table_stride, batch);
+  CacheType type;
+  if (st == TM_OK) st = check_cache_type(dtype, cache_dtype, key_scale, value_scale, &type);
+  if (st == TM_OK) st = check_cache(num_pages, key_page_stride, kv_heads, "key_cache", elem_bytes(type));
+  if (st == TM_OK) st = check_cache(num_pages, value_page_stride, kv_heads, "value_cache", elem_bytes(type));
+  if (st == TM_OK) st = check_stride(query_stride, heads * kHeadDim, batch * rows, "query");
+  if (st == TM_OK) st = check_scale(scale);
+  if (st != TM_OK || batch == 0 || rows == 0) return st;
+  st = check_aligned({query, key_cache, value_cache, out});
+  if (st == TM_OK) st = check_element(block_table, 4);
+  if (st == TM_OK) st = check_element(seq_lens, 4);
+  if (st != TM_OK) return st;
+  const CachedPlan plan = cached_plan(batch, rows, heads, kv_heads, table_cols, window, sinks);
+  st = check_units(plan.units);
+  if (st == TM_OK) st = check_workspace(workspace, workspace_bytes, plan.workspace_bytes);
+  if (st != TM_OK) return st;
+  const Range written[] = {{out, batch * rows * heads * kHeadBytes, "out"},
+                           {workspace, plan.workspace_bytes, "workspace"}};
+  const Range read[] = {
+      {query, rows_bytes(batch * rows, query_stride, heads * kHeadDim), "query"},
+      {key_cache, cache_bytes(num_pages, key_page_stride, kv_heads, elem_bytes(type)), "key_cache"},
+      {value_cache, cache_bytes(num_pages, value_page_stride, kv_heads, elem_bytes(type)), "value_cache"},
+      {key_scale, key_scale ? kv_heads * 4 : 0, "key_scale"},
+      {value_scale, value_scale ? kv_heads * 4 : 0, "value_scale"},
+      {block_table, table_bytes(batch, table_stride, table_cols), "block_table"},
+      {seq_lens, batch * 4, "seq_lens"}};
+  st = check_overlap(written, read);
+  if (st != TM_OK) return st;
+  CachedParams p{};
+  p.query = static_cast<const uint16_t*>(query);
+  p.query_stride = query_stride;
+  p.key_cache = static_cast<const char*>(key_cache);
+  p.value_cache = static_cast<const char*>(value_cache);
+  p.key_page_stride = key_page_stride * elem_bytes(type);
+  p.value_page_stride = value_page_stride * elem_bytes(type);
+  p.key_scale = key_scale;
+  p.value_scale = value_scale;
+  p.block_table = block_table;
+  p.table_stride = table_stride;
+  p.seq_lens = seq_lens;
+  p.out = static_cast<uint16_t*>(out);
+  p.counters = static_cast<unsigned long long*>(workspace);
+  p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
+  p.epoch = workspace_tag(workspace);
+  p.table_cols = (int)table_cols;
+  p.batch = (int)batch;
+  p.rows = (int)rows;
+  p.heads = (int)heads;
+  p.kv_heads = (int)kv_heads;
+  p.group = (int)(heads / kv_heads);
+  p.num_pages = (int)num_pages;
+  p.window = (int)(window >= INT32_MAX ? -1 : window);  // past every position: all keys
+  p.sinks = (int)std::min<int64_t>(sinks, table_cols * kPageSize);
+  p.row_parts = plan.row_parts;
+  p.workgroups = plan.workgroups;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  return launched(launch_cached_attention(p, plan.shape, dtype == TM_FP16, type, static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"

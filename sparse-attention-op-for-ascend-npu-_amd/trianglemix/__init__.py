@@ -11,7 +11,8 @@ plus ``router`` (per-layer routing), ``vllm_rocm`` (the vLLM-ROCm seam:
 ``register`` patches vLLM v1's Triton attention backend), ``counters``
 (structured counter log and its run aggregator), ``cache`` (paged KV write),
 ``pages`` (attention over selected pages), ``tree`` (attention of draft
-trees), ``calibrate`` (crossover gates), ``cabi`` (C ABI binding) and
+trees), ``rotary`` (position rotation, rotated cache write), ``cached``
+(attention over 8-bit and 16-bit caches), ``calibrate`` (crossover gates), ``cabi`` (C ABI binding) and
 ``workload`` (seeded synthetic chunks, work accounting).
 """
 

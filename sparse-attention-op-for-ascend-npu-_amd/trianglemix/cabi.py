@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABI in ``include/trianglemix.h`` and ``include/trianglemix_pages.h``.
+"""ctypes binding of the C ABI in ``include/trianglemix.h``, ``include/trianglemix_pages.h`` and
+``include/trianglemix_cached.h``.
 
 For callers that do not go through ``torch.ops`` (and for the parity tests,
 which exercise the C boundary directly).  Tensors are only used for their
@@ -250,3 +251,50 @@ def tree_attention(query, key, value, key_cache, value_cache, block_table, conte
         block_table.data_ptr(), block_table.stride(0), context_lens.data_ptr(), tree_offsets.data_ptr(),
         tree_mask.data_ptr(), out.data_ptr(), total, batch, heads, kv, cols, key_cache.shape[0], float(scale),
         _dtype(query), ws_ptr, ws_bytes, st))
+
+
+def _cache_dtype(tensor) -> int:
+    import torch
+
+    return 2 if tensor.dtype is torch.float8_e4m3fn else _dtype(tensor)  # TM_E4M3
+
+
+def _pointer(tensor):
+    return None if tensor is None else tensor.data_ptr()
+
+
+def rotate_positions(x, positions, freqs, out, *, interleaved: bool = False, magnitude: float = 1.0, stream=None) -> None:
+    """``rotary.rotate`` through the C ABI."""
+    lib = load_hip_library()
+    _check(lib.tm_rotate_positions(
+        x.data_ptr(), x.stride(0), positions.data_ptr(), freqs.data_ptr(), out.data_ptr(), out.stride(0), x.shape[0],
+        x.shape[1], 2 * freqs.shape[0], int(interleaved), float(magnitude), _dtype(x), _stream(x, stream)))
+
+
+def rotate_and_cache(query, key, value, positions, slot_mapping, freqs, query_out, key_cache, value_cache, *,
+                     interleaved: bool = False, magnitude: float = 1.0, key_scale=None, value_scale=None,
+                     stream=None) -> None:
+    """``rotary.rotate_and_cache`` through the C ABI."""
+    lib = load_hip_library()
+    _check(lib.tm_rotate_and_cache(
+        query.data_ptr(), query.stride(0), key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0),
+        positions.data_ptr(), slot_mapping.data_ptr(), freqs.data_ptr(), query_out.data_ptr(), query_out.stride(0),
+        key_cache.data_ptr(), key_cache.stride(0), value_cache.data_ptr(), value_cache.stride(0), _pointer(key_scale),
+        _pointer(value_scale), query.shape[0], query.shape[1], key_cache.shape[2], key_cache.shape[0], 2 * freqs.shape[0],
+        int(interleaved), float(magnitude), _dtype(query), _cache_dtype(key_cache), _stream(query, stream)))
+
+
+def cached_attention(query, key_cache, value_cache, block_table, seq_lens, out, *, scale: float, window: int = -1,
+                     sinks: int = 0, key_scale=None, value_scale=None, stream=None, workspace=None) -> None:
+    """``cached.cached_attention`` through the C ABI."""
+    lib = load_hip_library()
+    st = _stream(query, stream)
+    (batch, cols), heads, kv = block_table.shape, query.shape[1], key_cache.shape[2]
+    rows = _rows_per_request(query, batch)
+    need = _need(lib.tm_cached_attention_workspace_size, batch, rows, heads, kv, cols, window, sinks)
+    _held, ws_ptr, ws_bytes = _workspace_of(query, need, workspace, st)
+    _check(lib.tm_cached_attention(
+        query.data_ptr(), query.stride(0), key_cache.data_ptr(), key_cache.stride(0), value_cache.data_ptr(),
+        value_cache.stride(0), _pointer(key_scale), _pointer(value_scale), block_table.data_ptr(), block_table.stride(0),
+        seq_lens.data_ptr(), out.data_ptr(), batch, rows, heads, kv, cols, key_cache.shape[0], window, sinks, float(scale),
+        _dtype(query), _cache_dtype(key_cache), ws_ptr, ws_bytes, st))

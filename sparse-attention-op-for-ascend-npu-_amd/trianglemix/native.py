@@ -91,12 +91,18 @@ def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
         "tm_selected_page_attention": [vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, *[i64] * 7, f32, i32, vp, i64, vp],
         "tm_tree_attention": [vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, *[i64] * 6, f32, i32,
                               vp, i64, vp],
+        "tm_rotate_positions": [vp, i64, vp, vp, vp, *[i64] * 4, i32, f32, i32, vp],
+        "tm_rotate_and_cache": [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, i64, vp, i64, vp, vp, *[i64] * 5, i32,
+                                f32, i32, i32, vp],
+        "tm_cached_attention": [vp, i64, vp, i64, vp, i64, vp, vp, vp, i64, vp, vp, *[i64] * 8, f32, i32, i32, vp, i64, vp],
     }.items():
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name).argtypes = args
     for name in ("tm_select_pages", "tm_selected_page_attention", "tm_tree_attention"):
         size = getattr(lib, f"{name}_workspace_size")
         size.restype, size.argtypes = i64, [i64] * 5
+    lib.tm_cached_attention_workspace_size.restype = i64
+    lib.tm_cached_attention_workspace_size.argtypes = [i64] * 7
     del i32p
     return lib
 
