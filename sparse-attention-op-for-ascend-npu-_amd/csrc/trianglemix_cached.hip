@@ -53,8 +53,7 @@ namespace {
 typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * 64;
+#define TM_INLINED __attribute__((always_inline))  // a call would put all that a lambda names into memory
 
 // Max / sum over the four lanes that hold one row (l, l ^ 16, l ^ 32, l ^ 48).
 __device__ __forceinline__ float row_max(float x) {
@@ -69,6 +68,18 @@ __device__ __forceinline__ float row_sum(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+
+// Sum over the wave, and over its lanes up to this one.
+__device__ __forceinline__ int wave_prefix(int x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int add = __shfl_up(x, d);
+    if (lane >= d) x += add;
+  }
+  return x;
+}
+__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_prefix(x), 63); }
 
 // The bits of two 16-bit numbers of type Type from two e4m3 ones.
 template <class Type, bool kHigh>
@@ -197,39 +208,37 @@ __device__ __forceinline__ void v_operands(const T& tile, int w, u32x4_t& even, 
   }
 }
 
-// A request's pages that some row of it may attend: `sink_pages` from the first
-// on, then first_page .. end_page - 1; at least one unit where it has rows.
-struct Pages {
-  int sink_pages, first_page, end_page;
-  __device__ __forceinline__ Pages(const CachedParams& p, int len) {
-    end_page = (min(len, p.table_cols * kPageSize) + kPageSize - 1) / kPageSize;
-    const int first_key = p.window < 0 ? 0 : max(0, max(0, len - p.rows) - p.window);
-    first_page = min(first_key / kPageSize, end_page);
-    sink_pages = min((int)(((unsigned)p.sinks + kPageSize - 1) / kPageSize), first_page);
+// The 32-key tiles that rows at first_pos .. last_pos may attend: `sinks` from the
+// first on, then first .. end - 1; at least one where there is a row.
+struct Tiles {
+  int sinks, first, end, count;
+  __device__ __forceinline__ Tiles(const CachedParams& p, int first_pos, int last_pos) {
+    end = (min(max(last_pos, -1) + 1, p.table_cols * kPageSize) + kKvTile - 1) / kKvTile;
+    const int first_key = p.window < 0 ? 0 : max(0, max(0, first_pos) - p.window);
+    first = min(first_key / kKvTile, end);
+    sinks = min((int)(((unsigned)p.sinks + kKvTile - 1) / kKvTile), first);
+    count = last_pos < 0 ? 0 : max(1, sinks + end - first);
   }
-  __device__ __forceinline__ int units(int len) const {
-    return len > 0 ? max(1, sink_pages + end_page - first_page) : 0;
-  }
-  __device__ __forceinline__ int logical(int i) const { return i < sink_pages ? i : first_page + (i - sink_pages); }
+  __device__ __forceinline__ int tile(int i) const { return i < sinks ? i : first + (i - sinks); }
 };
 
 typedef const __attribute__((address_space(4))) int32_t* ConstInts;  // read by scalar loads
 
-template <class Type, CacheType kCache, int NT>
-__global__ void __launch_bounds__(kThreads, kCache == CacheType::kE4m3 ? (NT > 2 ? 1 : 2) : (NT > 1 ? 1 : 2)) cached_attention_kernel(const CachedParams p) {
+template <class Type, CacheType kCache, int NT, int kWaves>
+__global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const CachedParams p) {
+  constexpr int kThreads = 64 * kWaves, kWaveShift = kWaves == 8 ? 3 : 2;
   typedef Tile<Type, kCache> Share;
   typedef typename Share::Weight Weight;
   typedef typename Type::elem elem;
   constexpr int kRows = 16 * NT;
-  constexpr int kDepth = kCache == CacheType::kE4m3 && NT == 1 ? 3 : 2;  // tiles in registers, the one in use among them
+  constexpr int kDepth = 2;  // tiles in registers, the one in use among them
   constexpr int kHeadBytes = kHeadDim * Share::kElemBytes;
   constexpr float kWeightBits = std::is_same_v<Weight, Fp16> ? 7.0f : 0.0f;
-  constexpr int kRecord = kRows * (kHeadDim + 2);  // floats of a partial: O, row max, row sum
 
   __shared__ __attribute__((aligned(16))) float o_lds[kWaves][16 * kHeadDim];
   __shared__ float s_max[kWaves][kRows], s_sum[kWaves][kRows];
   __shared__ float join[kThreads][10];
-  __shared__ unsigned s_odd[kRows][3][4];  // note_odd: a bit a dim, for +infinity, -infinity, NaN
+  __shared__ unsigned s_odd[kWaves * kRows][3][4];  // note_odd: a bit a dim, for +infinity, -infinity, NaN
   __shared__ int s_last;
 
   const int tid = threadIdx.x;
@@ -237,469 +246,534 @@ __global__ void __launch_bounds__(kThreads, kCache == CacheType::kE4m3 ? (NT > 2
   const int lane = tid & 63;
   const int col = lane & 15;  // row of the wave's 16-row tile
   const int quad = lane >> 4;
+  const int run = blockIdx.x;
   const int G = p.group;
+  const GroupDivider by_group(p.group);
   const int token_bytes = p.kv_heads * kHeadBytes;
-  const int heads_parts = p.kv_heads * p.row_parts;
+  // this wave's head, row tile and keys among the workgroup's
+  const int slots = kWaves >> p.key_shift, slot = wave & (slots - 1), key_part = wave >> (kWaveShift - p.key_shift);
+  const int row_tiles = 1 << p.row_shift, row_tile = slot & (row_tiles - 1);
+  const int head_shift = kWaveShift - p.key_shift - p.row_shift, head_part = slot >> p.row_shift;
+  const int head_groups = p.kv_heads >> head_shift;
+  const int slot_rows = row_tiles > 1 ? kRows : min(kRows, p.part_tokens * G);  // of a partial's record
+  // The merge of partials: 16 threads a row; where the rows leave threads over, `parts`
+  // of them share a row's partials, of which each loads kFlight at a time.
+  constexpr int kRowsAtOnce = kThreads / 16, kFlight = 8;
+  const int record_rows = slots * slot_rows;
+  int row_slots = 1;
+  while (row_slots < record_rows && row_slots < kRowsAtOnce) row_slots *= 2;
+  const int parts = kRowsAtOnce / row_slots;
+  const int cluster = kFlight * parts;  // shares that are merged at once
 
-  auto clear_odd = [&]() {
-    for (int i = tid; i < kRows * 12; i += kThreads) (&s_odd[0][0][0])[i] = 0;
-  };
-  clear_odd();
+  for (int i = tid; i < kWaves * kRows * 12; i += kThreads) (&s_odd[0][0][0])[i] = 0;
   __syncthreads();
 
-  // ---- the plan: requests base .. base + 63 one a lane, their running unit counts ----
-  auto len_of = [&](int b) { return b < p.batch ? max(p.seq_lens[b], 0) : 0; };
-  int base = 0, len64 = 0, upto64 = 0, before64 = 0;  // before64: units of the requests in front of base
-  auto load_requests = [&]() {
-    len64 = len_of(base + lane);
-    upto64 = Pages(p, len64).units(len64) * heads_parts;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int add = __shfl_up(upto64, d);
-      if (lane >= d) upto64 += add;
+  // ---- this workgroup's group, and its tiles lo .. hi - 1, share `share` of `shares` ----
+  int request, head_group, part = 0, share, shares, each, first_share;
+  auto len_of = [&](int b) TM_INLINED { return b < p.batch ? max(p.seq_lens[b], 0) : 0; };
+  int len;
+  if (p.row_parts == 1) {
+    // Every group is cut into as many shares as its tiles take at `least` a share, the
+    // same for all and enough to keep all groups' shares within the grid.
+    auto tiles_of = [&](int n) TM_INLINED { return Tiles(p, n - p.rows, n - 1).count; };
+    int len64 = len_of(lane);
+    int tiles64 = tiles_of(len64);
+    int total = tiles64;
+    for (int b = 64 + lane; b < p.batch + lane; b += 64) total += tiles_of(len_of(b));
+    total = wave_sum(total);
+    // Sure: sum(ceil(tiles / least)) is at most total / least and a share more a group.
+    // One block of requests: the smallest such number by halves from total / workgroups on.
+    int least = max(p.min_tiles, (int)(((unsigned)(total * head_groups) + (unsigned)p.full_shares - 1u) / (unsigned)p.full_shares));
+    if (p.batch <= 64 && least > p.min_tiles) {
+      int low = max(p.min_tiles, (int)((unsigned)(total * head_groups) / (unsigned)p.workgroups));
+#pragma unroll 1
+      for (int i = 0; i < p.halvings && low < least; ++i) {
+        const int mid = (int)(((unsigned)low + (unsigned)least) >> 1);
+        const int all = wave_sum((int)((unsigned)(tiles64 + mid - 1) / (unsigned)mid)) * head_groups;
+        if (all <= p.workgroups) least = mid;
+        else low = mid + 1;
+      }
     }
-    upto64 += before64;
-  };
-  load_requests();
-  int total = __builtin_amdgcn_readlane(upto64, 63);
-  for (int b = 64; b < p.batch; b += 64) {
-    const int len = len_of(b + lane);
-    int sum = Pages(p, len).units(len) * heads_parts;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-    total += __builtin_amdgcn_readfirstlane(sum);
-  }
-  const int usual = (int)((unsigned)total / (unsigned)(heads_parts * p.batch));
-  const int per_run = max(min_run_units(usual, kRows > kMostStreamRows ? kMostStreamRows : kRows),
-                          (int)((unsigned)(total + p.workgroups - 1) / (unsigned)p.workgroups));
-  const int run = run_of_workgroup();
-  int unit = min(run, total / per_run + 1) * per_run;
-  const int unit_end = min(total, unit + per_run);
-
-  while (unit < unit_end) {
-    // ---- the group, and its units lo .. hi - 1 of this run ----
-    while (__builtin_amdgcn_readlane(upto64, 63) <= unit) {
-      before64 = __builtin_amdgcn_readlane(upto64, 63);
+    int base = 0, before = 0, shares64, upto64;  // the requests base .. base + 63, one a lane
+    for (;;) {
+      // no more shares than are merged at once, where that leaves them short
+      const int each64 = max(least, min((tiles64 + cluster - 1) / cluster, 8 << p.key_shift));
+      shares64 = (int)((unsigned)(tiles64 + each64 - 1) / (unsigned)each64);
+      upto64 = before + wave_prefix(shares64 * head_groups);
+      if (__builtin_amdgcn_readlane(upto64, 63) > run) break;
+      before = __builtin_amdgcn_readlane(upto64, 63);
       base += 64;
-      load_requests();
+      if (base >= p.batch) return;  // more workgroups than shares
+      len64 = len_of(base + lane);
+      tiles64 = tiles_of(len64);
     }
-    const int in_block = __ffsll((unsigned long long)__ballot(upto64 > unit)) - 1;
-    const int request = base + in_block;
-    const int len = __builtin_amdgcn_readlane(len64, in_block);
-    const Pages pages(p, len);
-    const int units = pages.units(len);
-    const int id = (unit - (__builtin_amdgcn_readlane(upto64, in_block) - units * heads_parts)) / units;
-    const int first = __builtin_amdgcn_readlane(upto64, in_block) - (heads_parts - id) * units;  // its first unit
-    const int kv_head = id / p.row_parts;
-    const int row_base = (id % p.row_parts) * kRows;
-    const int lo = unit - first, hi = min(unit_end - first, units);
-    const bool whole = lo == 0 && hi == units;
-    const int valid_rows = min(kRows, p.rows * G - row_base);
-    const int pos0 = len - p.rows;  // position of token 0; a negative one is no row
-    const int first_pos = pos0 + row_base / G, last_pos = pos0 + (row_base + valid_rows - 1) / G;
-    const int tokens = min(len, p.table_cols * kPageSize);  // with a key
+    const int in_block = __ffsll((unsigned long long)__ballot(upto64 > run)) - 1;
+    request = base + in_block;
+    len = __builtin_amdgcn_readlane(len64, in_block);
+    shares = __builtin_amdgcn_readlane(shares64, in_block);
+    const int at = run - (__builtin_amdgcn_readlane(upto64, in_block) - shares * head_groups);
+    // the shares of neighbouring heads side by side: they read neighbouring numbers
+    share = at / head_groups;
+    head_group = at - share * head_groups;
+    first_share = run - at + head_group;
+  } else {
+    unsigned id = (unsigned)run;
+    head_group = (int)(id % (unsigned)head_groups);
+    id /= (unsigned)head_groups;
+    share = (int)(id % (unsigned)p.splits);
+    id /= (unsigned)p.splits;
+    request = (int)(id % (unsigned)p.batch);
+    part = p.row_parts - 1 - (int)(id / (unsigned)p.batch);  // later rows attend more keys
+    if (part < 0) return;  // the grid is a multiple of 8
+    len = __builtin_amdgcn_readfirstlane(len_of(request));
+    first_share = run - share * head_groups;
+  }
+  const int part_tokens = min(p.part_tokens, p.rows - part * p.part_tokens);
+  const int part_rows = part_tokens * G;
+  const int pos0 = len - p.rows + part * p.part_tokens;  // of the part's first token; a negative one is no row
+  const Tiles tiles(p, pos0, pos0 + part_tokens - 1);
+  if (p.row_parts > 1) {
+    each = (tiles.count + p.splits - 1) / p.splits;
+    shares = each > 0 ? (tiles.count + each - 1) / each : 0;
+    if (share >= shares) return;
+  } else {
+    each = (tiles.count + shares - 1) / shares;  // as even as they come
+    shares = (tiles.count + each - 1) / each;
+    if (share >= shares) return;
+  }
+  const int lo = share * each, hi = min(lo + each, tiles.count);
+  // Record and arrival word of share s of the group: those of the workgroup that has it.
+  const int share_step = head_groups;
+  const int record_bytes = slots * slot_rows * (kHeadDim + 2) * 4;
+  auto record = [&](int s) TM_INLINED { return (unsigned)(first_share + s * share_step) * (unsigned)record_bytes; };
+  const int tokens = min(len, p.table_cols * kPageSize);  // with a key
+  const bool whole = shares == 1;
+  const int kv_head = (head_group << head_shift) + head_part;
+  const int row_base = row_tile * kRows;  // this wave's rows in the part
+  const int valid_rows = min(kRows, part_rows - row_base);  // none: the wave only takes part in the joins
+  const int first_pos = pos0 + by_group.token(row_base);
+  const int last_pos = valid_rows > 0 ? pos0 + by_group.token(row_base + valid_rows - 1) : -1;
+  const int row0 = request * p.rows + part * p.part_tokens;  // of query and out
 
-    // ---- Q ----
-    i16x8_t q[NT][4];
-    int row_pos[NT];
+  // ---- Q ----
+  i16x8_t q[NT][4];
+  int row_pos[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int r = row_base + 16 * n + col;
-      const int t = (int)((unsigned)r / (unsigned)G);
-      const bool ok = 16 * n + col < valid_rows;
-      row_pos[n] = ok ? pos0 + t : -1;
-      const uint16_t* const from =
-          p.query + (int64_t)(request * p.rows + t) * p.query_stride + (int64_t)(kv_head * G + (r - t * G)) * kHeadDim;
+  for (int n = 0; n < NT; ++n) {
+    const int r = row_base + 16 * n + col;
+    const int t = by_group.token(r);
+    const bool ok = 16 * n + col < valid_rows;
+    row_pos[n] = ok ? pos0 + t : -1;
+    const uint16_t* const from =
+        p.query + (int64_t)(row0 + t) * p.query_stride + (int64_t)(kv_head * G + (r - t * G)) * kHeadDim;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      q[n][c] = i16x8_t{};
+      if (ok) q[n][c] = *reinterpret_cast<const i16x8_t*>(from + Share::q_dim(c, quad));
+    }
+  }
+
+  float c2 = p.scale_log2;
+  if constexpr (kCache == CacheType::kE4m3) c2 *= p.key_scale[kv_head];
+
+  // ---- tiles: step i of key part k is tile lo + (i << key_shift) + k of the list ----
+  const ConstInts table = (ConstInts)(p.block_table + (int64_t)request * p.table_stride);
+  const int steps = ((hi - lo - 1) >> p.key_shift) + 1;
+  auto tile_of = [&](int step) TM_INLINED { return tiles.tile(lo + (step << p.key_shift) + key_part); };
+  auto entry = [&](int step) TM_INLINED {  // page of the cache, or -1
+    int phys = -1;
+    const int t = tile_of(step);
+    if (lo + (step << p.key_shift) + key_part < hi && t < tiles.end) phys = table[t / (kPageSize / kKvTile)];
+    return (unsigned)phys < (unsigned)p.num_pages ? phys : -1;
+  };
+  auto first_key = [&](int step) TM_INLINED { return tile_of(step) * kKvTile; };
+  // the first key that the last row's window holds, and that the first row's does
+  const int last_low = p.window < 0 ? 0 : max(last_pos, 0) - p.window;
+  const int first_low = p.window < 0 ? 0 : max(first_pos, 0) - p.window;
+  // Keys of the tile that are in memory, 0 where no row attends any of them.
+  auto valid_keys = [&](int step, int phys) TM_INLINED {
+    const int key0 = first_key(step);
+    if (phys < 0 || key0 > last_pos || (key0 + 31 < first_low && key0 >= p.sinks)) return 0;
+    return min(32, tokens - key0);
+  };
+  auto value_tile = [&](int step, int phys) TM_INLINED {
+    return p.value_cache + max(phys, 0) * p.value_page_stride + kv_head * kHeadBytes + (first_key(step) % kPageSize) * token_bytes;
+  };
+  int k_off[2], v_off[8];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) k_off[u] = (8 * (col >> 2) + 4 * u + (col & 3)) * token_bytes + 16 * quad;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v_off[j] = (8 * quad + j) * token_bytes + 8 * Share::kElemBytes * col;
+  auto load = [&](Share& t, int step, int phys) TM_INLINED {
+    const int valid = valid_keys(step, phys);
+    const int range = valid > 0 ? (valid - 1) * token_bytes + kHeadBytes : 0;
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(p.key_cache + max(phys, 0) * p.key_page_stride + kv_head * kHeadBytes +
+                (first_key(step) % kPageSize) * token_bytes),
+        (short)0, range, kBufferFlags);
+    const __amdgpu_buffer_rsrc_t vr =
+        __builtin_amdgcn_make_buffer_rsrc((void*)value_tile(step, phys), (short)0, range, kBufferFlags);
+    t.load(kr, vr, k_off, v_off);
+  };
+
+  float m_run[NT], l_run[NT];
+  f32x4_t o[8][NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m_run[n] = -INFINITY;
+    l_run[n] = 0.0f;
+#pragma unroll
+    for (int m = 0; m < 8; ++m) o[m][n] = f32x4_t{};
+  }
+
+  // Notes the V entries of a tile that are no finite numbers for the rows that attend
+  // them, apart from the product: 0 * NaN would reach the others too.
+  auto note_odd = [&](int step, int phys) TM_INLINED {
+    const int key0 = first_key(step), keys = valid_keys(step, phys);
+    const int pos = pos0 + by_group.token(row_base + lane);  // of row `lane`
+    const char* at = value_tile(step, phys);
+#pragma unroll 1
+    for (int k = 0; k < keys; ++k, at += token_bytes) {
+      const int lower = Share::odd_kind(at, lane), upper = Share::odd_kind(at, lane + 64);
+      const int key = key0 + k;
+      const bool seen =
+          lane < valid_rows && key <= pos && (p.window < 0 || key >= max(pos, 0) - p.window || key < p.sinks);
+#pragma unroll 1
+      for (int kind = 1; kind < 4; ++kind) {
+        const unsigned long long lo64 = __ballot(lower == kind), hi64 = __ballot(upper == kind);
+        if (seen && (lo64 | hi64) != 0) {
+          unsigned* const to = s_odd[slot * kRows + lane][kind - 1];
+          atomicOr(to, (unsigned)lo64);
+          atomicOr(to + 1, (unsigned)(lo64 >> 32));
+          atomicOr(to + 2, (unsigned)hi64);
+          atomicOr(to + 3, (unsigned)(hi64 >> 32));
+        }
+      }
+    }
+  };
+
+  auto compute = [&](Share& t, int step, int phys) TM_INLINED {
+    if (valid_keys(step, phys) == 0) return;
+    const int key0 = first_key(step);
+    const bool masked = key0 + 31 > first_pos || (key0 < last_low && key0 + 31 >= p.sinks);
+    f32x4_t s[2][NT];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[u][n] = f32x4_t{};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        q[n][c] = i16x8_t{};
-        if (ok) q[n][c] = *reinterpret_cast<const i16x8_t*>(from + Share::q_dim(c, quad));
+        const i16x8_t a = t.k_operand(u, c);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[u][n] = Type::mfma16(a, q[n][c], s[u][n]);
       }
     }
-
-    float c2 = p.scale_log2, v_scale = 1.0f;
-    if constexpr (kCache == CacheType::kE4m3) {
-      c2 *= p.key_scale[kv_head];
-      v_scale = p.value_scale[kv_head];
-    }
-
-    // ---- pages ----
-    const ConstInts table = (ConstInts)(p.block_table + (int64_t)request * p.table_stride);
-    auto entry = [&](int i) {  // page of the cache, or -1
-      int phys = -1;
-      if (i < hi && pages.logical(i) < pages.end_page) phys = table[pages.logical(i)];
-      return (unsigned)phys < (unsigned)p.num_pages ? phys : -1;
-    };
-    int k_off[2], v_off[8];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) k_off[u] = (32 * wave + 8 * (col >> 2) + 4 * u + (col & 3)) * token_bytes + 16 * quad;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v_off[j] = (32 * wave + 8 * quad + j) * token_bytes + 8 * Share::kElemBytes * col;
-    auto valid_keys = [&](int i, int phys) {
-      return phys < 0 ? 0 : min(kPageSize, tokens - pages.logical(i) * kPageSize);
-    };
-    auto value_page = [&](int phys) {
-      return p.value_cache + max(phys, 0) * p.value_page_stride + kv_head * kHeadBytes;
-    };
-    auto load = [&](Share& t, int i, int phys) {
-      const int valid = valid_keys(i, phys);
-      const int range = valid > 0 ? (valid - 1) * token_bytes + kHeadBytes : 0;
-      const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)(p.key_cache + max(phys, 0) * p.key_page_stride + kv_head * kHeadBytes), (short)0, range, kBufferFlags);
-      const __amdgpu_buffer_rsrc_t vr =
-          __builtin_amdgcn_make_buffer_rsrc((void*)value_page(phys), (short)0, range, kBufferFlags);
-      t.load(kr, vr, k_off, v_off);
-    };
-
-    float m_run[NT], l_run[NT];
-    f32x4_t o[8][NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      m_run[n] = -INFINITY;
-      l_run[n] = 0.0f;
-#pragma unroll
-      for (int m = 0; m < 8; ++m) o[m][n] = f32x4_t{};
-    }
-
-    // Notes the V entries of a tile that are no finite numbers for the rows that attend
-    // them, apart from the product: 0 * NaN would reach the others too.
-    auto note_odd = [&](int i, int phys) {
-      const int key0 = pages.logical(i) * kPageSize + 32 * wave;
-      const int keys = min(32, valid_keys(i, phys) - 32 * wave);
-      const int pos = pos0 + (int)((unsigned)(row_base + lane) / (unsigned)G);  // of row `lane`
-      const char* at = value_page(phys) + 32 * wave * token_bytes;
-#pragma unroll 1
-      for (int k = 0; k < keys; ++k, at += token_bytes) {
-        const int lower = Share::odd_kind(at, lane), upper = Share::odd_kind(at, lane + 64);
-        const int key = key0 + k;
-        const bool seen =
-            lane < valid_rows && key <= pos && (p.window < 0 || key >= max(pos, 0) - p.window || key < p.sinks);
-#pragma unroll 1
-        for (int kind = 1; kind < 4; ++kind) {
-          const unsigned long long lo64 = __ballot(lower == kind), hi64 = __ballot(upper == kind);
-          if (seen && (lo64 | hi64) != 0) {
-            unsigned* const to = s_odd[lane][kind - 1];
-            atomicOr(to, (unsigned)lo64);
-            atomicOr(to + 1, (unsigned)(lo64 >> 32));
-            atomicOr(to + 2, (unsigned)hi64);
-            atomicOr(to + 3, (unsigned)(hi64 >> 32));
-          }
-        }
-      }
-    };
-
-    auto compute = [&](Share& t, int i, int phys) {
-      const int key0 = pages.logical(i) * kPageSize + 32 * wave;
-      // the first key that the last row's window holds, and that the first row's does
-      const int last_low = p.window < 0 ? 0 : max(last_pos, 0) - p.window;
-      const int first_low = p.window < 0 ? 0 : max(first_pos, 0) - p.window;
-      if (phys < 0 || key0 > last_pos || (key0 + 31 < first_low && key0 >= p.sinks)) return;
-      const bool masked = key0 + 31 > first_pos || (key0 < last_low && key0 + 31 >= p.sinks);
-      f32x4_t s[2][NT];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) s[u][n] = f32x4_t{};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const i16x8_t a = t.k_operand(u, c);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) s[u][n] = Type::mfma16(a, q[n][c], s[u][n]);
-        }
-      }
-      if (masked) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int low = p.window < 0 ? 0 : max(row_pos[n], 0) - p.window;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int key = key0 + 8 * quad + e;
-            const bool seen = key <= row_pos[n] && (key >= low || key < p.sinks);
-            s[e >> 2][n][e & 3] = seen ? s[e >> 2][n][e & 3] : -INFINITY;
-          }
-        }
-      }
-      i16x8_t pb[NT];
+    if (masked) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, s[e >> 2][n][e & 3]);
-        top = row_max(top) * c2;
-        if (__any(top > m_run[n] + kLazyRescale)) {
-          const float m_new = fmaxf(m_run[n], top);
-          const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run[n] - m_new);
-          l_run[n] *= alpha;
-#pragma unroll
-          for (int m = 0; m < 8; ++m) o[m][n] *= alpha;
-          m_run[n] = m_new;
-        }
-        const float shift = kWeightBits - (m_run[n] == -INFINITY ? 0.0f : m_run[n]);
-        typename Weight::vec weight;
-        float add = 0.0f;
+        const int low = p.window < 0 ? 0 : max(row_pos[n], 0) - p.window;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][n][e & 3], c2, shift));
-          add += x;
-          weight[e] = (typename Weight::elem)x;
-        }
-        l_run[n] += add;
-        pb[n] = __builtin_bit_cast(i16x8_t, weight);
-      }
-      if (masked && __builtin_expect(__any(t.odd_value()) != 0, 0)) {
-        note_odd(i, phys);
-        t.keep_finite();
-      }
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        __builtin_amdgcn_sched_barrier(0);
-        u32x4_t even, odd;
-        v_operands(t, w, even, odd);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          o[2 * w][n] = Weight::mfma16(__builtin_bit_cast(i16x8_t, even), pb[n], o[2 * w][n]);
-          o[2 * w + 1][n] = Weight::mfma16(__builtin_bit_cast(i16x8_t, odd), pb[n], o[2 * w + 1][n]);
+          const int key = key0 + 8 * quad + e;
+          const bool seen = key <= row_pos[n] && (key >= low || key < p.sinks);
+          s[e >> 2][n][e & 3] = seen ? s[e >> 2][n][e & 3] : -INFINITY;
         }
       }
-    };
-
-    // Tile slot s holds page i + s; the page kDepth - 1 ahead is on its way.
-    Share tile[kDepth];
-    int phys[kDepth];
-#pragma unroll
-    for (int s = 0; s < kDepth; ++s) phys[s] = entry(lo + s);
-#pragma unroll
-    for (int s = 0; s + 1 < kDepth; ++s) load(tile[s], lo + s, phys[s]);
-    for (int i = lo; i < hi; i += kDepth) {
-#pragma unroll
-      for (int s = 0; s < kDepth; ++s) {
-        constexpr int kAhead = kDepth - 1;
-        const int slot = (s + kAhead) % kDepth;
-        load(tile[slot], i + s + kAhead, phys[slot]);
-        const int own = phys[s];
-        phys[s] = entry(i + s + kDepth);
-        if (i + s < hi) compute(tile[s], i + s, own);
-      }
     }
-
-    // ---- the waves' sums, 16 rows at a time through LDS ----
+    i16x8_t pb[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float l = row_sum(l_run[n]);
-      m_run[n] = row_shift(m_run[n], l);
-      if (quad == 0) {
-        s_max[wave][16 * n + col] = m_run[n];
-        s_sum[wave][16 * n + col] = l;
-      }
-    }
-    // 16 threads a row, 8 dims each.
-    const int r16 = tid >> 4, c8 = tid & 15;
-    auto store_row = [&](int r, const float* acc, float l) {
-      const int at = row_base + r;
-      const int t = (int)((unsigned)at / (unsigned)G);
-      if (pos0 + t < 0) return;  // before the request's first token: no row
-      const float inv = l > 0.0f ? v_scale / l : 0.0f;
-      // a NaN sum fails the comparison, and must reach the result
-      const float scale = (__float_as_uint(l) & 0x7fffffffu) > 0x7f800000u ? l : inv;
-      typename Type::vec y;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = (elem)(acc[e] * scale);
-      *reinterpret_cast<typename Type::vec*>(
-          p.out + ((int64_t)(request * p.rows + t) * p.heads + kv_head * G + (at - t * G)) * kHeadDim + 8 * c8) = y;
-    };
-    // the workgroups that share the group, and where their partials lie
-    const int first_run = (int)((unsigned)first / (unsigned)per_run);
-    const int last_run = (int)((unsigned)(first + units - 1) / (unsigned)per_run);
-    auto record = [&](int r) { return (unsigned)(2 * r + (r == first_run ? 1 : 0)) * (kRecord * 4u); };
-    const __amdgpu_buffer_rsrc_t rec = __builtin_amdgcn_make_buffer_rsrc(
-        (void*)p.partials, (short)0, whole ? 0 : (int)((unsigned)p.workgroups * 2u * (kRecord * 4u)), kBufferFlags);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      __syncthreads();
-      if (16 * n >= valid_rows) break;
       float top = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < kWaves; ++k) top = fmaxf(top, s_max[k][16 * n + col]);
-      const float weight = m_run[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - top);
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, s[e >> 2][n][e & 3]);
+      top = row_max(top) * c2;
+      if (__any(top > m_run[n] + kLazyRescale)) {
+        const float m_new = fmaxf(m_run[n], top);
+        const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run[n] - m_new);
+        l_run[n] *= alpha;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {  // dims 32 quad + 8 e + 4 half ..
-          f32x4_t x;
-#pragma unroll
-          for (int m = 0; m < 4; ++m) x[m] = m_run[n] == -INFINITY ? 0.0f : o[4 * half + m][n][e] * weight;
-          const int chunk = (8 * quad + 2 * e + half) ^ col;
-          *reinterpret_cast<f32x4_t*>(&o_lds[wave][col * kHeadDim + 4 * chunk]) = x;
-        }
+        for (int m = 0; m < 8; ++m) o[m][n] *= alpha;
+        m_run[n] = m_new;
       }
-      __syncthreads();
-      const int r = 16 * n + r16;
-      if (r < valid_rows) {
-        float all = -INFINITY;
+      const float shift = kWeightBits - (m_run[n] == -INFINITY ? 0.0f : m_run[n]);
+      typename Weight::vec weight;
+      float add = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kWaves; ++k) all = fmaxf(all, s_max[k][r]);
-        float l = 0.0f, acc[8] = {};
+      for (int e = 0; e < 8; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e >> 2][n][e & 3], c2, shift));
+        add += x;
+        weight[e] = (typename Weight::elem)x;
+      }
+      l_run[n] += add;
+      pb[n] = __builtin_bit_cast(i16x8_t, weight);
+    }
+    if (masked && __builtin_expect(__any(t.odd_value()) != 0, 0)) {
+      note_odd(step, phys);
+      t.keep_finite();
+    }
 #pragma unroll
-        for (int k = 0; k < kWaves; ++k) {
-          const float mk = s_max[k][r];
-          l += mk == -INFINITY ? 0.0f : s_sum[k][r] * __builtin_amdgcn_exp2f(mk - all);
+    for (int w = 0; w < 4; ++w) {
+      __builtin_amdgcn_sched_barrier(0);
+      u32x4_t even, odd;
+      v_operands(t, w, even, odd);
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const f32x4_t x =
-                *reinterpret_cast<const f32x4_t*>(&o_lds[k][r16 * kHeadDim + 4 * ((2 * c8 + half) ^ r16)]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[4 * half + e] += x[e];
-          }
-        }
-#pragma unroll
-        for (int kind = 0; kind < 3; ++kind) {
-          const unsigned odd = s_odd[r][kind][c8 >> 2] >> (8 * (c8 & 3)) & 0xffu;
-          // bits, and no number that is taken for finite
-          float value = __uint_as_float(kind == 0 ? 0x7f800000u : kind == 1 ? 0xff800000u : 0x7fc00000u);
-          asm volatile("" : "+v"(value));
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc[e] += odd >> e & 1 ? value : 0.0f;
-        }
-        if (whole) {
-          store_row(r, acc, l);
-        } else {
-          const unsigned at = record(run);
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const f32x4_t x = {acc[4 * half], acc[4 * half + 1], acc[4 * half + 2], acc[4 * half + 3]};
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, x), rec,
-                                                   at + (r * kHeadDim + 8 * c8 + 4 * half) * 4, 0, kCpolAgent);
-          }
-          if (c8 == 0) {
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(all), rec, at + (kRows * kHeadDim + r) * 4, 0,
-                                                  kCpolAgent);
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), rec, at + (kRows * (kHeadDim + 1) + r) * 4, 0,
-                                                  kCpolAgent);
-          }
-        }
+      for (int n = 0; n < NT; ++n) {
+        o[2 * w][n] = Weight::mfma16(__builtin_bit_cast(i16x8_t, even), pb[n], o[2 * w][n]);
+        o[2 * w + 1][n] = Weight::mfma16(__builtin_bit_cast(i16x8_t, odd), pb[n], o[2 * w + 1][n]);
       }
     }
+  };
 
-    if (!whole) {
-      // ---- the workgroup that arrives last merges ----
-      wait_dma();  // this wave's partial stores have completed
-      __syncthreads();
-      unsigned long long* const word = p.counters + first_run;
-      if (tid == 0) {
-        s_last = (int)(count_arrival(word, p.epoch) == (unsigned long long)(last_run - first_run + 1));
-      }
-      __syncthreads();
-      if (s_last) {
-        // The word is left at this launch's tag with a count of zero for the next one.
-        if (tid == 0) __hip_atomic_store(word, p.epoch << kEpochShift, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        // 16 threads a row again; where the rows leave threads over, they share a
-        // row's partials (part pg of `parts` takes every parts-th) and join through
-        // LDS.  Four partials' loads are in flight at a time.
-        int row_slots = 1;
-        while (row_slots < valid_rows && row_slots < kThreads / 16) row_slots *= 2;
-        const int parts = kThreads / 16 / row_slots;
-        const int pg = r16 / row_slots;
-        for (int rb = 0; rb < valid_rows; rb += row_slots) {
-          const int r = rb + r16 % row_slots;
-          float top = -INFINITY, l = 0.0f, acc[8] = {};
-          if (r < valid_rows) {
-            for (int s0 = first_run + pg; s0 <= last_run; s0 += 4 * parts) {
-              float ms[4], ls[4];
-              f32x4_t x[4][2];
+  // Tile slot s holds step i + s; the step kDepth - 1 ahead is on its way.
+  Share tile[kDepth];
+  int phys[kDepth];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                // past the last one its loads fall outside the buffer's range
-                const int s = s0 + j * parts;
-                const unsigned at = s <= last_run ? record(s) : kOutOfRange;
-                ms[j] = __uint_as_float(
-                    __builtin_amdgcn_raw_buffer_load_b32(rec, at + (kRows * kHeadDim + r) * 4, 0, kCpolAgent));
-                ls[j] = __uint_as_float(
-                    __builtin_amdgcn_raw_buffer_load_b32(rec, at + (kRows * (kHeadDim + 1) + r) * 4, 0, kCpolAgent));
+  for (int s = 0; s < kDepth; ++s) phys[s] = entry(s);
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                  x[j][half] = __builtin_bit_cast(
-                      f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                                   rec, at + (r * kHeadDim + 8 * c8 + 4 * half) * 4, 0, kCpolAgent));
-                }
-              }
-              float next = top;
+  for (int s = 0; s + 1 < kDepth; ++s) load(tile[s], s, phys[s]);
+  for (int i = 0; i < steps; i += kDepth) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                if (s0 + j * parts > last_run) ms[j] = -INFINITY;
-                next = fmaxf(next, ms[j]);
-              }
-              const float shift = next == -INFINITY ? 0.0f : next;
-              const float keep = __builtin_amdgcn_exp2f(top - shift);
-              l *= keep;
+    for (int s = 0; s < kDepth; ++s) {
+      constexpr int kAhead = kDepth - 1;
+      const int ahead = (s + kAhead) % kDepth;
+      load(tile[ahead], i + s + kAhead, phys[ahead]);
+      const int own = phys[s];
+      phys[s] = entry(i + s + kDepth);
+      if (i + s < steps) compute(tile[s], i + s, own);
+    }
+  }
+
+  // ---- the key parts' sums, 16 rows of every slot at a time through LDS ----
 #pragma unroll
-              for (int e = 0; e < 8; ++e) acc[e] *= keep;
+  for (int n = 0; n < NT; ++n) {
+    const float l = row_sum(l_run[n]);
+    m_run[n] = row_shift(m_run[n], l);
+    if (quad == 0) {
+      s_max[wave][16 * n + col] = m_run[n];
+      s_sum[wave][16 * n + col] = l;
+    }
+  }
+  // 16 threads a row, 8 dims each.
+  const int r16 = tid >> 4, c8 = tid & 15;
+  auto store_row = [&](int of_slot, int r, const float* acc, float l) TM_INLINED {
+    const int at = (of_slot & (row_tiles - 1)) * kRows + r;
+    const int t = by_group.token(at);
+    if (pos0 + t < 0) return;  // before the request's first token: no row
+    const int head = (head_group << head_shift) + (of_slot >> p.row_shift);
+    float v_scale = 1.0f;
+    if constexpr (kCache == CacheType::kE4m3) v_scale = p.value_scale[head];
+    const float inv = l > 0.0f ? v_scale / l : 0.0f;
+    // a NaN sum fails the comparison, and must reach the result
+    const float scale = (__float_as_uint(l) & 0x7fffffffu) > 0x7f800000u ? l : inv;
+    typename Type::vec y;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float w = __builtin_amdgcn_exp2f(ms[j] - shift);
-                l += ls[j] * w;
+    for (int e = 0; e < 8; ++e) y[e] = (elem)(acc[e] * scale);
+    *reinterpret_cast<typename Type::vec*>(
+        p.out + ((int64_t)(row0 + t) * p.heads + head * G + (at - t * G)) * kHeadDim + 8 * c8) = y;
+  };
+  auto rows_of = [&](int of_slot) TM_INLINED { return min(kRows, part_rows - (of_slot & (row_tiles - 1)) * kRows); };
+  // a record: O of all slots' rows, then their row maxima and sums
+  const __amdgpu_buffer_rsrc_t rec = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)p.partials, (short)0, whole ? 0 : (int)((unsigned)p.workgroups * (unsigned)record_bytes),
+      kBufferFlags);
+  auto store_partial = [&](int s, int rr, const float* acc, float max, float l) TM_INLINED {
+    const unsigned at = record(s);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) acc[e] += x[j][e >> 2][e & 3] * w;
-              }
-              top = next;
-            }
-          }
-          if (parts > 1) {
-            __syncthreads();
+    for (int half = 0; half < 2; ++half) {
+      const f32x4_t x = {acc[4 * half], acc[4 * half + 1], acc[4 * half + 2], acc[4 * half + 3]};
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, x), rec,
+                                             at + (rr * kHeadDim + 8 * c8 + 4 * half) * 4, 0, kCpolAgent);
+    }
+    if (c8 == 0) {
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(max), rec, at + (record_rows * kHeadDim + rr) * 4, 0, kCpolAgent);
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), rec, at + (record_rows * (kHeadDim + 1) + rr) * 4, 0,
+                                            kCpolAgent);
+    }
+  };
 #pragma unroll
-            for (int e = 0; e < 8; ++e) join[tid][e] = acc[e];
-            join[tid][8] = top;
-            join[tid][9] = l;
-            __syncthreads();
-            if (pg == 0) {
-              float all = top;
-              for (int k = 1; k < parts; ++k) all = fmaxf(all, join[tid + k * 16 * row_slots][8]);
-              const float shift = all == -INFINITY ? 0.0f : all;
-              const float keep = __builtin_amdgcn_exp2f(top - shift);
-              l *= keep;
+  for (int n = 0; n < NT; ++n) {
+    __syncthreads();
+    if (16 * n >= min(kRows, part_rows)) break;
+    float top = -INFINITY;
+    for (int k = slot; k < kWaves; k += slots) top = fmaxf(top, s_max[k][16 * n + col]);
+    const float weight = m_run[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - top);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) acc[e] *= keep;
-              for (int k = 1; k < parts; ++k) {
-                const float* const from = join[tid + k * 16 * row_slots];
-                const float w = __builtin_amdgcn_exp2f(from[8] - shift);
-                l += from[9] * w;
+    for (int e = 0; e < 4; ++e) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) acc[e] += from[e] * w;
-              }
-            }
-          }
-          if (pg == 0 && r < valid_rows) store_row(r, acc, l);
-        }
+      for (int half = 0; half < 2; ++half) {  // dims 32 quad + 8 e + 4 half ..
+        f32x4_t x;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) x[m] = m_run[n] == -INFINITY ? 0.0f : o[4 * half + m][n][e] * weight;
+        const int chunk = (8 * quad + 2 * e + half) ^ col;
+        *reinterpret_cast<f32x4_t*>(&o_lds[wave][col * kHeadDim + 4 * chunk]) = x;
       }
     }
-    unit = first + hi;
     __syncthreads();
-    clear_odd();
+    const int slot_each = row_tiles > 1 ? 16 : min(16, part_rows - 16 * n);  // rows of a slot
+    for (int i = r16; i < slots * slot_each; i += kThreads / 16) {
+      const int of_slot = i / slot_each, at16 = i - of_slot * slot_each, r = 16 * n + at16;
+      if (r >= rows_of(of_slot)) continue;
+      float all = -INFINITY;
+      for (int k = of_slot; k < kWaves; k += slots) all = fmaxf(all, s_max[k][r]);
+      float l = 0.0f, acc[8] = {};
+      for (int k = of_slot; k < kWaves; k += slots) {
+        const float mk = s_max[k][r];
+        l += mk == -INFINITY ? 0.0f : s_sum[k][r] * __builtin_amdgcn_exp2f(mk - all);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const f32x4_t x =
+              *reinterpret_cast<const f32x4_t*>(&o_lds[k][at16 * kHeadDim + 4 * ((2 * c8 + half) ^ at16)]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[4 * half + e] += x[e];
+        }
+      }
+#pragma unroll
+      for (int kind = 0; kind < 3; ++kind) {
+        const unsigned odd = s_odd[of_slot * kRows + r][kind][c8 >> 2] >> (8 * (c8 & 3)) & 0xffu;
+        // bits, and no number that is taken for finite
+        float value = __uint_as_float(kind == 0 ? 0x7f800000u : kind == 1 ? 0xff800000u : 0x7fc00000u);
+        asm volatile("" : "+v"(value));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] += odd >> e & 1 ? value : 0.0f;
+      }
+      if (whole) {
+        store_row(of_slot, r, acc, l);
+      } else {
+        store_partial(share, of_slot * slot_rows + r, acc, all, l);
+      }
+    }
+  }
+
+  if (whole) return;
+
+  // ---- the shares: the workgroup that arrives last at a cluster of them merges it, the
+  // one that arrives last of the clusters those ----
+  for (int level = 0; level < 2; ++level) {
+    const int stride = level == 0 ? 1 : cluster;
+    const int from = level == 0 ? share / cluster * cluster : 0;  // the first share that is merged, then every stride-th
+    const int count = level == 0 ? min(cluster, shares - from) : (shares + cluster - 1) / cluster;
+    const bool last_level = level == 1 || shares <= cluster;
+    wait_dma();  // this wave's partial stores have completed
     __syncthreads();
+    // words: the cluster's first share's; the group's second share's
+    unsigned long long* const word = p.counters + first_share + (level == 0 ? from : 1) * head_groups;
+    if (tid == 0) {
+      s_last = (int)(count_arrival(word, p.epoch) == (unsigned long long)count);
+      // The word is left at this launch's tag with a count of zero for the next one.
+      if (s_last) __hip_atomic_store(word, p.epoch << kEpochShift, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!s_last) return;
+    // Part pg of a row's threads takes every parts-th partial; they join through LDS.
+    const int pg = r16 / row_slots;
+    for (int rb = 0; rb < record_rows; rb += row_slots) {
+      const int rr = rb + r16 % row_slots, of_slot = rr / slot_rows, r = rr - of_slot * slot_rows;
+      const bool held = rr < record_rows && r < rows_of(of_slot);
+      float top = -INFINITY, l = 0.0f, acc[8] = {};
+      if (held) {
+        for (int s0 = pg; s0 < count; s0 += kFlight * parts) {
+          float ms[kFlight], ls[kFlight];
+          f32x4_t x[kFlight][2];
+#pragma unroll
+          for (int j = 0; j < kFlight; ++j) {
+            // past the last one its loads fall outside the buffer's range
+            const int s = s0 + j * parts;
+            const unsigned at = s < count ? record(from + s * stride) : kOutOfRange;
+            ms[j] = __uint_as_float(
+                __builtin_amdgcn_raw_buffer_load_b32(rec, at + (record_rows * kHeadDim + rr) * 4, 0, kCpolAgent));
+            ls[j] = __uint_as_float(
+                __builtin_amdgcn_raw_buffer_load_b32(rec, at + (record_rows * (kHeadDim + 1) + rr) * 4, 0, kCpolAgent));
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              x[j][half] = __builtin_bit_cast(
+                  f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                               rec, at + (rr * kHeadDim + 8 * c8 + 4 * half) * 4, 0, kCpolAgent));
+            }
+          }
+          float next = top;
+#pragma unroll
+          for (int j = 0; j < kFlight; ++j) {
+            if (s0 + j * parts >= count) ms[j] = -INFINITY;
+            next = fmaxf(next, ms[j]);
+          }
+          const float shift = next == -INFINITY ? 0.0f : next;
+          const float keep = __builtin_amdgcn_exp2f(top - shift);
+          l *= keep;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] *= keep;
+#pragma unroll
+          for (int j = 0; j < kFlight; ++j) {
+            const float w = __builtin_amdgcn_exp2f(ms[j] - shift);
+            l += ls[j] * w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] += x[j][e >> 2][e & 3] * w;
+          }
+          top = next;
+        }
+      }
+      if (parts > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) join[tid][e] = acc[e];
+        join[tid][8] = top;
+        join[tid][9] = l;
+        __syncthreads();
+        if (pg == 0) {
+          float all = top;
+          for (int k = 1; k < parts; ++k) all = fmaxf(all, join[tid + k * 16 * row_slots][8]);
+          const float shift = all == -INFINITY ? 0.0f : all;
+          const float keep = __builtin_amdgcn_exp2f(top - shift);
+          l *= keep;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] *= keep;
+          for (int k = 1; k < parts; ++k) {
+            const float* const other = join[tid + k * 16 * row_slots];
+            const float w = __builtin_amdgcn_exp2f(other[8] - shift);
+            l += other[9] * w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] += other[e] * w;
+          }
+          top = all;
+        }
+      } else if (!last_level) {
+        __syncthreads();  // all have read the record that the result replaces
+      }
+      if (pg == 0 && held) {
+        if (last_level) store_row(of_slot, r, acc, l);
+        else store_partial(from, rr, acc, top, l);
+      }
+    }
+    if (last_level) return;
   }
 }
 
 template <class Type, CacheType kCache>
-hipError_t launch_shape(const CachedParams& p, int shape_rows, hipStream_t stream) {
-  const dim3 grid((unsigned)p.workgroups), block(kThreads);
-  switch (shape_rows) {
-    case 16: hipLaunchKernelGGL((cached_attention_kernel<Type, kCache, 1>), grid, block, 0, stream, p); break;
-    case 32: hipLaunchKernelGGL((cached_attention_kernel<Type, kCache, 2>), grid, block, 0, stream, p); break;
-    case 64: hipLaunchKernelGGL((cached_attention_kernel<Type, kCache, 4>), grid, block, 0, stream, p); break;
-    default: return hipErrorInvalidValue;
+hipError_t launch_shape(const CachedParams& p, CachedShape shape, hipStream_t stream) {
+  const dim3 grid((unsigned)p.workgroups), block(64 * shape.waves);
+  if (shape.rows == 16 && shape.waves == 4) {
+    hipLaunchKernelGGL((cached_attention_kernel<Type, kCache, 1, 4>), grid, block, 0, stream, p);
+  } else if (shape.rows == 16 && shape.waves == 8) {
+    hipLaunchKernelGGL((cached_attention_kernel<Type, kCache, 1, 8>), grid, block, 0, stream, p);
+  } else if (shape.rows == 32 && shape.waves == 8) {
+    hipLaunchKernelGGL((cached_attention_kernel<Type, kCache, 2, 8>), grid, block, 0, stream, p);
+  } else if (shape.rows == 64 && shape.waves == 4) {
+    hipLaunchKernelGGL((cached_attention_kernel<Type, kCache, 4, 4>), grid, block, 0, stream, p);
+  } else {
+    return hipErrorInvalidValue;
   }
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_cached_attention(const CachedParams& p, int shape_rows, bool fp16, CacheType cache,
+hipError_t launch_cached_attention(const CachedParams& p, CachedShape shape, bool fp16, CacheType cache,
                                    hipStream_t stream) {
   if (cache == CacheType::kE4m3) {
-    return fp16 ? launch_shape<Fp16, CacheType::kE4m3>(p, shape_rows, stream)
-                : launch_shape<Bf16, CacheType::kE4m3>(p, shape_rows, stream);
+    return fp16 ? launch_shape<Fp16, CacheType::kE4m3>(p, shape, stream)
+                : launch_shape<Bf16, CacheType::kE4m3>(p, shape, stream);
   }
-  return fp16 ? launch_shape<Fp16, CacheType::kSame>(p, shape_rows, stream)
-              : launch_shape<Bf16, CacheType::kSame>(p, shape_rows, stream);
+  return fp16 ? launch_shape<Fp16, CacheType::kSame>(p, shape, stream)
+              : launch_shape<Bf16, CacheType::kSame>(p, shape, stream);
 }
 
 }  // namespace tmx

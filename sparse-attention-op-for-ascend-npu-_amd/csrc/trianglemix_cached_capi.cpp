@@ -65,11 +65,13 @@ int check_cache_type(int dtype, int cache_dtype, const void* key_scale, const vo
 
 int elem_bytes(CacheType type) { return type == CacheType::kE4m3 ? 1 : 2; }
 
-int64_t pages_of(int64_t tokens) { return (tokens + kPageSize - 1) / kPageSize; }
+// Partial records of the groups that are cut.
+constexpr int64_t kMaxRecordBytes = int64_t(64) << 20;
 
 struct CachedPlan {
-  int shape, row_parts, workgroups;
-  int64_t units, workspace_bytes;
+  CachedShape shape;
+  int row_shift, key_shift, part_tokens, row_parts, splits, full_shares, min_tiles, halvings, workgroups;
+  int64_t tiles, workspace_bytes;
 };
 
 int check_cached(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t table_cols, int64_t window,
@@ -84,22 +86,75 @@ int check_cached(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, i
   return TM_OK;
 }
 
-// The pages that a request's rows can attend at most, its own included.
-int64_t most_units(int64_t rows, int64_t table_cols, int64_t window, int64_t sinks) {
-  if (window < 0 || window >= table_cols * kPageSize) return table_cols;
-  return std::min(table_cols, pages_of(window + rows - 1) + 1 + pages_of(std::min(sinks, table_cols * kPageSize)));
+// The 32-key tiles that a request's rows can attend at most.
+int64_t most_tiles(int64_t rows, int64_t table_cols, int64_t window, int64_t sinks) {
+  const int64_t all = table_cols * (kPageSize / kKvTile);
+  if (window < 0 || window >= table_cols * kPageSize) return all;
+  return std::min(all, (window + rows - 1) / kKvTile + 2 + (std::min(sinks, table_cols * kPageSize) + kKvTile - 1) / kKvTile);
 }
 
 CachedPlan cached_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t table_cols, int64_t window,
                        int64_t sinks) {
-  CachedPlan r;
-  const int64_t group_rows = rows * (heads / kv_heads);
-  r.shape = group_rows <= 16 ? 16 : group_rows <= 32 ? 32 : 64;
-  r.row_parts = (int)((group_rows + r.shape - 1) / r.shape);
-  r.units = batch * kv_heads * r.row_parts * most_units(rows, table_cols, window, sinks);
-  r.workgroups = (int)((std::min<int64_t>(2 * kComputeUnits, r.units) + 7) / 8 * 8);
-  r.workspace_bytes = kCounterBytes + 2 * int64_t(r.workgroups) * r.shape * (kHeadDim + 2) * 4;
+  CachedPlan r{};
+  const int64_t group = heads / kv_heads, group_rows = rows * group;
+  const int64_t tiles = most_tiles(rows, table_cols, window, sinks);
+  // Whether groups of 2^shift heads leave every CU 32 tiles.
+  const auto enough = [&](int shift) {
+    return kv_heads % (1 << shift) == 0 && batch * (kv_heads >> shift) * std::max<int64_t>(1, tiles / 32) >= kComputeUnits;
+  };
+  // A wave's rows and the row tiles of a workgroup's waves; what these leave of the
+  // waves goes to neighbouring KV heads, whose numbers lie side by side in memory (64
+  // requests of 2000 to 16384 tokens: 222 us with eight heads a workgroup, 234 with
+  // four, 283 with two), or to parts of the keys: where there is little to read or
+  // many rows, whose partials would cost more (32 requests of 5 tokens, 500 to 9000
+  // before them: 97 us with eight heads, 76 with four, 85 with two).
+  int most_shift;
+  if (group_rows <= 16) {
+    r.shape = {16, group_rows <= 4 && enough(3) && batch * kv_heads >= kComputeUnits ? 8 : 4};
+    most_shift = r.shape.waves == 8 ? 3 : 2;
+  } else if (group_rows <= 32) {
+    r.shape = {32, 8};
+    most_shift = 2;
+  } else {
+    r.shape = {64, 4};
+    r.row_shift = group_rows <= 64 ? 0 : group_rows <= 128 ? 1 : 2;
+    most_shift = group_rows <= 64 ? 1 : 0;
+  }
+  int head_shift = 0;
+  while (head_shift < most_shift && enough(head_shift + 1)) ++head_shift;
+  r.key_shift = (r.shape.waves == 8 ? 3 : 2) - r.row_shift - head_shift;
+  r.part_tokens = (int)std::min(rows, (int64_t(r.shape.rows) << r.row_shift) / group);
+  r.row_parts = (int)((rows + r.part_tokens - 1) / r.part_tokens);
+  const int64_t groups = batch * r.row_parts * (kv_heads >> head_shift);
+  r.tiles = groups * tiles;
+  const int64_t slot_rows = r.row_shift > 0 ? r.shape.rows : std::min<int64_t>(r.shape.rows, r.part_tokens * group);
+  const int64_t record_bytes = (slot_rows << (r.row_shift + head_shift)) * (kHeadDim + 2) * 4;
+  int64_t shares = groups;
+  if (r.row_parts > 1) {
+    r.splits = (int)std::max<int64_t>(1, std::min(kComputeUnits / groups, tiles >> r.key_shift));
+    shares = groups * r.splits;
+  } else {
+    r.full_shares = (int)std::max(kComputeUnits - groups, int64_t(kComputeUnits / 2));
+    if ((groups + r.full_shares) * record_bytes <= kMaxRecordBytes && groups + r.full_shares <= kCounterBytes / 8) {
+      r.min_tiles = 1 << r.key_shift;
+      // Half a microsecond, where the groups are so many that their last shares matter
+      // (without: 274 us in place of the 234 above with four heads).
+      r.halvings = tiles > 64 && groups >= kComputeUnits / 4 ? 5 : 0;
+      shares = std::min(groups + r.full_shares, r.tiles);
+    } else {
+      r.min_tiles = (int)tiles;  // no group is cut
+    }
+  }
+  r.workgroups = (int)((shares + 7) / 8 * 8);
+  r.workspace_bytes = shares > groups ? kCounterBytes + r.workgroups * record_bytes : 0;
   return r;
+}
+
+int check_tiles(int64_t tiles) {
+  if (tiles > kMaxUnits) {
+    return report(TM_ERR_UNSUPPORTED, "the call may read %lld tiles of 32 keys; the limit is %d", (long long)tiles, kMaxUnits);
+  }
+  return TM_OK;
 }
 
 }  // namespace
@@ -234,7 +289,7 @@ int64_t tm_cached_attention_workspace_size(int64_t batch, int64_t rows, int64_t 
   if (check_cached(batch, rows, heads, kv_heads, table_cols, window, sinks) != TM_OK) return -1;
   if (batch == 0 || rows == 0) return 0;
   const CachedPlan plan = cached_plan(batch, rows, heads, kv_heads, table_cols, window, sinks);
-  return check_units(plan.units) == TM_OK ? plan.workspace_bytes : -1;
+  return check_tiles(plan.tiles) == TM_OK ? plan.workspace_bytes : -1;
 }
 
 int tm_cached_attention(const void* query, int64_t query_stride, const void* key_cache, int64_t key_page_stride,
@@ -259,7 +314,7 @@ int tm_cached_attention(const void* query, int64_t query_stride, const void* key
   if (st == TM_OK) st = check_element(seq_lens, 4);
   if (st != TM_OK) return st;
   const CachedPlan plan = cached_plan(batch, rows, heads, kv_heads, table_cols, window, sinks);
-  st = check_units(plan.units);
+  st = check_tiles(plan.tiles);
   if (st == TM_OK) st = check_workspace(workspace, workspace_bytes, plan.workspace_bytes);
   if (st != TM_OK) return st;
   const Range written[] = {{out, batch * rows * heads * kHeadBytes, "out"},
@@ -287,9 +342,11 @@ int tm_cached_attention(const void* query, int64_t query_stride, const void* key
   p.table_stride = table_stride;
   p.seq_lens = seq_lens;
   p.out = static_cast<uint16_t*>(out);
-  p.counters = static_cast<unsigned long long*>(workspace);
-  p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
-  p.epoch = workspace_tag(workspace);
+  if (plan.workspace_bytes > 0) {
+    p.counters = static_cast<unsigned long long*>(workspace);
+    p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
+    p.epoch = workspace_tag(workspace);
+  }
   p.table_cols = (int)table_cols;
   p.batch = (int)batch;
   p.rows = (int)rows;
@@ -299,7 +356,14 @@ int tm_cached_attention(const void* query, int64_t query_stride, const void* key
   p.num_pages = (int)num_pages;
   p.window = (int)(window >= INT32_MAX ? -1 : window);  // past every position: all keys
   p.sinks = (int)std::min<int64_t>(sinks, table_cols * kPageSize);
+  p.row_shift = plan.row_shift;
+  p.key_shift = plan.key_shift;
+  p.part_tokens = plan.part_tokens;
   p.row_parts = plan.row_parts;
+  p.splits = plan.splits;
+  p.full_shares = plan.full_shares;
+  p.min_tiles = plan.min_tiles;
+  p.halvings = plan.halvings;
   p.workgroups = plan.workgroups;
   p.scale_log2 = scale * 1.4426950408889634f;
   return launched(launch_cached_attention(p, plan.shape, dtype == TM_FP16, type, static_cast<hipStream_t>(stream)));
