@@ -52,20 +52,24 @@ struct CachedParams {
   unsigned long long epoch;
   int table_cols, batch, rows, heads, kv_heads, group, num_pages;
   int window, sinks;  // window -1: all keys
-  // The waves of a workgroup: 2^row_shift row tiles times 2^key_shift parts of
+  // Few rows: the waves of a workgroup, 2^row_shift row tiles times 2^key_shift parts of
   // the keys times as many KV heads as that leaves.
   int row_shift, key_shift;
-  int part_tokens, row_parts;  // tokens of a workgroup's rows, and how many such parts a request has
-  int splits;                  // of every part's keys where there are more parts than one; else
-  int full_shares, min_tiles;  // shares by the requests' lengths, of at least min_tiles tiles,
+  int full_shares, min_tiles;  // shares of the keys, of at least min_tiles tiles, by the requests' lengths,
   int halvings;                // made even by so many steps
+  // Chunks: tokens of a workgroup's rows, how many such parts a request has, shares of
+  // every part's keys.
+  int part_tokens, row_parts, splits;
   int workgroups;              // of the grid
   float scale_log2;
 };
-// A wave's rows and a workgroup's waves: 16 x 4, 16 x 8, 32 x 8 or 64 x 4.
+// A wave's rows and a workgroup's waves: 16 x 4, 16 x 8 or 32 x 8.
 struct CachedShape {
   int rows, waves;
 };
+// Rows of a workgroup that attends for a chunk (more rows of a KV head than fit the shapes above).
+constexpr int kChunkRows = 256, kMostFewRows = 128;
+hipError_t launch_cached_chunks(const CachedParams& p, bool fp16, CacheType cache, hipStream_t stream);
 hipError_t launch_cached_attention(const CachedParams& p, CachedShape shape, bool fp16, CacheType cache,
                                    hipStream_t stream);
 

@@ -42,18 +42,10 @@
 
 #include <stdint.h>
 
-#include <type_traits>
-
-#include "trianglemix_cached.h"
-#include "trianglemix_lists.h"
+#include "trianglemix_cached_device.h"
 
 namespace tmx {
 namespace {
-
-typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
-
-#define TM_INLINED __attribute__((always_inline))  // a call would put all that a lambda names into memory
 
 // Max / sum over the four lanes that hold one row (l, l ^ 16, l ^ 32, l ^ 48).
 __device__ __forceinline__ float row_max(float x) {
@@ -80,16 +72,6 @@ __device__ __forceinline__ int wave_prefix(int x) {
   return x;
 }
 __device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_prefix(x), 63); }
-
-// The bits of two 16-bit numbers of type Type from two e4m3 ones.
-template <class Type, bool kHigh>
-__device__ __forceinline__ unsigned from_e4m3(unsigned x) {
-  if constexpr (std::is_same_v<Type, Fp16>) {
-    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, kHigh));
-  } else {
-    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, kHigh));
-  }
-}
 
 // A wave's share of a page, 32 keys: what its lanes load, and the operands made of it.
 template <class Type, CacheType kCache>
@@ -208,21 +190,6 @@ __device__ __forceinline__ void v_operands(const T& tile, int w, u32x4_t& even, 
   }
 }
 
-// The 32-key tiles that rows at first_pos .. last_pos may attend: `sinks` from the
-// first on, then first .. end - 1; at least one where there is a row.
-struct Tiles {
-  int sinks, first, end, count;
-  __device__ __forceinline__ Tiles(const CachedParams& p, int first_pos, int last_pos) {
-    end = (min(max(last_pos, -1) + 1, p.table_cols * kPageSize) + kKvTile - 1) / kKvTile;
-    const int first_key = p.window < 0 ? 0 : max(0, max(0, first_pos) - p.window);
-    first = min(first_key / kKvTile, end);
-    sinks = min((int)(((unsigned)p.sinks + kKvTile - 1) / kKvTile), first);
-    count = last_pos < 0 ? 0 : max(1, sinks + end - first);
-  }
-  __device__ __forceinline__ int tile(int i) const { return i < sinks ? i : first + (i - sinks); }
-};
-
-typedef const __attribute__((address_space(4))) int32_t* ConstInts;  // read by scalar loads
 
 template <class Type, CacheType kCache, int NT, int kWaves>
 __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const CachedParams p) {
@@ -246,7 +213,6 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
   const int lane = tid & 63;
   const int col = lane & 15;  // row of the wave's 16-row tile
   const int quad = lane >> 4;
-  const int run = blockIdx.x;
   const int G = p.group;
   const GroupDivider by_group(p.group);
   const int token_bytes = p.kv_heads * kHeadBytes;
@@ -255,97 +221,64 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
   const int row_tiles = 1 << p.row_shift, row_tile = slot & (row_tiles - 1);
   const int head_shift = kWaveShift - p.key_shift - p.row_shift, head_part = slot >> p.row_shift;
   const int head_groups = p.kv_heads >> head_shift;
-  const int slot_rows = row_tiles > 1 ? kRows : min(kRows, p.part_tokens * G);  // of a partial's record
-  // The merge of partials: 16 threads a row; where the rows leave threads over, `parts`
-  // of them share a row's partials, of which each loads kFlight at a time.
-  constexpr int kRowsAtOnce = kThreads / 16, kFlight = 8;
+  const int slot_rows = row_tiles > 1 ? kRows : min(kRows, p.rows * G);  // of a partial's record
   const int record_rows = slots * slot_rows;
-  int row_slots = 1;
-  while (row_slots < record_rows && row_slots < kRowsAtOnce) row_slots *= 2;
-  const int parts = kRowsAtOnce / row_slots;
-  const int cluster = kFlight * parts;  // shares that are merged at once
-
+  const int cluster = kPartialsInFlight * merge_parts<kThreads>(record_rows);  // shares that are merged at once
   for (int i = tid; i < kWaves * kRows * 12; i += kThreads) (&s_odd[0][0][0])[i] = 0;
   __syncthreads();
 
-  // ---- this workgroup's group, and its tiles lo .. hi - 1, share `share` of `shares` ----
-  int request, head_group, part = 0, share, shares, each, first_share;
+  // ---- this workgroup's group, and its tiles lo .. hi - 1, one of `shares` shares ----
+  // Every group is cut into as many shares as its tiles take at `least` a share, the
+  // same for all and enough to keep all groups' shares within the grid.
   auto len_of = [&](int b) TM_INLINED { return b < p.batch ? max(p.seq_lens[b], 0) : 0; };
-  int len;
-  if (p.row_parts == 1) {
-    // Every group is cut into as many shares as its tiles take at `least` a share, the
-    // same for all and enough to keep all groups' shares within the grid.
-    auto tiles_of = [&](int n) TM_INLINED { return Tiles(p, n - p.rows, n - 1).count; };
-    int len64 = len_of(lane);
-    int tiles64 = tiles_of(len64);
-    int total = tiles64;
-    for (int b = 64 + lane; b < p.batch + lane; b += 64) total += tiles_of(len_of(b));
-    total = wave_sum(total);
-    // Sure: sum(ceil(tiles / least)) is at most total / least and a share more a group.
-    // One block of requests: the smallest such number by halves from total / workgroups on.
-    int least = max(p.min_tiles, (int)(((unsigned)(total * head_groups) + (unsigned)p.full_shares - 1u) / (unsigned)p.full_shares));
-    if (p.batch <= 64 && least > p.min_tiles) {
-      int low = max(p.min_tiles, (int)((unsigned)(total * head_groups) / (unsigned)p.workgroups));
+  auto tiles_of = [&](int n) TM_INLINED { return Tiles<kKvTile>(p, n - p.rows, n - 1).count; };
+  int len64 = len_of(lane);
+  int tiles64 = tiles_of(len64);  // of requests base .. base + 63, one a lane
+  int total = tiles64;
+  for (int b = 64 + lane; b < p.batch + lane; b += 64) total += tiles_of(len_of(b));
+  total = wave_sum(total);
+  // Sure: sum(ceil(tiles / least)) is at most total / least and a share more a group.
+  // One block of requests: the smallest such number by halves from total / workgroups on.
+  int least = max(p.min_tiles, (int)(((unsigned)(total * head_groups) + (unsigned)p.full_shares - 1u) / (unsigned)p.full_shares));
+  if (p.batch <= 64 && least > p.min_tiles) {
+    int low = max(p.min_tiles, (int)((unsigned)(total * head_groups) / (unsigned)p.workgroups));
 #pragma unroll 1
-      for (int i = 0; i < p.halvings && low < least; ++i) {
-        const int mid = (int)(((unsigned)low + (unsigned)least) >> 1);
-        const int all = wave_sum((int)((unsigned)(tiles64 + mid - 1) / (unsigned)mid)) * head_groups;
-        if (all <= p.workgroups) least = mid;
-        else low = mid + 1;
-      }
+    for (int i = 0; i < p.halvings && low < least; ++i) {
+      const int mid = (int)(((unsigned)low + (unsigned)least) >> 1);
+      const int all = wave_sum((int)((unsigned)(tiles64 + mid - 1) / (unsigned)mid)) * head_groups;
+      if (all <= p.workgroups) least = mid;
+      else low = mid + 1;
     }
-    int base = 0, before = 0, shares64, upto64;  // the requests base .. base + 63, one a lane
-    for (;;) {
-      // no more shares than are merged at once, where that leaves them short
-      const int each64 = max(least, min((tiles64 + cluster - 1) / cluster, 8 << p.key_shift));
-      shares64 = (int)((unsigned)(tiles64 + each64 - 1) / (unsigned)each64);
-      upto64 = before + wave_prefix(shares64 * head_groups);
-      if (__builtin_amdgcn_readlane(upto64, 63) > run) break;
-      before = __builtin_amdgcn_readlane(upto64, 63);
-      base += 64;
-      if (base >= p.batch) return;  // more workgroups than shares
-      len64 = len_of(base + lane);
-      tiles64 = tiles_of(len64);
-    }
-    const int in_block = __ffsll((unsigned long long)__ballot(upto64 > run)) - 1;
-    request = base + in_block;
-    len = __builtin_amdgcn_readlane(len64, in_block);
-    shares = __builtin_amdgcn_readlane(shares64, in_block);
-    const int at = run - (__builtin_amdgcn_readlane(upto64, in_block) - shares * head_groups);
-    // the shares of neighbouring heads side by side: they read neighbouring numbers
-    share = at / head_groups;
-    head_group = at - share * head_groups;
-    first_share = run - at + head_group;
-  } else {
-    unsigned id = (unsigned)run;
-    head_group = (int)(id % (unsigned)head_groups);
-    id /= (unsigned)head_groups;
-    share = (int)(id % (unsigned)p.splits);
-    id /= (unsigned)p.splits;
-    request = (int)(id % (unsigned)p.batch);
-    part = p.row_parts - 1 - (int)(id / (unsigned)p.batch);  // later rows attend more keys
-    if (part < 0) return;  // the grid is a multiple of 8
-    len = __builtin_amdgcn_readfirstlane(len_of(request));
-    first_share = run - share * head_groups;
   }
-  const int part_tokens = min(p.part_tokens, p.rows - part * p.part_tokens);
-  const int part_rows = part_tokens * G;
-  const int pos0 = len - p.rows + part * p.part_tokens;  // of the part's first token; a negative one is no row
-  const Tiles tiles(p, pos0, pos0 + part_tokens - 1);
-  if (p.row_parts > 1) {
-    each = (tiles.count + p.splits - 1) / p.splits;
-    shares = each > 0 ? (tiles.count + each - 1) / each : 0;
-    if (share >= shares) return;
-  } else {
-    each = (tiles.count + shares - 1) / shares;  // as even as they come
-    shares = (tiles.count + each - 1) / each;
-    if (share >= shares) return;
+  const int run = blockIdx.x;
+  int base = 0, before = 0, shares64, upto64;
+  for (;;) {
+    // no more shares than are merged at once, where that leaves them short
+    const int each64 = max(least, min((tiles64 + cluster - 1) / cluster, 8 << p.key_shift));
+    shares64 = (int)((unsigned)(tiles64 + each64 - 1) / (unsigned)each64);
+    upto64 = before + wave_prefix(shares64 * head_groups);
+    if (__builtin_amdgcn_readlane(upto64, 63) > run) break;
+    before = __builtin_amdgcn_readlane(upto64, 63);
+    base += 64;
+    if (base >= p.batch) return;  // more workgroups than shares
+    len64 = len_of(base + lane);
+    tiles64 = tiles_of(len64);
   }
+  const int in_block = __ffsll((unsigned long long)__ballot(upto64 > run)) - 1;
+  const int request = base + in_block;
+  const int len = __builtin_amdgcn_readlane(len64, in_block);
+  int shares = __builtin_amdgcn_readlane(shares64, in_block);
+  const int at = run - (__builtin_amdgcn_readlane(upto64, in_block) - shares * head_groups);
+  // the shares of neighbouring heads side by side: they read neighbouring numbers
+  const int share = at / head_groups, head_group = at - share * head_groups;
+  const int part_rows = p.rows * G;
+  const int pos0 = len - p.rows;  // of the first token; a negative one is no row
+  const Tiles<kKvTile> tiles(p, pos0, len - 1);
+  const int each = (tiles.count + shares - 1) / shares;  // as even as they come
+  shares = (tiles.count + each - 1) / each;
+  if (share >= shares) return;
   const int lo = share * each, hi = min(lo + each, tiles.count);
-  // Record and arrival word of share s of the group: those of the workgroup that has it.
-  const int share_step = head_groups;
-  const int record_bytes = slots * slot_rows * (kHeadDim + 2) * 4;
-  auto record = [&](int s) TM_INLINED { return (unsigned)(first_share + s * share_step) * (unsigned)record_bytes; };
+  const Shares group(p, record_rows, run - at + head_group, head_groups, share, shares);
   const int tokens = min(len, p.table_cols * kPageSize);  // with a key
   const bool whole = shares == 1;
   const int kv_head = (head_group << head_shift) + head_part;
@@ -353,7 +286,7 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
   const int valid_rows = min(kRows, part_rows - row_base);  // none: the wave only takes part in the joins
   const int first_pos = pos0 + by_group.token(row_base);
   const int last_pos = valid_rows > 0 ? pos0 + by_group.token(row_base + valid_rows - 1) : -1;
-  const int row0 = request * p.rows + part * p.part_tokens;  // of query and out
+  const int row0 = request * p.rows;  // of query and out
 
   // ---- Q ----
   i16x8_t q[NT][4];
@@ -572,24 +505,6 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
         p.out + ((int64_t)(row0 + t) * p.heads + head * G + (at - t * G)) * kHeadDim + 8 * c8) = y;
   };
   auto rows_of = [&](int of_slot) TM_INLINED { return min(kRows, part_rows - (of_slot & (row_tiles - 1)) * kRows); };
-  // a record: O of all slots' rows, then their row maxima and sums
-  const __amdgpu_buffer_rsrc_t rec = __builtin_amdgcn_make_buffer_rsrc(
-      (void*)p.partials, (short)0, whole ? 0 : (int)((unsigned)p.workgroups * (unsigned)record_bytes),
-      kBufferFlags);
-  auto store_partial = [&](int s, int rr, const float* acc, float max, float l) TM_INLINED {
-    const unsigned at = record(s);
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const f32x4_t x = {acc[4 * half], acc[4 * half + 1], acc[4 * half + 2], acc[4 * half + 3]};
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, x), rec,
-                                             at + (rr * kHeadDim + 8 * c8 + 4 * half) * 4, 0, kCpolAgent);
-    }
-    if (c8 == 0) {
-      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(max), rec, at + (record_rows * kHeadDim + rr) * 4, 0, kCpolAgent);
-      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), rec, at + (record_rows * (kHeadDim + 1) + rr) * 4, 0,
-                                            kCpolAgent);
-    }
-  };
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     __syncthreads();
@@ -639,111 +554,22 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
       if (whole) {
         store_row(of_slot, r, acc, l);
       } else {
-        store_partial(share, of_slot * slot_rows + r, acc, all, l);
+        const int row = of_slot * slot_rows + r;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const f32x4_t x = {acc[4 * half], acc[4 * half + 1], acc[4 * half + 2], acc[4 * half + 3]};
+          group.store(share, row, 8 * c8 + 4 * half, x);
+        }
+        if (c8 == 0) group.store_sums(share, row, all, l);
       }
     }
   }
 
-  if (whole) return;
-
-  // ---- the shares: the workgroup that arrives last at a cluster of them merges it, the
-  // one that arrives last of the clusters those ----
-  for (int level = 0; level < 2; ++level) {
-    const int stride = level == 0 ? 1 : cluster;
-    const int from = level == 0 ? share / cluster * cluster : 0;  // the first share that is merged, then every stride-th
-    const int count = level == 0 ? min(cluster, shares - from) : (shares + cluster - 1) / cluster;
-    const bool last_level = level == 1 || shares <= cluster;
-    wait_dma();  // this wave's partial stores have completed
-    __syncthreads();
-    // words: the cluster's first share's; the group's second share's
-    unsigned long long* const word = p.counters + first_share + (level == 0 ? from : 1) * head_groups;
-    if (tid == 0) {
-      s_last = (int)(count_arrival(word, p.epoch) == (unsigned long long)count);
-      // The word is left at this launch's tag with a count of zero for the next one.
-      if (s_last) __hip_atomic_store(word, p.epoch << kEpochShift, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (!s_last) return;
-    // Part pg of a row's threads takes every parts-th partial; they join through LDS.
-    const int pg = r16 / row_slots;
-    for (int rb = 0; rb < record_rows; rb += row_slots) {
-      const int rr = rb + r16 % row_slots, of_slot = rr / slot_rows, r = rr - of_slot * slot_rows;
-      const bool held = rr < record_rows && r < rows_of(of_slot);
-      float top = -INFINITY, l = 0.0f, acc[8] = {};
-      if (held) {
-        for (int s0 = pg; s0 < count; s0 += kFlight * parts) {
-          float ms[kFlight], ls[kFlight];
-          f32x4_t x[kFlight][2];
-#pragma unroll
-          for (int j = 0; j < kFlight; ++j) {
-            // past the last one its loads fall outside the buffer's range
-            const int s = s0 + j * parts;
-            const unsigned at = s < count ? record(from + s * stride) : kOutOfRange;
-            ms[j] = __uint_as_float(
-                __builtin_amdgcn_raw_buffer_load_b32(rec, at + (record_rows * kHeadDim + rr) * 4, 0, kCpolAgent));
-            ls[j] = __uint_as_float(
-                __builtin_amdgcn_raw_buffer_load_b32(rec, at + (record_rows * (kHeadDim + 1) + rr) * 4, 0, kCpolAgent));
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              x[j][half] = __builtin_bit_cast(
-                  f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                               rec, at + (rr * kHeadDim + 8 * c8 + 4 * half) * 4, 0, kCpolAgent));
-            }
-          }
-          float next = top;
-#pragma unroll
-          for (int j = 0; j < kFlight; ++j) {
-            if (s0 + j * parts >= count) ms[j] = -INFINITY;
-            next = fmaxf(next, ms[j]);
-          }
-          const float shift = next == -INFINITY ? 0.0f : next;
-          const float keep = __builtin_amdgcn_exp2f(top - shift);
-          l *= keep;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc[e] *= keep;
-#pragma unroll
-          for (int j = 0; j < kFlight; ++j) {
-            const float w = __builtin_amdgcn_exp2f(ms[j] - shift);
-            l += ls[j] * w;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] += x[j][e >> 2][e & 3] * w;
-          }
-          top = next;
-        }
-      }
-      if (parts > 1) {
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 8; ++e) join[tid][e] = acc[e];
-        join[tid][8] = top;
-        join[tid][9] = l;
-        __syncthreads();
-        if (pg == 0) {
-          float all = top;
-          for (int k = 1; k < parts; ++k) all = fmaxf(all, join[tid + k * 16 * row_slots][8]);
-          const float shift = all == -INFINITY ? 0.0f : all;
-          const float keep = __builtin_amdgcn_exp2f(top - shift);
-          l *= keep;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc[e] *= keep;
-          for (int k = 1; k < parts; ++k) {
-            const float* const other = join[tid + k * 16 * row_slots];
-            const float w = __builtin_amdgcn_exp2f(other[8] - shift);
-            l += other[9] * w;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] += other[e] * w;
-          }
-          top = all;
-        }
-      } else if (!last_level) {
-        __syncthreads();  // all have read the record that the result replaces
-      }
-      if (pg == 0 && held) {
-        if (last_level) store_row(of_slot, r, acc, l);
-        else store_partial(from, rr, acc, top, l);
-      }
-    }
-    if (last_level) return;
+  if (!whole) {
+    merge_shares<kThreads>(
+        p, group, join, &s_last,
+        [&](int row) TM_INLINED { return row % slot_rows < rows_of(row / slot_rows); },
+        [&](int row, int, const float* acc, float l) TM_INLINED { store_row(row / slot_rows, row % slot_rows, acc, l); });
   }
 }
 
@@ -756,8 +582,6 @@ hipError_t launch_shape(const CachedParams& p, CachedShape shape, hipStream_t st
     hipLaunchKernelGGL((cached_attention_kernel<Type, kCache, 1, 8>), grid, block, 0, stream, p);
   } else if (shape.rows == 32 && shape.waves == 8) {
     hipLaunchKernelGGL((cached_attention_kernel<Type, kCache, 2, 8>), grid, block, 0, stream, p);
-  } else if (shape.rows == 64 && shape.waves == 4) {
-    hipLaunchKernelGGL((cached_attention_kernel<Type, kCache, 4, 4>), grid, block, 0, stream, p);
   } else {
     return hipErrorInvalidValue;
   }

@@ -102,6 +102,18 @@ CachedPlan cached_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_he
   const auto enough = [&](int shift) {
     return kv_heads % (1 << shift) == 0 && batch * (kv_heads >> shift) * std::max<int64_t>(1, tiles / 32) >= kComputeUnits;
   };
+  if (group_rows > kMostFewRows) {
+    // Chunks: workgroups of 256 rows, and as many shares of their keys as fill the GPU.
+    r.part_tokens = (int)(kChunkRows / group);
+    r.row_parts = (int)((rows + r.part_tokens - 1) / r.part_tokens);
+    const int64_t groups = batch * r.row_parts * kv_heads;
+    r.tiles = groups * tiles;
+    r.splits = (int)std::max<int64_t>(1, std::min(kComputeUnits / groups, tiles / 8));
+    r.workgroups = (int)(groups * r.splits);
+    const int64_t record_bytes = r.part_tokens * group * (kHeadDim + 2) * 4;
+    r.workspace_bytes = r.splits > 1 ? kCounterBytes + r.workgroups * record_bytes : 0;
+    return r;
+  }
   // A wave's rows and the row tiles of a workgroup's waves; what these leave of the
   // waves goes to neighbouring KV heads, whose numbers lie side by side in memory (64
   // requests of 2000 to 16384 tokens: 222 us with eight heads a workgroup, 234 with
@@ -112,38 +124,28 @@ CachedPlan cached_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_he
   if (group_rows <= 16) {
     r.shape = {16, group_rows <= 4 && enough(3) && batch * kv_heads >= kComputeUnits ? 8 : 4};
     most_shift = r.shape.waves == 8 ? 3 : 2;
-  } else if (group_rows <= 32) {
-    r.shape = {32, 8};
-    most_shift = 2;
   } else {
-    r.shape = {64, 4};
-    r.row_shift = group_rows <= 64 ? 0 : group_rows <= 128 ? 1 : 2;
-    most_shift = group_rows <= 64 ? 1 : 0;
+    r.shape = {32, 8};
+    r.row_shift = group_rows <= 32 ? 0 : group_rows <= 64 ? 1 : 2;
+    most_shift = 2 - r.row_shift;
   }
   int head_shift = 0;
   while (head_shift < most_shift && enough(head_shift + 1)) ++head_shift;
   r.key_shift = (r.shape.waves == 8 ? 3 : 2) - r.row_shift - head_shift;
-  r.part_tokens = (int)std::min(rows, (int64_t(r.shape.rows) << r.row_shift) / group);
-  r.row_parts = (int)((rows + r.part_tokens - 1) / r.part_tokens);
-  const int64_t groups = batch * r.row_parts * (kv_heads >> head_shift);
+  const int64_t groups = batch * (kv_heads >> head_shift);
   r.tiles = groups * tiles;
-  const int64_t slot_rows = r.row_shift > 0 ? r.shape.rows : std::min<int64_t>(r.shape.rows, r.part_tokens * group);
+  const int64_t slot_rows = r.row_shift > 0 ? r.shape.rows : std::min<int64_t>(r.shape.rows, group_rows);
   const int64_t record_bytes = (slot_rows << (r.row_shift + head_shift)) * (kHeadDim + 2) * 4;
   int64_t shares = groups;
-  if (r.row_parts > 1) {
-    r.splits = (int)std::max<int64_t>(1, std::min(kComputeUnits / groups, tiles >> r.key_shift));
-    shares = groups * r.splits;
+  r.full_shares = (int)std::max(kComputeUnits - groups, int64_t(kComputeUnits / 2));
+  if ((groups + r.full_shares) * record_bytes <= kMaxRecordBytes && groups + r.full_shares <= kCounterBytes / 8) {
+    r.min_tiles = 1 << r.key_shift;
+    // Half a microsecond, where the groups are so many that their last shares matter
+    // (without: 274 us in place of the 234 above with four heads).
+    r.halvings = tiles > 64 && groups >= kComputeUnits / 4 ? 5 : 0;
+    shares = std::min(groups + r.full_shares, r.tiles);
   } else {
-    r.full_shares = (int)std::max(kComputeUnits - groups, int64_t(kComputeUnits / 2));
-    if ((groups + r.full_shares) * record_bytes <= kMaxRecordBytes && groups + r.full_shares <= kCounterBytes / 8) {
-      r.min_tiles = 1 << r.key_shift;
-      // Half a microsecond, where the groups are so many that their last shares matter
-      // (without: 274 us in place of the 234 above with four heads).
-      r.halvings = tiles > 64 && groups >= kComputeUnits / 4 ? 5 : 0;
-      shares = std::min(groups + r.full_shares, r.tiles);
-    } else {
-      r.min_tiles = (int)tiles;  // no group is cut
-    }
+    r.min_tiles = (int)tiles;  // no group is cut
   }
   r.workgroups = (int)((shares + 7) / 8 * 8);
   r.workspace_bytes = shares > groups ? kCounterBytes + r.workgroups * record_bytes : 0;
@@ -366,7 +368,9 @@ int tm_cached_attention(const void* query, int64_t query_stride, const void* key
   p.halvings = plan.halvings;
   p.workgroups = plan.workgroups;
   p.scale_log2 = scale * 1.4426950408889634f;
-  return launched(launch_cached_attention(p, plan.shape, dtype == TM_FP16, type, static_cast<hipStream_t>(stream)));
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  return launched(plan.row_parts > 0 ? launch_cached_chunks(p, dtype == TM_FP16, type, s)
+                                     : launch_cached_attention(p, plan.shape, dtype == TM_FP16, type, s));
 }
 
 }  // extern "C"
