@@ -57,9 +57,10 @@ struct CachedParams {
   int row_shift, key_shift;
   int full_shares, min_tiles;  // shares of the keys, of at least min_tiles tiles, by the requests' lengths,
   int halvings;                // made even by so many steps
-  // Chunks: tokens of a workgroup's rows, how many such parts a request has, shares of
-  // every part's keys.
-  int part_tokens, row_parts, splits;
+  // Chunks: tokens of a workgroup's rows, how many such parts a request has; of all
+  // requests' parts, the latest first, full_parts have a workgroup a KV head, the
+  // others one for each of `splits` shares of their keys.
+  int part_tokens, row_parts, full_parts, splits;
   int workgroups;              // of the grid
   float scale_log2;
 };

@@ -223,7 +223,8 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
   const int head_groups = p.kv_heads >> head_shift;
   const int slot_rows = row_tiles > 1 ? kRows : min(kRows, p.rows * G);  // of a partial's record
   const int record_rows = slots * slot_rows;
-  const int cluster = kPartialsInFlight * merge_parts<kThreads>(record_rows);  // shares that are merged at once
+  constexpr int kFlight = 8, kEach = NT;  // of the merge
+  const int cluster = kFlight * merge_parts<kThreads>(record_rows);  // shares that are merged at once
   for (int i = tid; i < kWaves * kRows * 12; i += kThreads) (&s_odd[0][0][0])[i] = 0;
   __syncthreads();
 
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
   shares = (tiles.count + each - 1) / each;
   if (share >= shares) return;
   const int lo = share * each, hi = min(lo + each, tiles.count);
-  const Shares group(p, record_rows, run - at + head_group, head_groups, share, shares);
+  const Shares group(p, p.workgroups, record_rows, run - at + head_group, head_groups, share, shares);
   const int tokens = min(len, p.table_cols * kPageSize);  // with a key
   const bool whole = shares == 1;
   const int kv_head = (head_group << head_shift) + head_part;
@@ -566,7 +567,7 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
   }
 
   if (!whole) {
-    merge_shares<kThreads>(
+    merge_shares<kThreads, kFlight, kEach>(
         p, group, join, &s_last,
         [&](int row) TM_INLINED { return row % slot_rows < rows_of(row / slot_rows); },
         [&](int row, int, const float* acc, float l) TM_INLINED { store_row(row / slot_rows, row % slot_rows, acc, l); });

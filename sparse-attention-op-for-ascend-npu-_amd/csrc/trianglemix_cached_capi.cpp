@@ -70,7 +70,7 @@ constexpr int64_t kMaxRecordBytes = int64_t(64) << 20;
 
 struct CachedPlan {
   CachedShape shape;
-  int row_shift, key_shift, part_tokens, row_parts, splits, full_shares, min_tiles, halvings, workgroups;
+  int row_shift, key_shift, part_tokens, row_parts, full_parts, splits, full_shares, min_tiles, halvings, workgroups;
   int64_t tiles, workspace_bytes;
 };
 
@@ -103,15 +103,25 @@ CachedPlan cached_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_he
     return kv_heads % (1 << shift) == 0 && batch * (kv_heads >> shift) * std::max<int64_t>(1, tiles / 32) >= kComputeUnits;
   };
   if (group_rows > kMostFewRows) {
-    // Chunks: workgroups of 256 rows, and as many shares of their keys as fill the GPU.
+    // Chunks: workgroups of 256 rows, one a CU.  What does not fill the GPU's last round
+    // is shared out, into as many shares as end soonest: a share costs some seven
+    // steps besides its own (the start, its partial, the merge).
     r.part_tokens = (int)(kChunkRows / group);
     r.row_parts = (int)((rows + r.part_tokens - 1) / r.part_tokens);
-    const int64_t groups = batch * r.row_parts * kv_heads;
-    r.tiles = groups * tiles;
-    r.splits = (int)std::max<int64_t>(1, std::min(kComputeUnits / groups, tiles / 8));
-    r.workgroups = (int)(groups * r.splits);
+    const int64_t parts = batch * r.row_parts, steps = (tiles + 1) / 2;
+    r.tiles = parts * kv_heads * tiles;
+    r.full_parts = (int)(parts * kv_heads / kComputeUnits * kComputeUnits / kv_heads);
+    const int64_t rest = (parts - r.full_parts) * kv_heads;
+    const auto cost = [&](int64_t splits) {
+      return (rest * splits + kComputeUnits - 1) / kComputeUnits * ((steps + splits - 1) / splits + (splits > 1 ? 7 : 0));
+    };
+    r.splits = 1;
     const int64_t record_bytes = r.part_tokens * group * (kHeadDim + 2) * 4;
-    r.workspace_bytes = r.splits > 1 ? kCounterBytes + r.workgroups * record_bytes : 0;
+    for (int s = 2; s <= std::min<int64_t>(32, steps / 4) && rest * s * record_bytes <= kMaxRecordBytes; ++s) {
+      if (cost(s) < cost(r.splits)) r.splits = s;
+    }
+    r.workgroups = (int)(r.full_parts * kv_heads + rest * r.splits);
+    r.workspace_bytes = r.splits > 1 ? kCounterBytes + rest * r.splits * record_bytes : 0;
     return r;
   }
   // A wave's rows and the row tiles of a workgroup's waves; what these leave of the
@@ -362,6 +372,7 @@ int tm_cached_attention(const void* query, int64_t query_stride, const void* key
   p.key_shift = plan.key_shift;
   p.part_tokens = plan.part_tokens;
   p.row_parts = plan.row_parts;
+  p.full_parts = plan.full_parts;
   p.splits = plan.splits;
   p.full_shares = plan.full_shares;
   p.min_tiles = plan.min_tiles;

@@ -57,12 +57,12 @@ struct Shares {
   int first, step;  // workgroup of share 0, and from one share to the next
   int share, count;
 
-  __device__ __forceinline__ Shares(const CachedParams& p, int record_rows, int first_share, int share_step, int own,
-                                    int shares)
+  __device__ __forceinline__ Shares(const CachedParams& p, int records, int record_rows, int first_share, int share_step,
+                                    int own, int shares)
       : record_bytes((unsigned)record_rows * ((kHeadDim + 2) * 4)), rows(record_rows), first(first_share),
         step(share_step), share(own), count(shares) {
     partials = __builtin_amdgcn_make_buffer_rsrc(
-        (void*)p.partials, (short)0, shares > 1 ? (int)((unsigned)p.workgroups * record_bytes) : 0, kBufferFlags);
+        (void*)p.partials, (short)0, shares > 1 ? (int)((unsigned)records * record_bytes) : 0, kBufferFlags);
   }
   __device__ __forceinline__ unsigned record(int s) const { return (unsigned)(first + s * step) * record_bytes; }
   // Four dims of a row of record s; its maximum and sum.
@@ -80,22 +80,21 @@ struct Shares {
 // Merges a shared group once its partials are stored: the workgroup that arrives last
 // at a cluster of shares merges it, the one that arrives last of the clusters those
 // (the same sums whichever they are).  16 threads a row, 8 dims each; where the rows
-// leave threads over, `parts` of them share a row's partials and join through LDS.
-// Eight partials' loads are in flight at a time.  held(row): whether the record's row
+// leave threads over, `parts` of them share a row's partials and join through LDS.  A
+// thread has the loads of kFlight partials of kEach rows in flight.  held(row): whether the record's row
 // is one; out(row, c8, acc, sum): its dims 8 c8 .. + 7.  Every thread calls it.
-constexpr int kPartialsInFlight = 8;
 template <int kThreads>
 __device__ __forceinline__ int merge_parts(int rows) {
   int row_slots = 1;
   while (row_slots < rows && row_slots < kThreads / 16) row_slots *= 2;
   return kThreads / 16 / row_slots;
 }
-template <int kThreads, class Held, class Out>
+template <int kThreads, int kFlight, int kEach, class Held, class Out>
 __device__ __forceinline__ void merge_shares(const CachedParams& p, const Shares& shares, float (*join)[10], int* last,
                                              Held held, Out out) {
   const int tid = threadIdx.x, r16 = tid >> 4, c8 = tid & 15;
   const int parts = merge_parts<kThreads>(shares.rows), row_slots = kThreads / 16 / parts;
-  const int cluster = kPartialsInFlight * parts, pg = r16 / row_slots;
+  const int cluster = kFlight * parts, pg = r16 / row_slots;
   for (int level = 0; level < 2; ++level) {
     // the shares that are merged: `count` from `from` on, every stride-th
     const int stride = level == 0 ? 1 : cluster;
@@ -113,89 +112,106 @@ __device__ __forceinline__ void merge_shares(const CachedParams& p, const Shares
     }
     __syncthreads();
     if (!*last) return;
-    const int pg = r16 / row_slots;
-    for (int rb = 0; rb < shares.rows; rb += row_slots) {
-      const int row = rb + r16 % row_slots;
-      const bool ok = row < shares.rows && held(row);
-      float top = -INFINITY, l = 0.0f, acc[8] = {};
-      if (ok) {
-        for (int s0 = pg; s0 < count; s0 += kPartialsInFlight * parts) {
-          float ms[kPartialsInFlight], ls[kPartialsInFlight];
-          f32x4_t x[kPartialsInFlight][2];
+    for (int rb = 0; rb < shares.rows; rb += kEach * row_slots) {
+      float top[kEach], l[kEach], acc[kEach][8];
+      int row[kEach];
+      bool ok[kEach];
 #pragma unroll
-          for (int j = 0; j < kPartialsInFlight; ++j) {
-            // past the last one its loads fall outside the buffer's range
+      for (int i = 0; i < kEach; ++i) {
+        row[i] = rb + i * row_slots + r16 % row_slots;
+        ok[i] = row[i] < shares.rows && held(row[i]);
+        top[i] = -INFINITY;
+        l[i] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[i][e] = 0.0f;
+      }
+      for (int s0 = pg; s0 < count; s0 += kFlight * parts) {
+        float ms[kEach][kFlight], ls[kEach][kFlight];
+        f32x4_t x[kEach][kFlight][2];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+#pragma unroll
+          for (int j = 0; j < kFlight; ++j) {
+            // past the last one, and of what is no row, its loads fall outside the buffer's range
             const int s = s0 + j * parts;
-            const unsigned at = s < count ? shares.record(from + s * stride) : kOutOfRange;
-            ms[j] = __uint_as_float(
-                __builtin_amdgcn_raw_buffer_load_b32(shares.partials, at + (shares.rows * kHeadDim + row) * 4, 0, kCpolAgent));
-            ls[j] = __uint_as_float(
-                __builtin_amdgcn_raw_buffer_load_b32(shares.partials, at + (shares.rows * (kHeadDim + 1) + row) * 4, 0, kCpolAgent));
+            const unsigned at = s < count && ok[i] ? shares.record(from + s * stride) : kOutOfRange;
+            ms[i][j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                shares.partials, at + (shares.rows * kHeadDim + row[i]) * 4, 0, kCpolAgent));
+            ls[i][j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                shares.partials, at + (shares.rows * (kHeadDim + 1) + row[i]) * 4, 0, kCpolAgent));
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              x[j][half] = __builtin_bit_cast(
+              x[i][j][half] = __builtin_bit_cast(
                   f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                               shares.partials, at + (row * kHeadDim + 8 * c8 + 4 * half) * 4, 0, kCpolAgent));
+                               shares.partials, at + (row[i] * kHeadDim + 8 * c8 + 4 * half) * 4, 0, kCpolAgent));
             }
           }
-          float next = top;
+        }
 #pragma unroll
-          for (int j = 0; j < kPartialsInFlight; ++j) {
-            if (s0 + j * parts >= count) ms[j] = -INFINITY;
-            next = fmaxf(next, ms[j]);
+        for (int i = 0; i < kEach; ++i) {
+          float next = top[i];
+#pragma unroll
+          for (int j = 0; j < kFlight; ++j) {
+            if (s0 + j * parts >= count) ms[i][j] = -INFINITY;
+            next = fmaxf(next, ms[i][j]);
           }
           const float shift = next == -INFINITY ? 0.0f : next;
-          const float keep = __builtin_amdgcn_exp2f(top - shift);
-          l *= keep;
+          const float keep = __builtin_amdgcn_exp2f(top[i] - shift);
+          l[i] *= keep;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) acc[e] *= keep;
+          for (int e = 0; e < 8; ++e) acc[i][e] *= keep;
 #pragma unroll
-          for (int j = 0; j < kPartialsInFlight; ++j) {
-            const float w = __builtin_amdgcn_exp2f(ms[j] - shift);
-            l += ls[j] * w;
+          for (int j = 0; j < kFlight; ++j) {
+            const float w = __builtin_amdgcn_exp2f(ms[i][j] - shift);
+            l[i] += ls[i][j] * w;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] += x[j][e >> 2][e & 3] * w;
+            for (int e = 0; e < 8; ++e) acc[i][e] += x[i][j][e >> 2][e & 3] * w;
           }
-          top = next;
+          top[i] = next;
         }
       }
       if (parts > 1) {
-        __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) join[tid][e] = acc[e];
-        join[tid][8] = top;
-        join[tid][9] = l;
-        __syncthreads();
-        if (pg == 0) {
-          float all = top;
-          for (int k = 1; k < parts; ++k) all = fmaxf(all, join[tid + k * 16 * row_slots][8]);
-          const float shift = all == -INFINITY ? 0.0f : all;
-          const float keep = __builtin_amdgcn_exp2f(top - shift);
-          l *= keep;
+        for (int i = 0; i < kEach; ++i) {
+          __syncthreads();
 #pragma unroll
-          for (int e = 0; e < 8; ++e) acc[e] *= keep;
-          for (int k = 1; k < parts; ++k) {
-            const float* const other = join[tid + k * 16 * row_slots];
-            const float w = __builtin_amdgcn_exp2f(other[8] - shift);
-            l += other[9] * w;
+          for (int e = 0; e < 8; ++e) join[tid][e] = acc[i][e];
+          join[tid][8] = top[i];
+          join[tid][9] = l[i];
+          __syncthreads();
+          if (pg == 0) {
+            float all = top[i];
+            for (int k = 1; k < parts; ++k) all = fmaxf(all, join[tid + k * 16 * row_slots][8]);
+            const float shift = all == -INFINITY ? 0.0f : all;
+            const float keep = __builtin_amdgcn_exp2f(top[i] - shift);
+            l[i] *= keep;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] += other[e] * w;
+            for (int e = 0; e < 8; ++e) acc[i][e] *= keep;
+            for (int k = 1; k < parts; ++k) {
+              const float* const other = join[tid + k * 16 * row_slots];
+              const float w = __builtin_amdgcn_exp2f(other[8] - shift);
+              l[i] += other[9] * w;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) acc[i][e] += other[e] * w;
+            }
+            top[i] = all;
           }
-          top = all;
         }
       } else if (!last_level) {
-        __syncthreads();  // all have read the record that the result replaces
+        __syncthreads();  // all have read the records that the results replace
       }
-      if (pg == 0 && ok) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        if (pg != 0 || !ok[i]) continue;
         if (last_level) {
-          out(row, c8, acc, l);
+          out(row[i], c8, acc[i], l[i]);
         } else {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const f32x4_t x = {acc[4 * half], acc[4 * half + 1], acc[4 * half + 2], acc[4 * half + 3]};
-            shares.store(from, row, 8 * c8 + 4 * half, x);
+            const f32x4_t x = {acc[i][4 * half], acc[i][4 * half + 1], acc[i][4 * half + 2], acc[i][4 * half + 3]};
+            shares.store(from, row[i], 8 * c8 + 4 * half, x);
           }
-          if (c8 == 0) shares.store_sums(from, row, top, l);
+          if (c8 == 0) shares.store_sums(from, row[i], top[i], l[i]);
         }
       }
     }

@@ -105,8 +105,14 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
   unsigned id = blockIdx.x;
   const int kv_head = (int)(id % (unsigned)p.kv_heads);  // of one XCD where there are eight: it shares their keys
   id /= (unsigned)p.kv_heads;
-  const int share = (int)(id % (unsigned)p.splits);
-  id /= (unsigned)p.splits;
+  // The first p.full_parts parts (of all requests) have a workgroup a KV head, the others p.splits.
+  int splits = 1, share = 0;
+  if ((int)id >= p.full_parts) {
+    splits = p.splits;
+    id -= (unsigned)p.full_parts;
+    share = (int)(id % (unsigned)splits);
+    id = id / (unsigned)splits + (unsigned)p.full_parts;
+  }
   const int request = (int)(id % (unsigned)p.batch);
   const int part = p.row_parts - 1 - (int)(id / (unsigned)p.batch);  // later rows attend more keys
   const int len = max(p.seq_lens[request], 0);
@@ -115,10 +121,12 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
   const int pos0 = len - p.rows + part * p.part_tokens;  // of the part's first token; a negative one is no row
   const Tiles<kStepKeys> tiles(p, pos0, pos0 + part_tokens - 1);
   if (tiles.count == 0) return;
-  const int each = (tiles.count + p.splits - 1) / p.splits, shares = (tiles.count + each - 1) / each;
+  const int each = (tiles.count + splits - 1) / splits, shares = (tiles.count + each - 1) / each;
   if (share >= shares) return;
   const int lo = share * each, steps = min(each, tiles.count - lo);
-  const Shares group(p, min(kChunkRows, p.part_tokens * G), (int)blockIdx.x - share * p.kv_heads, p.kv_heads, share, shares);
+  const int unshared = p.full_parts * p.kv_heads;  // workgroups without records
+  const Shares group(p, p.workgroups - unshared, min(kChunkRows, p.part_tokens * G),
+                     (int)blockIdx.x - unshared - share * p.kv_heads, p.kv_heads, share, shares);
   const int tokens = min(len, p.table_cols * kPageSize);  // with a key
   const int row0 = request * p.rows + part * p.part_tokens;  // of query and out
   for (int i = tid; i < kChunkRows * 12; i += kThreads) (&s_odd[0][0][0])[i] = 0;
@@ -362,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
   }
   float(*const join)[10] = reinterpret_cast<float(*)[10]>(k_lds);
   static_assert(kThreads * 10 * 4 <= 2 * kSlotBytes, "the joined values fit the slots");
-  merge_shares<kThreads>(
+  merge_shares<kThreads, 4, 2>(
       p, group, join, &s_last, [&](int r) TM_INLINED { return r < part_rows; },
       [&](int r, int c8, const float* acc, float sum) TM_INLINED {
         if (pos0 + by_group.token(r) < 0) return;

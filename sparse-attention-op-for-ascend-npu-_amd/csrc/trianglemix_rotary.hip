@@ -80,13 +80,21 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(const RotatePara
     raw_a = *reinterpret_cast<const typename Type::vec*>(from + a_dim);
     raw_b = *reinterpret_cast<const typename Type::vec*>(from + b_dim);
   }
+  // What hangs on none of these is loaded beside them.
+  const double frequency = p.frequencies[min(lane, p.rotary_dim / 2 - 1)];
   int64_t slot = -1;
-  if constexpr (kCache) slot = p.slots[row];
+  float scale = 1.0f;
+  if constexpr (kCache) {
+    slot = p.slots[row];
+    if constexpr (kStored == CacheType::kE4m3) {
+      if (kind == 1 || kind == 2) scale = (kind == 1 ? p.key_scale : p.value_scale)[own];
+    }
+  }
   if (position < 0) return;  // no row
 
   float2 mine = {1.0f, 0.0f};
   if (lane < p.rotary_dim / 2) {
-    const double t = (double)position * (p.frequencies[lane] * 0.15915494309189533577);
+    const double t = (double)position * (frequency * 0.15915494309189533577);
     const float half_turns = 2.0f * (float)(t - rint(t));
     float s, c;
     sincospif(half_turns, &s, &c);
@@ -133,7 +141,6 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(const RotatePara
                                 : p.value_cache + slot / kPageSize * p.value_page_stride) +
                      (slot % kPageSize * p.kv_heads + own) * (kHeadDim * kBytes);
     if constexpr (kStored == CacheType::kE4m3) {
-      const float scale = kind == 1 ? p.key_scale[own] : p.value_scale[own];
       *reinterpret_cast<u32x2_t*>(to + a_dim) = to_e4m3(a, scale);
       *reinterpret_cast<u32x2_t*>(to + b_dim) = to_e4m3(b, scale);
     } else {
