@@ -68,9 +68,10 @@ struct CachedParams {
 struct CachedShape {
   int rows, waves;
 };
-// Rows of a workgroup that attends for a chunk (more rows of a KV head than fit the shapes above).
+// Chunks, of more rows of a KV head than kMostFewRows: workgroups of kChunkRows rows or
+// of half as many.
 constexpr int kChunkRows = 256, kMostFewRows = 128;
-hipError_t launch_cached_chunks(const CachedParams& p, bool fp16, CacheType cache, hipStream_t stream);
+hipError_t launch_cached_chunks(const CachedParams& p, int rows, bool fp16, CacheType cache, hipStream_t stream);
 hipError_t launch_cached_attention(const CachedParams& p, CachedShape shape, bool fp16, CacheType cache,
                                    hipStream_t stream);
 

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <array>
 
 #include "../../include/trianglemix_cached.h"
 #include "trianglemix_cached.h"
@@ -103,25 +104,35 @@ CachedPlan cached_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_he
     return kv_heads % (1 << shift) == 0 && batch * (kv_heads >> shift) * std::max<int64_t>(1, tiles / 32) >= kComputeUnits;
   };
   if (group_rows > kMostFewRows) {
-    // Chunks: workgroups of 256 rows, one a CU.  What does not fill the GPU's last round
-    // is shared out, into as many shares as end soonest: a share costs some seven
-    // steps besides its own (the start, its partial, the merge).
-    r.part_tokens = (int)(kChunkRows / group);
-    r.row_parts = (int)((rows + r.part_tokens - 1) / r.part_tokens);
-    const int64_t parts = batch * r.row_parts, steps = (tiles + 1) / 2;
-    r.tiles = parts * kv_heads * tiles;
-    r.full_parts = (int)(parts * kv_heads / kComputeUnits * kComputeUnits / kv_heads);
-    const int64_t rest = (parts - r.full_parts) * kv_heads;
-    const auto cost = [&](int64_t splits) {
-      return (rest * splits + kComputeUnits - 1) / kComputeUnits * ((steps + splits - 1) / splits + (splits > 1 ? 7 : 0));
-    };
-    r.splits = 1;
-    const int64_t record_bytes = r.part_tokens * group * (kHeadDim + 2) * 4;
-    for (int s = 2; s <= std::min<int64_t>(32, steps / 4) && rest * s * record_bytes <= kMaxRecordBytes; ++s) {
-      if (cost(s) < cost(r.splits)) r.splits = s;
+    // Chunks: workgroups of 256 rows, or of 128 with two key parts, one a CU.  What does
+    // not fill the GPU's last round is shared out.  Taken is what ends soonest by the
+    // time of a step of 64 keys and what a share costs besides (the start, its partial,
+    // the merge), in 0.1 us.  256 | 128 rows: 128 rows of 8192 tokens 65 | 52 us, 300 of
+    // 3000 58 | 41, 512 of 8192 104 | 120, 2048 of 32749 1079 | 1447.
+    const int64_t steps = (tiles + 1) / 2;
+    int64_t best = INT64_MAX;
+    for (const auto [most_rows, step, besides] : {std::array{kChunkRows, 20, 220}, std::array{kChunkRows / 2, 14, 120}}) {
+      const int64_t part_tokens = most_rows / group, row_parts = (rows + part_tokens - 1) / part_tokens;
+      const int64_t parts = batch * row_parts;
+      const int64_t full_parts = parts * kv_heads / kComputeUnits * kComputeUnits / kv_heads;
+      const int64_t rest = (parts - full_parts) * kv_heads;
+      const int64_t record_bytes = part_tokens * group * (kHeadDim + 2) * 4;
+      for (int64_t s = 1; s == 1 || (s <= steps / 4 && s <= 32 && rest * s * record_bytes <= kMaxRecordBytes); ++s) {
+        const int64_t rounds = full_parts * kv_heads / kComputeUnits;
+        const int64_t rest_rounds = (rest * s + kComputeUnits - 1) / kComputeUnits;
+        const int64_t time = rounds * steps * step + rest_rounds * ((steps + s - 1) / s * step + (s > 1 ? besides : 0));
+        if (time >= best) continue;
+        best = time;
+        r.shape.rows = most_rows;
+        r.part_tokens = (int)part_tokens;
+        r.row_parts = (int)row_parts;
+        r.full_parts = (int)full_parts;
+        r.splits = (int)s;
+        r.tiles = parts * kv_heads * tiles;
+        r.workgroups = (int)(full_parts * kv_heads + rest * s);
+        r.workspace_bytes = s > 1 ? kCounterBytes + rest * s * record_bytes : 0;
+      }
     }
-    r.workgroups = (int)(r.full_parts * kv_heads + rest * r.splits);
-    r.workspace_bytes = r.splits > 1 ? kCounterBytes + rest * r.splits * record_bytes : 0;
     return r;
   }
   // A wave's rows and the row tiles of a workgroup's waves; what these leave of the
@@ -380,7 +391,7 @@ int tm_cached_attention(const void* query, int64_t query_stride, const void* key
   p.workgroups = plan.workgroups;
   p.scale_log2 = scale * 1.4426950408889634f;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  return launched(plan.row_parts > 0 ? launch_cached_chunks(p, dtype == TM_FP16, type, s)
+  return launched(plan.row_parts > 0 ? launch_cached_chunks(p, plan.shape.rows, dtype == TM_FP16, type, s)
                                      : launch_cached_attention(p, plan.shape, dtype == TM_FP16, type, s));
 }
 

@@ -33,6 +33,7 @@ constexpr int kWaves = 8, kThreads = 64 * kWaves;
 constexpr int kStepKeys = 64;
 constexpr int kSlotBytes = kStepKeys * kRowBytes;  // 16 KB: K or V of one step
 static_assert(kWaves * 32 == kChunkRows && kPageSize % kStepKeys == 0, "a step stays inside a page");
+static_assert(kStepKeys == 2 * kKvTile, "a tile for each of two key parts");
 
 // What a thread carries of a step: 16 numbers of K and of V.
 template <class Type, CacheType kCache>
@@ -80,17 +81,20 @@ struct Staged<Type, CacheType::kE4m3> {
   __device__ __forceinline__ u32x4_t value_chunk(int half) const { return widened<Fp16>(v, half); }
 };
 
-template <class Type, CacheType kCache>
+template <class Type, CacheType kCache, int kKeyParts>
 __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedParams p) {
+  constexpr int kRowTiles = kWaves / kKeyParts, kRows = 32 * kRowTiles, kTiles = 2 / kKeyParts;  // a wave's tiles of a step
   typedef Staged<Type, kCache> Stage;
   typedef typename Stage::Weight Weight;
   typedef typename Type::elem elem;
   constexpr int kHeadBytes = kHeadDim * Stage::kElemBytes;
   constexpr float kWeightBits = std::is_same_v<Weight, Fp16> ? 7.0f : 0.0f;
 
-  __shared__ __attribute__((aligned(1024))) char k_lds[2][kSlotBytes];
-  __shared__ __attribute__((aligned(1024))) char v_lds[2][kSlotBytes];
-  __shared__ unsigned s_odd[kChunkRows][3][4];  // note_odd: a bit a dim, for +infinity, -infinity, NaN
+  __shared__ __attribute__((aligned(1024))) char kv_lds[4 * kSlotBytes];
+  char* const k_lds = kv_lds;
+  char* const v_lds = kv_lds + 2 * kSlotBytes;
+  __shared__ unsigned s_odd[kRows][3][4];  // note_odd: a bit a dim, for +infinity, -infinity, NaN
+  __shared__ float s_max[kWaves][32], s_sum[kWaves][32];
   __shared__ int s_last;
 
   const int tid = threadIdx.x;
@@ -125,14 +129,15 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
   if (share >= shares) return;
   const int lo = share * each, steps = min(each, tiles.count - lo);
   const int unshared = p.full_parts * p.kv_heads;  // workgroups without records
-  const Shares group(p, p.workgroups - unshared, min(kChunkRows, p.part_tokens * G),
+  const Shares group(p, p.workgroups - unshared, min(kRows, p.part_tokens * G),
                      (int)blockIdx.x - unshared - share * p.kv_heads, p.kv_heads, share, shares);
   const int tokens = min(len, p.table_cols * kPageSize);  // with a key
   const int row0 = request * p.rows + part * p.part_tokens;  // of query and out
-  for (int i = tid; i < kChunkRows * 12; i += kThreads) (&s_odd[0][0][0])[i] = 0;
+  for (int i = tid; i < kRows * 12; i += kThreads) (&s_odd[0][0][0])[i] = 0;
 
-  // ---- this wave's rows ----
-  const int row_base = 32 * wave, row = row_base + n;
+  // ---- this wave's rows, and its part of a step's keys ----
+  const int key_part = wave / kRowTiles;
+  const int row_base = 32 * (wave % kRowTiles), row = row_base + n;
   const int valid_rows = min(32, part_rows - row_base);  // none: the wave only loads
   const int token = by_group.token(row);
   const bool ok = n < valid_rows;
@@ -210,8 +215,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
     }
   };
   auto write = [&](int i) TM_INLINED {  // the staged step into its slot
-    char* const ks = k_lds[i & 1];
-    char* const vs = v_lds[i & 1];
+    char* const ks = k_lds + (i & 1) * kSlotBytes;
+    char* const vs = v_lds + (i & 1) * kSlotBytes;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = Stage::row(h), chunk = Stage::chunk(h);
@@ -242,30 +247,30 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
   auto compute = [&](int i, int phys) TM_INLINED {
     const int key0 = first_key(i);
     if (phys < 0 || key0 > last_pos || (key0 + kStepKeys - 1 < first_low && key0 >= p.sinks)) return;
-    const char* const ks = k_lds[i & 1];
-    const char* const vs = v_lds[i & 1];
-    f32x16_t s[2] = {};
+    const char* const ks = k_lds + (i & 1) * kSlotBytes;
+    const char* const vs = v_lds + (i & 1) * kSlotBytes;
+    f32x16_t s[kTiles] = {};
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const i16x8_t a = *reinterpret_cast<const i16x8_t*>(ks + t * kTileBytes + (k_off ^ (32 * c)));
+      for (int t = 0; t < kTiles; ++t) {
+        const i16x8_t a = *reinterpret_cast<const i16x8_t*>(ks + (t + key_part) * kTileBytes + (k_off ^ (32 * c)));
         s[t] = Type::mfma32(a, q[c], s[t]);
       }
     }
     if (key0 + kStepKeys - 1 > first_pos || (key0 < last_low && key0 + kStepKeys - 1 >= p.sinks)) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < kTiles; ++t) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          const int key = key0 + 32 * t + elem_key(v) + 4 * half;
+          const int key = key0 + 32 * (t + key_part) + elem_key(v) + 4 * half;
           s[t][v] = key <= row_pos && (key >= low || key < p.sinks) ? s[t][v] : -INFINITY;
         }
       }
     }
     float top = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < 16; ++v) top = fmaxf(top, fmaxf(s[0][v], s[1][v]));
+    for (int v = 0; v < 16; ++v) top = fmaxf(top, fmaxf(s[0][v], s[kTiles - 1][v]));
     top = half_max(top) * c2;
     if (__any(top > m_run + kLazyRescale)) {
       const float m_new = fmaxf(m_run, top);
@@ -276,10 +281,10 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
       m_run = m_new;
     }
     const float shift = kWeightBits - (m_run == -INFINITY ? 0.0f : m_run);
-    i16x8_t pb[4];
+    i16x8_t pb[2 * kTiles];
     float add = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2 * kTiles; ++j) {
       typename Weight::vec weight;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -291,10 +296,10 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
     }
     l_run += add;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2 * kTiles; ++j) {
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
-        const char* const at = vs + 16 * j * kRowBytes + (v_off ^ (64 * m));
+        const char* const at = vs + (16 * j + 32 * key_part) * kRowBytes + (v_off ^ (64 * m));
         const i16x4_t lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)(at));
         const i16x4_t hi4 =
             __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)(at + 8 * kRowBytes));
@@ -319,8 +324,43 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
   }
 
   // ---- results: this lane's row, dims 32 m + 8 v + 4 half .. + 3 ----
-  const float l = half_sum(l_run);
+  float l = half_sum(l_run);
   m_run = row_shift(m_run, l);
+  if constexpr (kKeyParts == 2) {
+    // the second key part's sums, register by register, to the waves that have the first
+    float* const parts = reinterpret_cast<float*>(kv_lds) + (row_base / 32) * (64 * 64) + lane;
+    static_assert(kRowTiles * 64 * 64 * 4 <= 4 * kSlotBytes, "they fit the slots");
+    if (half == 0) {
+      s_max[wave][n] = m_run;
+      s_sum[wave][n] = l;
+    }
+    __syncthreads();
+    const int other = wave ^ kRowTiles;
+    const float top = fmaxf(m_run, s_max[other][n]);
+    const float keep = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - top);
+    if (key_part == 1) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) parts[64 * (16 * m + v)] = m_run == -INFINITY ? 0.0f : o[m][v] * keep;
+      }
+    }
+    __syncthreads();
+    if (key_part == 0) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          o[m][v] = (m_run == -INFINITY ? 0.0f : o[m][v] * keep) + parts[64 * (16 * m + v)];
+        }
+      }
+      const float theirs = s_max[other][n];
+      l = (m_run == -INFINITY ? 0.0f : l * keep) +
+          (theirs == -INFINITY ? 0.0f : s_sum[other][n] * __builtin_amdgcn_exp2f(theirs - top));
+      m_run = top;
+    }
+  }
+  const bool writes = ok && key_part == 0;
 #pragma unroll
   for (int m = 0; m < 4; ++m) {
 #pragma unroll
@@ -341,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
     return p.out + ((int64_t)(row0 + t) * p.heads + kv_head * G + (r - t * G)) * kHeadDim;
   };
   if (shares == 1) {
-    if (!ok || row_pos < 0) return;  // before the request's first token: no row
+    if (!writes || row_pos < 0) return;  // before the request's first token: no row
     const float scale = scale_of(l);
     uint16_t* const to = out_row(row);
     typedef elem vec4 __attribute__((ext_vector_type(4)));
@@ -357,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
     }
     return;
   }
-  if (ok) {
+  if (writes) {
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
 #pragma unroll
@@ -368,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
     }
     if (half == 0) group.store_sums(share, row, m_run, l);
   }
-  float(*const join)[10] = reinterpret_cast<float(*)[10]>(k_lds);
+  float(*const join)[10] = reinterpret_cast<float(*)[10]>(kv_lds);
   static_assert(kThreads * 10 * 4 <= 2 * kSlotBytes, "the joined values fit the slots");
   merge_shares<kThreads, 4, 2>(
       p, group, join, &s_last, [&](int r) TM_INLINED { return r < part_rows; },
@@ -382,21 +422,24 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
       });
 }
 
-template <class Type>
-hipError_t launch_type(const CachedParams& p, CacheType cache, hipStream_t stream) {
+template <class Type, CacheType kCache>
+hipError_t launch_rows(const CachedParams& p, int rows, hipStream_t stream) {
   const dim3 grid((unsigned)p.workgroups), block(kThreads);
-  if (cache == CacheType::kE4m3) {
-    hipLaunchKernelGGL((cached_chunk_kernel<Type, CacheType::kE4m3>), grid, block, 0, stream, p);
+  if (rows == kChunkRows) {
+    hipLaunchKernelGGL((cached_chunk_kernel<Type, kCache, 1>), grid, block, 0, stream, p);
   } else {
-    hipLaunchKernelGGL((cached_chunk_kernel<Type, CacheType::kSame>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((cached_chunk_kernel<Type, kCache, 2>), grid, block, 0, stream, p);
   }
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_cached_chunks(const CachedParams& p, bool fp16, CacheType cache, hipStream_t stream) {
-  return fp16 ? launch_type<Fp16>(p, cache, stream) : launch_type<Bf16>(p, cache, stream);
+hipError_t launch_cached_chunks(const CachedParams& p, int rows, bool fp16, CacheType cache, hipStream_t stream) {
+  if (cache == CacheType::kE4m3) {
+    return fp16 ? launch_rows<Fp16, CacheType::kE4m3>(p, rows, stream) : launch_rows<Bf16, CacheType::kE4m3>(p, rows, stream);
+  }
+  return fp16 ? launch_rows<Fp16, CacheType::kSame>(p, rows, stream) : launch_rows<Bf16, CacheType::kSame>(p, rows, stream);
 }
 
 }  // namespace tmx
