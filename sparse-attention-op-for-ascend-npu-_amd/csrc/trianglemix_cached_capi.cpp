@@ -109,10 +109,10 @@ CachedPlan cached_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_he
     // time of a step of 64 keys and what a share costs besides (the start, its partial,
     // the merge), in 0.1 us.  256 | 128 rows: 128 rows of 8192 tokens 65 | 52 us, 300 of
     // 3000 58 | 41, 512 of 8192 104 | 120, 2048 of 32749 1079 | 1447.
-    const int64_t steps = (tiles + 1) / 2;
     int64_t best = INT64_MAX;
     for (const auto [most_rows, step, besides] : {std::array{kChunkRows, 20, 220}, std::array{kChunkRows / 2, 14, 120}}) {
       const int64_t part_tokens = most_rows / group, row_parts = (rows + part_tokens - 1) / part_tokens;
+      const int64_t tiles = most_tiles(part_tokens, table_cols, window, sinks), steps = (tiles + 1) / 2;
       const int64_t parts = batch * row_parts;
       const int64_t full_parts = parts * kv_heads / kComputeUnits * kComputeUnits / kv_heads;
       const int64_t rest = (parts - full_parts) * kv_heads;
