@@ -61,17 +61,29 @@ __device__ __forceinline__ float row_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Sum over the wave, and over its lanes up to this one.
+// Sum over the wave, and over its lanes up to this one: lanes 1, 2, 4 and 8 back in
+// their row of 16, then a row's last lane to the rows behind it (a move each in
+// place of a round trip through LDS: with divide_up 0.5 us a call less).
+template <int kControl, int kRowMask>
+__device__ __forceinline__ int moved(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, kControl, kRowMask, 0xf, false);
+}
 __device__ __forceinline__ int wave_prefix(int x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int add = __shfl_up(x, d);
-    if (lane >= d) x += add;
-  }
+  x += moved<0x111, 0xf>(x);  // row_shr:1
+  x += moved<0x112, 0xf>(x);
+  x += moved<0x114, 0xf>(x);
+  x += moved<0x118, 0xf>(x);
+  x += moved<0x142, 0xa>(x);  // row_bcast:15
+  x += moved<0x143, 0xc>(x);  // row_bcast:31
   return x;
 }
 __device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_prefix(x), 63); }
+
+// a / b rounded up, for a + b below 2^21: the quotient of a + b - 1/2 in 32 bits is off by less
+// than it is from the next whole number.
+__device__ __forceinline__ int divide_up(int a, int b) {
+  return (int)(((float)(a + b) - 0.5f) * __builtin_amdgcn_rcpf((float)b));
+}
 
 // A wave's share of a page, 32 keys: what its lanes load, and the operands made of it.
 template <class Type, CacheType kCache>
@@ -240,13 +252,15 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
   total = wave_sum(total);
   // Sure: sum(ceil(tiles / least)) is at most total / least and a share more a group.
   // One block of requests: the smallest such number by halves from total / workgroups on.
+  // (From the most tiles of a request on, every group is one share.)
   int least = max(p.min_tiles, (int)(((unsigned)(total * head_groups) + (unsigned)p.full_shares - 1u) / (unsigned)p.full_shares));
+  least = min(least, kMaxTableCols * (kPageSize / kKvTile));
   if (p.batch <= 64 && least > p.min_tiles) {
     int low = max(p.min_tiles, (int)((unsigned)(total * head_groups) / (unsigned)p.workgroups));
 #pragma unroll 1
     for (int i = 0; i < p.halvings && low < least; ++i) {
       const int mid = (int)(((unsigned)low + (unsigned)least) >> 1);
-      const int all = wave_sum((int)((unsigned)(tiles64 + mid - 1) / (unsigned)mid)) * head_groups;
+      const int all = wave_sum(divide_up(tiles64, mid)) * head_groups;
       if (all <= p.workgroups) least = mid;
       else low = mid + 1;
     }
@@ -255,8 +269,8 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
   int base = 0, before = 0, shares64, upto64;
   for (;;) {
     // no more shares than are merged at once, where that leaves them short
-    const int each64 = max(least, min((tiles64 + cluster - 1) / cluster, 8 << p.key_shift));
-    shares64 = (int)((unsigned)(tiles64 + each64 - 1) / (unsigned)each64);
+    const int each64 = max(least, min(divide_up(tiles64, cluster), 8 << p.key_shift));
+    shares64 = divide_up(tiles64, each64);
     upto64 = before + wave_prefix(shares64 * head_groups);
     if (__builtin_amdgcn_readlane(upto64, 63) > run) break;
     before = __builtin_amdgcn_readlane(upto64, 63);
@@ -271,12 +285,12 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
   int shares = __builtin_amdgcn_readlane(shares64, in_block);
   const int at = run - (__builtin_amdgcn_readlane(upto64, in_block) - shares * head_groups);
   // the shares of neighbouring heads side by side: they read neighbouring numbers
-  const int share = at / head_groups, head_group = at - share * head_groups;
+  const int share = __builtin_amdgcn_readfirstlane(divide_up(at + 1, head_groups)) - 1, head_group = at - share * head_groups;
   const int part_rows = p.rows * G;
   const int pos0 = len - p.rows;  // of the first token; a negative one is no row
   const Tiles<kKvTile> tiles(p, pos0, len - 1);
-  const int each = (tiles.count + shares - 1) / shares;  // as even as they come
-  shares = (tiles.count + each - 1) / each;
+  const int each = __builtin_amdgcn_readfirstlane(divide_up(tiles.count, shares));  // as even as they come
+  shares = __builtin_amdgcn_readfirstlane(divide_up(tiles.count, each));
   if (share >= shares) return;
   const int lo = share * each, hi = min(lo + each, tiles.count);
   const Shares group(p, p.workgroups, record_rows, run - at + head_group, head_groups, share, shares);

@@ -57,6 +57,13 @@ struct Staged<Type, CacheType::kSame> {
   }
   __device__ __forceinline__ u32x4_t key_chunk(int half) const { return k[half]; }
   __device__ __forceinline__ u32x4_t value_chunk(int half) const { return v[half]; }
+  // Whether some V number is not finite: a carry out of its exponent's place.
+  __device__ __forceinline__ bool odd_value() const {
+    unsigned odd = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) odd |= (v[e >> 2][e & 3] & 0x7fff7fffu) + (0x8000u - Type::kExp) * 0x10001u;
+    return (odd & 0x80008000u) != 0;
+  }
 };
 
 template <class Type>
@@ -79,6 +86,12 @@ struct Staged<Type, CacheType::kE4m3> {
   }
   __device__ __forceinline__ u32x4_t key_chunk(int half) const { return widened<Type>(k, half); }
   __device__ __forceinline__ u32x4_t value_chunk(int half) const { return widened<Fp16>(v, half); }
+  __device__ __forceinline__ bool odd_value() const {
+    unsigned odd = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) odd |= (v[e] & 0x7f7f7f7fu) + 0x01010101u;
+    return (odd & 0x80808080u) != 0;
+  }
 };
 
 template <class Type, CacheType kCache, int kKeyParts>
@@ -217,17 +230,13 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
   auto write = [&](int i) TM_INLINED {  // the staged step into its slot
     char* const ks = k_lds + (i & 1) * kSlotBytes;
     char* const vs = v_lds + (i & 1) * kSlotBytes;
+    const bool odd = __builtin_expect(__any(stage.odd_value()), 0);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = Stage::row(h), chunk = Stage::chunk(h);
       *reinterpret_cast<u32x4_t*>(ks + r * kRowBytes + 16 * k_slot(r, chunk)) = stage.key_chunk(h);
       u32x4_t x = stage.value_chunk(h);
-      unsigned odd = 0;  // a one in the exponent's place carries out where all its bits are set
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        odd |= ((x[e] & 0x7fff7fffu) + (0x8000u - Weight::kExp) * 0x10001u) & 0x80008000u;
-      }
-      if (__builtin_expect(__any(odd != 0), 0)) {
+      if (odd) {
         note_odd(first_key(i), r, chunk, x);
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = only_kind<Weight>(x[e], 0) | only_kind<Weight>(x[e] >> 16, 0) << 16;
@@ -244,12 +253,15 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
   const int v_key = 4 * half + ((lane & 15) >> 2), v_dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   const int v_off = v_key * kRowBytes + 16 * v_slot(v_key, v_dim >> 3) + 2 * (v_dim & 7);
 
-  auto compute = [&](int i, int phys) TM_INLINED {
+  auto active = [&](int i, int phys) TM_INLINED {  // whether some row of the wave attends some key of the step
     const int key0 = first_key(i);
-    if (phys < 0 || key0 > last_pos || (key0 + kStepKeys - 1 < first_low && key0 >= p.sinks)) return;
+    return phys >= 0 && key0 <= last_pos && (key0 + kStepKeys - 1 >= first_low || key0 < p.sinks);
+  };
+  f32x16_t s[kTiles];
+  auto scores = [&](int i) TM_INLINED {
     const char* const ks = k_lds + (i & 1) * kSlotBytes;
-    const char* const vs = v_lds + (i & 1) * kSlotBytes;
-    f32x16_t s[kTiles] = {};
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) s[t] = f32x16_t{};
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
 #pragma unroll
@@ -258,6 +270,10 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
         s[t] = Type::mfma32(a, q[c], s[t]);
       }
     }
+  };
+  auto values = [&](int i) TM_INLINED {
+    const int key0 = first_key(i);
+    const char* const vs = v_lds + (i & 1) * kSlotBytes;
     if (key0 + kStepKeys - 1 > first_pos || (key0 < last_low && key0 + kStepKeys - 1 >= p.sinks)) {
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
@@ -308,19 +324,26 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
     }
   };
 
-  int phys = entry(0), next = entry(1);
+  // Step i + 1 is staged when step i begins and is written while the matrix cores work
+  // at its scores; step i + 2 is loaded from then on.
+  int phys = entry(0), next = entry(1), behind = entry(2);
   load(0, phys);
   __syncthreads();  // s_odd is clear
   write(0);
+  load(1, next);
   __syncthreads();
   for (int i = 0; i < steps; ++i) {
-    if (i + 1 < steps) load(i + 1, next);
-    const int behind = entry(i + 2);
-    compute(i, phys);
+    const bool on = active(i, phys);
+    if (on) scores(i);
+    __builtin_amdgcn_sched_barrier(0);
     if (i + 1 < steps) write(i + 1);
-    __syncthreads();
+    load(i + 2, behind);
     phys = next;
     next = behind;
+    behind = entry(i + 3);
+    __builtin_amdgcn_sched_barrier(0);
+    if (on) values(i);
+    __syncthreads();
   }
 
   // ---- results: this lane's row, dims 32 m + 8 v + 4 half .. + 3 ----
