@@ -13,8 +13,9 @@
  * (cache_dtype TM_BF16 or TM_FP16, equal to dtype) or of e4m3 numbers (TM_E4M3:
  * 4 exponent bits of bias 7, 3 mantissa bits, largest 448, no infinities).  A
  * number of an e4m3 cache stands for itself times its KV head's scale,
- * key_scale / value_scale [kv_heads] fp32 (null for 16-bit caches).  Page
- * strides are in numbers, of 16 bytes in multiples.
+ * key_scale / value_scale [kv_heads] fp32 (null for 16-bit caches): positive,
+ * from 2^-126 to 2^126; others are not looked for and give numbers that mean
+ * nothing.  Page strides are in numbers, of 16 bytes in multiples.
  */
 #ifndef TRIANGLEMIX_CACHED_H
 #define TRIANGLEMIX_CACHED_H
@@ -76,13 +77,20 @@ int tm_rotate_and_cache(const void* query, int64_t query_stride, const void* key
  * The step's own keys are in the cache.  Single tokens (rows 1), a few drafted
  * ones, or a whole chunk.
  *
+ * A call may read 2^30 tiles of 32 keys, counted over the requests at the
+ * table's full width (the window's, where there is one) and the KV heads.  Keys
+ * of pages that the cache does not have, and keys past the table, are attended
+ * by no row.  Rows before a request's first token are none: their out is left as
+ * it was.
+ *
  * Numerics: scores, softmax statistics and sums in fp32.  The weights are rounded
  * to the cache's type for their product with V (fp16 over an e4m3 cache, whose
  * numbers are exact in it); the sum that they are divided by takes them
  * unrounded; the result is rounded once.  A row without keys gives zeros.  A key
- * whose score is -infinity counts as one that the row does not attend.  NaN, and
- * infinities in V, reach the rows that attend their key and no other; an
- * infinity whose weight rounds to zero may arrive as NaN.
+ * whose score is -infinity has the weight zero.  NaN in keys, and NaN and
+ * infinities in V, reach the rows that attend their key and no other, whatever
+ * the key's weight; an infinity may arrive as NaN where that weight rounds to
+ * zero or other infinities meet it.
  */
 int tm_cached_attention(const void* query, int64_t query_stride, const void* key_cache, int64_t key_page_stride,
                         const void* value_cache, int64_t value_page_stride, const float* key_scale,
@@ -94,7 +102,7 @@ int tm_cached_attention(const void* query, int64_t query_stride, const void* key
 
 /* Workspace bytes of that call, or -1 for what it refuses.  The workspace is
  * as that of tm_triangle_paged_sparse_attention: any contents, 16-byte
- * aligned, one per call in flight. */
+ * aligned, one per call in flight.  At most 64 MiB + 64 KiB. */
 int64_t tm_cached_attention_workspace_size(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads,
                                            int64_t table_cols, int64_t window, int64_t sinks);
 

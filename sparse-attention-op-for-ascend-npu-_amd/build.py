@@ -66,8 +66,8 @@ NO_NANS_DEFAULT = ["-Xarch_device", "-fno-honor-nans"]
 NO_NANS = {"trianglemix_select.hip": [], "trianglemix_rotary.hip": []}
 
 HIP_SOURCES = ["trianglemix_kernel.hip", "trianglemix_wide.hip", "trianglemix_cache.hip", "trianglemix_rows.hip",
-               "trianglemix_blocks.hip", "trianglemix_select.hip", "trianglemix_rotary.hip", "trianglemix_cached.hip", "trianglemix_chunks.hip",
-               "trianglemix_capi.cpp", "trianglemix_pages_capi.cpp", "trianglemix_cached_capi.cpp"]
+               "trianglemix_blocks.hip", "trianglemix_select.hip", "trianglemix_rotary.hip", "trianglemix_cached.hip",
+               "trianglemix_chunks.hip", "trianglemix_capi.cpp", "trianglemix_pages_capi.cpp", "trianglemix_cached_capi.cpp"]
 
 TORCH_SOURCES = ["trianglemix_torch.cpp", "trianglemix_pages_torch.cpp", "trianglemix_cached_torch.cpp"]
 

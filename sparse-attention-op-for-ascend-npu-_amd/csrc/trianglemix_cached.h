@@ -70,7 +70,7 @@ struct CachedShape {
 };
 // Chunks, of more rows of a KV head than kMostFewRows: workgroups of kChunkRows rows or
 // of half as many.
-constexpr int kChunkRows = 256, kMostFewRows = 128;
+constexpr int kChunkRows = 256, kMostFewRows = 64;
 hipError_t launch_cached_chunks(const CachedParams& p, int rows, bool fp16, CacheType cache, hipStream_t stream);
 hipError_t launch_cached_attention(const CachedParams& p, CachedShape shape, bool fp16, CacheType cache,
                                    hipStream_t stream);

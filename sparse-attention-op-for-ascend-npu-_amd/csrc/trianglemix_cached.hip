@@ -1,21 +1,33 @@
 // Attention of the last tokens of each request over its paged cache, of e4m3
 // numbers or of the queries' own 16-bit type, for MI355X (gfx950).
 //
-// Work.  A group is the query rows of a (request, KV head) that one workgroup
-// holds: all heads of the GQA group times the request's tokens, rows numbered
-// token * G + head, cut into row parts of 16 NT.  A unit is one page (128 keys)
-// of one group: the pages of the first `sinks` keys and those from the window's
-// first key of the request's first row on, or all.  The units of all groups, in a
-// row, are dealt to the workgroups in equal contiguous runs, as in
-// trianglemix_lists.h, with the same partials and merge for groups that a run's
-// end cuts: every workgroup streams the same number of pages whatever the lengths,
-// the grid does not depend on them, and the sums do not depend on which workgroup
-// merges them.
+// Work.  The rows are those of a request's last tokens, few enough for the waves of
+// a workgroup (trianglemix_chunks.hip has the others): all heads of a GQA group times
+// the tokens, numbered token * G + head.  A workgroup is four or eight waves, each
+// with a tile of 16 NT rows: of neighbouring KV heads (their numbers lie side by side
+// in memory, 128 bytes of e4m3 each: read by one workgroup they stream at 5.9 TB/s,
+// by one each at 4.6 to 5.7), of several row tiles, or with parts of the keys.  A group
+// is what a workgroup so covers.  Its 32-key tiles are the first `sinks` keys' and
+// those from the window's first key on, or all; others are not read.
 //
-// A workgroup is four waves over the same rows; wave w has keys 32 w .. 32 w + 31
-// of every page.  K and V go from memory into registers, kDepth - 1 tiles ahead:
-// a wave loads what it multiplies itself, so the page loop has neither LDS nor
-// barriers.  The waves' sums meet in LDS behind it.
+// Shares.  Every group's tiles are cut into equal shares, as many as the GPU holds
+// workgroups over all groups: lengths are read on the device, the grid does not
+// depend on them, a workgroup has one share.  (Equal runs over all groups in a row
+// keep the workgroups more even, but each then ends two or three groups, and pays
+// for the join of the waves, the partial and the next start each time: 64
+// requests of 2000 to 16384 tokens 222 us, with runs 225 to 240; a window of 512
+// keys 27 and 40.)  Partials are merged as in trianglemix_cached_device.h.
+//
+// K and V go from memory into registers, a tile ahead of the one in use: a wave loads
+// what it multiplies itself, so the loop has neither LDS nor barriers.  More tiles
+// ahead (two, three) and two workgroups a CU were no faster: 64 to 128 KB in flight a
+// CU are enough.  The waves' sums meet in LDS behind the loop.
+//
+// What bounds it: memory.  64 requests of 2000 to 16384 tokens (1.22 GB) 222 us, four
+// of 65536 to 131072 (0.83 GB) 149, at 5.5 TB/s over all and 5.9 within the loop; the
+// rest is the start (lengths, table and first tiles, each waiting for the one before: 3
+// us), the join and the merge (5 to 10).  One token of 8111 on two KV heads: 10.7
+// us, launch and round trips alone.
 //
 // Contractions (per wave, 32 keys x 16 NT rows, v_mfma_f32_16x16x32)
 //   S^T (keys x rows) = K Q^T     A = K, B = Q

@@ -107,8 +107,9 @@ CachedPlan cached_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_he
     // Chunks: workgroups of 256 rows, or of 128 with two key parts, one a CU.  What does
     // not fill the GPU's last round is shared out.  Taken is what ends soonest by the
     // time of a step of 64 keys and what a share costs besides (the start, its partial,
-    // the merge), in 0.1 us.  256 | 128 rows: 128 rows of 8192 tokens 65 | 52 us, 300 of
-    // 3000 58 | 41, 512 of 8192 104 | 120, 2048 of 32749 1079 | 1447.
+    // the merge), in 0.1 us.  256 | 128 rows, four heads to each of eight KV heads: 33
+    // tokens of 8192 49 | 38 us, 75 of 3000 48 | 34, 512 of 8192 94 | 99, 1000 of 20000
+    // 344 | 391, 2048 of 32749 1025 | 1213.
     int64_t best = INT64_MAX;
     for (const auto [most_rows, step, besides] : {std::array{kChunkRows, 20, 220}, std::array{kChunkRows / 2, 14, 120}}) {
       const int64_t part_tokens = most_rows / group, row_parts = (rows + part_tokens - 1) / part_tokens;
@@ -137,17 +138,19 @@ CachedPlan cached_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_he
   }
   // A wave's rows and the row tiles of a workgroup's waves; what these leave of the
   // waves goes to neighbouring KV heads, whose numbers lie side by side in memory (64
-  // requests of 2000 to 16384 tokens: 222 us with eight heads a workgroup, 234 with
-  // four, 283 with two), or to parts of the keys: where there is little to read or
+  // requests of 2000 to 16384 tokens: 221 us with eight heads a workgroup, 233 with
+  // four, 275 with two), or to parts of the keys: where there is little to read or
   // many rows, whose partials would cost more (32 requests of 5 tokens, 500 to 9000
-  // before them: 97 us with eight heads, 76 with four, 85 with two).
+  // before them: 99 us with eight heads, 77 with four, 80 with two).
+  // More than 64 rows are chunks (32 requests of 32 tokens, 500 to 9000 before them: as
+  // four row tiles a workgroup 237 us, as chunks 176; of 16 tokens 117 and 173).
   int most_shift;
   if (group_rows <= 16) {
     r.shape = {16, group_rows <= 4 && enough(3) && batch * kv_heads >= kComputeUnits ? 8 : 4};
     most_shift = r.shape.waves == 8 ? 3 : 2;
   } else {
     r.shape = {32, 8};
-    r.row_shift = group_rows <= 32 ? 0 : group_rows <= 64 ? 1 : 2;
+    r.row_shift = group_rows <= 32 ? 0 : 1;
     most_shift = 2 - r.row_shift;
   }
   int head_shift = 0;
@@ -161,8 +164,8 @@ CachedPlan cached_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_he
   r.full_shares = (int)std::max(kComputeUnits - groups, int64_t(kComputeUnits / 2));
   if ((groups + r.full_shares) * record_bytes <= kMaxRecordBytes && groups + r.full_shares <= kCounterBytes / 8) {
     r.min_tiles = 1 << r.key_shift;
-    // Half a microsecond, where the groups are so many that their last shares matter
-    // (without: 274 us in place of the 234 above with four heads).
+    // Half a microsecond, where the groups are so many that their last shares matter (32
+    // requests of 5 tokens: 79 us without, 77 with).
     r.halvings = tiles > 64 && groups >= kComputeUnits / 4 ? 5 : 0;
     shares = std::min(groups + r.full_shares, r.tiles);
   } else {

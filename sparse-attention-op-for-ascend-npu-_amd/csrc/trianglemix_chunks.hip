@@ -6,14 +6,23 @@
 // head), all heads of the GQA group times consecutive tokens, rows numbered token *
 // G + head.  A step is 64 keys.  Each goes from memory into registers a step ahead,
 // becomes 16-bit numbers there (e4m3: K of the queries' type, V fp16 with fp16
-// weights, both exact) and is written to LDS for all waves: once for 256 rows, where
-// waves that load their operands themselves convert them for each 32 or 64.  Two
-// slots of 32 KB; one barrier a step.
+// weights, both exact) and is written to LDS for all waves while the matrix cores work
+// at the step before's scores: once for 256 rows, where waves that load their operands
+// themselves convert them for each 32 or 64 (2048 rows of 32749 tokens: 1450 us so).
+// Two slots of 32 KB; one barrier a step.  Where 256 rows a workgroup leave CUs idle, a
+// workgroup has 128 rows and its waves one tile of a step each (two key parts, joined in
+// LDS at the end).
 //
 // Contractions (per wave, 32-key tiles x 32 rows, v_mfma_f32_32x32x16)
 //   S^T (keys x rows) = K Q^T     A = K rows from LDS, B = Q in registers
 //   O^T (dims x rows) += V^T P^T  A = V by ds_read_b64_tr_b16, B = P
 // with the operand layouts of trianglemix_device.h.
+//
+// What bounds it: 2048 rows of 32749 tokens 1025 us, 1039 TFLOP/s, where a library
+// product of 8192^3 reaches 1205; MFMAs are busy 44 % of the cycles, vector
+// instructions (exponentials, conversions) 46 %, LDS about as much.  512 rows of 8192
+// tokens: 94 us, 70 of them in the loop, the rest partials of four shares a part (34 MB)
+// and their merge.
 //
 // Parts whose keys are shared by several workgroups (few rows, many keys) are merged
 // as in trianglemix_cached_device.h.  Numerics as in trianglemix_cached.hip.  V entries

@@ -13,9 +13,9 @@
 // three and small head counts leave few lanes idle.
 //
 // Results go past the caches (non-temporal stores: 4096 tokens into an 8-bit cache
-// 18.0 us, 19.3 with plain ones).
+// 17.3 us, 18.5 with plain ones).
 //
-// What bounds it: memory for large chunks (8191 tokens of 40 heads 33.5 us, 5.0 TB/s as
+// What bounds it: memory for large chunks (8191 tokens of 40 heads 34.2 us, 4.9 TB/s as
 // a library copy), the launch and two dependent round
 // trips (position, then the rows' sines; the rows themselves are loaded beside
 // them) for a decoding step.
@@ -43,7 +43,7 @@ struct RotateFp16 { typedef f16x8_t vec; typedef _Float16 elem; };
 // Eight numbers as e4m3 of their quotients by `scale`: ties to even, +-448 for
 // what is larger, NaN for NaN.  The quotient is the product with the reciprocal and
 // one step of its error, the division's rounding at a third of its instructions
-// (4096 tokens: 18.0 us, with divisions 19.3); far beyond the range, where that step
+// (4096 tokens: 17.3 us, with divisions 18.0); far beyond the range, where that step
 // may overflow, the product alone says which end.
 __device__ __forceinline__ u32x2_t to_e4m3(const float* x, float scale) {
   const float reciprocal = 1.0f / scale;

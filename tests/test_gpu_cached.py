@@ -58,6 +58,19 @@ CASES = [
     ([900], 300, 8, 2, 64, 1),
     ([400], 1, 4, 1, 1 << 40, 1 << 40),
     ([700], 40, 4, 1, 200, 1000),         # sinks past the window's first key
+    ([7200] + [(53 * i) % 400 for i in range(39)], 1, 32, 8, -1, 0),  # eight KV heads a workgroup
+    ([(211 * i) % 3001 for i in range(70)], 1, 8, 4, -1, 0),          # more requests than a wave has lanes
+    ([20000, 700], 12, 16, 4, -1, 0),     # more shares than are merged at once
+    # chunks: more rows of a KV head than the waves of a workgroup hold
+    ([900, 64, 0, 1300], 64, 32, 8, -1, 0),
+    ([3000], 200, 8, 2, -1, 0),           # shared out over the keys
+    ([2500, 100], 150, 12, 4, 300, 5),
+    ([700, 50], 40, 32, 1, -1, 0),        # four tokens a workgroup
+    ([260, 1], 33, 4, 1, -1, 0),          # a part and four rows
+    ([900, 30], 13, 5, 1, -1, 0),         # 65 rows: one more than fits
+    ([600, 900], 11, 18, 3, -1, 0),       # 66 rows
+    ([640, 300], 7, 18, 2, 100, 3),       # 63 rows, nine heads a KV head
+    ([5000], 129, 8, 8, 700, 0),
 ]
 
 
@@ -114,7 +127,8 @@ def test_strides_bad_pages_and_lengths_past_the_table(gpu, cache):
 
 
 @pytest.mark.parametrize("cache", ["e4m3", "same"])
-@pytest.mark.parametrize("rows,heads,window,sinks", [(1, 8, -1, 0), (1, 8, 100, 4), (9, 8, -1, 0), (9, 8, 100, 4), (40, 12, 30, 4)])
+@pytest.mark.parametrize("rows,heads,window,sinks", [(1, 8, -1, 0), (1, 8, 100, 4), (9, 8, -1, 0), (9, 8, 100, 4), (40, 12, 30, 4),
+                                                    (130, 8, -1, 0)])
 def test_what_a_row_does_not_attend_cannot_reach_it(gpu, cache, rows, heads, window, sinks):
     """NaN behind the last token, in front of the window and at drafted tokens after a row's own position."""
     lens, kv = [700, 300], 2
@@ -138,7 +152,7 @@ def test_what_a_row_does_not_attend_cannot_reach_it(gpu, cache, rows, heads, win
 
 
 @pytest.mark.parametrize("cache,odd", [("e4m3", "nan"), ("same", "nan"), ("same", "inf"), ("same", "-inf"), ("same", "both")])
-@pytest.mark.parametrize("rows,window,sinks", [(1, -1, 0), (7, -1, 0), (7, 20, 3), (20, -1, 0)])
+@pytest.mark.parametrize("rows,window,sinks", [(1, -1, 0), (7, -1, 0), (7, 20, 3), (20, -1, 0), (40, -1, 0), (70, 20, 3)])
 def test_odd_values_reach_their_rows_and_dims(gpu, cache, odd, rows, window, sinks):
     """A value that is no finite number reaches the rows that attend its key, in its dim and KV head alone."""
     lens, kv, heads = [300, 170], 2, 8
@@ -163,17 +177,18 @@ def test_odd_values_reach_their_rows_and_dims(gpu, cache, odd, rows, window, sin
     assert ((got.double() - want).abs() <= tol)[fine].all()
 
 
-def test_nan_in_queries_and_keys(gpu):
-    lens, kv, heads, rows = [400], 2, 8, 6
+@pytest.mark.parametrize("rows", [6, 40, 100])
+def test_nan_in_queries_and_keys(gpu, rows):
+    lens, kv, heads = [400], 2, 8
     keys, values, table, ks, vs = make_any_cache(lens, kv, BF16, "e4m3", seed=41)
     query = make_rows(rows, heads, BF16, 42)
     query[2, 5, 9] = float("nan")
-    bits(keys)[int(table[0, 3]), 397 - 384, 0, 3] = 0x7f  # key 397: rows 3, 4 and 5 attend it
+    bits(keys)[int(table[0, 3]), 397 - 384, 0, 3] = 0x7f  # key 397: the last three rows attend it
     got = cached.cached_attention(query.to(gpu), keys.to(gpu), values.to(gpu), table.to(gpu), ints(lens, gpu), SCALE,
                                   **gpu_scales(ks, vs, gpu)).cpu()
     want = torch.zeros(rows, heads, dtype=torch.bool)
     want[2, 5] = True
-    want[3:, :4] = True
+    want[-3:, :4] = True
     assert torch.equal(got.isnan().all(dim=-1), want) and torch.equal(got.isnan().any(dim=-1), want)
 
 
@@ -231,6 +246,11 @@ def test_a_cache_behind_2_31_bytes(gpu):
     got = cached.cached_attention(query.to(gpu), keys, values, ints([used], gpu), ints(lens, gpu), SCALE,
                                   **gpu_scales(ks, vs, gpu)).cpu()
     assert ((got.double() - want).abs() <= attention_tolerance(want, size, v, vs, 640, BF16)).all()
+    many = make_rows(100, heads, BF16, 63)  # a chunk
+    want, size = OC.attention(many, k, v, torch.arange(5, dtype=torch.int32)[None], ints(lens), SCALE, -1, 0, ks, vs)
+    got = cached.cached_attention(many.to(gpu), keys, values, ints([used], gpu), ints(lens, gpu), SCALE,
+                                  **gpu_scales(ks, vs, gpu)).cpu()
+    assert ((got.double() - want).abs() - attention_tolerance(want, size, v, vs, 640, BF16)).max() <= 0
     # 16384 columns that repeat these pages: every key 3276 or 3277 times
     cols = 16384
     long = at.to(torch.int32).repeat(cols // 5 + 1)[:cols].view(1, cols).contiguous()
@@ -254,13 +274,14 @@ def test_many_requests(gpu):
     check(out.cpu(), want, size, values, vs, 300, lens, 1, before)
 
 
-def test_graph_replays_with_other_lengths(gpu):
-    """Two graphs of decoding steps from one pool, replayed in turn with lengths of their own and eager calls between."""
+@pytest.mark.parametrize("rows", [1, 6, 60])
+def test_graph_replays_with_other_lengths(gpu, rows):
+    """Two graphs of steps from one pool, replayed in turn with lengths of their own and eager calls between."""
     heads, kv, batch = 8, 2, 5
     keys, values, table, ks, vs = make_any_cache([2500, 1800, 2000, 900, 700], kv, BF16, "e4m3", seed=81)
     keys, values, table = keys.to(gpu), values.to(gpu), table.to(gpu)
     scales = gpu_scales(ks, vs, gpu)
-    query = make_rows(batch, heads, BF16, 82).to(gpu)
+    query = make_rows(batch * rows, heads, BF16, 82).to(gpu)
     lens = [ints([1] * batch, gpu) for _ in range(2)]
     outs = [torch.zeros_like(query) for _ in range(2)]
     cached.cached_attention(query, keys, values, table, lens[0], SCALE, out=outs[0], **scales)
@@ -289,7 +310,7 @@ def test_threads_and_streams(gpu, binding):
     keys, values, table, ks, vs = make_any_cache(lens, 2, BF16, "e4m3", seed=91)
     args = (keys.to(gpu), values.to(gpu), table.to(gpu), ints(lens, gpu))
     scales = gpu_scales(ks, vs, gpu)
-    queries = [make_rows(3 * r, 8, BF16, 92 + r).to(gpu) for r in (1, 5, 20)]
+    queries = [make_rows(3 * r, 8, BF16, 92 + r).to(gpu) for r in (1, 5, 60)]
 
     def call(i):
         out = torch.zeros_like(queries[i])
