@@ -24,11 +24,12 @@ def new_cache(num_pages: int, kv_heads: int, dtype=None, *, device=None):
 
 def head_scales(rows, margin: float = 1.0):
     """fp32 ``[kv_heads]`` scales that give the largest number of each head of ``rows [tokens, kv_heads, 128]``, times
-    ``margin``, the largest of an 8-bit cache; 1 for a head of zeros."""
+    ``margin``, the largest of an 8-bit cache; 1 for a head of zeros (and of numbers too small for a normal scale)."""
     import torch
 
     largest = rows.detach().abs().amax(dim=(0, 2)).float() * (margin / E4M3_MAX)
-    return torch.where(largest > 0, largest, torch.ones_like(largest)).contiguous()
+    normal = largest >= torch.finfo(torch.float32).tiny
+    return torch.where(normal, largest, torch.ones_like(largest)).contiguous()
 
 
 def cached_attention(query, key_cache, value_cache, block_table, seq_lens, softmax_scale: float, *, window: int = -1,
