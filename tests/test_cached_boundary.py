@@ -245,5 +245,7 @@ def test_head_scales():
     s = cached.head_scales(x)
     assert s.dtype == torch.float32 and torch.equal(s, torch.tensor([2.0, 2.0 / 448, 1.0]))
     assert torch.equal(cached.head_scales(x, margin=2.0), torch.tensor([4.0, 4.0 / 448, 1.0]))
+    x[1, 0, 4], x[2, 1, 7] = 2.0 ** -120, 2.0 ** -117  # 2^-120 / 448 is no normal number of 32 bits
+    assert torch.equal(cached.head_scales(x), torch.tensor([1.0, 2.0 ** -117 / 448, 1.0]))
     keys, values = cached.new_cache(3, 2, torch.float16)
     assert keys.shape == values.shape == (3, 128, 2, 128) and keys.dtype == torch.float16 and not keys.any()
