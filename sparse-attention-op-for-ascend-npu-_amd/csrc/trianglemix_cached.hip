@@ -513,9 +513,9 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
       s_sum[wave][16 * n + col] = l;
     }
   }
-  // 16 threads a row, 8 dims each.
-  const int r16 = tid >> 4, c8 = tid & 15;
-  auto store_row = [&](int of_slot, int r, const float* acc, float l) TM_INLINED {
+  // 16 threads a row, dims 4 c16 .. + 3 and 64 + 4 c16 .. + 3 each.
+  const int r16 = tid >> 4, c16 = tid & 15;
+  auto store = [&](int of_slot, int r, const float* acc, float l) TM_INLINED {
     const int at = (of_slot & (row_tiles - 1)) * kRows + r;
     const int t = by_group.token(at);
     if (pos0 + t < 0) return;  // before the request's first token: no row
@@ -525,11 +525,7 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
     const float inv = l > 0.0f ? v_scale / l : 0.0f;
     // a NaN sum fails the comparison, and must reach the result
     const float scale = (__float_as_uint(l) & 0x7fffffffu) > 0x7f800000u ? l : inv;
-    typename Type::vec y;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = (elem)(acc[e] * scale);
-    *reinterpret_cast<typename Type::vec*>(
-        p.out + ((int64_t)(row0 + t) * p.heads + head * G + (at - t * G)) * kHeadDim + 8 * c8) = y;
+    store_row<Type>(p.out + ((int64_t)(row0 + t) * p.heads + head * G + (at - t * G)) * kHeadDim, c16, acc, scale);
   };
   auto rows_of = [&](int of_slot) TM_INLINED { return min(kRows, part_rows - (of_slot & (row_tiles - 1)) * kRows); };
 #pragma unroll
@@ -564,30 +560,30 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const f32x4_t x =
-              *reinterpret_cast<const f32x4_t*>(&o_lds[k][at16 * kHeadDim + 4 * ((2 * c8 + half) ^ at16)]);
+              *reinterpret_cast<const f32x4_t*>(&o_lds[k][at16 * kHeadDim + 4 * ((16 * half + c16) ^ at16)]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[4 * half + e] += x[e];
         }
       }
 #pragma unroll
       for (int kind = 0; kind < 3; ++kind) {
-        const unsigned odd = s_odd[of_slot * kRows + r][kind][c8 >> 2] >> (8 * (c8 & 3)) & 0xffu;
+        const unsigned* const odd = s_odd[of_slot * kRows + r][kind] + (c16 >> 3);
         // bits, and no number that is taken for finite
         float value = __uint_as_float(kind == 0 ? 0x7f800000u : kind == 1 ? 0xff800000u : 0x7fc00000u);
         asm volatile("" : "+v"(value));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] += odd >> e & 1 ? value : 0.0f;
+        for (int e = 0; e < 8; ++e) acc[e] += odd[2 * (e >> 2)] >> (4 * (c16 & 7) + (e & 3)) & 1 ? value : 0.0f;
       }
       if (whole) {
-        store_row(of_slot, r, acc, l);
+        store(of_slot, r, acc, l);
       } else {
         const int row = of_slot * slot_rows + r;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const f32x4_t x = {acc[4 * half], acc[4 * half + 1], acc[4 * half + 2], acc[4 * half + 3]};
-          group.store(share, row, 8 * c8 + 4 * half, x);
+          group.store(share, row, 64 * half + 4 * c16, x);
         }
-        if (c8 == 0) group.store_sums(share, row, all, l);
+        if (c16 == 0) group.store_sums(share, row, all, l);
       }
     }
   }
@@ -596,7 +592,7 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
     merge_shares<kThreads, kFlight, kEach>(
         p, group, join, &s_last,
         [&](int row) TM_INLINED { return row % slot_rows < rows_of(row / slot_rows); },
-        [&](int row, int, const float* acc, float l) TM_INLINED { store_row(row / slot_rows, row % slot_rows, acc, l); });
+        [&](int row, const float* acc, float l) TM_INLINED { store(row / slot_rows, row % slot_rows, acc, l); });
   }
 }
 

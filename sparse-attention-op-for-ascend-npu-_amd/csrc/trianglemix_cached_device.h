@@ -77,12 +77,26 @@ struct Shares {
   }
 };
 
+// A row's numbers of the thread c16 of its 16, as merge_shares has them, times `scale`.
+template <class Type>
+__device__ __forceinline__ void store_row(uint16_t* row, int c16, const float* acc, float scale) {
+  typedef typename Type::elem vec4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    vec4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (typename Type::elem)(acc[4 * half + e] * scale);
+    *reinterpret_cast<vec4*>(row + 64 * half + 4 * c16) = y;
+  }
+}
+
 // Merges a shared group once its partials are stored: the workgroup that arrives last
 // at a cluster of shares merges it, the one that arrives last of the clusters those
-// (the same sums whichever they are).  16 threads a row, 8 dims each; where the rows
+// (the same sums whichever they are).  16 threads a row, dims 4 c16 .. + 3 and 64 + 4
+// c16 .. + 3 each (what they load or store at once lies side by side); where the rows
 // leave threads over, `parts` of them share a row's partials and join through LDS.  A
 // thread has the loads of kFlight partials of kEach rows in flight.  held(row): whether the record's row
-// is one; out(row, c8, acc, sum): its dims 8 c8 .. + 7.  Every thread calls it.
+// is one; out(row, acc, sum): the thread's dims of it.  Every thread calls it.
 template <int kThreads>
 __device__ __forceinline__ int merge_parts(int rows) {
   int row_slots = 1;
@@ -92,7 +106,7 @@ __device__ __forceinline__ int merge_parts(int rows) {
 template <int kThreads, int kFlight, int kEach, class Held, class Out>
 __device__ __forceinline__ void merge_shares(const CachedParams& p, const Shares& shares, float (*join)[10], int* last,
                                              Held held, Out out) {
-  const int tid = threadIdx.x, r16 = tid >> 4, c8 = tid & 15;
+  const int tid = threadIdx.x, r16 = tid >> 4, c16 = tid & 15;
   const int parts = merge_parts<kThreads>(shares.rows), row_slots = kThreads / 16 / parts;
   const int cluster = kFlight * parts, pg = r16 / row_slots;
   for (int level = 0; level < 2; ++level) {
@@ -143,7 +157,7 @@ __device__ __forceinline__ void merge_shares(const CachedParams& p, const Shares
             for (int half = 0; half < 2; ++half) {
               x[i][j][half] = __builtin_bit_cast(
                   f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                               shares.partials, at + (row[i] * kHeadDim + 8 * c8 + 4 * half) * 4, 0, kCpolAgent));
+                               shares.partials, at + (row[i] * kHeadDim + 64 * half + 4 * c16) * 4, 0, kCpolAgent));
             }
           }
         }
@@ -204,14 +218,14 @@ __device__ __forceinline__ void merge_shares(const CachedParams& p, const Shares
       for (int i = 0; i < kEach; ++i) {
         if (pg != 0 || !ok[i]) continue;
         if (last_level) {
-          out(row[i], c8, acc[i], l[i]);
+          out(row[i], acc[i], l[i]);
         } else {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const f32x4_t x = {acc[i][4 * half], acc[i][4 * half + 1], acc[i][4 * half + 2], acc[i][4 * half + 3]};
-            shares.store(from, row[i], 8 * c8 + 4 * half, x);
+            shares.store(from, row[i], 64 * half + 4 * c16, x);
           }
-          if (c8 == 0) shares.store_sums(from, row[i], top[i], l[i]);
+          if (c16 == 0) shares.store_sums(from, row[i], top[i], l[i]);
         }
       }
     }
