@@ -411,26 +411,10 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
     const int t = by_group.token(r);
     return p.out + ((int64_t)(row0 + t) * p.heads + kv_head * G + (r - t * G)) * kHeadDim;
   };
-  if (shares == 1) {
-    if (!ok || key_part != 0 || row_pos < 0) return;  // before the request's first token: no row
-    const float scale = scale_of(l);
-    uint16_t* const to = out_row(row);
-    typedef elem vec4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        vec4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (elem)(o[m][4 * v + e] * scale);
-        *reinterpret_cast<vec4*>(to + 32 * m + 8 * v + 4 * half) = y;
-      }
-    }
-    return;
-  }
   // 64 dims at a time through the wave's part of LDS, so that a store's lanes lie side by
   // side, 256 bytes of a row.
   if (key_part == 0) {
+    const float scale = shares > 1 ? 1.0f : scale_of(l);
     char* const own = kv_lds + (row_base / 32) * (4 * kSlotBytes / kRowTiles);
     static_assert(32 * 64 * 4 <= 4 * kSlotBytes / kWaves, "64 dims of 32 rows fit it");
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's own values: its LDS operations stay in order
@@ -441,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
       for (int c = 0; c < 16; c += 2) {  // dims 4 (c + half) .. + 3 of the 64
         const int m = 2 * side + (c >> 3), v = 4 * ((c & 7) >> 1);
         *reinterpret_cast<f32x4_t*>(own + 256 * n + 16 * ((c + half) ^ (n & 15))) =
-            f32x4_t{o[m][v], o[m][v + 1], o[m][v + 2], o[m][v + 3]};
+            f32x4_t{o[m][v] * scale, o[m][v + 1] * scale, o[m][v + 2] * scale, o[m][v + 3] * scale};
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -449,13 +433,20 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
       for (int i = 0; i < 8; ++i) {
         const int r = 4 * i + (lane >> 4), c = lane & 15;
         const f32x4_t x = *reinterpret_cast<const f32x4_t*>(own + 256 * r + 16 * (c ^ (r & 15)));
-        if (r < valid_rows) group.store(share, row_base + r, 64 * side + 4 * c, x);
+        if (r >= valid_rows) continue;
+        if (shares > 1) {
+          group.store(share, row_base + r, 64 * side + 4 * c, x);
+        } else if (pos0 + by_group.token(row_base + r) >= 0) {  // else before the request's first token: no row
+          typedef elem vec4 __attribute__((ext_vector_type(4)));
+          *reinterpret_cast<vec4*>(out_row(row_base + r) + 64 * side + 4 * c) = __builtin_convertvector(x, vec4);
+        }
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
-    if (ok && half == 0) group.store_sums(share, row, m_run, l);
+    if (shares > 1 && ok && half == 0) group.store_sums(share, row, m_run, l);
   }
+  if (shares == 1) return;
   float(*const join)[10] = reinterpret_cast<float(*)[10]>(kv_lds);
   static_assert(kThreads * 10 * 4 <= 2 * kSlotBytes, "the joined values fit the slots");
   merge_shares<kThreads, 4, 2>(
