@@ -77,8 +77,9 @@ int tm_rotate_and_cache(const void* query, int64_t query_stride, const void* key
  * The step's own keys are in the cache.  Single tokens (rows 1), a few drafted
  * ones, or a whole chunk.
  *
- * A call may read 2^30 tiles of 32 keys, counted over the requests at the
- * table's full width (the window's, where there is one) and the KV heads.  Keys
+ * A call may read 2^30 tiles of 32 keys, counted at the table's full width (the
+ * window's, where there is one) for each request, each KV head (KV heads that a
+ * workgroup has together count once) and, in chunks, each of their parts.  Keys
  * of pages that the cache does not have, and keys past the table, are attended
  * by no row.  Rows before a request's first token are none: their out is left as
  * it was.
@@ -100,7 +101,8 @@ int tm_cached_attention(const void* query, int64_t query_stride, const void* key
                         float scale, int dtype, int cache_dtype, void* workspace, int64_t workspace_bytes,
                         void* stream);
 
-/* Workspace bytes of that call, or -1 for what it refuses.  The workspace is
+/* Workspace bytes of that call over a cache of either type, or -1 for what it
+ * refuses over both.  The workspace is
  * as that of tm_triangle_paged_sparse_attention: any contents, 16-byte
  * aligned, one per call in flight.  At most 64 MiB + 64 KiB. */
 int64_t tm_cached_attention_workspace_size(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads,

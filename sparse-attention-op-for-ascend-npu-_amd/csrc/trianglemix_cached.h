@@ -68,9 +68,13 @@ struct CachedParams {
 struct CachedShape {
   int rows, waves;
 };
-// Chunks, of more rows of a KV head than kMostFewRows: workgroups of kChunkRows rows or
-// of half as many.
-constexpr int kChunkRows = 256, kMostFewRows = 64;
+// Chunks, of more rows of a KV head than most_few_rows: workgroups of kChunkRows rows or
+// of half as many.  (32 requests of 32 tokens, four heads a KV head, 500 to 9000 tokens
+// before them: 128 rows a workgroup that loads for itself 233 us, as chunks 178.  Of 16
+// tokens, 64 rows, 115 and 173 over 8-bit caches, 185 and 178 over 16-bit ones, whose tiles
+// fill the registers; 64 of up to 3000 tokens 110 | 124 and 167 | 131.)
+constexpr int kChunkRows = 256;
+constexpr int most_few_rows(CacheType type) { return type == CacheType::kE4m3 ? 64 : 32; }
 hipError_t launch_cached_chunks(const CachedParams& p, int rows, bool fp16, CacheType cache, hipStream_t stream);
 hipError_t launch_cached_attention(const CachedParams& p, CachedShape shape, bool fp16, CacheType cache,
                                    hipStream_t stream);

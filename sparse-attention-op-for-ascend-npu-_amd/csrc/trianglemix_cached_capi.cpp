@@ -94,8 +94,8 @@ int64_t most_tiles(int64_t rows, int64_t table_cols, int64_t window, int64_t sin
   return std::min(all, (window + rows - 1) / kKvTile + 2 + (std::min(sinks, table_cols * kPageSize) + kKvTile - 1) / kKvTile);
 }
 
-CachedPlan cached_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t table_cols, int64_t window,
-                       int64_t sinks) {
+CachedPlan cached_plan(CacheType type, int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t table_cols,
+                       int64_t window, int64_t sinks) {
   CachedPlan r{};
   const int64_t group = heads / kv_heads, group_rows = rows * group;
   const int64_t tiles = most_tiles(rows, table_cols, window, sinks);
@@ -103,15 +103,15 @@ CachedPlan cached_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_he
   const auto enough = [&](int shift) {
     return kv_heads % (1 << shift) == 0 && batch * (kv_heads >> shift) * std::max<int64_t>(1, tiles / 32) >= kComputeUnits;
   };
-  if (group_rows > kMostFewRows) {
+  if (group_rows > most_few_rows(type)) {
     // Chunks: workgroups of 256 rows, or of 128 with two key parts, one a CU.  What does
     // not fill the GPU's last round is shared out.  Taken is what ends soonest by the
     // time of a step of 64 keys and what a share costs besides (the start, its partial,
     // the merge), in 0.1 us.  256 | 128 rows, four heads to each of eight KV heads: 33
-    // tokens of 8192 49 | 38 us, 75 of 3000 48 | 34, 512 of 8192 94 | 99, 1000 of 20000
-    // 344 | 391, 2048 of 32749 1025 | 1213.
+    // tokens of 8192 40 | 32 us, 75 of 3000 36 | 28, 512 of 8192 88 | 100, 1000 of 20000
+    // 326 | 389, 2048 of 32749 1032 | 1220.
     int64_t best = INT64_MAX;
-    for (const auto [most_rows, step, besides] : {std::array{kChunkRows, 20, 220}, std::array{kChunkRows / 2, 14, 120}}) {
+    for (const auto [most_rows, step, besides] : {std::array{kChunkRows, 20, 120}, std::array{kChunkRows / 2, 14, 60}}) {
       const int64_t part_tokens = most_rows / group, row_parts = (rows + part_tokens - 1) / part_tokens;
       const int64_t tiles = most_tiles(part_tokens, table_cols, window, sinks), steps = (tiles + 1) / 2;
       const int64_t parts = batch * row_parts;
@@ -138,12 +138,10 @@ CachedPlan cached_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_he
   }
   // A wave's rows and the row tiles of a workgroup's waves; what these leave of the
   // waves goes to neighbouring KV heads, whose numbers lie side by side in memory (64
-  // requests of 2000 to 16384 tokens: 221 us with eight heads a workgroup, 233 with
+  // requests of 2000 to 16384 tokens: 219 us with eight heads a workgroup, 232 with
   // four, 275 with two), or to parts of the keys: where there is little to read or
   // many rows, whose partials would cost more (32 requests of 5 tokens, 500 to 9000
-  // before them: 99 us with eight heads, 77 with four, 80 with two).
-  // More than 64 rows are chunks (32 requests of 32 tokens, 500 to 9000 before them: as
-  // four row tiles a workgroup 237 us, as chunks 176; of 16 tokens 117 and 173).
+  // before them: 91 us with eight heads, 75 with four, 79 with two).
   int most_shift;
   if (group_rows <= 16) {
     r.shape = {16, group_rows <= 4 && enough(3) && batch * kv_heads >= kComputeUnits ? 8 : 4};
@@ -165,7 +163,7 @@ CachedPlan cached_plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_he
   if ((groups + r.full_shares) * record_bytes <= kMaxRecordBytes && groups + r.full_shares <= kCounterBytes / 8) {
     r.min_tiles = 1 << r.key_shift;
     // Half a microsecond, where the groups are so many that their last shares matter (32
-    // requests of 5 tokens: 79 us without, 77 with).
+    // requests of 5 tokens 77 us without, 75 with; of 16 tokens 143 and 115).
     r.halvings = tiles > 64 && groups >= kComputeUnits / 4 ? 5 : 0;
     shares = std::min(groups + r.full_shares, r.tiles);
   } else {
@@ -314,8 +312,14 @@ int64_t tm_cached_attention_workspace_size(int64_t batch, int64_t rows, int64_t 
   report(TM_OK, "%s", "");
   if (check_cached(batch, rows, heads, kv_heads, table_cols, window, sinks) != TM_OK) return -1;
   if (batch == 0 || rows == 0) return 0;
-  const CachedPlan plan = cached_plan(batch, rows, heads, kv_heads, table_cols, window, sinks);
-  return check_tiles(plan.tiles) == TM_OK ? plan.workspace_bytes : -1;
+  // What either cache type needs, of those whose call is not refused.
+  int64_t bytes = -1;
+  for (const CacheType type : {CacheType::kSame, CacheType::kE4m3}) {
+    const CachedPlan plan = cached_plan(type, batch, rows, heads, kv_heads, table_cols, window, sinks);
+    if (check_tiles(plan.tiles) == TM_OK) bytes = std::max(bytes, plan.workspace_bytes);
+  }
+  if (bytes >= 0) report(TM_OK, "%s", "");
+  return bytes;
 }
 
 int tm_cached_attention(const void* query, int64_t query_stride, const void* key_cache, int64_t key_page_stride,
@@ -339,7 +343,7 @@ int tm_cached_attention(const void* query, int64_t query_stride, const void* key
   if (st == TM_OK) st = check_element(block_table, 4);
   if (st == TM_OK) st = check_element(seq_lens, 4);
   if (st != TM_OK) return st;
-  const CachedPlan plan = cached_plan(batch, rows, heads, kv_heads, table_cols, window, sinks);
+  const CachedPlan plan = cached_plan(type, batch, rows, heads, kv_heads, table_cols, window, sinks);
   st = check_tiles(plan.tiles);
   if (st == TM_OK) st = check_workspace(workspace, workspace_bytes, plan.workspace_bytes);
   if (st != TM_OK) return st;

@@ -70,6 +70,8 @@ CASES = [
     ([900, 30], 13, 5, 1, -1, 0),         # 65 rows: one more than fits
     ([600, 900], 11, 18, 3, -1, 0),       # 66 rows
     ([640, 300], 7, 18, 2, 100, 3),       # 63 rows, nine heads a KV head
+    ([900, 30, 2000], 11, 9, 3, -1, 0),   # 33 rows
+    ([1100, 8, 700], 8, 8, 2, -1, 0),     # 32 rows
     ([5000], 129, 8, 8, 700, 0),
 ]
 
