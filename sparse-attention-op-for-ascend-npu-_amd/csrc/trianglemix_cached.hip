@@ -20,13 +20,13 @@
 //
 // K and V go from memory into registers, a tile ahead of the one in use: a wave loads
 // what it multiplies itself, so the loop has neither LDS nor barriers.  More tiles
-// ahead (two, three) and two workgroups a CU were no faster: 64 to 128 KB in flight a
-// CU are enough.  The waves' sums meet in LDS behind the loop.
+// ahead (two, three), two workgroups a CU and waves held together by a barrier a tile
+// were no faster: 64 to 128 KB in flight a CU are enough.  The waves' sums meet in LDS behind the loop.
 //
-// What bounds it: memory.  64 requests of 2000 to 16384 tokens (1.22 GB) 222 us, four
-// of 65536 to 131072 (0.83 GB) 149, at 5.5 TB/s over all and 5.9 within the loop; the
+// What bounds it: memory.  64 requests of 2000 to 16384 tokens (1.22 GB) 220 us, four
+// of 65536 to 131072 (0.83 GB) 148, at 5.6 TB/s over all and 5.9 within the loop; the
 // rest is the start (lengths, table and first tiles, each waiting for the one before: 3
-// us), the join and the merge (5 to 10).  One token of 8111 on two KV heads: 10.7
+// us), the join and the merge (5 to 10).  One token of 8111 on two KV heads: 10.3
 // us, launch and round trips alone.
 //
 // Contractions (per wave, 32 keys x 16 NT rows, v_mfma_f32_16x16x32)

@@ -18,11 +18,13 @@
 //   O^T (dims x rows) += V^T P^T  A = V by ds_read_b64_tr_b16, B = P
 // with the operand layouts of trianglemix_device.h.
 //
-// What bounds it: 2048 rows of 32749 tokens 1025 us, 1039 TFLOP/s, where a library
-// product of 8192^3 reaches 1205; MFMAs are busy 44 % of the cycles, vector
-// instructions (exponentials, conversions) 46 %, LDS about as much.  512 rows of 8192
-// tokens: 94 us, 70 of them in the loop, the rest partials of four shares a part (34 MB)
-// and their merge.
+// What bounds it: 2048 rows of 32749 tokens, 32 heads, 1035 us, 1030 TFLOP/s, where a
+// library product of 8192^3 reaches 1205: power, the clock is 2.1 of 2.4 GHz.  A
+// step takes 4300 cycles; MFMAs are busy 47 % of them, LDS 36 %, and the seven vector
+// instructions to an MFMA (exponentials, sums, conversions) about as long as the
+// MFMAs.  Waves half a step apart, so that one's exponentials run beside the other's
+// products, take the same time.  512 rows of 8192 tokens: 85 us, 71 of them in the
+// loop, the rest start, partials of four shares a part (34 MB) and their merge.
 //
 // Parts whose keys are shared by several workgroups (few rows, many keys) are merged
 // as in trianglemix_cached_device.h.  Numerics as in trianglemix_cached.hip.  V entries
