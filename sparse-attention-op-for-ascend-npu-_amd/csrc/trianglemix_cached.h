@@ -74,6 +74,10 @@ struct CachedShape {
 // tokens, 64 rows, 115 and 173 over 8-bit caches, 185 and 178 over 16-bit ones, whose tiles
 // fill the registers; 64 of up to 3000 tokens 110 | 124 and 167 | 131.)
 constexpr int kChunkRows = 256;
+// Steps of 64 keys that a share of a part has at least, also where the requests are far
+// shorter than their table is wide (one request of 128 rows of 300 tokens, 16384 columns:
+// 24 us, without 30; eight steps: 20, but 75 rows of 3000 tokens 42 and 35).
+constexpr int kLeastSteps = 4;
 constexpr int most_few_rows(CacheType type) { return type == CacheType::kE4m3 ? 64 : 32; }
 hipError_t launch_cached_chunks(const CachedParams& p, int rows, bool fp16, CacheType cache, hipStream_t stream);
 hipError_t launch_cached_attention(const CachedParams& p, CachedShape shape, bool fp16, CacheType cache,

@@ -118,7 +118,9 @@ CachedPlan cached_plan(CacheType type, int64_t batch, int64_t rows, int64_t head
       const int64_t full_parts = parts * kv_heads / kComputeUnits * kComputeUnits / kv_heads;
       const int64_t rest = (parts - full_parts) * kv_heads;
       const int64_t record_bytes = part_tokens * group * (kHeadDim + 2) * 4;
-      for (int64_t s = 1; s == 1 || (s <= steps / 4 && s <= 32 && rest * s * record_bytes <= kMaxRecordBytes); ++s) {
+      const int64_t most = std::clamp<int64_t>(rest > 0 ? kMaxRecordBytes / (rest * record_bytes) : 1, 1,
+                                               std::clamp<int64_t>(steps / kLeastSteps, 1, 32));
+      for (int64_t s = 1; s <= most; ++s) {
         const int64_t rounds = full_parts * kv_heads / kComputeUnits;
         const int64_t rest_rounds = (rest * s + kComputeUnits - 1) / kComputeUnits;
         const int64_t time = rounds * steps * step + rest_rounds * ((steps + s - 1) / s * step + (s > 1 ? besides : 0));

@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
   const int pos0 = len - p.rows + part * p.part_tokens;  // of the part's first token; a negative one is no row
   const Tiles<kStepKeys> tiles(p, pos0, pos0 + part_tokens - 1);
   if (tiles.count == 0) return;
-  const int each = (tiles.count + splits - 1) / splits, shares = (tiles.count + each - 1) / each;
+  const int each = max((tiles.count + splits - 1) / splits, kLeastSteps), shares = (tiles.count + each - 1) / each;
   if (share >= shares) return;
   const int lo = share * each, steps = min(each, tiles.count - lo);
   const int unshared = p.full_parts * p.kv_heads;  // workgroups without records

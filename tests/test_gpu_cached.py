@@ -263,6 +263,23 @@ def test_a_cache_behind_2_31_bytes(gpu):
     assert ((got.double() - want).abs() <= attention_tolerance(want, size, v, vs, cols * 128, BF16)).all()
 
 
+@pytest.mark.parametrize("cache", ["e4m3", "same"])
+@pytest.mark.parametrize("lens,rows,window,sinks", [([300], 128, -1, 0), ([40, 700, 0], 33, -1, 0), ([500, 90], 9, -1, 0), ([700, 70], 50, 200, 3),
+                                                    ([900, 3], 1, -1, 0)])
+def test_tables_far_wider_than_the_requests(gpu, cache, lens, rows, window, sinks):
+    """A table for two million tokens, as a captured call has it: nothing but the lengths bounds what is read."""
+    heads, kv = 8, 2
+    keys, values, table, ks, vs = make_any_cache(lens, kv, BF16, cache, seed=131)
+    query, before = make_rows(len(lens) * rows, heads, BF16, 132), make_rows(len(lens) * rows, heads, BF16, 133)
+    want, size = OC.attention(query, keys, values, table, ints(lens), SCALE, window, sinks, ks, vs)
+    wide = torch.full((len(lens), 16384), 1 << 30, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    out = before.to(gpu)
+    cached.cached_attention(query.to(gpu), keys.to(gpu), values.to(gpu), wide.to(gpu), ints(lens, gpu), SCALE, window=window,
+                            sinks=sinks, out=out, **gpu_scales(ks, vs, gpu))
+    check(out.cpu(), want, size, values, vs, max(lens), lens, rows, before)
+
+
 def test_many_requests(gpu):
     """1024 requests of 0 to 300 tokens: more than a wave's lanes hold lengths of."""
     lens = [(i * 37) % 301 for i in range(1024)]
