@@ -115,13 +115,13 @@ CachedPlan cached_plan(CacheType type, int64_t batch, int64_t rows, int64_t head
       const int64_t part_tokens = most_rows / group, row_parts = (rows + part_tokens - 1) / part_tokens;
       const int64_t tiles = most_tiles(part_tokens, table_cols, window, sinks), steps = (tiles + 1) / 2;
       const int64_t parts = batch * row_parts;
-      const int64_t full_parts = parts * kv_heads / kComputeUnits * kComputeUnits / kv_heads;
+      const int64_t rounds = parts * kv_heads / kComputeUnits;  // full ones, to a part: the last may leave CUs to the rest
+      const int64_t full_parts = rounds * kComputeUnits / kv_heads;
       const int64_t rest = (parts - full_parts) * kv_heads;
       const int64_t record_bytes = part_tokens * group * (kHeadDim + 2) * 4;
       const int64_t most = std::clamp<int64_t>(rest > 0 ? kMaxRecordBytes / (rest * record_bytes) : 1, 1,
                                                std::clamp<int64_t>(steps / kLeastSteps, 1, 32));
       for (int64_t s = 1; s <= most; ++s) {
-        const int64_t rounds = full_parts * kv_heads / kComputeUnits;
         const int64_t rest_rounds = (rest * s + kComputeUnits - 1) / kComputeUnits;
         const int64_t time = rounds * steps * step + rest_rounds * ((steps + s - 1) / s * step + (s > 1 ? besides : 0));
         if (time >= best) continue;
