@@ -160,9 +160,11 @@ CachedPlan cached_plan(CacheType type, int64_t batch, int64_t rows, int64_t head
   r.tiles = groups * tiles;
   const int64_t slot_rows = r.row_shift > 0 ? r.shape.rows : std::min<int64_t>(r.shape.rows, group_rows);
   const int64_t record_bytes = (slot_rows << (r.row_shift + head_shift)) * (kHeadDim + 2) * 4;
+  const auto grid = [](int64_t shares) { return (shares + 7) / 8 * 8; };  // each workgroup has a record and a word
   int64_t shares = groups;
   r.full_shares = (int)std::max(kComputeUnits - groups, int64_t(kComputeUnits / 2));
-  if ((groups + r.full_shares) * record_bytes <= kMaxRecordBytes && groups + r.full_shares <= kCounterBytes / 8) {
+  const int64_t most = grid(groups + r.full_shares);
+  if (most * record_bytes <= kMaxRecordBytes && most <= kCounterBytes / 8) {
     r.min_tiles = 1 << r.key_shift;
     // Half a microsecond, where the groups are so many that their last shares matter (32
     // requests of 5 tokens 77 us without, 75 with; of 16 tokens 143 and 115).
@@ -171,7 +173,7 @@ CachedPlan cached_plan(CacheType type, int64_t batch, int64_t rows, int64_t head
   } else {
     r.min_tiles = (int)tiles;  // no group is cut
   }
-  r.workgroups = (int)((shares + 7) / 8 * 8);
+  r.workgroups = (int)grid(shares);
   r.workspace_bytes = shares > groups ? kCounterBytes + r.workgroups * record_bytes : 0;
   return r;
 }
