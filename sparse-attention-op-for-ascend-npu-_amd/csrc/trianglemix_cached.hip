@@ -534,14 +534,17 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
     if (16 * n >= min(kRows, part_rows)) break;
     float top = -INFINITY;
     for (int k = slot; k < kWaves; k += slots) top = fmaxf(top, s_max[k][16 * n + col]);
-    const float weight = m_run[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - top);
+    // A row whose scores here are all -infinity: its weight is zero, and zero times an O that a NaN in V has
+    // reached is NaN, as it must be (the compiler takes no number for NaN: it does not see which this one is).
+    float weight = m_run[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - top);
+    asm volatile("" : "+v"(weight));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {  // dims 32 quad + 8 e + 4 half ..
         f32x4_t x;
 #pragma unroll
-        for (int m = 0; m < 4; ++m) x[m] = m_run[n] == -INFINITY ? 0.0f : o[4 * half + m][n][e] * weight;
+        for (int m = 0; m < 4; ++m) x[m] = o[4 * half + m][n][e] * weight;
         const int chunk = (8 * quad + 2 * e + half) ^ col;
         *reinterpret_cast<f32x4_t*>(&o_lds[wave][col * kHeadDim + 4 * chunk]) = x;
       }
