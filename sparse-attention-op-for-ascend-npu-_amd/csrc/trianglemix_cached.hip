@@ -522,10 +522,8 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
     const int head = (head_group << head_shift) + (of_slot >> p.row_shift);
     float v_scale = 1.0f;
     if constexpr (kCache == CacheType::kE4m3) v_scale = p.value_scale[head];
-    const float inv = l > 0.0f ? v_scale / l : 0.0f;
-    // a NaN sum fails the comparison, and must reach the result
-    const float scale = (__float_as_uint(l) & 0x7fffffffu) > 0x7f800000u ? l : inv;
-    store_row<Type>(p.out + ((int64_t)(row0 + t) * p.heads + head * G + (at - t * G)) * kHeadDim, c16, acc, scale);
+    store_row<Type>(p.out + ((int64_t)(row0 + t) * p.heads + head * G + (at - t * G)) * kHeadDim, c16, acc,
+                    inverse_sum(l), v_scale);
   };
   auto rows_of = [&](int of_slot) TM_INLINED { return min(kRows, part_rows - (of_slot & (row_tiles - 1)) * kRows); };
 #pragma unroll

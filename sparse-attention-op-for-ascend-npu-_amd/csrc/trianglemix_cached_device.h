@@ -77,15 +77,22 @@ struct Shares {
   }
 };
 
-// A row's numbers of the thread c16 of its 16, as merge_shares has them, times `scale`.
+// What a row's numbers are multiplied by, of their weights' sum: a NaN sum fails the comparison, and must reach the
+// result.  The values' scale is a factor of its own: in one with a small scale a large sum would leave no bits
+// (scales go down to 2^-126, sums of fp16 weights up to 2^28 and more).
+__device__ __forceinline__ float inverse_sum(float sum) {
+  return (__float_as_uint(sum) & 0x7fffffffu) > 0x7f800000u ? sum : sum > 0.0f ? 1.0f / sum : 0.0f;
+}
+
+// A row's numbers of the thread c16 of its 16, as merge_shares has them, times the two factors.
 template <class Type>
-__device__ __forceinline__ void store_row(uint16_t* row, int c16, const float* acc, float scale) {
+__device__ __forceinline__ void store_row(uint16_t* row, int c16, const float* acc, float inverse, float scale) {
   typedef typename Type::elem vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     vec4 y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = (typename Type::elem)(acc[4 * half + e] * scale);
+    for (int e = 0; e < 4; ++e) y[e] = (typename Type::elem)(acc[4 * half + e] * inverse * scale);
     *reinterpret_cast<vec4*>(row + 64 * half + 4 * c16) = y;
   }
 }

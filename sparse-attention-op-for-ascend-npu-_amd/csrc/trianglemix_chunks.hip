@@ -405,10 +405,6 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
       for (int v = 0; v < 16; ++v) o[m][v] += odd >> elem_key(v) & 1 ? value : 0.0f;
     }
   }
-  auto scale_of = [&](float sum) TM_INLINED {
-    // a NaN sum fails the comparison, and must reach the result
-    return (__float_as_uint(sum) & 0x7fffffffu) > 0x7f800000u ? sum : sum > 0.0f ? v_scale / sum : 0.0f;
-  };
   auto out_row = [&](int r) TM_INLINED {
     const int t = by_group.token(r);
     return p.out + ((int64_t)(row0 + t) * p.heads + kv_head * G + (r - t * G)) * kHeadDim;
@@ -416,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
   // 64 dims at a time through the wave's part of LDS, so that a store's lanes lie side by
   // side, 256 bytes of a row.
   if (key_part == 0) {
-    const float scale = shares > 1 ? 1.0f : scale_of(l);
+    const float inverse = shares > 1 ? 1.0f : inverse_sum(l), scale = shares > 1 ? 1.0f : v_scale;
     char* const own = kv_lds + (row_base / 32) * (4 * kSlotBytes / kRowTiles);
     static_assert(32 * 64 * 4 <= 4 * kSlotBytes / kWaves, "64 dims of 32 rows fit it");
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's own values: its LDS operations stay in order
@@ -427,7 +423,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
       for (int c = 0; c < 16; c += 2) {  // dims 4 (c + half) .. + 3 of the 64
         const int m = 2 * side + (c >> 3), v = 4 * ((c & 7) >> 1);
         *reinterpret_cast<f32x4_t*>(own + 256 * n + 16 * ((c + half) ^ (n & 15))) =
-            f32x4_t{o[m][v] * scale, o[m][v + 1] * scale, o[m][v + 2] * scale, o[m][v + 3] * scale};
+            f32x4_t{o[m][v] * inverse * scale, o[m][v + 1] * inverse * scale, o[m][v + 2] * inverse * scale,
+                    o[m][v + 3] * inverse * scale};
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -454,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
   merge_shares<kThreads, 4, 2>(
       p, group, join, &s_last, [&](int r) TM_INLINED { return r < part_rows; },
       [&](int r, const float* acc, float sum) TM_INLINED {
-        if (pos0 + by_group.token(r) >= 0) store_row<Type>(out_row(r), tid & 15, acc, scale_of(sum));
+        if (pos0 + by_group.token(r) >= 0) store_row<Type>(out_row(r), tid & 15, acc, inverse_sum(sum), v_scale);
       });
 }
 

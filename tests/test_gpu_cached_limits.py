@@ -71,3 +71,21 @@ def test_odd_values_at_keys_of_no_weight(gpu, dtype, requests, rows, heads, kv):
     want[[3, 64, 127]] = True
     assert torch.equal(got.isnan(), want.expand_as(got))
     assert not got[:rows, :, ~want].any() and got[rows:, :, ~want].isfinite().all() and got[rows:, :, ~want].any()
+
+
+@pytest.mark.parametrize("n,rows,heads", [(60, 1, 8), (100000, 1, 8), (100000, 8, 8), (100000, 20, 8), (20000, 300, 16)])
+def test_value_scales_of_any_size(gpu, n, rows, heads):
+    """From 2^-126 to 2^118, over sums of many weights: equal keys, so that a row is the mean of one number.
+
+    The weights are equal and exact; what is summed and multiplied in 32 bits stays below 2^-12, the rounding is half a step.
+    """
+    kv, pages = 4, -(-n // 128)
+    vs = torch.tensor([2.0 ** -126, 1.7 * 2.0 ** -126, 1.3 * 2.0 ** -118, 2.0 ** 118])
+    table = torch.arange(pages, dtype=torch.int32).view(1, -1)
+    keys, values = cached.new_cache(pages, kv)
+    values = torch.full(values.shape, 448.0).to(values.dtype)
+    query = make_rows(rows, heads, BF16, 5)
+    got = cached.cached_attention(query.to(gpu), keys.to(gpu), values.to(gpu), table.to(gpu), ints([n], gpu), SCALE,
+                                  **gpu_scales(torch.ones(kv), vs, gpu)).cpu()
+    want = (448.0 * vs.double()).repeat_interleave(heads // kv)[:, None].expand(rows, heads, 128)
+    assert ((got.double() - want).abs() <= (2.0 ** -12 + half_step(BF16)) * want).all()
