@@ -44,7 +44,9 @@ struct RotateFp16 { typedef f16x8_t vec; typedef _Float16 elem; };
 // what is larger, NaN for NaN.  The quotient is the product with the reciprocal and
 // one step of its error, the division's rounding at a third of its instructions
 // (4096 tokens: 17.3 us, with divisions 18.0); far beyond the range, where that step
-// may overflow, the product alone says which end.
+// may overflow, the product alone says which end.  By scales below 2^-90 the numbers are
+// divided: the error's step may be too small for a number of 32 bits there, and ties of
+// such quotients would go astray.
 __device__ __forceinline__ u32x2_t to_e4m3(const float* x, float scale) {
   const float reciprocal = 1.0f / scale;
   float y[8];
@@ -52,8 +54,15 @@ __device__ __forceinline__ u32x2_t to_e4m3(const float* x, float scale) {
   for (int e = 0; e < 8; ++e) {
     const float near = x[e] * reciprocal;
     const float step = __builtin_fmaf(__builtin_fmaf(-near, scale, x[e]), reciprocal, near);
-    const float q = fabsf(near) < 1024.0f ? __builtin_copysignf(step, near) : near;  // a zero keeps its sign
-    y[e] = (__float_as_uint(q) & 0x7fffffffu) > 0x7f800000u ? q : __builtin_amdgcn_fmed3f(q, -448.0f, 448.0f);
+    y[e] = fabsf(near) < 1024.0f ? __builtin_copysignf(step, near) : near;  // a zero keeps its sign
+  }
+  if (__builtin_expect(scale < 0x1p-90f, 0)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = x[e] / scale;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if ((__float_as_uint(y[e]) & 0x7fffffffu) <= 0x7f800000u) y[e] = __builtin_amdgcn_fmed3f(y[e], -448.0f, 448.0f);
   }
   u32x2_t r;
 #pragma unroll
