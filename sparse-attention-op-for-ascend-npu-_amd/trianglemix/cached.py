@@ -23,13 +23,14 @@ def new_cache(num_pages: int, kv_heads: int, dtype=None, *, device=None):
 
 
 def head_scales(rows, margin: float = 1.0):
-    """fp32 ``[kv_heads]`` scales that give the largest number of each head of ``rows [tokens, kv_heads, 128]``, times
-    ``margin``, the largest of an 8-bit cache; 1 for a head of zeros (and of numbers too small for a normal scale)."""
+    """fp32 ``[kv_heads]`` scales that give the largest finite number of each head of ``rows [tokens, kv_heads, 128]``,
+    times ``margin``, the largest of an 8-bit cache; 1 for a head of zeros (and of numbers too small for a normal scale)."""
     import torch
 
-    largest = rows.detach().abs().amax(dim=(0, 2)).float() * (margin / E4M3_MAX)
+    size = rows.detach().abs()
+    largest = size.masked_fill(~size.isfinite(), 0.0).amax(dim=(0, 2)).float() * (margin / E4M3_MAX)
     normal = largest >= torch.finfo(torch.float32).tiny
-    return torch.where(normal, largest, torch.ones_like(largest)).contiguous()
+    return torch.where(normal, largest.clamp(max=2.0 ** 126), torch.ones_like(largest)).contiguous()
 
 
 def cached_attention(query, key_cache, value_cache, block_table, seq_lens, softmax_scale: float, *, window: int = -1,
