@@ -590,7 +590,7 @@ __global__ void __launch_bounds__(64 * kWaves, 1) cached_attention_kernel(const 
   }
 
   if (!whole) {
-    merge_shares<kThreads, kFlight, kEach>(
+    merge_shares<kThreads, kFlight, kEach, true>(
         p, group, join, &s_last,
         [&](int row) TM_INLINED { return row % slot_rows < rows_of(row / slot_rows); },
         [&](int row, const float* acc, float l) TM_INLINED { store(row / slot_rows, row % slot_rows, acc, l); });

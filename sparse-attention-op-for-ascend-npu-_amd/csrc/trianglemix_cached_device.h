@@ -101,20 +101,21 @@ __device__ __forceinline__ void store_row(uint16_t* row, int c16, const float* a
 // at a cluster of shares merges it, the one that arrives last of the clusters those
 // (the same sums whichever they are).  16 threads a row, dims 4 c16 .. + 3 and 64 + 4
 // c16 .. + 3 each (what they load or store at once lies side by side); where the rows
-// leave threads over, `parts` of them share a row's partials and join through LDS.  A
-// thread has the loads of kFlight partials of kEach rows in flight.  held(row): whether the record's row
-// is one; out(row, acc, sum): the thread's dims of it.  Every thread calls it.
+// leave threads over, `parts` of them share a row's partials and join through LDS (kJoin;
+// without it they never are, and `join` is null).  A thread has the loads of kFlight
+// partials of kEach rows in flight.  held(row): whether the record's row is one; out(row,
+// acc, sum): the thread's dims of it.  Every thread calls it.
 template <int kThreads>
 __device__ __forceinline__ int merge_parts(int rows) {
   int row_slots = 1;
   while (row_slots < rows && row_slots < kThreads / 16) row_slots *= 2;
   return kThreads / 16 / row_slots;
 }
-template <int kThreads, int kFlight, int kEach, class Held, class Out>
+template <int kThreads, int kFlight, int kEach, bool kJoin, class Held, class Out>
 __device__ __forceinline__ void merge_shares(const CachedParams& p, const Shares& shares, float (*join)[10], int* last,
                                              Held held, Out out) {
   const int tid = threadIdx.x, r16 = tid >> 4, c16 = tid & 15;
-  const int parts = merge_parts<kThreads>(shares.rows), row_slots = kThreads / 16 / parts;
+  const int parts = kJoin ? merge_parts<kThreads>(shares.rows) : 1, row_slots = kThreads / 16 / parts;
   const int cluster = kFlight * parts, pg = r16 / row_slots;
   for (int level = 0; level < 2; ++level) {
     // the shares that are merged: `count` from `from` on, every stride-th

@@ -446,10 +446,9 @@ __global__ void __launch_bounds__(kThreads, 1) cached_chunk_kernel(const CachedP
     if (shares > 1 && ok && half == 0) group.store_sums(share, row, m_run, l);
   }
   if (shares == 1) return;
-  float(*const join)[10] = reinterpret_cast<float(*)[10]>(kv_lds);
-  static_assert(kThreads * 10 * 4 <= 2 * kSlotBytes, "the joined values fit the slots");
-  merge_shares<kThreads, 4, 2>(
-      p, group, join, &s_last, [&](int r) TM_INLINED { return r < part_rows; },
+  static_assert(kChunkRows / 2 - (kMaxGroup - 1) >= kThreads / 16, "a record's rows leave no thread over to join");
+  merge_shares<kThreads, 4, 2, false>(
+      p, group, nullptr, &s_last, [&](int r) TM_INLINED { return r < part_rows; },
       [&](int r, const float* acc, float sum) TM_INLINED {
         if (pos0 + by_group.token(r) >= 0) store_row<Type>(out_row(r), tid & 15, acc, inverse_sum(sum), v_scale);
       });
