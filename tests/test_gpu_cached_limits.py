@@ -8,6 +8,7 @@ import torch
 from cached_cases import attention_tolerance, bits, half_step, make_any_cache
 from pages_cases import SCALE, make_rows
 from trianglemix import cached
+from trianglemix.native import load_hip_library
 
 pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
@@ -89,3 +90,86 @@ def test_value_scales_of_any_size(gpu, n, rows, heads):
                                   **gpu_scales(torch.ones(kv), vs, gpu)).cpu()
     want = (448.0 * vs.double()).repeat_interleave(heads // kv)[:, None].expand(rows, heads, 128)
     assert ((got.double() - want).abs() <= (2.0 ** -12 + half_step(BF16)) * want).all()
+
+
+# requests, rows, heads, KV heads, window, first keys, columns of the table: four and eight waves of 16 rows, 32 rows with
+# one and two row tiles a workgroup, chunks of 128 and of 256 rows
+SHAPES = [(2, 4, 8, 2, -1, 0, 0), (2, 4, 8, 2, 40, 3, 0), (32, 2, 16, 8, -1, 0, 64), (32, 2, 16, 8, 40, 3, 300), (2, 8, 8, 2, -1, 0, 0),
+          (2, 8, 8, 2, 40, 3, 0), (2, 16, 8, 2, 40, 3, 0), (2, 50, 8, 2, -1, 0, 0), (2, 50, 8, 2, 40, 3, 0), (2, 150, 6, 2, 70, 130, 0),
+          (32, 64, 32, 8, -1, 0, 0), (32, 64, 32, 8, 40, 3, 0)]
+
+
+@pytest.mark.parametrize("cache,dtype", [("e4m3", BF16), ("same", BF16), ("same", FP16)])
+@pytest.mark.parametrize("requests,rows,heads,kv,window,sinks,cols", SHAPES)
+def test_rows_of_a_step_are_apart(gpu, cache, dtype, requests, rows, heads, kv, window, sinks, cols):
+    """NaN at a key that the step's later tokens alone attend, or the earlier ones' windows alone: these rows' results are
+    NaN, the others as without it."""
+    print(f"apart {requests} {rows} {heads}/{kv} {window} {sinks} {cols} {cache} {dtype}", flush=True)
+    lens = [700 if b % 2 == 0 else 300 for b in range(requests)]
+    keys, values, table, ks, vs = make_any_cache(lens, kv, dtype, cache, seed=rows + requests)
+    if cols:  # as a captured call's
+        wide = torch.full((requests, cols), -1, dtype=torch.int32)
+        wide[:, :table.shape[1]] = table
+        table = wide
+    query = make_rows(requests * rows, heads, dtype, 22)
+    want, size = definition(query, keys, values, table, lens, rows, window, sinks, ks, vs)
+    tol = attention_tolerance(want, size, values, vs, 700, dtype)
+    nan = bits(torch.tensor(float("nan")).to(keys.dtype))
+    # behind the step's middle; before it, at the first key that the first row's window holds
+    places = [(lambda n: n - rows // 2)] + ([lambda n: n - rows - window] if window >= 0 else [])
+    for place in places:
+        for poisoned in range(2):
+            both = [keys.clone(), values.clone()]
+            attends = torch.zeros(requests * rows, dtype=torch.bool)
+            for b, n in enumerate(lens):
+                k = place(n)
+                bits(both[poisoned])[int(table[b, k // 128]), k % 128] = nan
+                attends[b * rows:(b + 1) * rows] = seen_keys(n, rows, window, sinks)[:, k]
+            assert attends.any() and not attends.all()
+            got = cached.cached_attention(query.to(gpu), both[0].to(gpu), both[1].to(gpu), table.to(gpu), ints(lens, gpu),
+                                          SCALE, window=window, sinks=sinks, **gpu_scales(ks, vs, gpu)).cpu()
+            assert got[attends].isnan().all()
+            assert ((got.double() - want).abs() <= tol)[~attends].all()
+
+
+@pytest.mark.parametrize("cache", ["e4m3", "same"])
+@pytest.mark.parametrize("requests,rows,heads,kv,window,sinks", [
+    (1024, 1, 64, 64, -1, 0), (1024, 1, 64, 64, 100, 4), (256, 16, 32, 8, -1, 0), (1024, 5, 32, 8, -1, 0), (900, 5, 32, 8, 33, 2)])
+def test_batches_whose_groups_are_too_many_to_share(gpu, cache, requests, rows, heads, kv, window, sinks):
+    """As many groups as leave no memory for records: each is one workgroup's, of any length."""
+    print(f"unshared {requests} {rows} {heads}/{kv} {window} {cache}", flush=True)
+    lens = [(i * 37) % 301 for i in range(requests)]
+    keys, values, table, ks, vs = make_any_cache([300] * 40, kv, BF16, cache, seed=71)
+    table = table[torch.arange(requests) % 40].contiguous()  # requests that share pages
+    if cache == "e4m3" or rows * heads // kv <= 32:  # more rows over a 16-bit cache are a chunk's
+        size_of = load_hip_library().tm_cached_attention_workspace_size
+        assert size_of(requests, rows, heads, kv, table.shape[1], window, sinks) == 0
+    query = make_rows(requests * rows, heads, BF16, 72)
+    want, size = definition(query, keys, values, table, lens, rows, window, sinks, ks, vs)
+    before = torch.full(query.shape, 3.0, dtype=BF16)
+    out = before.to(gpu)
+    cached.cached_attention(query.to(gpu), keys.to(gpu), values.to(gpu), table.to(gpu), ints(lens, gpu), SCALE, window=window,
+                            sinks=sinks, out=out, **gpu_scales(ks, vs, gpu))
+    got = out.cpu()
+    held = ints(lens).repeat_interleave(rows) - rows + torch.arange(requests * rows) % rows >= 0
+    assert ((got.double() - want).abs() <= attention_tolerance(want, size, values, vs, 300, BF16))[held].all()
+    assert torch.equal(got[~held], before[~held])
+
+
+@pytest.mark.parametrize("cache", ["e4m3", "same"])
+@pytest.mark.parametrize("lens,rows,heads,kv,window,sinks", [
+    ([1100, 2000, 700], 1024, 15, 3, -1, 0), ([2100, 900], 1500, 20, 5, -1, 0), ([2048], 2048, 28, 7, 300, 5),
+    ([700, 1200], 700, 9, 9, -1, 0)])
+def test_chunks_of_odd_kv_heads(gpu, cache, lens, rows, heads, kv, window, sinks):
+    """KV heads that divide no round of the GPU, groups that divide no workgroup's rows."""
+    keys, values, table, ks, vs = make_any_cache(lens, kv, BF16, cache, seed=81)
+    query = make_rows(len(lens) * rows, heads, BF16, 82)
+    want, size = definition(query, keys, values, table, lens, rows, window, sinks, ks, vs)
+    before = torch.full(query.shape, 3.0, dtype=BF16)
+    out = before.to(gpu)
+    cached.cached_attention(query.to(gpu), keys.to(gpu), values.to(gpu), table.to(gpu), ints(lens, gpu), SCALE, window=window,
+                            sinks=sinks, out=out, **gpu_scales(ks, vs, gpu))
+    got = out.cpu()
+    held = ints(lens).repeat_interleave(rows) - rows + torch.arange(len(lens) * rows) % rows >= 0
+    assert ((got.double() - want).abs() <= attention_tolerance(want, size, values, vs, 2100, BF16))[held].all()
+    assert torch.equal(got[~held], before[~held])
