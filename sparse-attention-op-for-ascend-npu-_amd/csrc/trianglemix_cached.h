@@ -75,8 +75,9 @@ struct CachedShape {
 // fill the registers; 64 of up to 3000 tokens 110 | 124 and 167 | 131.)
 constexpr int kChunkRows = 256;
 // Steps of 64 keys that a share of a part has at least, also where the requests are far
-// shorter than their table is wide (one request of 128 rows of 300 tokens, 16384 columns:
-// 24 us, without 30; eight steps: 20, but 75 rows of 3000 tokens 42 and 35).
+// shorter than their table is wide (16384 columns, one request: 128 rows of 300 tokens 24
+// us, without a least 30, with eight steps 20; but 75 rows of 3000 tokens 36, with eight
+// 42.  In tables as wide as the request is long they take 17 and 27).
 constexpr int kLeastSteps = 4;
 constexpr int most_few_rows(CacheType type) { return type == CacheType::kE4m3 ? 64 : 32; }
 hipError_t launch_cached_chunks(const CachedParams& p, int rows, bool fp16, CacheType cache, hipStream_t stream);

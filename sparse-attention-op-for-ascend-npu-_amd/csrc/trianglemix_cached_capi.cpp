@@ -106,8 +106,10 @@ CachedPlan cached_plan(CacheType type, int64_t batch, int64_t rows, int64_t head
   if (group_rows > most_few_rows(type)) {
     // Chunks: workgroups of 256 rows, or of 128 with two key parts, one a CU.  What does
     // not fill the GPU's last round is shared out.  Taken is what ends soonest by the
-    // time of a step of 64 keys and what a share costs besides (the start, its partial,
-    // the merge), in 0.1 us.  256 | 128 rows, four heads to each of eight KV heads: 33
+    // time of a step of 64 keys and what a share costs besides (its partial and the merge),
+    // in 0.1 us; what every call costs (launch, start, results) is left out on both sides.
+    // Lengths are not known here: a request counts as long as its table is wide.
+    // 256 | 128 rows, four heads to each of eight KV heads: 33
     // tokens of 8192 40 | 32 us, 75 of 3000 36 | 28, 512 of 8192 88 | 100, 1000 of 20000
     // 326 | 389, 2048 of 32749 1032 | 1220.
     int64_t best = INT64_MAX;
@@ -143,7 +145,10 @@ CachedPlan cached_plan(CacheType type, int64_t batch, int64_t rows, int64_t head
   // requests of 2000 to 16384 tokens: 219 us with eight heads a workgroup, 232 with
   // four, 275 with two), or to parts of the keys: where there is little to read or
   // many rows, whose partials would cost more (32 requests of 5 tokens, 500 to 9000
-  // before them: 91 us with eight heads, 75 with four, 79 with two).
+  // before them: 91 us with eight heads, 75 with four, 79 with two).  So it is with five
+  // to sixteen rows of a head: four waves | eight, 32 requests of 4 tokens and of 500 to
+  // 9000 69 | 78 us, 1000 of a token and 100 to 900 with eight query heads a KV head 223 |
+  // 233; only of many long ones eight take less (64 of 4 tokens, 2000 to 16384: 242 | 231).
   int most_shift;
   if (group_rows <= 16) {
     r.shape = {16, group_rows <= 4 && enough(3) && batch * kv_heads >= kComputeUnits ? 8 : 4};

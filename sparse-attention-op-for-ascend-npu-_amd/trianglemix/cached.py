@@ -3,7 +3,9 @@
 ``rotary.rotate_and_cache`` fills the cache, ``cached_attention`` reads it: the last ``rows`` tokens of each request attend
 causally over its pages, all of them or a window behind the first few tokens.  An 8-bit cache
 (``torch.float8_e4m3fn``) holds e4m3 numbers with one fp32 scale for each KV head of K and of V: half the memory and
-half the traffic of a 16-bit one.  ``block_table`` and ``seq_lens`` are int32 on the GPU and are read there: a captured
+half the traffic of a 16-bit one.  The package's other operators (the sparse prefill and its dense companion, the
+cache write, page selection, trees) take 16-bit caches alone: ``new_cache(..., dtype=torch.bfloat16)`` makes one
+that both can use.  ``block_table`` and ``seq_lens`` are int32 on the GPU and are read there: a captured
 call can be replayed with others.  ``include/trianglemix_cached.h`` states every rule.
 """
 

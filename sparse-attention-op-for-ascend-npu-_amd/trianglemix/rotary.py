@@ -19,7 +19,8 @@ def frequencies(rotary_dim: int, base: float = 10000.0, *, stretch: float = 1.0,
     ``method`` says how: ``"positions"`` divides every frequency by ``stretch``; ``"base"`` enlarges the base so that the
     slowest pair is divided by it and the fastest is left alone; ``"parts"`` leaves alone the pairs that turn at least
     ``fast_turns`` times over ``trained_length`` positions, divides those of at most ``slow_turns``, and mixes linearly
-    in between (``magnitude`` belongs to it).
+    in between (``magnitude`` belongs to it).  Linearly in the turns: a model trained with a mix that is linear in the
+    pair's index has frequencies of its own, which the operators take as they are.
     """
     import torch
 
